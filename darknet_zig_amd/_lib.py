@@ -1,11 +1,12 @@
-"""ctypes binding of libdkz.so, the C ABI declared in include/dkz_ops.h.
+"""ctypes binding of libdkz.so, the C ABI declared in include/dkz_ops.h, and of
+its companion libdkz_dense.so (include/dkz_dense.h).
 
 This is the Python-side equivalent of the extern declarations a Zig host would
 write against the same header. Every exported symbol is listed in SIGNATURES;
 tests check the table against the header and the built library.
 
-There is deliberately no fallback: if libdkz.so has not been built (or cannot
-be loaded), load() raises and nothing runs.
+There is deliberately no fallback: if a library has not been built (or cannot
+be loaded), load() and load_dense() raise and nothing runs.
 """
 
 from __future__ import annotations
@@ -15,11 +16,14 @@ import os
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libdkz.so"
+DENSE_LIB_NAME = "libdkz_dense.so"
 
 _p = C.c_void_p
 _i = C.c_int
 _f = C.c_float
 _sz = C.c_size_t
+_u = C.c_uint
+_u64 = C.c_ulonglong
 
 # name -> (restype, argtypes), in the order of include/dkz_ops.h.
 SIGNATURES: dict[str, tuple] = {
@@ -83,7 +87,42 @@ SIGNATURES: dict[str, tuple] = {
     "dkz_batchnorm_backward_noalloc": (_i, [_i, _i, _i, _i] + [_p] * 11),
 }
 
+# The same for include/dkz_dense.h.
+_drop = [_f, _f, _u, _u64]  # prob, scale, seed, first
+DENSE_SIGNATURES: dict[str, tuple] = {
+    "dkz_dense_last_error_context": (C.c_char_p, []),
+    "dkz_seeded_dropout": (_i, [_i, _i, _p, _p, *_drop, _i, _p]),
+    "dkz_linear_forward_workspace": (_i, [_i] * 4 + [C.POINTER(_sz)]),
+    "dkz_linear_forward": (_i, [_i] * 5 + _drop + [_p] * 7 + [_sz]),
+    "dkz_linear_backward_workspace": (_i, [_i] * 4 + [C.POINTER(_sz)]),
+    "dkz_linear_backward": (_i, [_i] * 5 + _drop + [_p] * 5 + [_f] + [_p] * 4 + [_sz]),
+    "dkz_linear_cross_entropy_forward_workspace": (_i, [_i] * 4 + [C.POINTER(_sz)] * 2),
+    "dkz_linear_cross_entropy_forward": (_i, [_i] * 4 + [_p] * 7 + [_sz]),
+    "dkz_linear_cross_entropy_backward_workspace": (_i, [_i] * 4 + [C.POINTER(_sz)] * 2),
+    "dkz_linear_cross_entropy_backward": (_i, [_i] * 4 + [_p] * 6 + [_f, _f] + [_p] * 4 + [_sz]),
+}
+
 _LIB: C.CDLL | None = None
+_DENSE: C.CDLL | None = None
+
+
+def _open(p: Path, signatures: dict[str, tuple]) -> C.CDLL:
+    if not p.exists():
+        raise ImportError(
+            f"{p} is not built; the HIP tensor-op libraries are required "
+            "(build them with `python -m darknet_zig_amd.build`)"
+        )
+    lib = C.CDLL(str(p))
+    for name, (res, args) in signatures.items():
+        fn = getattr(lib, name)  # AttributeError names a missing export
+        fn.restype = res
+        fn.argtypes = args
+    return lib
+
+
+def _path() -> Path:
+    env = os.environ.get("DKZ_LIBRARY")
+    return Path(env) if env else LIB_PATH
 
 
 def load(path: Path | str | None = None) -> C.CDLL:
@@ -95,18 +134,17 @@ def load(path: Path | str | None = None) -> C.CDLL:
     global _LIB
     if _LIB is not None and path is None:
         return _LIB
-    env = os.environ.get("DKZ_LIBRARY")
-    p = Path(path) if path is not None else Path(env) if env else LIB_PATH
-    if not p.exists():
-        raise ImportError(
-            f"{p} is not built; the HIP tensor-op library is required "
-            "(build it with `python -m darknet_zig_amd.build`)"
-        )
-    lib = C.CDLL(str(p))
-    for name, (res, args) in SIGNATURES.items():
-        fn = getattr(lib, name)  # AttributeError names a missing export
-        fn.restype = res
-        fn.argtypes = args
+    lib = _open(Path(path) if path is not None else _path(), SIGNATURES)
     if path is None:
         _LIB = lib
     return lib
+
+
+def load_dense() -> C.CDLL:
+    """Loads libdkz_dense.so (once), which lies beside libdkz.so and shares its
+    stream and sync-after-launch switch. Raises if absent."""
+    global _DENSE
+    if _DENSE is None:
+        load()
+        _DENSE = _open(_path().resolve().parent / DENSE_LIB_NAME, DENSE_SIGNATURES)
+    return _DENSE

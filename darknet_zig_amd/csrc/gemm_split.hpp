@@ -602,8 +602,11 @@ constexpr int min_waves() { return BM * BN >= 128 * 128 ? 2 : BM * BN >= 128 * 6
 // needed and the results are the same. Tiles are 64x64 (their sums take 32
 // registers; a 128x128 tile's would take 128), each a part of the g.tile_bm x
 // g.tile_bn tile whose pieces it adds up, or the 32x128 ones.
-template <int BM, int BN, Operand AK, Operand BK, bool ORDERED = false>
-__global__ __launch_bounds__(kBlock, (min_waves<BM, BN>() - (ORDERED ? 2 : 0))) void gemm_split_kernel(SplitArgs g) {
+//
+// Epi: none, and C is alpha * the product + beta * C; or one object, whose
+// put(row, col, value) takes every element of the product instead.
+template <int BM, int BN, Operand AK, Operand BK, bool ORDERED = false, class... Epi>
+__global__ __launch_bounds__(kBlock, (min_waves<BM, BN>() - (ORDERED ? 2 : 0))) void gemm_split_kernel(SplitArgs g, Epi... epi) {
     constexpr int kRowsOfWaves = BM == 32 ? 1 : 2;  // 32-row tiles: four waves side by side
     constexpr int WM = BM / kRowsOfWaves, WN = BN * kRowsOfWaves / 4, TM = WM / 32, TN = WN / 32;
     constexpr int RA = BM == 32 ? 64 : BM;  // rows of A staged (of a 32-row tile, the last row again)
@@ -903,6 +906,14 @@ __global__ __launch_bounds__(kBlock, (min_waves<BM, BN>() - (ORDERED ? 2 : 0))) 
                                   : g.partial + (size_t)slot * g.m * g.n + j;
             const uint32_t ld = !part ? g.ldc : streams ? BN : g.n;
             float out[16];
+            if constexpr (sizeof...(Epi) != 0) {
+                if (!part) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (row(r) < g.m) (epi.put(row(r), j, big[ti][tj][r]), ...);
+                    continue;
+                }
+            }
             if (part) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) out[r] = big[ti][tj][r];
@@ -941,8 +952,8 @@ __global__ __launch_bounds__(kBlock, (min_waves<BM, BN>() - (ORDERED ? 2 : 0))) 
 // partials, 16 beyond, where one lane's loads would take a round trip to memory
 // for every few partials ([1,50176]x[50176,9], 448 of them: 50 us with one lane,
 // 3.2 with 16).
-template <bool V4, int GROUPS>
-__global__ __launch_bounds__(kBlock) void split_reduce_kernel(SplitArgs g) {
+template <bool V4, int GROUPS, class... Epi>
+__global__ __launch_bounds__(kBlock) void split_reduce_kernel(SplitArgs g, Epi... epi) {
     using T = std::conditional_t<V4, float4, float>;
     constexpr uint32_t kW = V4 ? 4 : 1, kOuts = kBlock / GROUPS;
     constexpr int kInFlight = 8;
@@ -975,6 +986,11 @@ __global__ __launch_bounds__(kBlock) void split_reduce_kernel(SplitArgs g) {
     }
     if (!in) return;
     const uint32_t e = v * kW, i = e / g.n, j = e - i * g.n;
+    if constexpr (sizeof...(Epi) != 0) {
+#pragma unroll
+        for (uint32_t x = 0; x < kW; ++x) (epi.put(i, j + x, (float)s[x]), ...);
+        return;
+    }
     float *cp = c_column(g.c, j, g, 0, 0) + (size_t)i * g.ldc;
     T o;
 #pragma unroll
@@ -985,8 +1001,8 @@ __global__ __launch_bounds__(kBlock) void split_reduce_kernel(SplitArgs g) {
 // The streamed tiles' epilogue: adds a tile's pieces in k order (in f64), then as above.
 // A lane takes four consecutive columns of one row, eight pieces in flight; V4:
 // they are 16 aligned bytes of C.
-template <bool V4>
-__global__ __launch_bounds__(kBlock) void stream_reduce_kernel(SplitArgs g) {
+template <bool V4, class... Epi>
+__global__ __launch_bounds__(kBlock) void stream_reduce_kernel(SplitArgs g, Epi... epi) {
     constexpr int kPieces = 8;
     const uint32_t tile_floats = g.tile_bm << g.tile_bn_log2;
     const uint32_t e = 4 * (blockIdx.x * kBlock + threadIdx.x), t = e / tile_floats, at = e - t * tile_floats;
@@ -1008,6 +1024,12 @@ __global__ __launch_bounds__(kBlock) void stream_reduce_kernel(SplitArgs g) {
         for (int u = 0; u < kPieces; ++u)
 #pragma unroll
             for (int x = 0; x < 4; ++x) s[x] += b + u <= last ? (double)::dkz::lane(p[u], x) : 0.0;
+    }
+    if constexpr (sizeof...(Epi) != 0) {
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x)
+            if (j + x < g.n) (epi.put(i, j + x, (float)s[x]), ...);
+        return;
     }
     if constexpr (V4) {
         float *cp = c_column(g.c, j, g, 0, 0) + (size_t)i * g.ldc;

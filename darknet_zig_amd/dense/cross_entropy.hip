@@ -1,0 +1,550 @@
+// cross_entropy.hip -- softmax cross-entropy of a linear layer over many
+// classes without its logits, forward and backward.
+//
+// Forward, bf16: the product's epilogue reduces every wave's part of a row of
+// logits to its maximum m and s = sum of exp(z - m), and a second launch merges
+// a row's (m, s) pairs. Backward: the product again, its epilogue making
+// d = s_r * (onehot - exp(z - lse)) for a piece of the classes, which the two
+// products for the gradients then read. fp32: the logits of a piece are written
+// to the workspace and reduced, or replaced by d, there.
+#include <algorithm>
+
+#include "dense_internal.hpp"
+#include "epilogue.hpp"
+#include "product.hpp"
+#include "product_f32.hpp"
+
+namespace dkz {
+namespace {
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+// exp(x) by the exponential instruction: its argument x * log2(e) is rounded in
+// fp32, so the result is within |x| * 2^-24 of it, and about 1e-6 for the
+// probabilities that matter. NaN in, NaN out.
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+
+// The sum s and maximum m of a set of logits, s relative to m: the pair of none is (0, -inf).
+struct Stat {
+    float m, s;
+};
+// Merges another set. fmaxf passes over NaNs, which stay in s. A set of -infinities has s 0.
+__device__ __forceinline__ Stat merge(Stat a, Stat b) {
+    const float m = fmaxf(a.m, b.m);
+    const float base = m == neg_inf() ? 0.0f : m;
+    return {m, a.s * expf_cw(a.m - base) + b.s * expf_cw(b.m - base)};
+}
+
+// A row's results from the pair of all its logits and its target's logit.
+__device__ __forceinline__ void finish_row(Stat t, bool target, float z, float *loss, float *lse) {
+    // No class left: log(0). A sum that is NaN stays so.
+    const float l = t.s == 0.0f ? neg_inf() : t.m + logf(t.s);
+    *lse = l;
+    // -inf - -inf: the probability 0 of a target among no classes.
+    *loss = !target ? 0.0f : l == neg_inf() ? __builtin_inff() : l - z;
+}
+
+// ---- bf16 forward ----
+
+template <int WAVES_C>
+struct StatEpilogue {
+    const float *biases;
+    const int *targets;
+    Stat *stats;          // [rows][parts]: part = column tile * WAVES_C + wave column
+    float *target_logit;  // [rows]
+    uint32_t parts;
+
+    template <int TR, int TC, int WR, int WC>
+    __device__ __forceinline__ void tile(f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
+                                         uint32_t rows, uint32_t cols, uint32_t, uint32_t tc, char *) const {
+        static_assert(WC == WAVES_C, "the parts are the waves' columns");
+        const uint32_t lane = threadIdx.x & 63, wave_c = (threadIdx.x >> 6) % WC;
+        const uint32_t cl = c0 + wc0 + 4 * (lane >> 5);
+#pragma unroll
+        for (int j = 0; j < TR; ++j) {
+            const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
+            const uint32_t t = r < rows ? (uint32_t)targets[r] : ~0u;
+            float m = neg_inf();
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const uint32_t c = cl + 32 * i + 8 * (e >> 2) + (e & 3);
+                    float z = acc[i][j][e];
+                    if (biases != nullptr && c < cols) z += biases[c];
+                    if (c >= cols) z = neg_inf();
+                    else if (c == t) target_logit[r] = z;
+                    acc[i][j][e] = z;
+                    m = fmaxf(m, z);
+                }
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float base = m == neg_inf() ? 0.0f : m;
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s += exp_fast(acc[i][j][e] - base);
+            s += __shfl_xor(s, 32);
+            if (r < rows && lane < 32) stats[(uint64_t)r * parts + tc * WC + wave_c] = {m, s};
+        }
+    }
+};
+
+// A wave a row: merges its parts.
+__global__ __launch_bounds__(kBlock) void merge_stats_kernel(const Stat *stats, uint32_t parts, const int *targets,
+                                                            const float *target_logit, uint32_t rows, uint32_t classes, float *loss,
+                                                            float *lse) {
+    const uint32_t r = blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    if (r >= rows) return;
+    Stat t{neg_inf(), 0.0f};
+    for (uint32_t i = lane; i < parts; i += kWave) t = merge(t, stats[(uint64_t)r * parts + i]);
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) t = merge(t, {__shfl_xor(t.m, x), __shfl_xor(t.s, x)});
+    const bool target = (uint32_t)targets[r] < classes;
+    if (lane == 0) finish_row(t, target, target ? target_logit[r] : 0.0f, loss + r, lse + r);
+}
+
+// ---- the gradient of a logit ----
+
+struct RowGradient {
+    const int *targets;
+    const float *lse, *row_scales;
+    float scale;
+    uint32_t classes;
+
+    // s_r and lse_r; s_r 0 for a row that has no gradient (then p is not looked at).
+    __device__ __forceinline__ void row(uint32_t r, uint32_t &target, float &s, float &l) const {
+        target = (uint32_t)targets[r];
+        l = lse[r];
+        s = row_scales != nullptr ? scale * row_scales[r] : scale;
+        if (target >= classes || l == neg_inf()) target = ~0u;
+    }
+};
+
+// d = s_r * (onehot - exp(z - lse)), rounded to bf16 for the products that read
+// it, and each wave's unrounded column sums to `sums` (null: not wanted).
+template <int WAVES_R>
+struct GradientEpilogue {
+    const float *biases;  // of the piece
+    RowGradient rows_of;
+    __bf16 *d;
+    uint32_t ldd, first;  // first: the piece's first class
+    float *sums;          // [row tiles * WAVES_R][cols]
+
+    template <int TR, int TC, int WR, int WC>
+    __device__ __forceinline__ void tile(const f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
+                                         uint32_t rows, uint32_t cols, uint32_t tr, uint32_t, char *) const {
+        static_assert(WR == WAVES_R, "the sums are the waves' rows");
+        const uint32_t lane = threadIdx.x & 63, wave_r = (threadIdx.x >> 6) / WC;
+        const uint32_t cl = c0 + wc0 + 4 * (lane >> 5);
+        uint32_t target[TR];
+        float s[TR], l[TR];
+#pragma unroll
+        for (int j = 0; j < TR; ++j) {
+            const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
+            target[j] = ~0u;
+            s[j] = l[j] = 0.0f;
+            if (r < rows) rows_of.row(r, target[j], s[j], l[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < TC; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t c = cl + 32 * i + 8 * q;
+                float sum[4] = {};
+#pragma unroll
+                for (int j = 0; j < TR; ++j) {
+                    const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
+                    float4 v;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        float z = acc[i][j][4 * q + x];
+                        if (biases != nullptr && c + x < cols) z += biases[c + x];
+                        const float p = exp_fast(z - l[j]);
+                        const float g = s[j] * ((target[j] == first + c + x ? 1.0f : 0.0f) - p);
+                        lane_of(v, x) = target[j] == ~0u || c + x >= cols ? 0.0f : g;
+                        sum[x] += lane_of(v, x);
+                    }
+                    if (r < rows && c < ldd) store4(d, (uint64_t)r * ldd + c, v);
+                }
+                if (sums != nullptr) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                        for (int o = 1; o < 32; o *= 2) sum[x] += __shfl_xor(sum[x], o);
+                        if ((lane & 31) == 0 && c + x < cols) sums[(uint64_t)(tr * WR + wave_r) * cols + c + x] = sum[x];
+                    }
+                }
+            }
+    }
+    static __device__ __forceinline__ float &lane_of(float4 &v, int x) { return ::dkz::lane(v, x); }
+};
+
+// ---- fp32 ----
+
+// Logits with their bias, to the workspace.
+struct LogitEpilogue {
+    const float *biases;
+    float *out;
+    uint32_t ld;
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
+        out[(uint64_t)r * ld + c] = biases != nullptr ? z + biases[c] : z;
+    }
+};
+
+// A workgroup a row: the pair of a piece's logits merged into the row's; the last piece finishes the row.
+__global__ __launch_bounds__(kBlock) void row_stats_kernel(const float *z, uint32_t ld, uint32_t cols, uint32_t first, uint32_t classes,
+                                                          const int *targets, Stat *run, float *target_logit, float *loss,
+                                                          float *lse) {
+    __shared__ Stat waves[kBlock / kWave];
+    const uint32_t r = blockIdx.x;
+    const float *row = z + (uint64_t)r * ld;
+    float m = neg_inf();
+    for (uint32_t c = threadIdx.x; c < cols; c += kBlock) m = fmaxf(m, row[c]);
+    const float base = m == neg_inf() ? 0.0f : m;
+    float s = 0.0f;
+    for (uint32_t c = threadIdx.x; c < cols; c += kBlock) s += expf_cw(row[c] - base);
+    Stat t{m, s};
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) t = merge(t, {__shfl_xor(t.m, x), __shfl_xor(t.s, x)});
+    if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = t;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < kBlock / kWave; ++w) t = merge(t, waves[w]);
+    if (first != 0) t = merge(run[r], t);
+    const uint32_t target = (uint32_t)targets[r];
+    if (target - first < cols) target_logit[r] = row[target - first];
+    run[r] = t;
+    if (first + cols == classes) finish_row(t, target < classes, target < classes ? target_logit[r] : 0.0f, loss + r, lse + r);
+}
+
+constexpr uint32_t kGradRows = 64;  // rows a workgroup of logit_gradient_kernel takes
+
+// A piece's logits become d; a thread a column, and its sum of kGradRows rows to `sums`.
+__global__ __launch_bounds__(kBlock) void logit_gradient_kernel(float *z, uint32_t ld, uint32_t rows, uint32_t cols, uint32_t first,
+                                                               RowGradient rows_of, float *sums) {
+    const uint32_t c = blockIdx.x * kBlock + threadIdx.x, r0 = blockIdx.y * kGradRows;
+    if (c >= cols) return;
+    float sum = 0.0f;
+    for (uint32_t r = r0; r < min(r0 + kGradRows, rows); ++r) {
+        uint32_t target;
+        float s, l;
+        rows_of.row(r, target, s, l);
+        float *at = z + (uint64_t)r * ld + c;
+        const float p = expf_cw(*at - l);
+        const float g = target == ~0u ? 0.0f : s * ((target == first + c ? 1.0f : 0.0f) - p);
+        *at = g;
+        sum += g;
+    }
+    if (sums != nullptr) sums[(uint64_t)blockIdx.y * cols + c] = sum;
+}
+
+// Rows whose classes are none: lse -infinity, no target, no loss.
+__global__ __launch_bounds__(kBlock) void no_classes_kernel(uint32_t rows, float *loss, float *lse) {
+    const uint32_t r = blockIdx.x * kBlock + threadIdx.x;
+    if (r >= rows) return;
+    loss[r] = 0.0f;
+    lse[r] = neg_inf();
+}
+
+// ---- plans ----
+
+// Bytes of a piece's logits or d at most where the workspace has room for it:
+// enough rows and columns for whole rounds of tiles, and little beside the
+// weights of a class count that needs it.
+constexpr uint64_t kPieceBytes = 512ull << 20;
+constexpr uint64_t kLeastPiece = 256;  // classes
+
+// The classes of a piece that fits `bytes` at `per_class` bytes a class, a multiple of 64.
+inline uint64_t piece_of(uint64_t classes, uint64_t most_bytes, uint64_t per_class) {
+    const uint64_t fit = per_class == 0 ? classes : most_bytes / per_class / 64 * 64;
+    return std::min(std::max(fit, kLeastPiece), round_up(classes, 64));
+}
+
+constexpr uint32_t kTile = 128, kWavesR = 2, kWavesC = 2;
+
+struct ForwardPlan {
+    uint64_t piece;  // fp32
+    uint64_t logits, stats, target, partial;
+    uint64_t total() const { return logits + stats + target + partial; }
+};
+ForwardPlan forward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t classes, uint64_t piece_bytes) {
+    ForwardPlan p{};
+    p.target = padded(4 * rows);
+    if (type == DKZ_F32) {
+        p.piece = piece_of(classes, piece_bytes, 4 * rows);
+        p.logits = padded(4 * rows * p.piece);
+        p.stats = padded(sizeof(Stat) * rows);
+        const uint64_t last = classes % p.piece;
+        p.partial = std::max(classes >= p.piece ? f32_partial_bytes(rows, p.piece, inputs) : 0, f32_partial_bytes(rows, last, inputs));
+    } else {
+        p.stats = padded(sizeof(Stat) * rows * div_up(classes, kTile) * kWavesC);
+    }
+    return p;
+}
+
+struct BackwardPlan {
+    uint64_t piece, d, sums, accumulate, partial;
+    uint64_t total() const { return d + sums + accumulate + partial; }
+};
+BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t classes, uint64_t piece_bytes) {
+    BackwardPlan p{};
+    const uint64_t size = type_size(type);
+    p.piece = piece_of(classes, piece_bytes, size * rows);
+    p.d = padded(size * rows * p.piece);
+    const uint64_t last = classes % p.piece, whole = classes >= p.piece ? p.piece : 0;
+    if (type == DKZ_F32) {
+        p.sums = padded(4 * p.piece * div_up(rows, kGradRows));
+        for (const uint64_t n : {whole, last}) {
+            if (n == 0) continue;
+            p.partial = std::max({p.partial, f32_partial_bytes(rows, n, inputs), f32_partial_bytes(n, inputs, rows),
+                                  f32_partial_bytes(rows, inputs, n)});
+        }
+    } else {
+        p.sums = padded(4 * p.piece * div_up(rows, kTile) * kWavesR);
+        // The input gradient of several pieces is summed in fp32.
+        if (classes > p.piece) p.accumulate = padded(4 * rows * inputs);
+        for (const uint64_t n : {whole, last}) {
+            if (n == 0) continue;
+            p.partial = std::max({p.partial, plan_product(n, inputs, rows, true).partial_bytes(n, inputs),
+                                  plan_product(rows, inputs, n, true).partial_bytes(rows, inputs)});
+        }
+    }
+    return p;
+}
+
+// The plan with the largest piece, of powers of two of kPieceBytes, that `bytes` has room for.
+template <class Plan>
+bool fit_plan(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int type, uint64_t rows, uint64_t inputs, uint64_t classes,
+              uint64_t bytes, Plan &plan) {
+    for (uint64_t most = kPieceBytes;; most /= 2) {
+        plan = make(type, rows, inputs, classes, most);
+        if (plan.total() <= bytes) return true;
+        if (most == 0) return false;
+    }
+}
+
+// Input gradients of all pieces but the last, in fp32.
+struct AddEpilogue : QuadEpilogue<AddEpilogue> {
+    float *sum;
+    uint32_t ld;
+    bool begin, vec;
+    __device__ __forceinline__ void quad(uint32_t r, uint32_t c, uint32_t cols, float4 z) const {
+        const uint64_t at = (uint64_t)r * ld + c;
+        if (!vec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < cols) sum[at + i] = begin ? lane(z, i) : sum[at + i] + lane(z, i);
+            return;
+        }
+        if (!begin) {
+            const float4 o = load4(sum, at);
+            z = make_float4(z.x + o.x, z.y + o.y, z.z + o.z, z.w + o.w);
+        }
+        store4(sum, at, z);
+    }
+};
+// The last piece's, added to them and rounded.
+struct LastEpilogue : QuadEpilogue<LastEpilogue> {
+    const float *sum;
+    __bf16 *out;
+    uint32_t ld;
+    bool vec;
+    __device__ __forceinline__ void quad(uint32_t r, uint32_t c, uint32_t cols, float4 z) const {
+        const uint64_t at = (uint64_t)r * ld + c;
+        if (!vec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < cols) store1(out, at + i, sum[at + i] + lane(z, i));
+            return;
+        }
+        const float4 o = load4(sum, at);
+        store4(out, at, make_float4(z.x + o.x, z.y + o.y, z.z + o.z, z.w + o.w));
+    }
+};
+
+int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const void *input, const void *weights,
+            const float *biases, const int *targets, float *loss, float *lse, const ForwardPlan &plan, Workspace ws) {
+    constexpr const char *kName = "linear_cross_entropy";
+    if (classes == 0)
+        return launch("linear_cross_entropy_none", no_classes_kernel, dim3(div_up(rows, kBlock)), dim3(kBlock), (uint32_t)rows, loss, lse);
+    float *target_logit = ws.take<float>(plan.target / 4);
+    Stat *stats = ws.take<Stat>(plan.stats / sizeof(Stat));
+    if (type == DKZ_BF16) {
+        const uint32_t parts = div_up(classes, kTile) * kWavesC;
+        const StatEpilogue<kWavesC> epi{biases, targets, stats, target_logit, parts};
+        const ProductPlan p{kTile, kTile, 1, (uint32_t)round_up(inputs, kSlabK)};
+        DKZ_TRY((run_product<false, false>(kName, static_cast<const __bf16 *>(input), inputs, static_cast<const __bf16 *>(weights), inputs,
+                                           rows, classes, inputs, p, nullptr, epi)));
+        return launch("linear_cross_entropy_merge", merge_stats_kernel, dim3(div_up(rows, kBlock / kWave)), dim3(kBlock), stats, parts,
+                      targets, target_logit, (uint32_t)rows, (uint32_t)classes, loss, lse);
+    }
+    float *logits = ws.take<float>(plan.logits / 4), *partial = ws.take<float>(plan.partial / 4);
+    for (uint64_t first = 0; first < classes; first += plan.piece) {
+        const uint64_t n = std::min(plan.piece, classes - first);
+        const LogitEpilogue epi{biases != nullptr ? biases + first : nullptr, logits, (uint32_t)n};
+        DKZ_TRY((run_f32<kRowMajor, kRowMajor>(kName, static_cast<const float *>(input), inputs,
+                                               static_cast<const float *>(weights) + first * inputs, inputs, 0.0f, (float *)nullptr, n,
+                                               rows, n, inputs, partial, epi)));
+        DKZ_TRY(launch("linear_cross_entropy_stats", row_stats_kernel, dim3((uint32_t)rows), dim3(kBlock), logits, (uint32_t)n, (uint32_t)n,
+                       (uint32_t)first, (uint32_t)classes, targets, stats, target_logit, loss, lse));
+    }
+    return 0;
+}
+
+constexpr const char *kWeights = "linear_cross_entropy_weights", *kInput = "linear_cross_entropy_input";
+
+int backward_f32(uint64_t rows, uint64_t inputs, uint64_t classes, const float *input, const float *weights, const float *biases,
+                 const RowGradient &grad, float beta, float *bias_updates, float *weight_updates, float *input_delta,
+                 const BackwardPlan &plan, Workspace ws) {
+    float *d = ws.take<float>(plan.d / 4), *sums = ws.take<float>(plan.sums / 4), *partial = ws.take<float>(plan.partial / 4);
+    for (uint64_t first = 0; first < classes; first += plan.piece) {
+        const uint64_t n = std::min(plan.piece, classes - first), chunks = div_up(rows, kGradRows);
+        const float *w = weights + first * inputs;
+        if (rows != 0) {
+            const LogitEpilogue epi{biases != nullptr ? biases + first : nullptr, d, (uint32_t)n};
+            DKZ_TRY((run_f32<kRowMajor, kRowMajor>("linear_cross_entropy_logits", input, inputs, w, inputs, 0.0f, (float *)nullptr, n, rows,
+                                                   n, inputs, partial, epi)));
+            DKZ_TRY(launch("linear_cross_entropy_gradient", logit_gradient_kernel, dim3(div_up(n, kBlock), (uint32_t)chunks), dim3(kBlock),
+                           d, (uint32_t)n, (uint32_t)rows, (uint32_t)n, (uint32_t)first, grad, bias_updates != nullptr ? sums : nullptr));
+        }
+        if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
+        if (weight_updates != nullptr)
+            DKZ_TRY((run_f32<kColMajor, kColMajor>(kWeights, d, n, input, inputs, beta, weight_updates + first * inputs, inputs, n, inputs,
+                                                   rows, partial)));
+        if (input_delta != nullptr)
+            DKZ_TRY((run_f32<kRowMajor, kColMajor>(kInput, d, n, w, inputs, first == 0 ? 0.0f : 1.0f, input_delta, inputs, rows, inputs, n,
+                                                   partial)));
+    }
+    return 0;
+}
+
+int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16 *input, const __bf16 *weights, const float *biases,
+                  const RowGradient &grad, float beta, float *bias_updates, __bf16 *weight_updates, __bf16 *input_delta,
+                  const BackwardPlan &plan, Workspace ws) {
+    __bf16 *d = ws.take<__bf16>(plan.d / 2);
+    float *sums = ws.take<float>(plan.sums / 4), *accumulate = ws.take<float>(plan.accumulate / 4);
+    float *partial = ws.take<float>(plan.partial / 4);
+    for (uint64_t first = 0; first < classes; first += plan.piece) {
+        const uint64_t n = std::min(plan.piece, classes - first), chunks = (uint64_t)div_up(rows, kTile) * kWavesR, ldd = round_up(n, 8);
+        const __bf16 *w = weights + first * inputs;
+        const GradientEpilogue<kWavesR> epi{biases != nullptr ? biases + first : nullptr, grad, d, (uint32_t)ldd, (uint32_t)first,
+                                            bias_updates != nullptr ? sums : nullptr};
+        const ProductPlan p{kTile, kTile, 1, (uint32_t)round_up(inputs, kSlabK)};
+        DKZ_TRY((run_product<false, false>("linear_cross_entropy_gradient", input, inputs, w, inputs, rows, n, inputs, p, nullptr, epi)));
+        if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
+        if (weight_updates != nullptr)
+            DKZ_TRY((run_product<true, true>(kWeights, d, ldd, input, inputs, n, inputs, rows, plan_product(n, inputs, rows, true), partial,
+                                             store_epilogue<__bf16>(weight_updates + first * inputs, nullptr, inputs, beta))));
+        if (input_delta == nullptr) continue;
+        const ProductPlan pi = plan_product(rows, inputs, n, true);
+        const bool vec = inputs % 4 == 0, last = first + n == classes;
+        if (last && first == 0) {
+            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial,
+                                              store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f))));
+        } else if (last) {
+            LastEpilogue e;
+            e.sum = accumulate;
+            e.out = input_delta;
+            e.ld = (uint32_t)inputs;
+            e.vec = vec && aligned4(input_delta, DKZ_BF16);
+            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial, e)));
+        } else {
+            AddEpilogue e;
+            e.sum = accumulate;
+            e.ld = (uint32_t)inputs;
+            e.begin = first == 0;
+            e.vec = vec;
+            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial, e)));
+        }
+    }
+    return 0;
+}
+
+}  // namespace
+}  // namespace dkz
+
+using namespace dkz;
+
+extern "C" {
+
+int dkz_linear_cross_entropy_forward_workspace(int type, int rows, int inputs, int classes, size_t *least, size_t *best) {
+    DKZ_REQUIRE(least != nullptr && best != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
+    DKZ_REQUIRE_ELEMS(rows, inputs);
+    DKZ_REQUIRE_ELEMS(classes, inputs);
+    const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes;
+    *least = m == 0 || n == 0 ? 0 : (size_t)forward_plan(type, m, k, n, 0).total();
+    *best = m == 0 || n == 0 ? 0 : (size_t)forward_plan(type, m, k, n, kPieceBytes).total();
+    return 0;
+}
+
+int dkz_linear_cross_entropy_forward(int type, int rows, int inputs, int classes, const void *input, const void *weights,
+                                     const float *biases, const int *targets, float *loss, float *lse, void *workspace,
+                                     size_t workspace_bytes) {
+    DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
+    DKZ_REQUIRE_ELEMS(rows, inputs);
+    DKZ_REQUIRE_ELEMS(classes, inputs);
+    if (rows == 0) return 0;
+    DKZ_REQUIRE(targets != nullptr && loss != nullptr && lse != nullptr);
+    DKZ_REQUIRE(inputs == 0 || classes == 0 || (input != nullptr && weights != nullptr));
+    const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes, size = type_size(type);
+    ForwardPlan plan{};
+    if (n != 0) {
+        DKZ_REQUIRE(workspace != nullptr && aligned16(workspace));
+        DKZ_REQUIRE(fit_plan(forward_plan, type, m, k, n, workspace_bytes, plan));
+    }
+    const Span writes[] = {{loss, 4 * m}, {lse, 4 * m}, {workspace, plan.total()}};
+    const Span reads[] = {{input, m * k * size}, {weights, n * k * size}, {biases, 4 * n}, {targets, 4 * m}};
+    DKZ_REQUIRE(disjoint(writes, reads));
+    return forward(type, m, k, n, input, weights, biases, targets, loss, lse, plan, {static_cast<char *>(workspace), plan.total()});
+}
+
+int dkz_linear_cross_entropy_backward_workspace(int type, int rows, int inputs, int classes, size_t *least, size_t *best) {
+    DKZ_REQUIRE(least != nullptr && best != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
+    DKZ_REQUIRE_ELEMS(rows, inputs);
+    DKZ_REQUIRE_ELEMS(classes, inputs);
+    const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes;
+    *least = n == 0 ? 0 : (size_t)backward_plan(type, m, k, n, 0).total();
+    *best = n == 0 ? 0 : (size_t)backward_plan(type, m, k, n, kPieceBytes).total();
+    return 0;
+}
+
+int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classes, const void *input, const void *weights,
+                                      const float *biases, const int *targets, const float *lse, const float *row_scales,
+                                      float scale, float beta, float *bias_updates, void *weight_updates, void *input_delta,
+                                      void *workspace, size_t workspace_bytes) {
+    DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
+    DKZ_REQUIRE_ELEMS(rows, inputs);
+    DKZ_REQUIRE_ELEMS(classes, inputs);
+    const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes, size = type_size(type);
+    if (bias_updates == nullptr && weight_updates == nullptr && input_delta == nullptr) return 0;
+    if (m != 0 && n != 0) {
+        DKZ_REQUIRE(targets != nullptr && lse != nullptr);
+        DKZ_REQUIRE(k == 0 || (input != nullptr && weights != nullptr));
+    }
+    BackwardPlan plan{};
+    if (n != 0) {
+        DKZ_REQUIRE(backward_plan(type, m, k, n, 0).total() == 0 || (workspace != nullptr && aligned16(workspace)));
+        DKZ_REQUIRE(fit_plan(backward_plan, type, m, k, n, workspace_bytes, plan));
+    }
+    const Span writes[] = {{bias_updates, 4 * n}, {weight_updates, n * k * size}, {input_delta, m * k * size}, {workspace, plan.total()}};
+    const Span reads[] = {{input, m * k * size}, {weights, n * k * size}, {biases, 4 * n}, {targets, 4 * m}, {lse, 4 * m}, {row_scales, 4 * m}};
+    DKZ_REQUIRE(disjoint(writes, reads));
+    const RowGradient grad{targets, lse, row_scales, scale, (uint32_t)n};
+    const Workspace ws{static_cast<char *>(workspace), plan.total()};
+    if (n == 0) {  // no class pulls at the input
+        if (input_delta == nullptr || m * k == 0) return 0;
+        if (type == DKZ_F32)
+            return run_f32<kRowMajor, kColMajor>(kInput, (const float *)nullptr, 0, (const float *)nullptr, k, 0.0f,
+                                                 static_cast<float *>(input_delta), k, m, k, 0, nullptr);
+        return run_product<false, true>(kInput, nullptr, 0, nullptr, k, m, k, 0, plan_product(m, k, 0, true), nullptr,
+                                        store_epilogue<__bf16>(input_delta, nullptr, k, 0.0f));
+    }
+    if (type == DKZ_F32)
+        return backward_f32(m, k, n, static_cast<const float *>(input), static_cast<const float *>(weights), biases, grad, beta,
+                            bias_updates, static_cast<float *>(weight_updates), static_cast<float *>(input_delta), plan, ws);
+    return backward_bf16(m, k, n, static_cast<const __bf16 *>(input), static_cast<const __bf16 *>(weights), biases, grad, beta, bias_updates,
+                         static_cast<__bf16 *>(weight_updates), static_cast<__bf16 *>(input_delta), plan, ws);
+}
+
+}  // extern "C"

@@ -1,0 +1,143 @@
+// dense_internal.hpp -- what the sources of libdkz_dense.so share: the element
+// types, the argument checks and the caller's workspace. The stream, the
+// sync-after-launch switch and the launch helper are dkz_internal.hpp's, over
+// libdkz.so's own state (runtime.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "dkz_dense.h"
+#include "dkz_device.hpp"
+#include "dkz_internal.hpp"
+
+namespace dkz {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// ---- elements: arithmetic is fp32, a bf16 is rounded to nearest even once, as it is stored ----
+
+template <class T>
+__device__ __forceinline__ float load1(const T *p, uint64_t i) {
+    return (float)p[i];
+}
+template <class T>
+__device__ __forceinline__ void store1(T *p, uint64_t i, float v) {
+    p[i] = (T)v;
+}
+// Four consecutive elements at 4 * sizeof(T) alignment.
+template <class T>
+__device__ __forceinline__ float4 load4(const T *p, uint64_t i) {
+    if constexpr (sizeof(T) == 4) {
+        return *reinterpret_cast<const float4 *>(p + i);
+    } else {
+        const bf16x4 v = *reinterpret_cast<const bf16x4 *>(p + i);
+        return make_float4((float)v.x, (float)v.y, (float)v.z, (float)v.w);
+    }
+}
+template <class T>
+__device__ __forceinline__ void store4(T *p, uint64_t i, float4 v) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(p + i) = v;
+    } else {
+        const f32x4 f = {v.x, v.y, v.z, v.w};
+        *reinterpret_cast<bf16x4 *>(p + i) = __builtin_convertvector(f, bf16x4);
+    }
+}
+
+inline bool type_ok(int type) { return type == DKZ_F32 || type == DKZ_BF16; }
+inline uint64_t type_size(int type) { return type == DKZ_F32 ? 4 : 2; }
+
+// Whether n elements at p may be moved four at a time.
+inline bool aligned4(const void *p, int type) { return ((uintptr_t)p & (4 * type_size(type) - 1)) == 0; }
+
+// Whether [a, a + an) and [b, b + bn) share a byte; a null pointer shares none.
+inline bool overlap(const void *a, uint64_t an, const void *b, uint64_t bn) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a != nullptr && b != nullptr && an != 0 && bn != 0 && x < y + bn && y < x + an;
+}
+
+struct Span {
+    const void *p;
+    uint64_t bytes;
+};
+// Whether no span of `writes` shares a byte with one of `reads`, or with another of `writes`.
+template <int W, int R>
+inline bool disjoint(const Span (&writes)[W], const Span (&reads)[R]) {
+    for (int i = 0; i < W; ++i) {
+        for (const Span &r : reads)
+            if (overlap(writes[i].p, writes[i].bytes, r.p, r.bytes)) return false;
+        for (int j = 0; j < i; ++j)
+            if (overlap(writes[i].p, writes[i].bytes, writes[j].p, writes[j].bytes)) return false;
+    }
+    return true;
+}
+
+// ---- draws ----
+
+__device__ __forceinline__ uint32_t draw_hash(uint32_t x) {  // Wellons' lowbias32, as rand_uniform's
+    x ^= x >> 16;
+    x *= 0x7feb352du;
+    x ^= x >> 15;
+    x *= 0x846ca68bu;
+    x ^= x >> 16;
+    return x;
+}
+
+// Element i's draw is the top 24 bits of hash(seed ^ hash(low word of i) ^
+// hash(0x9e3779b9 * high word)), times 2^-24; below 2^32 elements, where the
+// last hash is 0, it is rand_uniform's. A draw is below prob exactly when its
+// 24 bits are below ceil(prob * 2^24) (the host's limit; 0: nothing falls out).
+struct Draws {
+    uint64_t first;
+    uint32_t seed, limit;
+    float scale;
+
+    __device__ __forceinline__ bool dropped(uint64_t i) const {
+        i += first;
+        const uint32_t high = (uint32_t)(i >> 32);
+        const uint32_t key = seed ^ (high ? draw_hash(0x9e3779b9u * high) : 0u);
+        return draw_hash(key ^ draw_hash((uint32_t)i)) >> 8 < limit;
+    }
+    // A select, not a multiply: a dropped NaN or infinity is 0.
+    __device__ __forceinline__ float apply(float v, uint64_t i) const { return dropped(i) ? 0.0f : v * scale; }
+};
+
+inline Draws make_draws(float prob, float scale, unsigned int seed, unsigned long long first) {
+    // prob * 2^24 is exact in fp32 unless it overflows; a NaN drops nothing, as the comparison with it says.
+    const float x = prob * 16777216.0f;
+    const uint32_t limit = !(x > 0.0f) ? 0u : x >= 16777216.0f ? 1u << 24 : (uint32_t)x + ((float)(uint32_t)x < x);
+    return {first, seed, limit, scale};
+}
+
+// ---- the caller's workspace, handed out from its start ----
+
+struct Workspace {
+    char *at;
+    uint64_t left;
+
+    template <class T>
+    T *take(uint64_t n) {
+        const uint64_t bytes = (n * sizeof(T) + 255) / 256 * 256;
+        if (bytes > left) return nullptr;
+        T *p = reinterpret_cast<T *>(at);
+        at += bytes;
+        left -= bytes;
+        return p;
+    }
+};
+inline uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+inline uint64_t round_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+
+}  // namespace dkz
+
+// Matrices past the ABI's largest element count (less what rounds a load up) are refused.
+#define DKZ_REQUIRE_ELEMS(a, b) DKZ_REQUIRE((uint64_t)(a) * (uint64_t)(b) + 3 <= kMaxElems)
+
+// A call's workspace: `need` bytes at a 16-byte boundary.
+#define DKZ_REQUIRE_WORKSPACE(need) \
+    DKZ_REQUIRE((need) == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= (need)))

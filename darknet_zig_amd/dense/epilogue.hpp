@@ -1,0 +1,165 @@
+// epilogue.hpp -- what becomes of a product's elements: epilogues of both
+// product kernels (put: one element; quad: four of a row), and the column sums
+// behind the bias gradients.
+#pragma once
+
+#include "dense_internal.hpp"
+#include "product.hpp"
+
+namespace dkz {
+namespace {
+
+constexpr bool uses_exp(int act) {
+    return act == kLogistic || act == kLoggy || act == kElu || act == kSelu || act == kTanh;
+}
+
+// The activation `act` of n values: EXP, one of those that take an exponential; else one of the others.
+template <bool EXP, int N>
+__device__ __forceinline__ void activate_all(int act, float (&x)[N]) {
+#define DKZ_ACT(A)                                                      \
+    case A:                                                             \
+        if constexpr (uses_exp(A) == EXP) {                             \
+            _Pragma("unroll") for (int i = 0; i < N; ++i) x[i] = activate<A>(x[i]); \
+        }                                                               \
+        break;
+    switch (act) {
+        DKZ_ACT(kLogistic) DKZ_ACT(kRelu) DKZ_ACT(kRelie) DKZ_ACT(kRamp) DKZ_ACT(kTanh) DKZ_ACT(kPlse) DKZ_ACT(kLeaky)
+        DKZ_ACT(kElu) DKZ_ACT(kLoggy) DKZ_ACT(kStair) DKZ_ACT(kHardtan) DKZ_ACT(kLhtan) DKZ_ACT(kSelu)
+        default: break;
+    }
+#undef DKZ_ACT
+}
+
+// The gradient at an activation's output.
+__device__ __forceinline__ float gradient_any(int act, float y) {
+#define DKZ_GRAD(A) \
+    case A: return gradient<A>(y);
+    switch (act) {
+        DKZ_GRAD(kLogistic) DKZ_GRAD(kRelu) DKZ_GRAD(kRelie) DKZ_GRAD(kRamp) DKZ_GRAD(kTanh) DKZ_GRAD(kPlse)
+        DKZ_GRAD(kLeaky) DKZ_GRAD(kElu) DKZ_GRAD(kLoggy) DKZ_GRAD(kStair) DKZ_GRAD(kHardtan) DKZ_GRAD(kLhtan) DKZ_GRAD(kSelu)
+        default: return 1.0f;
+    }
+#undef DKZ_GRAD
+}
+
+// out = dropout(activation(z + bias)) + residual. Matrices have `ld` columns
+// and no gaps, so that r * ld + c is also the draw's element.
+template <class T, bool EXP>
+struct LinearEpilogue : QuadEpilogue<LinearEpilogue<T, EXP>> {
+    const float *biases;
+    const T *residual;
+    T *activated, *output;
+    uint32_t ld;
+    int act;
+    bool vec;  // rows start at multiples of four elements: four at a time
+    Draws draws;
+
+    template <int N>
+    __device__ __forceinline__ void finish(uint64_t at, float (&a)[N]) const {  // a: activated
+        if (draws.limit != 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) a[i] = draws.apply(a[i], at + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) a[i] *= draws.scale;
+        }
+    }
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
+        const uint64_t at = (uint64_t)r * ld + c;
+        float a[1] = {biases != nullptr ? z + biases[c] : z};
+        activate_all<EXP>(act, a);
+        if (activated != nullptr) store1(activated, at, a[0]);
+        finish(at, a);
+        store1(output, at, residual != nullptr ? a[0] + load1(residual, at) : a[0]);
+    }
+    __device__ __forceinline__ void quad(uint32_t r, uint32_t c, uint32_t cols, float4 z) const {
+        if (!vec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < cols) put(r, c + i, lane(z, i));
+            return;
+        }
+        const uint64_t at = (uint64_t)r * ld + c;
+        float a[4] = {z.x, z.y, z.z, z.w};
+        if (biases != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] += biases[c + i];
+        }
+        activate_all<EXP>(act, a);
+        if (activated != nullptr) store4(activated, at, make_float4(a[0], a[1], a[2], a[3]));
+        finish(at, a);
+        if (residual != nullptr) {
+            const float4 b = load4(residual, at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] += lane(b, i);
+        }
+        store4(output, at, make_float4(a[0], a[1], a[2], a[3]));
+    }
+};
+
+// out = z + beta * old + add, old being out's own value. beta 0 does not read it.
+template <class T>
+struct StoreEpilogue : QuadEpilogue<StoreEpilogue<T>> {
+    T *out;
+    const T *add;
+    uint32_t ld;
+    float beta;
+    bool vec;
+
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
+        const uint64_t at = (uint64_t)r * ld + c;
+        if (beta != 0.0f) z += beta * load1(out, at);
+        store1(out, at, add != nullptr ? z + load1(add, at) : z);
+    }
+    __device__ __forceinline__ void quad(uint32_t r, uint32_t c, uint32_t cols, float4 z) const {
+        if (!vec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < cols) put(r, c + i, lane(z, i));
+            return;
+        }
+        const uint64_t at = (uint64_t)r * ld + c;
+        if (beta != 0.0f) {
+            const float4 o = load4(out, at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lane(z, i) += beta * lane(o, i);
+        }
+        if (add != nullptr) {
+            const float4 b = load4(add, at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lane(z, i) += lane(b, i);
+        }
+        store4(out, at, z);
+    }
+};
+
+template <class T>
+StoreEpilogue<T> store_epilogue(void *out, const void *add, uint64_t ld, float beta) {
+    StoreEpilogue<T> e;
+    e.out = static_cast<T *>(out);
+    e.add = static_cast<const T *>(add);
+    e.ld = (uint32_t)ld;
+    e.beta = beta;
+    constexpr uintptr_t mask = 4 * sizeof(T) - 1;
+    e.vec = ld % 4 == 0 && (((uintptr_t)out | (uintptr_t)add) & mask) == 0;
+    return e;
+}
+
+// updates[c] = beta * updates[c] + the sum of column c of partial[chunks][cols], in f64.
+__global__ __launch_bounds__(kBlock) void column_sums_kernel(const float *partial, uint32_t chunks, uint32_t cols, float beta,
+                                                            float *updates) {
+    const uint32_t c = blockIdx.x * kBlock + threadIdx.x;
+    if (c >= cols) return;
+    double s = 0.0;
+    for (uint32_t i = 0; i < chunks; ++i) s += (double)partial[(uint64_t)i * cols + c];
+    updates[c] = beta == 0.0f ? (float)s : beta * updates[c] + (float)s;
+}
+
+inline int add_column_sums(const float *partial, uint64_t chunks, uint64_t cols, float beta, float *updates) {
+    if (cols == 0) return 0;
+    return launch("bias_updates", column_sums_kernel, dim3(div_up(cols, kBlock)), dim3(kBlock), partial, (uint32_t)chunks,
+                  (uint32_t)cols, beta, updates);
+}
+
+}  // namespace
+}  // namespace dkz

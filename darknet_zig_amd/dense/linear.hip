@@ -1,0 +1,218 @@
+// linear.hip -- a connected layer with its epilogue in the product (bias,
+// activation, dropout, residual), and its backward pass.
+#include "dense_internal.hpp"
+#include "epilogue.hpp"
+#include "product.hpp"
+#include "product_f32.hpp"
+
+namespace dkz {
+namespace {
+
+template <class T, bool EXP>
+LinearEpilogue<T, EXP> linear_epilogue(uint64_t outputs, int act, const Draws &draws, const float *biases,
+                                       const void *residual, void *activated, void *output) {
+    LinearEpilogue<T, EXP> e;
+    e.biases = biases;
+    e.residual = static_cast<const T *>(residual);
+    e.activated = static_cast<T *>(activated);
+    e.output = static_cast<T *>(output);
+    e.ld = (uint32_t)outputs;
+    e.act = act;
+    constexpr uintptr_t mask = 4 * sizeof(T) - 1;
+    e.vec = outputs % 4 == 0 && (((uintptr_t)residual | (uintptr_t)activated | (uintptr_t)output) & mask) == 0;
+    e.draws = draws;
+    return e;
+}
+
+template <bool EXP>
+int forward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act, const Draws &draws, const void *input,
+            const void *weights, const float *biases, const void *residual, void *activated, void *output, Workspace ws) {
+    constexpr const char *kName = "linear_forward";
+    if (type == DKZ_F32) {
+        float *partial = ws.take<float>(f32_partial_bytes(rows, outputs, inputs) / 4);
+        return run_f32<kRowMajor, kRowMajor>(kName, static_cast<const float *>(input), inputs,
+                                             static_cast<const float *>(weights), inputs, 0.0f, (float *)nullptr, outputs, rows,
+                                             outputs, inputs, partial,
+                                             linear_epilogue<float, EXP>(outputs, act, draws, biases, residual, activated, output));
+    }
+    const ProductPlan p = plan_product(rows, outputs, inputs, true);
+    float *partial = ws.take<float>(p.partial_bytes(rows, outputs) / 4);
+    return run_product<false, false>(kName, static_cast<const __bf16 *>(input), inputs, static_cast<const __bf16 *>(weights),
+                                     inputs, rows, outputs, inputs, p, partial,
+                                     linear_epilogue<__bf16, EXP>(outputs, act, draws, biases, residual, activated, output));
+}
+
+uint64_t forward_bytes(int type, uint64_t rows, uint64_t inputs, uint64_t outputs) {
+    if (type == DKZ_F32) return f32_partial_bytes(rows, outputs, inputs);
+    return plan_product(rows, outputs, inputs, true).partial_bytes(rows, outputs);
+}
+
+// ---- backward ----
+
+constexpr uint32_t kDeltaRows = 64;  // rows a workgroup of delta_kernel takes
+
+// d = dropout(delta) * gradient(activated), stored to d (null: not) in rows of
+// ldd, and the sums of kDeltaRows rows' columns to partial (null: not).
+template <class T>
+__global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *activated, uint32_t rows, uint32_t cols, int act,
+                                                      Draws draws, T *d, uint32_t ldd, float *partial) {
+    const uint32_t c = blockIdx.x * kBlock + threadIdx.x, r0 = blockIdx.y * kDeltaRows;
+    if (c >= ldd) return;
+    float s = 0.0f;
+    for (uint32_t r = r0; r < min(r0 + kDeltaRows, rows); ++r) {
+        float v = 0.0f;
+        if (c < cols) {
+            const uint64_t at = (uint64_t)r * cols + c;
+            v = load1(delta, at);
+            v = draws.limit != 0 ? draws.apply(v, at) : v * draws.scale;
+            if (act != kLinear) v *= gradient_any(act, load1(activated, at));
+            s += v;
+        }
+        if (d != nullptr) store1(d, (uint64_t)r * ldd + c, v);
+    }
+    if (partial != nullptr && c < cols) partial[(uint64_t)blockIdx.y * cols + c] = s;
+}
+
+// Leading dimension of d in the workspace: whole 16-byte chunks.
+inline uint64_t delta_ld(int type, uint64_t outputs) { return round_up(outputs, type == DKZ_F32 ? 4 : 8); }
+
+struct BackwardPlan {
+    uint64_t d_bytes, sum_bytes, partial_bytes;
+    uint64_t total() const { return d_bytes + sum_bytes + partial_bytes; }
+};
+BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t outputs) {
+    BackwardPlan p;
+    p.d_bytes = padded(rows * delta_ld(type, outputs) * type_size(type));
+    p.sum_bytes = padded(4 * outputs * div_up(rows, kDeltaRows));
+    if (type == DKZ_F32)
+        p.partial_bytes = std::max(f32_partial_bytes(rows, inputs, outputs), f32_partial_bytes(outputs, inputs, rows));
+    else
+        p.partial_bytes = std::max(plan_product(rows, inputs, outputs, true).partial_bytes(rows, inputs),
+                                   plan_product(outputs, inputs, rows, true).partial_bytes(outputs, inputs));
+    return p;
+}
+
+template <class T>
+int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act, const Draws &draws, const void *input,
+             const void *weights, const void *activated, const void *delta, const void *input_residual, float beta,
+             float *bias_updates, void *weight_updates, void *input_delta, Workspace ws) {
+    const BackwardPlan plan = backward_plan(type, rows, inputs, outputs);
+    T *d = ws.take<T>(plan.d_bytes / sizeof(T));
+    float *sums = ws.take<float>(plan.sum_bytes / 4), *partial = ws.take<float>(plan.partial_bytes / 4);
+    uint64_t ldd = delta_ld(type, outputs);
+    const bool products = weight_updates != nullptr || input_delta != nullptr;
+    // The delta itself where nothing changes it.
+    const bool same = act == kLinear && draws.limit == 0 && draws.scale == 1.0f;
+    if (same || !products) {
+        d = nullptr;
+        ldd = outputs;
+    }
+    if (rows != 0 && outputs != 0 && (bias_updates != nullptr || d != nullptr))
+        DKZ_TRY(launch("linear_backward_delta", delta_kernel<T>, dim3(div_up(ldd, kBlock), div_up(rows, kDeltaRows)), dim3(kBlock),
+                       static_cast<const T *>(delta), static_cast<const T *>(activated), (uint32_t)rows, (uint32_t)outputs, act,
+                       draws, d, (uint32_t)ldd, bias_updates != nullptr ? sums : nullptr));
+    if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, div_up(rows, kDeltaRows), outputs, beta, bias_updates));
+    const T *dd = d != nullptr ? d : static_cast<const T *>(delta);
+    const T *x = static_cast<const T *>(input), *w = static_cast<const T *>(weights);
+    constexpr const char *kWeights = "linear_backward_weights", *kInput = "linear_backward_input";
+    if constexpr (sizeof(T) == 4) {
+        if (weight_updates != nullptr)
+            DKZ_TRY((run_f32<kColMajor, kColMajor>(kWeights, dd, ldd, x, inputs, beta, static_cast<float *>(weight_updates),
+                                                   inputs, outputs, inputs, rows, partial)));
+        if (input_delta != nullptr)
+            DKZ_TRY((run_f32<kRowMajor, kColMajor>(kInput, dd, ldd, w, inputs, 0.0f, (float *)nullptr, inputs, rows, inputs,
+                                                   outputs, partial, store_epilogue<T>(input_delta, input_residual, inputs, 0.0f))));
+    } else {
+        if (weight_updates != nullptr)
+            DKZ_TRY((run_product<true, true>(kWeights, dd, ldd, x, inputs, outputs, inputs, rows,
+                                             plan_product(outputs, inputs, rows, true), partial,
+                                             store_epilogue<T>(weight_updates, nullptr, inputs, beta))));
+        if (input_delta != nullptr)
+            DKZ_TRY((run_product<false, true>(kInput, dd, ldd, w, inputs, rows, inputs, outputs,
+                                              plan_product(rows, inputs, outputs, true), partial,
+                                              store_epilogue<T>(input_delta, input_residual, inputs, 0.0f))));
+    }
+    return 0;
+}
+
+}  // namespace
+}  // namespace dkz
+
+using namespace dkz;
+
+extern "C" {
+
+int dkz_linear_forward_workspace(int type, int rows, int inputs, int outputs, size_t *bytes) {
+    DKZ_REQUIRE(bytes != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
+    DKZ_REQUIRE_ELEMS(rows, inputs);
+    DKZ_REQUIRE_ELEMS(outputs, inputs);
+    DKZ_REQUIRE_ELEMS(rows, outputs);
+    *bytes = (size_t)forward_bytes(type, (uint64_t)rows, (uint64_t)inputs, (uint64_t)outputs);
+    return 0;
+}
+
+int dkz_linear_forward(int type, int rows, int inputs, int outputs, int activation, float prob, float scale, unsigned int seed,
+                       unsigned long long first, const void *input, const void *weights, const float *biases,
+                       const void *residual, void *activated, void *output, void *workspace, size_t workspace_bytes) {
+    DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
+    DKZ_REQUIRE(activation >= 0 && activation < kActCount);
+    DKZ_REQUIRE_ELEMS(rows, inputs);
+    DKZ_REQUIRE_ELEMS(outputs, inputs);
+    DKZ_REQUIRE_ELEMS(rows, outputs);
+    if (rows == 0 || outputs == 0) return 0;
+    DKZ_REQUIRE(output != nullptr && (inputs == 0 || (input != nullptr && weights != nullptr)));
+    const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)outputs, size = type_size(type);
+    const uint64_t need = forward_bytes(type, m, k, n), in = m * k * size, w = n * k * size, out = m * n * size;
+    DKZ_REQUIRE_WORKSPACE(need);
+    const Span writes[] = {{output, out}, {activated, out}, {workspace, need}};
+    const Span reads[] = {{input, in}, {weights, w}, {biases, 4 * n}, {residual == output ? nullptr : residual, out}};
+    DKZ_REQUIRE(disjoint(writes, reads));
+    const Draws draws = make_draws(prob, scale, seed, first);
+    const Workspace ws{static_cast<char *>(workspace), need};
+    return uses_exp(activation)
+               ? forward<true>(type, m, k, n, activation, draws, input, weights, biases, residual, activated, output, ws)
+               : forward<false>(type, m, k, n, activation, draws, input, weights, biases, residual, activated, output, ws);
+}
+
+int dkz_linear_backward_workspace(int type, int rows, int inputs, int outputs, size_t *bytes) {
+    DKZ_REQUIRE(bytes != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
+    DKZ_REQUIRE_ELEMS(rows, inputs);
+    DKZ_REQUIRE_ELEMS(outputs, inputs);
+    DKZ_REQUIRE_ELEMS(rows, outputs);
+    *bytes = (size_t)backward_plan(type, (uint64_t)rows, (uint64_t)inputs, (uint64_t)outputs).total();
+    return 0;
+}
+
+int dkz_linear_backward(int type, int rows, int inputs, int outputs, int activation, float prob, float scale, unsigned int seed,
+                        unsigned long long first, const void *input, const void *weights, const void *activated,
+                        const void *delta, const void *input_residual, float beta, float *bias_updates, void *weight_updates,
+                        void *input_delta, void *workspace, size_t workspace_bytes) {
+    DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
+    DKZ_REQUIRE(activation >= 0 && activation < kActCount);
+    DKZ_REQUIRE_ELEMS(rows, inputs);
+    DKZ_REQUIRE_ELEMS(outputs, inputs);
+    DKZ_REQUIRE_ELEMS(rows, outputs);
+    const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)outputs, size = type_size(type);
+    const uint64_t in = m * k * size, w = n * k * size, out = m * n * size;
+    const bool products = out != 0 && in + w != 0 && (weight_updates != nullptr || input_delta != nullptr);
+    if (out != 0 && (products || bias_updates != nullptr)) {
+        DKZ_REQUIRE(delta != nullptr && (activation == kLinear || activated != nullptr));
+        DKZ_REQUIRE(in == 0 || weight_updates == nullptr || input != nullptr);
+        DKZ_REQUIRE(w == 0 || input_delta == nullptr || weights != nullptr);
+    }
+    const uint64_t need = backward_plan(type, m, k, n).total();
+    DKZ_REQUIRE_WORKSPACE(need);
+    const Span writes[] = {{bias_updates, 4 * n}, {weight_updates, w}, {input_delta, in}, {workspace, need}};
+    const Span reads[] = {{input, in}, {weights, w}, {activated, out}, {delta, out},
+                          {input_residual == input_delta ? nullptr : input_residual, in}};
+    DKZ_REQUIRE(disjoint(writes, reads));
+    const Draws draws = make_draws(prob, scale, seed, first);
+    const Workspace ws{static_cast<char *>(workspace), need};
+    if (type == DKZ_F32)
+        return backward<float>(type, m, k, n, activation, draws, input, weights, activated, delta, input_residual, beta,
+                               bias_updates, weight_updates, input_delta, ws);
+    return backward<__bf16>(type, m, k, n, activation, draws, input, weights, activated, delta, input_residual, beta,
+                            bias_updates, weight_updates, input_delta, ws);
+}
+
+}  // extern "C"

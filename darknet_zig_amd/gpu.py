@@ -13,6 +13,10 @@ code and tests written against the reference read the same here:
   must()/panic (gpu.zig:51-55, 444-464).
 
 Host arrays are numpy arrays (float32, or int32 for maxpool indexes).
+
+The fused dense operators at the end (`seededDropout`, `linear*`) have no single
+gpu.zig counterpart. They go to libdkz_dense.so and take fp32 or bf16 tensors:
+a bf16 tensor of n elements is a Buf of (n + 1) // 2 four-byte elements.
 """
 
 from __future__ import annotations
@@ -515,4 +519,123 @@ def batchnormBackward(
             _p(variance), _p(scales), _p(bias_updates), _p(scale_updates), _p(mean_delta), _p(variance_delta),
         ),
         "batchnorm_backward",
+    )
+
+
+# ---- the dense operators of libdkz_dense.so (include/dkz_dense.h): connected
+# layers with their epilogue, dropout without a stored mask, and softmax
+# cross-entropy without stored logits. `type` is F32 or BF16. Workspaces are
+# the caller's: allocate what the *Workspace function says, in bytes. ----
+
+F32, BF16 = 0, 1
+
+
+def _must_dense(code: int, what: str) -> None:
+    if code != 0:
+        raise GpuError(code, what, _lib.load_dense().dkz_dense_last_error_context().decode(errors="replace"))
+
+
+def _bytes(b: Buf | None) -> int:
+    return 0 if b is None or b.ptr is None else 4 * b.len
+
+
+def seededDropout(
+    n: int, x_type: int, x: Buf, residual: Buf | None, prob: float, scale: float, seed: int, first: int, y_type: int,
+    y: Buf,
+) -> None:
+    """y = dropout(x) + residual with randUniform's draws, none of them stored;
+    the backward pass is the same call on the gradient."""
+    _must_dense(_lib.load_dense().dkz_seeded_dropout(n, x_type, _p(x), _p(residual), prob, scale, seed & 0xFFFFFFFF,
+                                                     first, y_type, _p(y)), "seeded_dropout")
+
+
+def linearForwardWorkspace(type: int, rows: int, inputs: int, outputs: int) -> int:
+    need = C.c_size_t(0)
+    _must_dense(_lib.load_dense().dkz_linear_forward_workspace(type, rows, inputs, outputs, C.byref(need)),
+                "linear_forward_workspace")
+    return need.value
+
+
+def linearForward(
+    type: int, rows: int, inputs: int, outputs: int, activation: int, prob: float, scale: float, seed: int, first: int,
+    input: Buf, weights: Buf, biases: Buf | None, residual: Buf | None, activated: Buf | None, output: Buf,
+    workspace: Buf | None,
+) -> None:
+    _must_dense(
+        _lib.load_dense().dkz_linear_forward(
+            type, rows, inputs, outputs, int(activation), prob, scale, seed & 0xFFFFFFFF, first, _p(input), _p(weights),
+            _p(biases), _p(residual), _p(activated), _p(output), _p(workspace), _bytes(workspace),
+        ),
+        "linear_forward",
+    )
+
+
+def linearBackwardWorkspace(type: int, rows: int, inputs: int, outputs: int) -> int:
+    need = C.c_size_t(0)
+    _must_dense(_lib.load_dense().dkz_linear_backward_workspace(type, rows, inputs, outputs, C.byref(need)),
+                "linear_backward_workspace")
+    return need.value
+
+
+def linearBackward(
+    type: int, rows: int, inputs: int, outputs: int, activation: int, prob: float, scale: float, seed: int, first: int,
+    input: Buf, weights: Buf, activated: Buf | None, delta: Buf, input_residual: Buf | None, beta: float,
+    bias_updates: Buf | None, weight_updates: Buf | None, input_delta: Buf | None, workspace: Buf | None,
+) -> None:
+    _must_dense(
+        _lib.load_dense().dkz_linear_backward(
+            type, rows, inputs, outputs, int(activation), prob, scale, seed & 0xFFFFFFFF, first, _p(input), _p(weights),
+            _p(activated), _p(delta), _p(input_residual), beta, _p(bias_updates), _p(weight_updates), _p(input_delta),
+            _p(workspace), _bytes(workspace),
+        ),
+        "linear_backward",
+    )
+
+
+def linearCrossEntropyForwardWorkspace(type: int, rows: int, inputs: int, classes: int) -> tuple[int, int]:
+    """(least, best): what any call needs, and what the fastest way takes."""
+    least, best = C.c_size_t(0), C.c_size_t(0)
+    _must_dense(
+        _lib.load_dense().dkz_linear_cross_entropy_forward_workspace(type, rows, inputs, classes, C.byref(least),
+                                                                     C.byref(best)),
+        "linear_cross_entropy_forward_workspace",
+    )
+    return least.value, best.value
+
+
+def linearCrossEntropyForward(
+    type: int, rows: int, inputs: int, classes: int, input: Buf, weights: Buf, biases: Buf | None, targets: Buf,
+    loss: Buf, lse: Buf, workspace: Buf | None,
+) -> None:
+    _must_dense(
+        _lib.load_dense().dkz_linear_cross_entropy_forward(
+            type, rows, inputs, classes, _p(input), _p(weights), _p(biases), _p(targets), _p(loss), _p(lse),
+            _p(workspace), _bytes(workspace),
+        ),
+        "linear_cross_entropy_forward",
+    )
+
+
+def linearCrossEntropyBackwardWorkspace(type: int, rows: int, inputs: int, classes: int) -> tuple[int, int]:
+    """(least, best): what any call needs, and what the fastest way takes."""
+    least, best = C.c_size_t(0), C.c_size_t(0)
+    _must_dense(
+        _lib.load_dense().dkz_linear_cross_entropy_backward_workspace(type, rows, inputs, classes, C.byref(least),
+                                                                      C.byref(best)),
+        "linear_cross_entropy_backward_workspace",
+    )
+    return least.value, best.value
+
+
+def linearCrossEntropyBackward(
+    type: int, rows: int, inputs: int, classes: int, input: Buf, weights: Buf, biases: Buf | None, targets: Buf,
+    lse: Buf, row_scales: Buf | None, scale: float, beta: float, bias_updates: Buf | None, weight_updates: Buf | None,
+    input_delta: Buf | None, workspace: Buf | None,
+) -> None:
+    _must_dense(
+        _lib.load_dense().dkz_linear_cross_entropy_backward(
+            type, rows, inputs, classes, _p(input), _p(weights), _p(biases), _p(targets), _p(lse), _p(row_scales), scale,
+            beta, _p(bias_updates), _p(weight_updates), _p(input_delta), _p(workspace), _bytes(workspace),
+        ),
+        "linear_cross_entropy_backward",
     )
