@@ -46,18 +46,16 @@ __device__ __forceinline__ void finish_row(Stat t, bool target, float z, float *
 
 // ---- bf16 forward ----
 
-template <int WAVES_C>
 struct StatEpilogue {
     const float *biases;
     const int *targets;
-    Stat *stats;          // [rows][parts]: part = column tile * WAVES_C + wave column
+    Stat *stats;          // [rows][parts]: part = column tile * the workgroup's wave columns + wave column
     float *target_logit;  // [rows]
     uint32_t parts;
 
     template <int TR, int TC, int WR, int WC>
     __device__ __forceinline__ void tile(f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
                                          uint32_t rows, uint32_t cols, uint32_t, uint32_t tc, char *) const {
-        static_assert(WC == WAVES_C, "the parts are the waves' columns");
         const uint32_t lane = threadIdx.x & 63, wave_c = (threadIdx.x >> 6) % WC;
         const uint32_t cl = c0 + wc0 + 4 * (lane >> 5);
 #pragma unroll
@@ -122,62 +120,64 @@ struct RowGradient {
 };
 
 // d = s_r * (onehot - exp(z - lse)), rounded to bf16 for the products that read
-// it, and each wave's unrounded column sums to `sums` (null: not wanted).
-template <int WAVES_R>
+// it, and each wave's unrounded column sums to `sums` (null: not wanted). The
+// tile passes through LDS as TileEpilogue's does.
 struct GradientEpilogue {
     const float *biases;  // of the piece
     RowGradient rows_of;
-    __bf16 *d;
-    uint32_t ldd, first;  // first: the piece's first class
-    float *sums;          // [row tiles * WAVES_R][cols]
+    __bf16 *d;            // 16-byte aligned
+    uint32_t ldd, first;  // ldd: a multiple of eight; first: the piece's first class
+    float *sums;          // [row tiles * the workgroup's wave rows][cols]
 
     template <int TR, int TC, int WR, int WC>
     __device__ __forceinline__ void tile(const f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
-                                         uint32_t rows, uint32_t cols, uint32_t tr, uint32_t, char *) const {
-        static_assert(WR == WAVES_R, "the sums are the waves' rows");
-        const uint32_t lane = threadIdx.x & 63, wave_r = (threadIdx.x >> 6) / WC;
-        const uint32_t cl = c0 + wc0 + 4 * (lane >> 5);
-        uint32_t target[TR];
-        float s[TR], l[TR];
+                                         uint32_t rows, uint32_t cols, uint32_t tr, uint32_t, char *lds) const {
+        constexpr uint32_t kCols = TC * 32, kLanes = kCols / 8, kStep = kWave / kLanes, kMask = kCols / 4 - 1;
+        const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        float4 *part = reinterpret_cast<float4 *>(lds) + wave * (32 * kCols / 4);
+        const uint32_t c = c0 + wc0 + lane % kLanes * 8;
+        float bias[8], sum[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bias[i] = c + i >= cols ? neg_inf() : biases != nullptr ? biases[c + i] : 0.0f;
 #pragma unroll
         for (int j = 0; j < TR; ++j) {
-            const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
-            target[j] = ~0u;
-            s[j] = l[j] = 0.0f;
-            if (r < rows) rows_of.row(r, target[j], s[j], l[j]);
-        }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int i = 0; i < TC; ++i)
+            for (int i = 0; i < TC; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t c = cl + 32 * i + 8 * q;
-                float sum[4] = {};
+                for (int q = 0; q < 4; ++q)
+                    part[(lane & 31) * (kCols / 4) + ((8 * i + 2 * q + (lane >> 5)) ^ (lane & 31 & kMask))] =
+                        make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+            for (uint32_t x = lane / kLanes; x < 32; x += kStep) {
+                const uint32_t r = r0 + wr0 + 32 * j + x, at = x * (kCols / 4), chunk = lane % kLanes * 2;
+                if (r >= rows) break;
+                const float4 a = part[at + (chunk ^ (x & kMask))], b = part[at + ((chunk + 1) ^ (x & kMask))];
+                uint32_t target;
+                float s, l;
+                rows_of.row(r, target, s, l);
+                float v[8];
 #pragma unroll
-                for (int j = 0; j < TR; ++j) {
-                    const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
-                    float4 v;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        float z = acc[i][j][4 * q + x];
-                        if (biases != nullptr && c + x < cols) z += biases[c + x];
-                        const float p = exp_fast(z - l[j]);
-                        const float g = s[j] * ((target[j] == first + c + x ? 1.0f : 0.0f) - p);
-                        lane_of(v, x) = target[j] == ~0u || c + x >= cols ? 0.0f : g;
-                        sum[x] += lane_of(v, x);
-                    }
-                    if (r < rows && c < ldd) store4(d, (uint64_t)r * ldd + c, v);
+                for (int i = 0; i < 8; ++i) {
+                    // A column past the last class: exp(-infinity), and no target. NaN logits stay in rows that have a gradient.
+                    const float p = c + i < cols ? exp_fast(::dkz::lane(i < 4 ? a : b, i & 3) + bias[i] - l) : 0.0f;
+                    v[i] = target == ~0u ? 0.0f : s * ((target == first + c + i ? 1.0f : 0.0f) - p);
+                    sum[i] += v[i];
                 }
-                if (sums != nullptr) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-#pragma unroll
-                        for (int o = 1; o < 32; o *= 2) sum[x] += __shfl_xor(sum[x], o);
-                        if ((lane & 31) == 0 && c + x < cols) sums[(uint64_t)(tr * WR + wave_r) * cols + c + x] = sum[x];
-                    }
-                }
+                if (c < ldd) store8(d, (uint64_t)r * ldd + c, v);
             }
+        }
+        if (sums == nullptr) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int o = kLanes; o < kWave; o *= 2) sum[i] += __shfl_xor(sum[i], o);
+            if (lane < kLanes && c + i < cols) sums[(uint64_t)(tr * WR + wave / WC) * cols + c + i] = sum[i];
+        }
     }
-    static __device__ __forceinline__ float &lane_of(float4 &v, int x) { return ::dkz::lane(v, x); }
 };
 
 // ---- fp32 ----
@@ -261,7 +261,8 @@ inline uint64_t piece_of(uint64_t classes, uint64_t most_bytes, uint64_t per_cla
     return std::min(std::max(fit, kLeastPiece), round_up(classes, 64));
 }
 
-constexpr uint32_t kTile = 128, kWavesR = 2, kWavesC = 2;
+// Tiles of the products whose epilogue looks at whole rows or columns: K stays whole.
+inline ProductPlan whole_plan(uint64_t rows, uint64_t classes, uint64_t inputs) { return plan_product(rows, classes, inputs, false); }
 
 struct ForwardPlan {
     uint64_t piece;  // fp32
@@ -278,7 +279,8 @@ ForwardPlan forward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t clas
         const uint64_t last = classes % p.piece;
         p.partial = std::max(classes >= p.piece ? f32_partial_bytes(rows, p.piece, inputs) : 0, f32_partial_bytes(rows, last, inputs));
     } else {
-        p.stats = padded(sizeof(Stat) * rows * div_up(classes, kTile) * kWavesC);
+        const ProductPlan t = whole_plan(rows, classes, inputs);
+        p.stats = padded(sizeof(Stat) * rows * div_up(classes, t.bc) * t.wc);
     }
     return p;
 }
@@ -301,11 +303,12 @@ BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t cl
                                   f32_partial_bytes(rows, inputs, n)});
         }
     } else {
-        p.sums = padded(4 * p.piece * div_up(rows, kTile) * kWavesR);
         // The input gradient of several pieces is summed in fp32.
         if (classes > p.piece) p.accumulate = padded(4 * rows * inputs);
         for (const uint64_t n : {whole, last}) {
             if (n == 0) continue;
+            const ProductPlan t = whole_plan(rows, n, inputs);
+            p.sums = std::max(p.sums, padded(4 * n * div_up(rows, t.br) * t.wr));
             p.partial = std::max({p.partial, plan_product(n, inputs, rows, true).partial_bytes(n, inputs),
                                   plan_product(rows, inputs, n, true).partial_bytes(rows, inputs)});
         }
@@ -325,41 +328,48 @@ bool fit_plan(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int typ
 }
 
 // Input gradients of all pieces but the last, in fp32.
-struct AddEpilogue : QuadEpilogue<AddEpilogue> {
+struct AddEpilogue : TileEpilogue<AddEpilogue> {
     float *sum;
     uint32_t ld;
     bool begin, vec;
-    __device__ __forceinline__ void quad(uint32_t r, uint32_t c, uint32_t cols, float4 z) const {
+    struct Columns {};
+    __device__ __forceinline__ bool whole() const { return vec; }
+    __device__ __forceinline__ Columns columns(uint32_t) const { return {}; }
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
         const uint64_t at = (uint64_t)r * ld + c;
-        if (!vec) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < cols) sum[at + i] = begin ? lane(z, i) : sum[at + i] + lane(z, i);
-            return;
-        }
+        sum[at] = begin ? z : sum[at] + z;
+    }
+    __device__ __forceinline__ void row(const Columns &, uint32_t r, uint32_t c, float (&z)[8]) const {
+        const uint64_t at = (uint64_t)r * ld + c;
         if (!begin) {
-            const float4 o = load4(sum, at);
-            z = make_float4(z.x + o.x, z.y + o.y, z.z + o.z, z.w + o.w);
+            float o[8];
+            load8(sum, at, o);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] += o[i];
         }
-        store4(sum, at, z);
+        store8(sum, at, z);
     }
 };
 // The last piece's, added to them and rounded.
-struct LastEpilogue : QuadEpilogue<LastEpilogue> {
+struct LastEpilogue : TileEpilogue<LastEpilogue> {
     const float *sum;
     __bf16 *out;
     uint32_t ld;
     bool vec;
-    __device__ __forceinline__ void quad(uint32_t r, uint32_t c, uint32_t cols, float4 z) const {
+    struct Columns {};
+    __device__ __forceinline__ bool whole() const { return vec; }
+    __device__ __forceinline__ Columns columns(uint32_t) const { return {}; }
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
         const uint64_t at = (uint64_t)r * ld + c;
-        if (!vec) {
+        store1(out, at, sum[at] + z);
+    }
+    __device__ __forceinline__ void row(const Columns &, uint32_t r, uint32_t c, float (&z)[8]) const {
+        const uint64_t at = (uint64_t)r * ld + c;
+        float o[8];
+        load8(sum, at, o);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < cols) store1(out, at + i, sum[at + i] + lane(z, i));
-            return;
-        }
-        const float4 o = load4(sum, at);
-        store4(out, at, make_float4(z.x + o.x, z.y + o.y, z.z + o.z, z.w + o.w));
+        for (int i = 0; i < 8; ++i) z[i] += o[i];
+        store8(out, at, z);
     }
 };
 
@@ -371,9 +381,9 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const vo
     float *target_logit = ws.take<float>(plan.target / 4);
     Stat *stats = ws.take<Stat>(plan.stats / sizeof(Stat));
     if (type == DKZ_BF16) {
-        const uint32_t parts = div_up(classes, kTile) * kWavesC;
-        const StatEpilogue<kWavesC> epi{biases, targets, stats, target_logit, parts};
-        const ProductPlan p{kTile, kTile, 1, (uint32_t)round_up(inputs, kSlabK)};
+        const ProductPlan p = whole_plan(rows, classes, inputs);
+        const uint32_t parts = div_up(classes, p.bc) * p.wc;
+        const StatEpilogue epi{biases, targets, stats, target_logit, parts};
         DKZ_TRY((run_product<false, false>(kName, static_cast<const __bf16 *>(input), inputs, static_cast<const __bf16 *>(weights), inputs,
                                            rows, classes, inputs, p, nullptr, epi)));
         return launch("linear_cross_entropy_merge", merge_stats_kernel, dim3(div_up(rows, kBlock / kWave)), dim3(kBlock), stats, parts,
@@ -426,11 +436,12 @@ int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16
     float *sums = ws.take<float>(plan.sums / 4), *accumulate = ws.take<float>(plan.accumulate / 4);
     float *partial = ws.take<float>(plan.partial / 4);
     for (uint64_t first = 0; first < classes; first += plan.piece) {
-        const uint64_t n = std::min(plan.piece, classes - first), chunks = (uint64_t)div_up(rows, kTile) * kWavesR, ldd = round_up(n, 8);
+        const uint64_t n = std::min(plan.piece, classes - first), ldd = round_up(n, 8);
+        const ProductPlan p = whole_plan(rows, n, inputs);
+        const uint64_t chunks = (uint64_t)div_up(rows, p.br) * p.wr;
         const __bf16 *w = weights + first * inputs;
-        const GradientEpilogue<kWavesR> epi{biases != nullptr ? biases + first : nullptr, grad, d, (uint32_t)ldd, (uint32_t)first,
+        const GradientEpilogue epi{biases != nullptr ? biases + first : nullptr, grad, d, (uint32_t)ldd, (uint32_t)first,
                                             bias_updates != nullptr ? sums : nullptr};
-        const ProductPlan p{kTile, kTile, 1, (uint32_t)round_up(inputs, kSlabK)};
         DKZ_TRY((run_product<false, false>("linear_cross_entropy_gradient", input, inputs, w, inputs, rows, n, inputs, p, nullptr, epi)));
         if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
         if (weight_updates != nullptr)
@@ -438,24 +449,24 @@ int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16
                                              store_epilogue<__bf16>(weight_updates + first * inputs, nullptr, inputs, beta))));
         if (input_delta == nullptr) continue;
         const ProductPlan pi = plan_product(rows, inputs, n, true);
-        const bool vec = inputs % 4 == 0, last = first + n == classes;
+        const bool last = first + n == classes;
         if (last && first == 0) {
             DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial,
-                                              store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f))));
+                                              store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f), true)));
         } else if (last) {
             LastEpilogue e;
             e.sum = accumulate;
             e.out = input_delta;
             e.ld = (uint32_t)inputs;
-            e.vec = vec && aligned4(input_delta, DKZ_BF16);
-            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial, e)));
+            e.vec = eights(inputs, input_delta);
+            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial, e, true)));
         } else {
             AddEpilogue e;
             e.sum = accumulate;
             e.ld = (uint32_t)inputs;
             e.begin = first == 0;
-            e.vec = vec;
-            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial, e)));
+            e.vec = eights(inputs, accumulate);
+            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial, e, true)));
         }
     }
     return 0;

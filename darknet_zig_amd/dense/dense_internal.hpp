@@ -28,31 +28,33 @@ template <class T>
 __device__ __forceinline__ void store1(T *p, uint64_t i, float v) {
     p[i] = (T)v;
 }
-// Four consecutive elements at 4 * sizeof(T) alignment.
+// Eight consecutive elements on a 16-byte boundary.
 template <class T>
-__device__ __forceinline__ float4 load4(const T *p, uint64_t i) {
+__device__ __forceinline__ void load8(const T *p, uint64_t i, float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
-        return *reinterpret_cast<const float4 *>(p + i);
+        const float4 a = reinterpret_cast<const float4 *>(p + i)[0], b = reinterpret_cast<const float4 *>(p + i)[1];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = lane(x < 4 ? a : b, x & 3);
     } else {
-        const bf16x4 v = *reinterpret_cast<const bf16x4 *>(p + i);
-        return make_float4((float)v.x, (float)v.y, (float)v.z, (float)v.w);
+        const bf16x8 a = *reinterpret_cast<const bf16x8 *>(p + i);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = (float)a[x];
     }
 }
 template <class T>
-__device__ __forceinline__ void store4(T *p, uint64_t i, float4 v) {
+__device__ __forceinline__ void store8(T *p, uint64_t i, const float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(p + i) = v;
+        reinterpret_cast<float4 *>(p + i)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(p + i)[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-        const f32x4 f = {v.x, v.y, v.z, v.w};
-        *reinterpret_cast<bf16x4 *>(p + i) = __builtin_convertvector(f, bf16x4);
+        typedef float f32x8 __attribute__((ext_vector_type(8)));
+        const f32x8 f = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+        *reinterpret_cast<bf16x8 *>(p + i) = __builtin_convertvector(f, bf16x8);
     }
 }
 
 inline bool type_ok(int type) { return type == DKZ_F32 || type == DKZ_BF16; }
 inline uint64_t type_size(int type) { return type == DKZ_F32 ? 4 : 2; }
-
-// Whether n elements at p may be moved four at a time.
-inline bool aligned4(const void *p, int type) { return ((uintptr_t)p & (4 * type_size(type) - 1)) == 0; }
 
 // Whether [a, a + an) and [b, b + bn) share a byte; a null pointer shares none.
 inline bool overlap(const void *a, uint64_t an, const void *b, uint64_t bn) {
@@ -103,7 +105,27 @@ struct Draws {
         return draw_hash(key ^ draw_hash((uint32_t)i)) >> 8 < limit;
     }
     // A select, not a multiply: a dropped NaN or infinity is 0.
-    __device__ __forceinline__ float apply(float v, uint64_t i) const { return dropped(i) ? 0.0f : v * scale; }
+    __device__ __forceinline__ float apply(float v, uint64_t i) const {
+        v *= scale;
+        return limit != 0 && dropped(i) ? 0.0f : v;
+    }
+    // Elements i .. i + N - 1.
+    template <int N>
+    __device__ __forceinline__ void apply(float (&v)[N], uint64_t i) const {
+#pragma unroll
+        for (int x = 0; x < N; ++x) v[x] *= scale;
+        if (limit == 0) return;
+        i += first;
+        const uint32_t low = (uint32_t)i, high = (uint32_t)(i >> 32);
+        const uint32_t key = seed ^ (high ? draw_hash(0x9e3779b9u * high) : 0u);
+        if (low + (N - 1) >= low) {  // one high word
+#pragma unroll
+            for (int x = 0; x < N; ++x) v[x] = draw_hash(key ^ draw_hash(low + x)) >> 8 < limit ? 0.0f : v[x];
+        } else {
+#pragma unroll
+            for (int x = 0; x < N; ++x) v[x] = dropped(i - first + x) ? 0.0f : v[x];
+        }
+    }
 };
 
 inline Draws make_draws(float prob, float scale, unsigned int seed, unsigned long long first) {

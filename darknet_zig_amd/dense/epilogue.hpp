@@ -45,93 +45,92 @@ __device__ __forceinline__ float gradient_any(int act, float y) {
 // out = dropout(activation(z + bias)) + residual. Matrices have `ld` columns
 // and no gaps, so that r * ld + c is also the draw's element.
 template <class T, bool EXP>
-struct LinearEpilogue : QuadEpilogue<LinearEpilogue<T, EXP>> {
+struct LinearEpilogue : TileEpilogue<LinearEpilogue<T, EXP>> {
     const float *biases;
     const T *residual;
     T *activated, *output;
     uint32_t ld;
     int act;
-    bool vec;  // rows start at multiples of four elements: four at a time
+    bool vec;
     Draws draws;
 
-    template <int N>
-    __device__ __forceinline__ void finish(uint64_t at, float (&a)[N]) const {  // a: activated
-        if (draws.limit != 0) {
+    struct Columns {
+        float bias[8];
+    };
+    __device__ __forceinline__ bool whole() const { return vec; }
+    __device__ __forceinline__ Columns columns(uint32_t c) const {
+        Columns s = {};
+        if (vec && biases != nullptr) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) a[i] = draws.apply(a[i], at + i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) a[i] *= draws.scale;
+            for (int i = 0; i < 8; ++i) s.bias[i] = biases[c + i];
         }
+        return s;
     }
     __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
         const uint64_t at = (uint64_t)r * ld + c;
         float a[1] = {biases != nullptr ? z + biases[c] : z};
         activate_all<EXP>(act, a);
         if (activated != nullptr) store1(activated, at, a[0]);
-        finish(at, a);
+        draws.apply(a, at);
         store1(output, at, residual != nullptr ? a[0] + load1(residual, at) : a[0]);
     }
-    __device__ __forceinline__ void quad(uint32_t r, uint32_t c, uint32_t cols, float4 z) const {
-        if (!vec) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < cols) put(r, c + i, lane(z, i));
-            return;
-        }
+    __device__ __forceinline__ void row(const Columns &s, uint32_t r, uint32_t c, float (&a)[8]) const {
         const uint64_t at = (uint64_t)r * ld + c;
-        float a[4] = {z.x, z.y, z.z, z.w};
+        float add[8] = {};
+        if (residual != nullptr) load8(residual, at, add);
         if (biases != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] += biases[c + i];
+            for (int i = 0; i < 8; ++i) a[i] += s.bias[i];
         }
         activate_all<EXP>(act, a);
-        if (activated != nullptr) store4(activated, at, make_float4(a[0], a[1], a[2], a[3]));
-        finish(at, a);
+        if (activated != nullptr) store8(activated, at, a);
+        draws.apply(a, at);
         if (residual != nullptr) {
-            const float4 b = load4(residual, at);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] += lane(b, i);
+            for (int i = 0; i < 8; ++i) a[i] += add[i];
         }
-        store4(output, at, make_float4(a[0], a[1], a[2], a[3]));
+        store8(output, at, a);
     }
 };
 
 // out = z + beta * old + add, old being out's own value. beta 0 does not read it.
 template <class T>
-struct StoreEpilogue : QuadEpilogue<StoreEpilogue<T>> {
+struct StoreEpilogue : TileEpilogue<StoreEpilogue<T>> {
     T *out;
     const T *add;
     uint32_t ld;
     float beta;
     bool vec;
 
+    struct Columns {};
+    __device__ __forceinline__ bool whole() const { return vec; }
+    __device__ __forceinline__ Columns columns(uint32_t) const { return {}; }
     __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
         const uint64_t at = (uint64_t)r * ld + c;
         if (beta != 0.0f) z += beta * load1(out, at);
         store1(out, at, add != nullptr ? z + load1(add, at) : z);
     }
-    __device__ __forceinline__ void quad(uint32_t r, uint32_t c, uint32_t cols, float4 z) const {
-        if (!vec) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < cols) put(r, c + i, lane(z, i));
-            return;
-        }
+    __device__ __forceinline__ void row(const Columns &, uint32_t r, uint32_t c, float (&z)[8]) const {
         const uint64_t at = (uint64_t)r * ld + c;
+        float x[8];
         if (beta != 0.0f) {
-            const float4 o = load4(out, at);
+            load8(out, at, x);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lane(z, i) += beta * lane(o, i);
+            for (int i = 0; i < 8; ++i) z[i] += beta * x[i];
         }
         if (add != nullptr) {
-            const float4 b = load4(add, at);
+            load8(add, at, x);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lane(z, i) += lane(b, i);
+            for (int i = 0; i < 8; ++i) z[i] += x[i];
         }
-        store4(out, at, z);
+        store8(out, at, z);
     }
 };
+
+// Whether matrices with rows of ld elements may be moved eight at a time.
+inline bool eights(uint64_t ld, const void *a, const void *b = nullptr, const void *c = nullptr) {
+    return ld % 8 == 0 && aligned16(a) && aligned16(b) && aligned16(c);
+}
 
 template <class T>
 StoreEpilogue<T> store_epilogue(void *out, const void *add, uint64_t ld, float beta) {
@@ -140,8 +139,7 @@ StoreEpilogue<T> store_epilogue(void *out, const void *add, uint64_t ld, float b
     e.add = static_cast<const T *>(add);
     e.ld = (uint32_t)ld;
     e.beta = beta;
-    constexpr uintptr_t mask = 4 * sizeof(T) - 1;
-    e.vec = ld % 4 == 0 && (((uintptr_t)out | (uintptr_t)add) & mask) == 0;
+    e.vec = eights(ld, out, add);
     return e;
 }
 

@@ -18,8 +18,7 @@ LinearEpilogue<T, EXP> linear_epilogue(uint64_t outputs, int act, const Draws &d
     e.output = static_cast<T *>(output);
     e.ld = (uint32_t)outputs;
     e.act = act;
-    constexpr uintptr_t mask = 4 * sizeof(T) - 1;
-    e.vec = outputs % 4 == 0 && (((uintptr_t)residual | (uintptr_t)activated | (uintptr_t)output) & mask) == 0;
+    e.vec = eights(outputs, residual, activated, output);
     e.draws = draws;
     return e;
 }
@@ -64,7 +63,7 @@ __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *
         if (c < cols) {
             const uint64_t at = (uint64_t)r * cols + c;
             v = load1(delta, at);
-            v = draws.limit != 0 ? draws.apply(v, at) : v * draws.scale;
+            v = draws.apply(v, at);
             if (act != kLinear) v *= gradient_any(act, load1(activated, at));
             s += v;
         }
@@ -130,7 +129,7 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
         if (input_delta != nullptr)
             DKZ_TRY((run_product<false, true>(kInput, dd, ldd, w, inputs, rows, inputs, outputs,
                                               plan_product(rows, inputs, outputs, true), partial,
-                                              store_epilogue<T>(input_delta, input_residual, inputs, 0.0f))));
+                                              store_epilogue<T>(input_delta, input_residual, inputs, 0.0f), d != nullptr)));
     }
     return 0;
 }

@@ -24,6 +24,7 @@ namespace {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr uint32_t kSlabK = 64;
@@ -109,12 +110,128 @@ __device__ __forceinline__ bf16x8 fragment(const char *lds, uint32_t row, int st
     }
 }
 
+// A slab of R rows of an operand on its way straight to LDS (buffer loads with
+// the lds bit: a wave's 64 lanes fill 1024 consecutive bytes, so the chunk
+// permutation is applied to the addresses read). For operands whose rows lie on
+// 16-byte boundaries. Chunks past `rows` or `kend` read past the buffer's end,
+// which gives zeros.
+template <int R, bool MC, int THREADS>
+struct Direct {
+    static constexpr int kLoads = R * (int)kSlabK / 8 / THREADS;
+    static constexpr uint32_t kOutside = 0x80000000u;
+    uint32_t off[kLoads];  // bytes from the slab's first element; kOutside: past the rows
+    uint32_t k[kLoads];    // the chunk's first k in the slab
+
+    __device__ __forceinline__ void init(uint32_t ld, uint32_t r0, uint32_t rows) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t c = threadIdx.x + i * THREADS;
+            const uint32_t line = MC ? c / (R / 8) : c / 8, slot = MC ? c % (R / 8) : c % 8;
+            const uint32_t chunk = MC ? slot ^ ((line & 3) * 4 & (R / 8 - 1)) : slot ^ (line & 7);
+            k[i] = MC ? line : chunk * 8;
+            off[i] = r0 + (MC ? chunk * 8 : line) < rows ? (line * ld + chunk * 8) * 2 : kOutside;
+        }
+    }
+    // p: element (r0, k0); left: k from k0 to the end. In asm, so that the
+    // compiler does not make every later read of LDS wait for it: the loop below
+    // waits itself (await_loads).
+    __device__ __forceinline__ void load(const __bf16 *p, uint32_t left, uint32_t lds) const {
+        const uint64_t at = (uint64_t)p;
+        const i32x4 buf = {(int)(uint32_t)at, (int)(uint32_t)(at >> 32), (int)kOutside, 0x00020000};
+        const uint32_t to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :
+                         : "s"(to + i * THREADS * 16), "v"(k[i] < left ? off[i] : kOutside), "s"(buf)
+                         : "m0");
+    }
+};
+
+// Waits for this wave's reads of LDS and loads to it, then for the workgroup's other waves.
+__device__ __forceinline__ void await_loads() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Epilogues that treat every element by itself derive from this and give
+//   put(r, c, z)            one element;
+//   whole()                 whether eight columns from a multiple of eight on may be
+//                           moved at once, as
+//   row(state, r, c, z[8])  with state = columns(c), what the columns share (biases).
+// A wave passes its part of the tile through LDS, 32 rows at a time: there a
+// lane wrote four columns of its row at once, here it takes eight of one of
+// four rows, so that rows are read and written in whole lines and the columns a
+// lane sees stay the same. (Straight from the registers, a lane having four
+// columns of each of 32 rows, the code is unrolled for every four, and a
+// dropout, bias and activation took 700 us of 8192x4096x16384's 1660.) Chunks of
+// four columns are permuted by chunk ^ row.
+template <class Self>
+struct TileEpilogue {
+    template <int TR, int TC, int WR, int WC>
+    __device__ __forceinline__ void tile(const f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
+                                         uint32_t rows, uint32_t cols, uint32_t, uint32_t, char *lds) const {
+        constexpr uint32_t kCols = TC * 32, kLanes = kCols / 8, kStep = kWave / kLanes, kMask = kCols / 4 - 1;
+        const Self &self = *static_cast<const Self *>(this);
+        const uint32_t lane = threadIdx.x & 63;
+        float4 *part = reinterpret_cast<float4 *>(lds) + (threadIdx.x >> 6) * (32 * kCols / 4);
+        const uint32_t c = c0 + wc0 + lane % kLanes * 8;
+        const bool whole = self.whole() && c0 + wc0 + kCols <= cols;
+        const auto state = self.columns(whole ? c : 0);
+#pragma unroll
+        for (int j = 0; j < TR; ++j) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    part[(lane & 31) * (kCols / 4) + ((8 * i + 2 * q + (lane >> 5)) ^ (lane & 31 & kMask))] =
+                        make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const uint32_t top = r0 + wr0 + 32 * j;
+            if (whole) {
+#pragma unroll 2
+                for (uint32_t x = lane / kLanes; x < 32; x += kStep) {
+                    const uint32_t at = x * (kCols / 4), chunk = lane % kLanes * 2;
+                    const float4 a = part[at + (chunk ^ (x & kMask))], b = part[at + ((chunk + 1) ^ (x & kMask))];
+                    float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    if (top + x < rows) self.row(state, top + x, c, z);
+                }
+            } else {
+                for (uint32_t x = 0; x < 32 && top + x < rows; ++x)
+                    for (uint32_t y = lane; y < kCols; y += kWave)
+                        if (c0 + wc0 + y < cols) {
+                            const float4 &q = part[x * (kCols / 4) + ((y / 4) ^ (x & kMask))];
+                            self.put(top + x, c0 + wc0 + y, reinterpret_cast<const float *>(&q)[y % 4]);
+                        }
+            }
+        }
+    }
+};
+
+// A split's sums, to be joined.
+struct PartialEpilogue : TileEpilogue<PartialEpilogue> {
+    float *out;
+    uint32_t ld;  // a multiple of eight
+    __device__ __forceinline__ PartialEpilogue(float *out, uint32_t ld) : out(out), ld(ld) {}
+    struct Columns {};
+    __device__ __forceinline__ Columns columns(uint32_t) const { return {}; }
+    __device__ __forceinline__ bool whole() const { return true; }
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const { out[(uint64_t)r * ld + c] = z; }
+    __device__ __forceinline__ void row(const Columns &, uint32_t r, uint32_t c, const float (&z)[8]) const {
+        float4 *to = reinterpret_cast<float4 *>(out + (uint64_t)r * ld + c);
+        to[0] = make_float4(z[0], z[1], z[2], z[3]);
+        to[1] = make_float4(z[4], z[5], z[6], z[7]);
+    }
+};
+
 // acc[i][j][e] is (r, c) = (32 * j + lane % 32, 32 * i + 8 * (e / 4) + 4 * (lane / 32) + e % 4) of the wave's part.
-template <int BR, int BC, int WR, int WC, bool VMC, bool UMC, class Epi>
+template <int BR, int BC, int WR, int WC, bool VMC, bool UMC, bool ALIGNED, class Epi>
 __global__ __launch_bounds__(64 * WR * WC) void product_kernel(ProductArgs g, Epi epi) {
     constexpr int kThreads = 64 * WR * WC, kTR = BR / WR / 32, kTC = BC / WC / 32;
-    constexpr int kV = BR * kSlabK * 2, kU = BC * kSlabK * 2;
-    __shared__ __align__(16) char lds[2 * (kV + kU)];
+    constexpr uint32_t kV = BR * kSlabK * 2, kStage = kV + BC * kSlabK * 2;
+    __shared__ __align__(1024) char lds[2 * kStage];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t tiles = g.tiles_r * g.tiles_c;
     const uint32_t w = xcd_run(blockIdx.x, tiles * g.splits), split = w / tiles;
@@ -131,133 +248,179 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(ProductArgs g, Ep
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
-    Staged<BR, VMC, kThreads> sv;
-    Staged<BC, UMC, kThreads> su;
-    if (kbeg < kend) {
-        sv.load(g.v, g.ldv, r0, g.rows, kbeg, kend);
-        su.load(g.u, g.ldu, c0, g.cols, kbeg, kend);
-        sv.store(lds);
-        su.store(lds + kV);
-        __syncthreads();
-        uint32_t cur = 0;
+    struct Fragments {
+        bf16x8 u[kTC], v[kTR];
+    };
+    auto read = [&](Fragments &f, uint32_t stage, int s) __attribute__((always_inline)) {
+        const char *at = lds + stage * kStage;
+#pragma unroll
+        for (int i = 0; i < kTC; ++i) f.u[i] = fragment<BC, UMC>(at + kV, wc0 + 32 * i, s);
+#pragma unroll
+        for (int j = 0; j < kTR; ++j) f.v[j] = fragment<BR, VMC>(at, wr0 + 32 * j, s);
+    };
+    auto multiply = [&](const Fragments &f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kTC; ++i)
+#pragma unroll
+            for (int j = 0; j < kTR; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.u[i], f.v[j], acc[i][j], 0, 0, 0);
+    };
+    static_assert(kSlabK == 64, "four steps a slab");
+
+    if constexpr (ALIGNED) {
+        // Two slabs of LDS. A wave reads a step's operands while it multiplies
+        // the step before; when it has read a slab's last ones and its loads of
+        // the next slab have landed, it meets the others, begins the loads of
+        // the slab after next into the one just read, and multiplies on.
+        if (kbeg < kend) {
+            Direct<BR, VMC, kThreads> dv;
+            Direct<BC, UMC, kThreads> du;
+            dv.init(g.ldv, r0, g.rows);
+            du.init(g.ldu, c0, g.cols);
+            const __bf16 *pv = g.v + (VMC ? (uint64_t)kbeg * g.ldv + r0 : (uint64_t)r0 * g.ldv + kbeg);
+            const __bf16 *pu = g.u + (UMC ? (uint64_t)kbeg * g.ldu + c0 : (uint64_t)c0 * g.ldu + kbeg);
+            const uint64_t sv = VMC ? (uint64_t)kSlabK * g.ldv : kSlabK, su = UMC ? (uint64_t)kSlabK * g.ldu : kSlabK;
+            const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+            int32_t left = (int32_t)(kend - kbeg);  // k from the next slab to load on
+            auto fetch = [&](uint32_t stage) __attribute__((always_inline)) {
+                if (left > 0) {
+                    dv.load(pv, (uint32_t)left, base + stage * kStage);
+                    du.load(pu, (uint32_t)left, base + stage * kStage + kV);
+                    pv += sv;
+                    pu += su;
+                    left -= (int32_t)kSlabK;
+                }
+            };
+            uint32_t slabs = (kend - kbeg + kSlabK - 1) / kSlabK, stage = 0;
+            // The compiler would read an operand where it is used, and wait for it.
+            auto ahead = [&](Fragments &next, uint32_t stage, int s, const Fragments &now) __attribute__((always_inline)) {
+                read(next, stage, s);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(now);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            Fragments a, b;
+            fetch(0);
+            fetch(1);
+            await_loads();
+            read(a, 0, 0);
 #pragma unroll 1
-        for (uint32_t k0 = kbeg; k0 < kend; k0 += kSlabK, cur ^= 1) {
-            const bool more = k0 + kSlabK < kend;
-            if (more) {
-                sv.load(g.v, g.ldv, r0, g.rows, k0 + kSlabK, kend);
-                su.load(g.u, g.ldu, c0, g.cols, k0 + kSlabK, kend);
+            for (; slabs != 0; --slabs) {
+                ahead(b, stage, 1, a);
+                ahead(a, stage, 2, b);
+                ahead(b, stage, 3, a);
+                await_loads();
+                fetch(stage);
+                stage ^= 1;
+                ahead(a, stage, 0, b);  // past the last slab: an old one, not multiplied
             }
-            const char *lv = lds + cur * (kV + kU), *lu = lv + kV;
-#pragma unroll
-            for (int s = 0; s < (int)kSlabK / 16; ++s) {
-                bf16x8 fu[kTC], fv[kTR];
-#pragma unroll
-                for (int i = 0; i < kTC; ++i) fu[i] = fragment<BC, UMC>(lu, wc0 + 32 * i, s);
-#pragma unroll
-                for (int j = 0; j < kTR; ++j) fv[j] = fragment<BR, VMC>(lv, wr0 + 32 * j, s);
-#pragma unroll
-                for (int i = 0; i < kTC; ++i)
-#pragma unroll
-                    for (int j = 0; j < kTR; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fu[i], fv[j], acc[i][j], 0, 0, 0);
-            }
-            if (more) {
-                char *to = lds + (cur ^ 1) * (kV + kU);
-                sv.store(to);
-                su.store(to + kV);
-            }
+        }
+    } else {
+        Staged<BR, VMC, kThreads> sv;
+        Staged<BC, UMC, kThreads> su;
+        if (kbeg < kend) {
+            sv.load(g.v, g.ldv, r0, g.rows, kbeg, kend);
+            su.load(g.u, g.ldu, c0, g.cols, kbeg, kend);
+            sv.store(lds);
+            su.store(lds + kV);
             __syncthreads();
+            uint32_t stage = 0;
+#pragma unroll 1
+            for (uint32_t k0 = kbeg; k0 < kend; k0 += kSlabK) {
+                const bool more = k0 + kSlabK < kend;
+                if (more) {
+                    sv.load(g.v, g.ldv, r0, g.rows, k0 + kSlabK, kend);
+                    su.load(g.u, g.ldu, c0, g.cols, k0 + kSlabK, kend);
+                }
+                Fragments f;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    read(f, stage, s);
+                    multiply(f);
+                }
+                stage ^= 1;
+                if (more) {
+                    sv.store(lds + stage * kStage);
+                    su.store(lds + stage * kStage + kV);
+                }
+                __syncthreads();
+            }
         }
     }
 
     if (g.splits > 1) {
-        float *to = g.partial + (uint64_t)split * g.rows * g.ldp;
-#pragma unroll
-        for (int j = 0; j < kTR; ++j) {
-            const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
-            if (r >= g.rows) continue;
-#pragma unroll
-            for (int i = 0; i < kTC; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint32_t c = c0 + wc0 + 32 * i + 8 * q + 4 * (lane >> 5);
-                    if (c < g.cols)
-                        *reinterpret_cast<float4 *>(to + (uint64_t)r * g.ldp + c) =
-                            make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-                }
-        }
+        const PartialEpilogue part{g.partial + (uint64_t)split * g.rows * g.ldp, g.ldp};
+        part.template tile<kTR, kTC, WR, WC>(acc, r0, c0, wr0, wc0, g.rows, g.cols, tr, tc, lds);
         return;
     }
     epi.template tile<kTR, kTC, WR, WC>(acc, r0, c0, wr0, wc0, g.rows, g.cols, tr, tc, lds);
 }
 
-// The join of a split product: adds a quad's partials in split order, in f64, and passes it to the epilogue.
+// The join of a split product: adds eight columns' partials in split order, in f64, and passes them to the epilogue.
 template <class Epi>
 __global__ __launch_bounds__(kBlock) void join_kernel(ProductArgs g, Epi epi) {
-    const uint32_t quads = g.ldp / 4, q = blockIdx.x * kBlock + threadIdx.x;
-    if (q >= g.rows * quads) return;
-    const uint32_t r = q / quads, c = (q - r * quads) * 4;
+    const uint32_t eights = g.ldp / 8, e = blockIdx.x * kBlock + threadIdx.x;
+    if (e >= g.rows * eights) return;
+    const uint32_t r = e / eights, c = (e - r * eights) * 8;
     const float *from = g.partial + (uint64_t)r * g.ldp + c;
-    double s[4] = {};
+    double s[8] = {};
     for (uint32_t p = 0; p < g.splits; ++p) {
-        const float4 x = *reinterpret_cast<const float4 *>(from + (uint64_t)p * g.rows * g.ldp);
-        s[0] += (double)x.x;
-        s[1] += (double)x.y;
-        s[2] += (double)x.z;
-        s[3] += (double)x.w;
+        const float4 *at = reinterpret_cast<const float4 *>(from + (uint64_t)p * g.rows * g.ldp);
+        const float4 x = at[0], y = at[1];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] += (double)lane(i < 4 ? x : y, i & 3);
     }
-    epi.quad(r, c, g.cols, make_float4((float)s[0], (float)s[1], (float)s[2], (float)s[3]));
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)s[i];
+    if (epi.whole() && c + 8 <= g.cols) {
+        epi.row(epi.columns(c), r, c, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < g.cols) epi.put(r, c + i, v[i]);
+    }
 }
 
-// Epilogues that treat every element by itself derive from this: quad(r, c,
-// cols, v) takes columns c .. c + 3 of row r, of which those below cols exist.
-template <class Self>
-struct QuadEpilogue {
-    template <int TR, int TC, int WR, int WC>
-    __device__ __forceinline__ void tile(const f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
-                                         uint32_t rows, uint32_t cols, uint32_t, uint32_t, char *) const {
-        const uint32_t lane = threadIdx.x & 63;
-#pragma unroll
-        for (int j = 0; j < TR; ++j) {
-            const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
-            if (r >= rows) continue;
-#pragma unroll
-            for (int i = 0; i < TC; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint32_t c = c0 + wc0 + 32 * i + 8 * q + 4 * (lane >> 5);
-                    if (c < cols)
-                        static_cast<const Self *>(this)->quad(
-                            r, c, cols, make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
-                }
-        }
-    }
-};
-
-// How a product is cut: tiles of br x bc, K in `splits` ranges of k_chunk.
+// How a product is cut: tiles of br x bc, each by wr x wc waves; K in `splits` ranges of k_chunk.
 struct ProductPlan {
-    uint32_t br, bc, splits, k_chunk;
+    uint32_t br, bc, wr, wc, splits, k_chunk;
     uint64_t partial_bytes(uint64_t rows, uint64_t cols) const {
-        return splits > 1 ? padded(4 * (uint64_t)splits * rows * round_up(cols, 4)) : 0;
+        return splits > 1 ? padded(4 * (uint64_t)splits * rows * round_up(cols, 8)) : 0;
     }
 };
 
 inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool may_split) {
-    (void)rows;
-    (void)cols;
     (void)may_split;
-    return {128, 128, 1, (uint32_t)round_up(k, kSlabK)};
+    const uint32_t t = rows > 128 && cols > 128 && div_up(rows, 256) * div_up(cols, 256) >= 200 ? 256 : 128;
+    return {t, t, t == 256 ? 4u : 2u, 2, 1, (uint32_t)round_up(k, kSlabK)};
 }
 
+// Whether an operand's rows start on 16-byte boundaries and are within the
+// loads' 32-bit offsets of each other. A k-contiguous one is whole chunks long
+// (`k` of them, or zeros to the end of the last).
+template <bool MC>
+inline bool direct_ok(const void *p, uint64_t ld, uint64_t k, bool zeros) {
+    return aligned16(p) && ld % 8 == 0 && ld < (1u << 22) && (MC || k % 8 == 0 || zeros);
+}
+
+template <int BR, int BC, int WR, int WC, bool VMC, bool UMC, class Epi>
+int launch_product(const char *name, dim3 grid, bool aligned, const ProductArgs &g, const Epi &epi) {
+    const dim3 block(64 * WR * WC);
+    if (aligned) return launch(name, product_kernel<BR, BC, WR, WC, VMC, UMC, true, Epi>, grid, block, g, epi);
+    return launch(name, product_kernel<BR, BC, WR, WC, VMC, UMC, false, Epi>, grid, block, g, epi);
+}
+
+// zeros: rows of v end in zeros up to a whole chunk.
 template <bool VMC, bool UMC, class Epi>
 int run_product(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu, uint64_t rows, uint64_t cols,
-                uint64_t k, const ProductPlan &p, float *partial, const Epi &epi) {
+                uint64_t k, const ProductPlan &p, float *partial, const Epi &epi, bool zeros = false) {
     if (rows == 0 || cols == 0) return 0;
     ProductArgs g{v, u, (uint32_t)ldv, (uint32_t)ldu, (uint32_t)rows, (uint32_t)cols, (uint32_t)k, div_up(rows, p.br),
-                  div_up(cols, p.bc), p.splits, p.k_chunk, partial, (uint32_t)round_up(cols, 4)};
+                  div_up(cols, p.bc), p.splits, p.k_chunk, partial, (uint32_t)round_up(cols, 8)};
     const dim3 grid((uint32_t)((uint64_t)g.tiles_r * g.tiles_c * g.splits));
-    DKZ_TRY(launch(name, product_kernel<128, 128, 2, 2, VMC, UMC, Epi>, grid, dim3(256), g, epi));
-    return 0;
+    const bool aligned = direct_ok<VMC>(v, ldv, k, zeros) && direct_ok<UMC>(u, ldu, k, false);
+    if (p.br == 256) return launch_product<256, 256, 4, 2, VMC, UMC>(name, grid, aligned, g, epi);
+    return launch_product<128, 128, 2, 2, VMC, UMC>(name, grid, aligned, g, epi);
 }
 
 }  // namespace
