@@ -11,7 +11,7 @@
 
 #include "dense_internal.hpp"
 #include "epilogue.hpp"
-#include "product.hpp"
+#include "product_plan.hpp"
 #include "product_f32.hpp"
 
 namespace dkz {
@@ -86,6 +86,18 @@ struct StatEpilogue {
             if (r < rows && lane < 32) stats[(uint64_t)r * parts + tc * WC + wave_c] = {m, s};
         }
     }
+    // Few rows: COLS lanes hold a row's part.
+    template <int COLS>
+    __device__ __forceinline__ void skinny(uint32_t r, uint32_t c, float z, uint32_t rows, uint32_t cols, uint32_t part) const {
+        if (c >= cols) z = neg_inf();
+        else if (biases != nullptr) z += biases[c];
+        if (r < rows && c < cols && c == (uint32_t)targets[r]) target_logit[r] = z;
+        const float m = seg_max<COLS>(z), base = m == neg_inf() ? 0.0f : m;
+        float s = exp_fast(z - base);
+#pragma unroll
+        for (int x = 1; x < COLS; x *= 2) s += __shfl_xor(s, x);
+        if (r < rows && (threadIdx.x & (COLS - 1)) == 0) stats[(uint64_t)r * parts + part] = {m, s};
+    }
 };
 
 // A wave a row: merges its parts.
@@ -127,7 +139,7 @@ struct GradientEpilogue {
     RowGradient rows_of;
     __bf16 *d;            // 16-byte aligned
     uint32_t ldd, first;  // ldd: a multiple of eight; first: the piece's first class
-    float *sums;          // [row tiles * the workgroup's wave rows][cols]
+    float *sums;          // [parts of the rows][cols]
 
     template <int TR, int TC, int WR, int WC>
     __device__ __forceinline__ void tile(const f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
@@ -177,6 +189,21 @@ struct GradientEpilogue {
             for (int o = kLanes; o < kWave; o *= 2) sum[i] += __shfl_xor(sum[i], o);
             if (lane < kLanes && c + i < cols) sums[(uint64_t)(tr * WR + wave / WC) * cols + c + i] = sum[i];
         }
+    }
+    // Few rows: one element, and every row its own part of the sums.
+    template <int COLS>
+    __device__ __forceinline__ void skinny(uint32_t r, uint32_t c, float z, uint32_t row_count, uint32_t cols, uint32_t) const {
+        if (r >= row_count || c >= ldd) return;
+        float v = 0.0f;
+        uint32_t target;
+        float s, l;
+        rows_of.row(r, target, s, l);
+        if (c < cols && target != ~0u) {
+            const float p = exp_fast((biases != nullptr ? z + biases[c] : z) - l);
+            v = s * ((target == first + c ? 1.0f : 0.0f) - p);
+        }
+        store1(d, (uint64_t)r * ldd + c, v);
+        if (sums != nullptr && c < cols) sums[(uint64_t)r * cols + c] = v;
     }
 };
 
@@ -262,7 +289,7 @@ inline uint64_t piece_of(uint64_t classes, uint64_t most_bytes, uint64_t per_cla
 }
 
 // Tiles of the products whose epilogue looks at whole rows or columns: K stays whole.
-inline ProductPlan whole_plan(uint64_t rows, uint64_t classes, uint64_t inputs) { return plan_product(rows, classes, inputs, false); }
+inline ProductPlan whole_plan(uint64_t rows, uint64_t classes, uint64_t inputs) { return plan_product(rows, classes, inputs, true, false); }
 
 struct ForwardPlan {
     uint64_t piece;  // fp32
@@ -280,7 +307,7 @@ ForwardPlan forward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t clas
         p.partial = std::max(classes >= p.piece ? f32_partial_bytes(rows, p.piece, inputs) : 0, f32_partial_bytes(rows, last, inputs));
     } else {
         const ProductPlan t = whole_plan(rows, classes, inputs);
-        p.stats = padded(sizeof(Stat) * rows * div_up(classes, t.bc) * t.wc);
+        p.stats = padded(sizeof(Stat) * rows * t.row_parts(classes));
     }
     return p;
 }
@@ -308,9 +335,9 @@ BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t cl
         for (const uint64_t n : {whole, last}) {
             if (n == 0) continue;
             const ProductPlan t = whole_plan(rows, n, inputs);
-            p.sums = std::max(p.sums, padded(4 * n * div_up(rows, t.br) * t.wr));
-            p.partial = std::max({p.partial, plan_product(n, inputs, rows, true).partial_bytes(n, inputs),
-                                  plan_product(rows, inputs, n, true).partial_bytes(rows, inputs)});
+            p.sums = std::max(p.sums, padded(4 * n * t.column_parts(rows)));
+            p.partial = std::max({p.partial, plan_product(n, inputs, rows, false, true).partial_bytes(n, inputs),
+                                  plan_product(rows, inputs, n, false, true).partial_bytes(rows, inputs)});
         }
     }
     return p;
@@ -382,7 +409,7 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const vo
     Stat *stats = ws.take<Stat>(plan.stats / sizeof(Stat));
     if (type == DKZ_BF16) {
         const ProductPlan p = whole_plan(rows, classes, inputs);
-        const uint32_t parts = div_up(classes, p.bc) * p.wc;
+        const uint32_t parts = (uint32_t)p.row_parts(classes);
         const StatEpilogue epi{biases, targets, stats, target_logit, parts};
         DKZ_TRY((run_product<false, false>(kName, static_cast<const __bf16 *>(input), inputs, static_cast<const __bf16 *>(weights), inputs,
                                            rows, classes, inputs, p, nullptr, epi)));
@@ -438,17 +465,17 @@ int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16
     for (uint64_t first = 0; first < classes; first += plan.piece) {
         const uint64_t n = std::min(plan.piece, classes - first), ldd = round_up(n, 8);
         const ProductPlan p = whole_plan(rows, n, inputs);
-        const uint64_t chunks = (uint64_t)div_up(rows, p.br) * p.wr;
+        const uint64_t chunks = p.column_parts(rows);
         const __bf16 *w = weights + first * inputs;
         const GradientEpilogue epi{biases != nullptr ? biases + first : nullptr, grad, d, (uint32_t)ldd, (uint32_t)first,
                                             bias_updates != nullptr ? sums : nullptr};
         DKZ_TRY((run_product<false, false>("linear_cross_entropy_gradient", input, inputs, w, inputs, rows, n, inputs, p, nullptr, epi)));
         if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
         if (weight_updates != nullptr)
-            DKZ_TRY((run_product<true, true>(kWeights, d, ldd, input, inputs, n, inputs, rows, plan_product(n, inputs, rows, true), partial,
+            DKZ_TRY((run_product<true, true>(kWeights, d, ldd, input, inputs, n, inputs, rows, plan_product(n, inputs, rows, false, true), partial,
                                              store_epilogue<__bf16>(weight_updates + first * inputs, nullptr, inputs, beta))));
         if (input_delta == nullptr) continue;
-        const ProductPlan pi = plan_product(rows, inputs, n, true);
+        const ProductPlan pi = plan_product(rows, inputs, n, false, true);
         const bool last = first + n == classes;
         if (last && first == 0) {
             DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial,
@@ -548,7 +575,7 @@ int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classe
         if (type == DKZ_F32)
             return run_f32<kRowMajor, kColMajor>(kInput, (const float *)nullptr, 0, (const float *)nullptr, k, 0.0f,
                                                  static_cast<float *>(input_delta), k, m, k, 0, nullptr);
-        return run_product<false, true>(kInput, nullptr, 0, nullptr, k, m, k, 0, plan_product(m, k, 0, true), nullptr,
+        return run_product<false, true>(kInput, nullptr, 0, nullptr, k, m, k, 0, plan_product(m, k, 0, false, true), nullptr,
                                         store_epilogue<__bf16>(input_delta, nullptr, k, 0.0f));
     }
     if (type == DKZ_F32)

@@ -2,7 +2,7 @@
 // activation, dropout, residual), and its backward pass.
 #include "dense_internal.hpp"
 #include "epilogue.hpp"
-#include "product.hpp"
+#include "product_plan.hpp"
 #include "product_f32.hpp"
 
 namespace dkz {
@@ -34,7 +34,7 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act,
                                              outputs, inputs, partial,
                                              linear_epilogue<float, EXP>(outputs, act, draws, biases, residual, activated, output));
     }
-    const ProductPlan p = plan_product(rows, outputs, inputs, true);
+    const ProductPlan p = plan_product(rows, outputs, inputs, true, true);
     float *partial = ws.take<float>(p.partial_bytes(rows, outputs) / 4);
     return run_product<false, false>(kName, static_cast<const __bf16 *>(input), inputs, static_cast<const __bf16 *>(weights),
                                      inputs, rows, outputs, inputs, p, partial,
@@ -43,7 +43,7 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act,
 
 uint64_t forward_bytes(int type, uint64_t rows, uint64_t inputs, uint64_t outputs) {
     if (type == DKZ_F32) return f32_partial_bytes(rows, outputs, inputs);
-    return plan_product(rows, outputs, inputs, true).partial_bytes(rows, outputs);
+    return plan_product(rows, outputs, inputs, true, true).partial_bytes(rows, outputs);
 }
 
 // ---- backward ----
@@ -51,25 +51,68 @@ uint64_t forward_bytes(int type, uint64_t rows, uint64_t inputs, uint64_t output
 constexpr uint32_t kDeltaRows = 64;  // rows a workgroup of delta_kernel takes
 
 // d = dropout(delta) * gradient(activated), stored to d (null: not) in rows of
-// ldd, and the sums of kDeltaRows rows' columns to partial (null: not).
-template <class T>
+// ldd, and the sums of kDeltaRows rows' columns to partial (null: not). Bound by
+// memory: a thread takes W columns (eight where rows start on 16-byte
+// boundaries) of eight rows, all of its loads issued before the first is used;
+// the eight sums of a column's threads are added in row order.
+template <class T, int W>
 __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *activated, uint32_t rows, uint32_t cols, int act,
                                                       Draws draws, T *d, uint32_t ldd, float *partial) {
-    const uint32_t c = blockIdx.x * kBlock + threadIdx.x, r0 = blockIdx.y * kDeltaRows;
-    if (c >= ldd) return;
-    float s = 0.0f;
-    for (uint32_t r = r0; r < min(r0 + kDeltaRows, rows); ++r) {
-        float v = 0.0f;
-        if (c < cols) {
-            const uint64_t at = (uint64_t)r * cols + c;
-            v = load1(delta, at);
-            v = draws.apply(v, at);
-            if (act != kLinear) v *= gradient_any(act, load1(activated, at));
-            s += v;
+    constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes, kEach = kDeltaRows / kGroups;
+    __shared__ float sums[kGroups][kLanes * W + 4];
+    const uint32_t x = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const uint32_t c = (blockIdx.x * kLanes + x) * W, r0 = blockIdx.y * kDeltaRows + group * kEach;
+    const bool in = c < cols;  // W == 8: cols is a multiple of it, and ldd is cols
+    float v[kEach][W], y[kEach][W], s[W] = {};
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        const uint64_t at = (uint64_t)min(r0 + i, rows - 1) * cols + (in ? c : 0);
+        if constexpr (W == 8) load8(delta, at, v[i]);
+        else v[i][0] = load1(delta, at);
+        if (act != kLinear) {
+            if constexpr (W == 8) load8(activated, at, y[i]);
+            else y[i][0] = load1(activated, at);
         }
-        if (d != nullptr) store1(d, (uint64_t)r * ldd + c, v);
     }
-    if (partial != nullptr && c < cols) partial[(uint64_t)blockIdx.y * cols + c] = s;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t r = r0 + i;
+        if (r >= rows) break;
+        draws.apply(v[i], (uint64_t)r * cols + c);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (act != kLinear) v[i][w] *= gradient_any(act, y[i][w]);
+            if (!in) v[i][w] = 0.0f;  // the rows' padding
+            s[w] += v[i][w];
+        }
+        if (d != nullptr && c < ldd) {
+            if constexpr (W == 8) store8(d, (uint64_t)r * ldd + c, v[i]);
+            else store1(d, (uint64_t)r * ldd + c, v[i][0]);
+        }
+    }
+    if (partial == nullptr) return;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sums[group][x * W + w] = s[w];
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < kLanes * W; e += kBlock) {
+        float t = sums[0][e];
+#pragma unroll
+        for (uint32_t i = 1; i < kGroups; ++i) t += sums[i][e];
+        const uint32_t column = blockIdx.x * kLanes * W + e;
+        if (column < cols) partial[(uint64_t)blockIdx.y * cols + column] = t;
+    }
+}
+
+template <class T>
+int run_delta(const T *delta, const T *activated, uint64_t rows, uint64_t cols, int act, const Draws &draws, T *d, uint64_t ldd,
+              float *partial) {
+    constexpr const char *kName = "linear_backward_delta";
+    const dim3 block(kBlock);
+    if (eights(cols, delta, act != kLinear ? activated : nullptr))
+        return launch(kName, delta_kernel<T, 8>, dim3(div_up(cols, 32 * 8), div_up(rows, kDeltaRows)), block, delta, activated,
+                      (uint32_t)rows, (uint32_t)cols, act, draws, d, (uint32_t)ldd, partial);
+    return launch(kName, delta_kernel<T, 1>, dim3(div_up(ldd, 32), div_up(rows, kDeltaRows)), block, delta, activated, (uint32_t)rows,
+                  (uint32_t)cols, act, draws, d, (uint32_t)ldd, partial);
 }
 
 // Leading dimension of d in the workspace: whole 16-byte chunks.
@@ -86,8 +129,8 @@ BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t ou
     if (type == DKZ_F32)
         p.partial_bytes = std::max(f32_partial_bytes(rows, inputs, outputs), f32_partial_bytes(outputs, inputs, rows));
     else
-        p.partial_bytes = std::max(plan_product(rows, inputs, outputs, true).partial_bytes(rows, inputs),
-                                   plan_product(outputs, inputs, rows, true).partial_bytes(outputs, inputs));
+        p.partial_bytes = std::max(plan_product(rows, inputs, outputs, false, true).partial_bytes(rows, inputs),
+                                   plan_product(outputs, inputs, rows, false, true).partial_bytes(outputs, inputs));
     return p;
 }
 
@@ -107,9 +150,8 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
         ldd = outputs;
     }
     if (rows != 0 && outputs != 0 && (bias_updates != nullptr || d != nullptr))
-        DKZ_TRY(launch("linear_backward_delta", delta_kernel<T>, dim3(div_up(ldd, kBlock), div_up(rows, kDeltaRows)), dim3(kBlock),
-                       static_cast<const T *>(delta), static_cast<const T *>(activated), (uint32_t)rows, (uint32_t)outputs, act,
-                       draws, d, (uint32_t)ldd, bias_updates != nullptr ? sums : nullptr));
+        DKZ_TRY(run_delta(static_cast<const T *>(delta), static_cast<const T *>(activated), rows, outputs, act, draws, d, ldd,
+                          bias_updates != nullptr ? sums : nullptr));
     if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, div_up(rows, kDeltaRows), outputs, beta, bias_updates));
     const T *dd = d != nullptr ? d : static_cast<const T *>(delta);
     const T *x = static_cast<const T *>(input), *w = static_cast<const T *>(weights);
@@ -124,11 +166,11 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
     } else {
         if (weight_updates != nullptr)
             DKZ_TRY((run_product<true, true>(kWeights, dd, ldd, x, inputs, outputs, inputs, rows,
-                                             plan_product(outputs, inputs, rows, true), partial,
+                                             plan_product(outputs, inputs, rows, false, true), partial,
                                              store_epilogue<T>(weight_updates, nullptr, inputs, beta))));
         if (input_delta != nullptr)
             DKZ_TRY((run_product<false, true>(kInput, dd, ldd, w, inputs, rows, inputs, outputs,
-                                              plan_product(rows, inputs, outputs, true), partial,
+                                              plan_product(rows, inputs, outputs, false, true), partial,
                                               store_epilogue<T>(input_delta, input_residual, inputs, 0.0f), d != nullptr)));
     }
     return 0;

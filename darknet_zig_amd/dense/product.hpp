@@ -167,6 +167,11 @@ __device__ __forceinline__ void await_loads() {
 // four columns are permuted by chunk ^ row.
 template <class Self>
 struct TileEpilogue {
+    // Few rows (product_skinny.hpp): one element, if it is there.
+    template <int COLS>
+    __device__ __forceinline__ void skinny(uint32_t r, uint32_t c, float z, uint32_t rows, uint32_t cols, uint32_t) const {
+        if (r < rows && c < cols) static_cast<const Self *>(this)->put(r, c, z);
+    }
     template <int TR, int TC, int WR, int WC>
     __device__ __forceinline__ void tile(const f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
                                          uint32_t rows, uint32_t cols, uint32_t, uint32_t, char *lds) const {
@@ -379,48 +384,6 @@ __global__ __launch_bounds__(kBlock) void join_kernel(ProductArgs g, Epi epi) {
         for (int i = 0; i < 8; ++i)
             if (c + i < g.cols) epi.put(r, c + i, v[i]);
     }
-}
-
-// How a product is cut: tiles of br x bc, each by wr x wc waves; K in `splits` ranges of k_chunk.
-struct ProductPlan {
-    uint32_t br, bc, wr, wc, splits, k_chunk;
-    uint64_t partial_bytes(uint64_t rows, uint64_t cols) const {
-        return splits > 1 ? padded(4 * (uint64_t)splits * rows * round_up(cols, 8)) : 0;
-    }
-};
-
-inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool may_split) {
-    (void)may_split;
-    const uint32_t t = rows > 128 && cols > 128 && div_up(rows, 256) * div_up(cols, 256) >= 200 ? 256 : 128;
-    return {t, t, t == 256 ? 4u : 2u, 2, 1, (uint32_t)round_up(k, kSlabK)};
-}
-
-// Whether an operand's rows start on 16-byte boundaries and are within the
-// loads' 32-bit offsets of each other. A k-contiguous one is whole chunks long
-// (`k` of them, or zeros to the end of the last).
-template <bool MC>
-inline bool direct_ok(const void *p, uint64_t ld, uint64_t k, bool zeros) {
-    return aligned16(p) && ld % 8 == 0 && ld < (1u << 22) && (MC || k % 8 == 0 || zeros);
-}
-
-template <int BR, int BC, int WR, int WC, bool VMC, bool UMC, class Epi>
-int launch_product(const char *name, dim3 grid, bool aligned, const ProductArgs &g, const Epi &epi) {
-    const dim3 block(64 * WR * WC);
-    if (aligned) return launch(name, product_kernel<BR, BC, WR, WC, VMC, UMC, true, Epi>, grid, block, g, epi);
-    return launch(name, product_kernel<BR, BC, WR, WC, VMC, UMC, false, Epi>, grid, block, g, epi);
-}
-
-// zeros: rows of v end in zeros up to a whole chunk.
-template <bool VMC, bool UMC, class Epi>
-int run_product(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu, uint64_t rows, uint64_t cols,
-                uint64_t k, const ProductPlan &p, float *partial, const Epi &epi, bool zeros = false) {
-    if (rows == 0 || cols == 0) return 0;
-    ProductArgs g{v, u, (uint32_t)ldv, (uint32_t)ldu, (uint32_t)rows, (uint32_t)cols, (uint32_t)k, div_up(rows, p.br),
-                  div_up(cols, p.bc), p.splits, p.k_chunk, partial, (uint32_t)round_up(cols, 8)};
-    const dim3 grid((uint32_t)((uint64_t)g.tiles_r * g.tiles_c * g.splits));
-    const bool aligned = direct_ok<VMC>(v, ldv, k, zeros) && direct_ok<UMC>(u, ldu, k, false);
-    if (p.br == 256) return launch_product<256, 256, 4, 2, VMC, UMC>(name, grid, aligned, g, epi);
-    return launch_product<128, 128, 2, 2, VMC, UMC>(name, grid, aligned, g, epi);
 }
 
 }  // namespace

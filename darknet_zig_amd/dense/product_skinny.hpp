@@ -1,0 +1,147 @@
+// product_skinny.hpp -- bf16 products of few rows (a token, a handful of
+// sequences): every weight is read once and used for a few rows, so the time is
+// the weights' way from memory.
+//
+// A workgroup takes 16 * CT columns and all rows, its waves a share of K each:
+// no LDS on the way, a lane loads eight k of a weight row (16 bytes at any
+// alignment) straight into an operand of v_mfma_f32_16x16x32_bf16 and eight of
+// an input row, which the caches hold, into the other. Each wave keeps two
+// steps of 64 k in flight beside the one it multiplies. The waves' sums meet in
+// LDS in wave order, and the epilogue takes them from there.
+#pragma once
+
+#include "dense_internal.hpp"
+#include "product.hpp"
+
+namespace dkz {
+namespace {
+
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kSkinnyRows = 64;  // rows at most
+
+template <int RT, int CT, int WAVES, bool UMC, class Epi>
+__global__ __launch_bounds__(64 * WAVES) void skinny_kernel(ProductArgs g, Epi epi) {
+    static_assert(!UMC, "weights with k contiguous");
+    constexpr int kCols = 16 * CT, kRows = 16 * RT, kPitch = kCols + 4;
+    __shared__ __align__(16) float sums[WAVES][kRows][kPitch];
+    // In a scalar, so that what depends on it is a branch: matrix instructions take no notice of masked lanes.
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, group = lane >> 4;
+    const uint32_t c0 = xcd_run(blockIdx.x, gridDim.x) * kCols;
+    // This wave's K: whole steps of 64 but for the last wave's end.
+    const uint32_t steps = (g.k + 63) / 64, per = (steps + WAVES - 1) / WAVES;
+    const uint32_t first = min(wave * per, steps), last = min(first + per, steps);
+
+    f32x4v acc[CT][RT] = {};
+    const short *pu[CT], *pv[RT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i)  // columns past the end repeat the last one, rows the last row: not stored
+        pu[i] = reinterpret_cast<const short *>(g.u) + (uint64_t)min(c0 + 16 * i + l16, g.cols - 1) * g.ldu + 16 * group;
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+        pv[j] = reinterpret_cast<const short *>(g.v) + (uint64_t)min(16 * j + l16, g.rows - 1) * g.ldv + 16 * group;
+
+    // A step's k 16 * group + 0 .. 15 of a row, in two operands: both sides name the same k by the same lane and place.
+    struct Step {
+        s16x8 u[CT][2], v[RT][2];
+    };
+    auto load = [&](Step &s, uint32_t step) __attribute__((always_inline)) {
+        const uint32_t k = step * 64;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < CT; ++i) s.u[i][h] = *reinterpret_cast<const s16x8u *>(pu[i] + k + 8 * h);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) s.v[j][h] = *reinterpret_cast<const s16x8u *>(pv[j] + k + 8 * h);
+        }
+    };
+    auto load_end = [&](Step &s, uint32_t step) __attribute__((always_inline)) {  // k past the end read as 0
+        const uint32_t k = step * 64 + 16 * group;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const bool in = k + 8 * h + x < g.k;
+#pragma unroll
+                for (int i = 0; i < CT; ++i) s.u[i][h][x] = in ? pu[i][step * 64 + 8 * h + x] : (short)0;
+#pragma unroll
+                for (int j = 0; j < RT; ++j) s.v[j][h][x] = in ? pv[j][step * 64 + 8 * h + x] : (short)0;
+            }
+    };
+    auto multiply = [&](const Step &s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int j = 0; j < RT; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, s.u[i][h]),
+                                                                       __builtin_bit_cast(bf16x8, s.v[j][h]), acc[i][j], 0, 0, 0);
+    };
+    const bool ragged = last == steps && first < last && g.k % 64 != 0;
+    const uint32_t whole = last - ragged;
+    if (first < whole) {
+        constexpr int kAhead = RT * CT >= 4 ? 2 : 4;  // steps in flight
+        Step s[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) load(s[a], min(first + a, whole - 1));
+#pragma unroll 1
+        for (uint32_t step = first; step < whole; step += kAhead) {
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                if (step + a < whole) multiply(s[a]);
+                load(s[a], min(step + a + kAhead, whole - 1));  // past the end: the last one again, not multiplied
+            }
+        }
+    }
+    if (ragged) {
+        Step s;
+        load_end(s, whole);
+        multiply(s);
+    }
+    // acc[i][j][e] is column 16 * i + 4 * group + e of row 16 * j + l16.
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+            *reinterpret_cast<f32x4v *>(&sums[wave][16 * j + l16][16 * i + 4 * group]) = acc[i][j];
+    __syncthreads();
+    // A thread an element, the columns along the lanes.
+    for (uint32_t e = threadIdx.x; e < kRows * kCols; e += 64 * WAVES) {
+        const uint32_t r = e / kCols, c = e % kCols;
+        float z = sums[0][r][c];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) z += sums[w][r][c];
+        epi.template skinny<kCols>(r, c0 + c, z, g.rows, g.cols, c0 / kCols);
+    }
+}
+
+// Columns of a workgroup: 32 where that fills the chip, else 16.
+inline uint32_t skinny_columns(uint64_t cols) { return cols >= 32 * 512 ? 32 : 16; }
+
+template <class Epi>
+int run_skinny(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu, uint64_t rows, uint64_t cols, uint64_t k,
+               const Epi &epi) {
+    ProductArgs g{};
+    g.v = v;
+    g.u = u;
+    g.ldv = (uint32_t)ldv;
+    g.ldu = (uint32_t)ldu;
+    g.rows = (uint32_t)rows;
+    g.cols = (uint32_t)cols;
+    g.k = (uint32_t)k;
+    const uint32_t width = skinny_columns(cols);
+    const dim3 grid(div_up(cols, width));
+    if (width == 32) {
+        if (rows <= 16) return launch(name, skinny_kernel<1, 2, 4, false, Epi>, grid, dim3(256), g, epi);
+        if (rows <= 32) return launch(name, skinny_kernel<2, 2, 4, false, Epi>, grid, dim3(256), g, epi);
+        return launch(name, skinny_kernel<4, 2, 4, false, Epi>, grid, dim3(256), g, epi);
+    }
+    if (rows <= 16) return launch(name, skinny_kernel<1, 1, 8, false, Epi>, grid, dim3(512), g, epi);
+    if (rows <= 32) return launch(name, skinny_kernel<2, 1, 8, false, Epi>, grid, dim3(512), g, epi);
+    return launch(name, skinny_kernel<4, 1, 8, false, Epi>, grid, dim3(512), g, epi);
+}
+
+}  // namespace
+}  // namespace dkz
