@@ -27,13 +27,20 @@ typedef short s16x8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-constexpr uint32_t kSlabK = 64;
+// The chunk of 16 bytes that slot `slot` of line `line` of a slab in LDS holds (and the other way round). A line is a row's BK k,
+// or (MC) one k's R rows; the permutation puts lines that are read together into different banks.
+template <int R, int BK, bool MC>
+__device__ __forceinline__ uint32_t permuted(uint32_t line, uint32_t slot) {
+    if constexpr (MC) return slot ^ ((line & 3) * 4 & (R / 8 - 1));
+    else if constexpr (BK == 64) return slot ^ (line >> 1 & 7);
+    else return slot ^ (line >> 2 & 3);
+}
 
 struct ProductArgs {
     const __bf16 *v, *u;  // row side, column side
     uint32_t ldv, ldu;
     uint32_t rows, cols, k;
-    uint32_t tiles_r, tiles_c, splits, k_chunk;  // k_chunk: a split's K, a multiple of kSlabK
+    uint32_t tiles_r, tiles_c, splits, k_chunk;  // k_chunk: a split's K, a multiple of the slab's depth
     float *partial;                              // splits > 1: [splits][rows][ldp]
     uint32_t ldp;
 };
@@ -54,10 +61,10 @@ __device__ __forceinline__ void tile_of(uint32_t t, uint32_t tiles_r, uint32_t t
 
 // A slab of R rows of an operand on its way to LDS through registers, whatever
 // its alignment. MC: row-contiguous.
-template <int R, bool MC, int THREADS>
+template <int R, int BK, bool MC, int THREADS>
 struct Staged {
-    static constexpr int kChunks = R * (int)kSlabK / 8 / THREADS;
-    static_assert(kChunks * 8 * THREADS == R * (int)kSlabK, "whole chunks a thread");
+    static constexpr int kChunks = R * BK / 8 / THREADS, kLine = MC ? R / 8 : BK / 8;  // kLine: chunks a line
+    static_assert(kChunks * 8 * THREADS == R * BK, "whole chunks a thread");
     s16x8 v[kChunks];
 
     // Rows past `rows` and k past `kend` read as 0.
@@ -65,7 +72,7 @@ struct Staged {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             const uint32_t c = threadIdx.x + i * THREADS;
-            const uint32_t row = r0 + (MC ? c % (R / 8) * 8 : c / 8), k = k0 + (MC ? c / (R / 8) : c % 8 * 8);
+            const uint32_t row = r0 + (MC ? c % kLine * 8 : c / kLine), k = k0 + (MC ? c / kLine : c % kLine * 8);
             const short *at = reinterpret_cast<const short *>(p) + (MC ? (uint64_t)k * ld + row : (uint64_t)row * ld + k);
             s16x8 x = {};
             if (row < rows && k < kend) {
@@ -85,24 +92,23 @@ struct Staged {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             const uint32_t c = threadIdx.x + i * THREADS;
-            const uint32_t line = MC ? c / (R / 8) : c / 8, chunk = MC ? c % (R / 8) : c % 8;
-            const uint32_t to = MC ? line * (R / 8) + (chunk ^ ((line & 3) * 4 & (R / 8 - 1))) : line * 8 + (chunk ^ (line & 7));
-            *reinterpret_cast<s16x8 *>(lds + to * 16) = v[i];
+            const uint32_t line = c / kLine;
+            *reinterpret_cast<s16x8 *>(lds + (line * kLine + permuted<R, BK, MC>(line, c % kLine)) * 16) = v[i];
         }
     }
 };
 
 // Rows row .. row + 31 of a slab in LDS, k 16 * step + 8 * (lane / 32) + 0 .. 7, as an MFMA operand.
-template <int R, bool MC>
+template <int R, int BK, bool MC>
 __device__ __forceinline__ bf16x8 fragment(const char *lds, uint32_t row, int step) {
     const uint32_t lane = threadIdx.x & 63;
     if constexpr (!MC) {
         const uint32_t r = row + (lane & 31), chunk = 2 * step + (lane >> 5);
-        return *reinterpret_cast<const bf16x8 *>(lds + r * 128 + ((chunk ^ (r & 7)) * 16));
+        return *reinterpret_cast<const bf16x8 *>(lds + r * (BK * 2) + permuted<R, BK, MC>(r, chunk) * 16);
     } else {
         // Lane a of a group of sixteen names four rows of k line a / 4.
         const uint32_t a = lane & 15, k = 16 * step + 8 * (lane >> 5) + a / 4, r = row + (lane & 16) + 4 * (a & 3);
-        const uint32_t at = k * (R * 2) + (((r >> 3) ^ ((k & 3) * 4 & (R / 8 - 1))) * 16) + (r & 4) * 2;
+        const uint32_t at = k * (R * 2) + permuted<R, BK, MC>(k, r >> 3) * 16 + (r & 4) * 2;
         const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(lds + at));
         const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(lds + at + 4 * R * 2));
         const s16x8 both = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -115,9 +121,10 @@ __device__ __forceinline__ bf16x8 fragment(const char *lds, uint32_t row, int st
 // permutation is applied to the addresses read). For operands whose rows lie on
 // 16-byte boundaries. Chunks past `rows` or `kend` read past the buffer's end,
 // which gives zeros.
-template <int R, bool MC, int THREADS>
+template <int R, int BK, bool MC, int THREADS>
 struct Direct {
-    static constexpr int kLoads = R * (int)kSlabK / 8 / THREADS;
+    static constexpr int kLoads = R * BK / 8 / THREADS, kLine = MC ? R / 8 : BK / 8;
+    static_assert(kLoads * 8 * THREADS == R * BK, "whole loads a thread");
     static constexpr uint32_t kOutside = 0x80000000u;
     uint32_t off[kLoads];  // bytes from the slab's first element; kOutside: past the rows
     uint32_t k[kLoads];    // the chunk's first k in the slab
@@ -126,37 +133,37 @@ struct Direct {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const uint32_t c = threadIdx.x + i * THREADS;
-            const uint32_t line = MC ? c / (R / 8) : c / 8, slot = MC ? c % (R / 8) : c % 8;
-            const uint32_t chunk = MC ? slot ^ ((line & 3) * 4 & (R / 8 - 1)) : slot ^ (line & 7);
+            const uint32_t line = c / kLine, chunk = permuted<R, BK, MC>(line, c % kLine);
             k[i] = MC ? line : chunk * 8;
             off[i] = r0 + (MC ? chunk * 8 : line) < rows ? (line * ld + chunk * 8) * 2 : kOutside;
         }
     }
-    // p: element (r0, k0); left: k from k0 to the end. In asm, so that the
-    // compiler does not make every later read of LDS wait for it: the loop below
-    // waits itself (await_loads).
-    __device__ __forceinline__ void load(const __bf16 *p, uint32_t left, uint32_t lds) const {
+    // Load i of a slab to LDS address `to` (the slab's). p: element (r0, k0);
+    // left: k from k0 to the end, 0 past it. In asm, so that the compiler does
+    // not make every later read of LDS wait for it: the loop below waits itself
+    // (await_loads).
+    __device__ __forceinline__ void load(int i, const __bf16 *p, uint32_t left, uint32_t to) const {
         const uint64_t at = (uint64_t)p;
         const i32x4 buf = {(int)(uint32_t)at, (int)(uint32_t)(at >> 32), (int)kOutside, 0x00020000};
-        const uint32_t to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :
-                         : "s"(to + i * THREADS * 16), "v"(k[i] < left ? off[i] : kOutside), "s"(buf)
-                         : "m0");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :
+                     : "s"(to + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024 + i * THREADS * 16),
+                       "v"(k[i] < left ? off[i] : kOutside), "s"(buf)
+                     : "m0");
     }
 };
 
-// Waits for this wave's reads of LDS and loads to it, then for the workgroup's other waves.
+// Waits for this wave's reads of LDS and all but its last N loads to it, then for the workgroup's other waves.
+template <int N>
 __device__ __forceinline__ void await_loads() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    static_assert(N < 64, "the counter has six bits");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 // Epilogues that treat every element by itself derive from this and give
 //   put(r, c, z)            one element;
-//   whole()                 whether eight columns from a multiple of eight on may be
-//                           moved at once, as
+//   whole()                 whether rows are whole eights of columns on 16-byte
+//                           boundaries, to be moved as
 //   row(state, r, c, z[8])  with state = columns(c), what the columns share (biases).
 // A wave passes its part of the tile through LDS, 32 rows at a time: there a
 // lane wrote four columns of its row at once, here it takes eight of one of
@@ -180,8 +187,8 @@ struct TileEpilogue {
         const uint32_t lane = threadIdx.x & 63;
         float4 *part = reinterpret_cast<float4 *>(lds) + (threadIdx.x >> 6) * (32 * kCols / 4);
         const uint32_t c = c0 + wc0 + lane % kLanes * 8;
-        const bool whole = self.whole() && c0 + wc0 + kCols <= cols;
-        const auto state = self.columns(whole ? c : 0);
+        const bool whole = self.whole();
+        const auto state = self.columns(whole ? min(c, cols - 8) : 0);
 #pragma unroll
         for (int j = 0; j < TR; ++j) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -201,15 +208,18 @@ struct TileEpilogue {
                     const uint32_t at = x * (kCols / 4), chunk = lane % kLanes * 2;
                     const float4 a = part[at + (chunk ^ (x & kMask))], b = part[at + ((chunk + 1) ^ (x & kMask))];
                     float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                    if (top + x < rows) self.row(state, top + x, c, z);
+                    if (top + x < rows && c < cols) self.row(state, top + x, c, z);
                 }
-            } else {
-                for (uint32_t x = 0; x < 32 && top + x < rows; ++x)
-                    for (uint32_t y = lane; y < kCols; y += kWave)
-                        if (c0 + wc0 + y < cols) {
-                            const float4 &q = part[x * (kCols / 4) + ((y / 4) ^ (x & kMask))];
-                            self.put(top + x, c0 + wc0 + y, reinterpret_cast<const float *>(&q)[y % 4]);
-                        }
+            } else {  // a lane a column
+                const uint32_t r_end = rows > top ? min(rows - top, 32u) : 0;
+                for (uint32_t y = lane; y < kCols; y += kWave) {
+                    if (c0 + wc0 + y >= cols) break;
+#pragma unroll 4
+                    for (uint32_t x = 0; x < r_end; ++x) {
+                        const float4 &q = part[x * (kCols / 4) + ((y / 4) ^ (x & kMask))];
+                        self.put(top + x, c0 + wc0 + y, reinterpret_cast<const float *>(&q)[y % 4]);
+                    }
+                }
             }
         }
     }
@@ -232,12 +242,20 @@ struct PartialEpilogue : TileEpilogue<PartialEpilogue> {
 };
 
 // acc[i][j][e] is (r, c) = (32 * j + lane % 32, 32 * i + 8 * (e / 4) + 4 * (lane / 32) + e % 4) of the wave's part.
-template <int BR, int BC, int WR, int WC, bool VMC, bool UMC, bool ALIGNED, class Epi>
-__global__ __launch_bounds__(64 * WR * WC) void product_kernel(ProductArgs g, Epi epi) {
-    constexpr int kThreads = 64 * WR * WC, kTR = BR / WR / 32, kTC = BC / WC / 32;
-    constexpr uint32_t kV = BR * kSlabK * 2, kStage = kV + BC * kSlabK * 2;
-    __shared__ __align__(1024) char lds[2 * kStage];
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+// Tile: its rows and columns, the waves that share them, the slab's depth and how many slabs LDS holds.
+template <int BR_, int BC_, int WR_, int WC_, int BK_, int STAGES_>
+struct Tile {
+    static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_, BK = BK_, STAGES = STAGES_, kThreads = 64 * WR * WC;
+};
+
+template <class T, bool VMC, bool UMC, bool ALIGNED, class Epi>
+__global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs g, Epi epi) {
+    constexpr int BR = T::BR, BC = T::BC, WR = T::WR, WC = T::WC, BK = T::BK, kThreads = T::kThreads;
+    constexpr int kTR = BR / WR / 32, kTC = BC / WC / 32, kSteps = BK / 16, kStages = ALIGNED ? T::STAGES : 2;
+    constexpr uint32_t kV = BR * BK * 2, kStage = kV + BC * BK * 2;
+    constexpr uint32_t kEpilogue = WR * WC * 32 * (kTC * 32) * 4;
+    __shared__ __align__(1024) char lds[kStages * kStage > kEpilogue ? kStages * kStage : kEpilogue];
+    const uint32_t wave = threadIdx.x >> 6;
     const uint32_t tiles = g.tiles_r * g.tiles_c;
     const uint32_t w = xcd_run(blockIdx.x, tiles * g.splits), split = w / tiles;
     uint32_t tr, tc;
@@ -256,12 +274,14 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(ProductArgs g, Ep
     struct Fragments {
         bf16x8 u[kTC], v[kTR];
     };
-    auto read = [&](Fragments &f, uint32_t stage, int s) __attribute__((always_inline)) {
+    auto read_one = [&](Fragments &f, uint32_t stage, int s, int o) __attribute__((always_inline)) {
         const char *at = lds + stage * kStage;
+        if (o < kTC) f.u[o] = fragment<BC, BK, UMC>(at + kV, wc0 + 32 * o, s);
+        else f.v[o - kTC] = fragment<BR, BK, VMC>(at, wr0 + 32 * (o - kTC), s);
+    };
+    auto read = [&](Fragments &f, uint32_t stage, int s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kTC; ++i) f.u[i] = fragment<BC, UMC>(at + kV, wc0 + 32 * i, s);
-#pragma unroll
-        for (int j = 0; j < kTR; ++j) f.v[j] = fragment<BR, VMC>(at, wr0 + 32 * j, s);
+        for (int o = 0; o < kTC + kTR; ++o) read_one(f, stage, s, o);
     };
     auto multiply = [&](const Fragments &f) __attribute__((always_inline)) {
 #pragma unroll
@@ -269,59 +289,88 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(ProductArgs g, Ep
 #pragma unroll
             for (int j = 0; j < kTR; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.u[i], f.v[j], acc[i][j], 0, 0, 0);
     };
-    static_assert(kSlabK == 64, "four steps a slab");
 
     if constexpr (ALIGNED) {
-        // Two slabs of LDS. A wave reads a step's operands while it multiplies
-        // the step before; when it has read a slab's last ones and its loads of
-        // the next slab have landed, it meets the others, begins the loads of
-        // the slab after next into the one just read, and multiplies on.
+        // LDS holds kStages slabs. A wave reads a step's operands while it
+        // multiplies the step before; when it has read a slab's last ones and
+        // its loads of the next slab have landed, it meets the others, and
+        // loads the slab kStages on into the place of the one just read, a few
+        // loads a step between the multiplications: issued all at once they
+        // hold up every wave of the workgroup for the time that the loads'
+        // 64 KB take (4096^3, 256x256 tiles: 115.5 us at once, 108.2 spread).
         if (kbeg < kend) {
-            Direct<BR, VMC, kThreads> dv;
-            Direct<BC, UMC, kThreads> du;
+            Direct<BR, BK, VMC, kThreads> dv;
+            Direct<BC, BK, UMC, kThreads> du;
+            constexpr int kLoads = dv.kLoads + du.kLoads;
             dv.init(g.ldv, r0, g.rows);
             du.init(g.ldu, c0, g.cols);
             const __bf16 *pv = g.v + (VMC ? (uint64_t)kbeg * g.ldv + r0 : (uint64_t)r0 * g.ldv + kbeg);
             const __bf16 *pu = g.u + (UMC ? (uint64_t)kbeg * g.ldu + c0 : (uint64_t)c0 * g.ldu + kbeg);
-            const uint64_t sv = VMC ? (uint64_t)kSlabK * g.ldv : kSlabK, su = UMC ? (uint64_t)kSlabK * g.ldu : kSlabK;
+            const uint64_t sv = VMC ? (uint64_t)BK * g.ldv : BK, su = UMC ? (uint64_t)BK * g.ldu : BK;
             const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-            int32_t left = (int32_t)(kend - kbeg);  // k from the next slab to load on
-            auto fetch = [&](uint32_t stage) __attribute__((always_inline)) {
-                if (left > 0) {
-                    dv.load(pv, (uint32_t)left, base + stage * kStage);
-                    du.load(pu, (uint32_t)left, base + stage * kStage + kV);
-                    pv += sv;
-                    pu += su;
-                    left -= (int32_t)kSlabK;
-                }
+            uint32_t left = kend - kbeg, to = base;  // of the slab that is being loaded
+            auto load = [&](int i) __attribute__((always_inline)) {
+                if (i < dv.kLoads) dv.load(i, pv, left, to);
+                else du.load(i - dv.kLoads, pu, left, to + kV);
             };
-            uint32_t slabs = (kend - kbeg + kSlabK - 1) / kSlabK, stage = 0;
-            // The compiler would read an operand where it is used, and wait for it.
-            auto ahead = [&](Fragments &next, uint32_t stage, int s, const Fragments &now) __attribute__((always_inline)) {
-                read(next, stage, s);
-                __builtin_amdgcn_sched_barrier(0);
-                multiply(now);
-                __builtin_amdgcn_sched_barrier(0);
+            auto next_slab = [&]() __attribute__((always_inline)) {
+                pv += sv;
+                pu += su;
+                left = left > (uint32_t)BK ? left - BK : 0;
             };
-            Fragments a, b;
-            fetch(0);
-            fetch(1);
-            await_loads();
-            read(a, 0, 0);
-#pragma unroll 1
-            for (; slabs != 0; --slabs) {
-                ahead(b, stage, 1, a);
-                ahead(a, stage, 2, b);
-                ahead(b, stage, 3, a);
-                await_loads();
-                fetch(stage);
-                stage ^= 1;
-                ahead(a, stage, 0, b);  // past the last slab: an old one, not multiplied
+            // One step: multiplies, and between the multiplications reads the next operands and issues loads from .. end - 1 of
+            // the slab. (The compiler would read an operand where it is used, and wait for it.)
+            auto step = [&](Fragments &next, uint32_t stage, int s, const Fragments &now, int from, int end) __attribute__((always_inline)) {
+                constexpr int kEach = kTC * kTR;
+#pragma unroll
+                for (int i = 0; i < kTC; ++i)
+#pragma unroll
+                    for (int j = 0; j < kTR; ++j) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now.u[i], now.v[j], acc[i][j], 0, 0, 0);
+                        const int m = i * kTR + j, n = end - from;
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int o = 0; o < kTC + kTR; ++o)
+                            if (o * kEach / (kTC + kTR) == m) read_one(next, stage, s, o);
+#pragma unroll
+                        for (int x = 0; x < n; ++x)
+                            if (x * kEach / n == m) load(from + x);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            };
+            // Past the end of K the loads write zeros, and go on: their count is what the waits go by.
+            static_assert(kSteps % 2 == 0, "steps alternate between two sets of operands");
+            constexpr int kParts = kSteps > 2 ? kSteps - 1 : kSteps, kPart = (kLoads + kParts - 1) / kParts;
+            constexpr auto part = [](int p) { return p * kPart < kLoads ? p * kPart : kLoads; };
+            Fragments f[2];
+#pragma unroll
+            for (int s = 0; s < kStages; ++s) {
+                to = base + s * kStage;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) load(i);
+                next_slab();
             }
+            await_loads<(kStages - 1) * kLoads>();
+            read(f[0], 0, 0);
+#pragma unroll
+            for (int s = 0; s + 1 < kSteps; ++s) step(f[(s + 1) & 1], 0, s + 1, f[s & 1], 0, 0);
+            uint32_t stage = 0;
+#pragma unroll 1
+            for (uint32_t slabs = (kend - kbeg + BK - 1) / BK; slabs > 1; --slabs) {
+                await_loads<(kStages - 2) * kLoads>();
+                to = base + stage * kStage;
+                stage = stage + 1 == (uint32_t)kStages ? 0 : stage + 1;
+                step(f[0], stage, 0, f[1], part(0), part(1));
+#pragma unroll
+                for (int s = 0; s + 1 < kSteps; ++s) step(f[(s + 1) & 1], stage, s + 1, f[s & 1], part(s + 1), part(s + 2));
+                next_slab();
+            }
+            multiply(f[1]);
+            await_loads<0>();  // LDS is the epilogue's now
         }
     } else {
-        Staged<BR, VMC, kThreads> sv;
-        Staged<BC, UMC, kThreads> su;
+        Staged<BR, BK, VMC, kThreads> sv;
+        Staged<BC, BK, UMC, kThreads> su;
         if (kbeg < kend) {
             sv.load(g.v, g.ldv, r0, g.rows, kbeg, kend);
             su.load(g.u, g.ldu, c0, g.cols, kbeg, kend);
@@ -330,15 +379,15 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(ProductArgs g, Ep
             __syncthreads();
             uint32_t stage = 0;
 #pragma unroll 1
-            for (uint32_t k0 = kbeg; k0 < kend; k0 += kSlabK) {
-                const bool more = k0 + kSlabK < kend;
+            for (uint32_t k0 = kbeg; k0 < kend; k0 += BK) {
+                const bool more = k0 + BK < kend;
                 if (more) {
-                    sv.load(g.v, g.ldv, r0, g.rows, k0 + kSlabK, kend);
-                    su.load(g.u, g.ldu, c0, g.cols, k0 + kSlabK, kend);
+                    sv.load(g.v, g.ldv, r0, g.rows, k0 + BK, kend);
+                    su.load(g.u, g.ldu, c0, g.cols, k0 + BK, kend);
                 }
                 Fragments f;
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
+                for (int s = 0; s < kSteps; ++s) {
                     read(f, stage, s);
                     multiply(f);
                 }

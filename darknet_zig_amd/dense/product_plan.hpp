@@ -8,6 +8,9 @@
 namespace dkz {
 namespace {
 
+typedef Tile<256, 256, 4, 2, 64, 2> Tile256;
+typedef Tile<128, 128, 2, 2, 64, 2> Tile128;
+
 // How a product is cut: tiles of br x bc, each by wr x wc waves; K in `splits`
 // ranges of k_chunk. br 0: the kernel for few rows.
 struct ProductPlan {
@@ -26,7 +29,7 @@ inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool n
     (void)may_split;
     if (nt && rows <= kSkinnyRows) return {0, 0, 0, 0, 1, 0};
     const uint32_t t = rows > 128 && cols > 128 && div_up(rows, 256) * div_up(cols, 256) >= 200 ? 256 : 128;
-    return {t, t, t == 256 ? 4u : 2u, 2, 1, (uint32_t)round_up(k, kSlabK)};
+    return {t, t, t == 256 ? 4u : 2u, 2, 1, (uint32_t)round_up(k, 64)};
 }
 
 // Whether an operand's rows start on 16-byte boundaries and are within the
@@ -37,11 +40,11 @@ inline bool direct_ok(const void *p, uint64_t ld, uint64_t k, bool zeros) {
     return aligned16(p) && ld % 8 == 0 && ld < (1u << 22) && (MC || k % 8 == 0 || zeros);
 }
 
-template <int BR, int BC, int WR, int WC, bool VMC, bool UMC, class Epi>
+template <class T, bool VMC, bool UMC, class Epi>
 int launch_product(const char *name, dim3 grid, bool aligned, const ProductArgs &g, const Epi &epi) {
-    const dim3 block(64 * WR * WC);
-    if (aligned) return launch(name, product_kernel<BR, BC, WR, WC, VMC, UMC, true, Epi>, grid, block, g, epi);
-    return launch(name, product_kernel<BR, BC, WR, WC, VMC, UMC, false, Epi>, grid, block, g, epi);
+    const dim3 block(T::kThreads);
+    if (aligned) return launch(name, product_kernel<T, VMC, UMC, true, Epi>, grid, block, g, epi);
+    return launch(name, product_kernel<T, VMC, UMC, false, Epi>, grid, block, g, epi);
 }
 
 // zeros: rows of v end in zeros up to a whole chunk.
@@ -55,8 +58,8 @@ int run_product(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u
                   div_up(cols, p.bc), p.splits, p.k_chunk, partial, (uint32_t)round_up(cols, 8)};
     const dim3 grid((uint32_t)((uint64_t)g.tiles_r * g.tiles_c * g.splits));
     const bool aligned = direct_ok<VMC>(v, ldv, k, zeros) && direct_ok<UMC>(u, ldu, k, false);
-    if (p.br == 256) return launch_product<256, 256, 4, 2, VMC, UMC>(name, grid, aligned, g, epi);
-    return launch_product<128, 128, 2, 2, VMC, UMC>(name, grid, aligned, g, epi);
+    if (p.br == 256) return launch_product<Tile256, VMC, UMC>(name, grid, aligned, g, epi);
+    return launch_product<Tile128, VMC, UMC>(name, grid, aligned, g, epi);
 }
 
 }  // namespace
