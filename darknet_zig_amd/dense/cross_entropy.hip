@@ -47,6 +47,7 @@ __device__ __forceinline__ void finish_row(Stat t, bool target, float z, float *
 // ---- bf16 forward ----
 
 struct StatEpilogue {
+    static constexpr bool kElementwise = false;
     const float *biases;
     const int *targets;
     Stat *stats;          // [rows][parts]: part = column tile * the workgroup's wave columns + wave column
@@ -100,18 +101,30 @@ struct StatEpilogue {
     }
 };
 
-// A wave a row: merges its parts.
+// A workgroup a row: merges its parts.
 __global__ __launch_bounds__(kBlock) void merge_stats_kernel(const Stat *stats, uint32_t parts, const int *targets,
-                                                            const float *target_logit, uint32_t rows, uint32_t classes, float *loss,
-                                                            float *lse) {
-    const uint32_t r = blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    if (r >= rows) return;
+                                                            const float *target_logit, uint32_t classes, float *loss, float *lse) {
+    __shared__ Stat waves[kBlock / kWave];
+    const uint32_t r = blockIdx.x;
+    const Stat *row = stats + (uint64_t)r * parts;
     Stat t{neg_inf(), 0.0f};
-    for (uint32_t i = lane; i < parts; i += kWave) t = merge(t, stats[(uint64_t)r * parts + i]);
+    for (uint32_t i = threadIdx.x; i < parts; i += 4 * kBlock) {
+        Stat next[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) next[u] = row[min(i + u * kBlock, parts - 1)];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+            if (i + u * kBlock < parts) t = merge(t, next[u]);
+    }
 #pragma unroll
     for (int x = 1; x < kWave; x *= 2) t = merge(t, {__shfl_xor(t.m, x), __shfl_xor(t.s, x)});
+    if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = t;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+#pragma unroll
+    for (int w = 1; w < kBlock / kWave; ++w) t = merge(t, waves[w]);
     const bool target = (uint32_t)targets[r] < classes;
-    if (lane == 0) finish_row(t, target, target ? target_logit[r] : 0.0f, loss + r, lse + r);
+    finish_row(t, target, target ? target_logit[r] : 0.0f, loss + r, lse + r);
 }
 
 // ---- the gradient of a logit ----
@@ -135,6 +148,7 @@ struct RowGradient {
 // it, and each wave's unrounded column sums to `sums` (null: not wanted). The
 // tile passes through LDS as TileEpilogue's does.
 struct GradientEpilogue {
+    static constexpr bool kElementwise = false;
     const float *biases;  // of the piece
     RowGradient rows_of;
     __bf16 *d;            // 16-byte aligned
@@ -354,9 +368,10 @@ bool fit_plan(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int typ
     }
 }
 
-// Input gradients of all pieces but the last, in fp32.
-struct AddEpilogue : TileEpilogue<AddEpilogue> {
+// The input gradient of one of several pieces: added up in fp32, the last one rounded to out.
+struct PieceEpilogue : TileEpilogue<PieceEpilogue> {
     float *sum;
+    __bf16 *out;  // null but for the last piece
     uint32_t ld;
     bool begin, vec;
     struct Columns {};
@@ -364,7 +379,9 @@ struct AddEpilogue : TileEpilogue<AddEpilogue> {
     __device__ __forceinline__ Columns columns(uint32_t) const { return {}; }
     __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
         const uint64_t at = (uint64_t)r * ld + c;
-        sum[at] = begin ? z : sum[at] + z;
+        if (!begin) z += sum[at];
+        if (out != nullptr) store1(out, at, z);
+        else sum[at] = z;
     }
     __device__ __forceinline__ void row(const Columns &, uint32_t r, uint32_t c, float (&z)[8]) const {
         const uint64_t at = (uint64_t)r * ld + c;
@@ -374,29 +391,8 @@ struct AddEpilogue : TileEpilogue<AddEpilogue> {
 #pragma unroll
             for (int i = 0; i < 8; ++i) z[i] += o[i];
         }
-        store8(sum, at, z);
-    }
-};
-// The last piece's, added to them and rounded.
-struct LastEpilogue : TileEpilogue<LastEpilogue> {
-    const float *sum;
-    __bf16 *out;
-    uint32_t ld;
-    bool vec;
-    struct Columns {};
-    __device__ __forceinline__ bool whole() const { return vec; }
-    __device__ __forceinline__ Columns columns(uint32_t) const { return {}; }
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
-        const uint64_t at = (uint64_t)r * ld + c;
-        store1(out, at, sum[at] + z);
-    }
-    __device__ __forceinline__ void row(const Columns &, uint32_t r, uint32_t c, float (&z)[8]) const {
-        const uint64_t at = (uint64_t)r * ld + c;
-        float o[8];
-        load8(sum, at, o);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] += o[i];
-        store8(out, at, z);
+        if (out != nullptr) store8(out, at, z);
+        else store8(sum, at, z);
     }
 };
 
@@ -413,8 +409,8 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const vo
         const StatEpilogue epi{biases, targets, stats, target_logit, parts};
         DKZ_TRY((run_product<false, false>(kName, static_cast<const __bf16 *>(input), inputs, static_cast<const __bf16 *>(weights), inputs,
                                            rows, classes, inputs, p, nullptr, epi)));
-        return launch("linear_cross_entropy_merge", merge_stats_kernel, dim3(div_up(rows, kBlock / kWave)), dim3(kBlock), stats, parts,
-                      targets, target_logit, (uint32_t)rows, (uint32_t)classes, loss, lse);
+        return launch("linear_cross_entropy_merge", merge_stats_kernel, dim3((uint32_t)rows), dim3(kBlock), stats, parts, targets,
+                      target_logit, (uint32_t)classes, loss, lse);
     }
     float *logits = ws.take<float>(plan.logits / 4), *partial = ws.take<float>(plan.partial / 4);
     for (uint64_t first = 0; first < classes; first += plan.piece) {
@@ -476,23 +472,16 @@ int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16
                                              store_epilogue<__bf16>(weight_updates + first * inputs, nullptr, inputs, beta))));
         if (input_delta == nullptr) continue;
         const ProductPlan pi = plan_product(rows, inputs, n, false, true);
-        const bool last = first + n == classes;
-        if (last && first == 0) {
+        if (n == classes) {
             DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial,
                                               store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f), true)));
-        } else if (last) {
-            LastEpilogue e;
-            e.sum = accumulate;
-            e.out = input_delta;
-            e.ld = (uint32_t)inputs;
-            e.vec = eights(inputs, input_delta);
-            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial, e, true)));
         } else {
-            AddEpilogue e;
+            PieceEpilogue e;
             e.sum = accumulate;
+            e.out = first + n == classes ? input_delta : nullptr;
             e.ld = (uint32_t)inputs;
             e.begin = first == 0;
-            e.vec = eights(inputs, accumulate);
+            e.vec = eights(inputs, accumulate, e.out);
             DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial, e, true)));
         }
     }

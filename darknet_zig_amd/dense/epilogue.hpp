@@ -30,14 +30,17 @@ __device__ __forceinline__ void activate_all(int act, float (&x)[N]) {
 #undef DKZ_ACT
 }
 
-// The gradient at an activation's output.
-__device__ __forceinline__ float gradient_any(int act, float y) {
-#define DKZ_GRAD(A) \
-    case A: return gradient<A>(y);
+// d[i] *= the gradient at the activation's output y[i].
+template <int N>
+__device__ __forceinline__ void gradient_all(int act, const float (&y)[N], float (&d)[N]) {
+#define DKZ_GRAD(A)                                                             \
+    case A:                                                                     \
+        _Pragma("unroll") for (int i = 0; i < N; ++i) d[i] *= gradient<A>(y[i]); \
+        break;
     switch (act) {
         DKZ_GRAD(kLogistic) DKZ_GRAD(kRelu) DKZ_GRAD(kRelie) DKZ_GRAD(kRamp) DKZ_GRAD(kTanh) DKZ_GRAD(kPlse)
         DKZ_GRAD(kLeaky) DKZ_GRAD(kElu) DKZ_GRAD(kLoggy) DKZ_GRAD(kStair) DKZ_GRAD(kHardtan) DKZ_GRAD(kLhtan) DKZ_GRAD(kSelu)
-        default: return 1.0f;
+        default: break;
     }
 #undef DKZ_GRAD
 }

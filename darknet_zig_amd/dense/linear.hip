@@ -79,9 +79,9 @@ __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *
         const uint32_t r = r0 + i;
         if (r >= rows) break;
         draws.apply(v[i], (uint64_t)r * cols + c);
+        if (act != kLinear) gradient_all(act, y[i], v[i]);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            if (act != kLinear) v[i][w] *= gradient_any(act, y[i][w]);
             if (!in) v[i][w] = 0.0f;  // the rows' padding
             s[w] += v[i][w];
         }

@@ -25,6 +25,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // The chunk of 16 bytes that slot `slot` of line `line` of a slab in LDS holds (and the other way round). A line is a row's BK k,
@@ -67,25 +68,35 @@ struct Staged {
     static_assert(kChunks * 8 * THREADS == R * BK, "whole chunks a thread");
     s16x8 v[kChunks];
 
-    // Rows past `rows` and k past `kend` read as 0.
+    // Rows past `rows` and k past `kend` read as 0. A chunk that ends past its
+    // line's end is the line's last eight elements, shifted: no branches but the
+    // workgroup's, so that a thread's loads are all on their way at once.
     __device__ __forceinline__ void load(const __bf16 *p, uint32_t ld, uint32_t r0, uint32_t rows, uint32_t k0, uint32_t kend) {
+        const short *base = reinterpret_cast<const short *>(p);
+        const bool inside = r0 + R <= rows && k0 + BK <= kend;
+        const uint32_t length = MC ? rows : kend, lines = MC ? kend : rows;
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             const uint32_t c = threadIdx.x + i * THREADS;
-            const uint32_t row = r0 + (MC ? c % kLine * 8 : c / kLine), k = k0 + (MC ? c / kLine : c % kLine * 8);
-            const short *at = reinterpret_cast<const short *>(p) + (MC ? (uint64_t)k * ld + row : (uint64_t)row * ld + k);
-            s16x8 x = {};
-            if (row < rows && k < kend) {
-                const uint32_t n = MC ? rows - row : kend - k;
-                if (n >= 8) {
-                    x = *reinterpret_cast<const s16x8u *>(at);
-                } else {
+            const uint32_t along = (MC ? r0 : k0) + c % kLine * 8, line = (MC ? k0 : r0) + c / kLine;
+            if (inside) {
+                v[i] = *reinterpret_cast<const s16x8u *>(base + (uint64_t)line * ld + along);
+            } else if (length >= 8) {
+                const uint32_t from = min(along, length - 8), shift = along - from;
+                const s16x8 x = *reinterpret_cast<const s16x8u *>(base + (uint64_t)min(line, lines - 1) * ld + from);
+                const u64x2 w = __builtin_bit_cast(u64x2, x);
+                const uint64_t lo = shift & 4 ? w.y : w.x, hi = shift & 4 ? 0 : w.y;
+                const uint32_t bits = (shift & 3) * 16;
+                const bool none = shift >= 8 || line >= lines;
+                const u64x2 y = {none ? 0 : lo >> bits | hi << 1 << (63 - bits), none ? 0 : hi >> bits};
+                v[i] = __builtin_bit_cast(s16x8, y);
+            } else {
+                s16x8 x = {};
 #pragma unroll
-                    for (int j = 0; j < 7; ++j)
-                        if (j < (int)n) x[j] = at[j];
-                }
+                for (int j = 0; j < 7; ++j)
+                    if (line < lines && along + j < length) x[j] = base[(uint64_t)line * ld + along + j];
+                v[i] = x;
             }
-            v[i] = x;
         }
     }
     __device__ __forceinline__ void store(char *lds) const {
@@ -174,6 +185,7 @@ __device__ __forceinline__ void await_loads() {
 // four columns are permuted by chunk ^ row.
 template <class Self>
 struct TileEpilogue {
+    static constexpr bool kElementwise = true;  // the K of a product may be cut, and the pieces joined
     // Few rows (product_skinny.hpp): one element, if it is there.
     template <int COLS>
     __device__ __forceinline__ void skinny(uint32_t r, uint32_t c, float z, uint32_t rows, uint32_t cols, uint32_t) const {
