@@ -302,13 +302,10 @@ inline uint64_t piece_of(uint64_t classes, uint64_t most_bytes, uint64_t per_cla
     return std::min(std::max(fit, kLeastPiece), round_up(classes, 64));
 }
 
-// Tiles of the products whose epilogue looks at whole rows or columns: K stays whole.
-inline ProductPlan whole_plan(uint64_t rows, uint64_t classes, uint64_t inputs) { return plan_product(rows, classes, inputs, true, false); }
-
 struct ForwardPlan {
     uint64_t piece;  // fp32
-    uint64_t logits, stats, target, partial;
-    uint64_t total() const { return logits + stats + target + partial; }
+    uint64_t logits, stats, target, packed, partial;
+    uint64_t total() const { return logits + stats + target + packed + partial; }
 };
 ForwardPlan forward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t classes, uint64_t piece_bytes) {
     ForwardPlan p{};
@@ -320,15 +317,17 @@ ForwardPlan forward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t clas
         const uint64_t last = classes % p.piece;
         p.partial = std::max(classes >= p.piece ? f32_partial_bytes(rows, p.piece, inputs) : 0, f32_partial_bytes(rows, last, inputs));
     } else {
-        const ProductPlan t = whole_plan(rows, classes, inputs);
-        p.stats = padded(sizeof(Stat) * rows * t.row_parts(classes));
+        if (!few_rows(rows)) p.packed = packed_bytes(rows, inputs) + packed_bytes(classes, inputs);
+        p.stats = padded(sizeof(Stat) * rows * most_of_plans(rows, classes, inputs, true, false, [&](const ProductPlan &t) {
+                             return t.row_parts(classes);
+                         }));
     }
     return p;
 }
 
 struct BackwardPlan {
-    uint64_t piece, d, sums, accumulate, partial;
-    uint64_t total() const { return d + sums + accumulate + partial; }
+    uint64_t piece, d, sums, accumulate, packed, partial;
+    uint64_t total() const { return d + sums + accumulate + packed + partial; }
 };
 BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t classes, uint64_t piece_bytes) {
     BackwardPlan p{};
@@ -344,14 +343,15 @@ BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t cl
                                   f32_partial_bytes(rows, inputs, n)});
         }
     } else {
+        if (rows != 0) p.packed = packed_bytes(rows, inputs) + packed_bytes(classes, inputs);
         // The input gradient of several pieces is summed in fp32.
         if (classes > p.piece) p.accumulate = padded(4 * rows * inputs);
         for (const uint64_t n : {whole, last}) {
             if (n == 0) continue;
-            const ProductPlan t = whole_plan(rows, n, inputs);
-            p.sums = std::max(p.sums, padded(4 * n * t.column_parts(rows)));
-            p.partial = std::max({p.partial, plan_product(n, inputs, rows, false, true).partial_bytes(n, inputs),
-                                  plan_product(rows, inputs, n, false, true).partial_bytes(rows, inputs)});
+            p.sums = std::max(p.sums, padded(4 * n * most_of_plans(rows, n, inputs, true, false, [&](const ProductPlan &t) {
+                                                 return t.column_parts(rows);
+                                             })));
+            p.partial = std::max({p.partial, most_partial_bytes(n, inputs, rows, false), most_partial_bytes(rows, inputs, n, false)});
         }
     }
     return p;
@@ -373,26 +373,20 @@ struct PieceEpilogue : TileEpilogue<PieceEpilogue> {
     float *sum;
     __bf16 *out;  // null but for the last piece
     uint32_t ld;
-    bool begin, vec;
-    struct Columns {};
-    __device__ __forceinline__ bool whole() const { return vec; }
-    __device__ __forceinline__ Columns columns(uint32_t) const { return {}; }
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
-        const uint64_t at = (uint64_t)r * ld + c;
-        if (!begin) z += sum[at];
-        if (out != nullptr) store1(out, at, z);
-        else sum[at] = z;
-    }
-    __device__ __forceinline__ void row(const Columns &, uint32_t r, uint32_t c, float (&z)[8]) const {
-        const uint64_t at = (uint64_t)r * ld + c;
+    bool begin, words;
+    __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
+    __device__ __forceinline__ bool in_words() const { return words; }
+    template <bool STEP_ROW, int N>
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, uint32_t n, const float (&)[N], float (&z)[N]) const {
+        const uint64_t at = (uint64_t)r * ld + c, step = STEP_ROW ? ld : 1;
         if (!begin) {
-            float o[8];
-            load8(sum, at, o);
+            float o[N];
+            load_n(sum, at, step, n, o);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] += o[i];
+            for (int i = 0; i < N; ++i) z[i] += o[i];
         }
-        if (out != nullptr) store8(out, at, z);
-        else store8(sum, at, z);
+        if (out != nullptr) store_n(out, at, step, n, z);
+        else store_n(sum, at, step, n, z);
     }
 };
 
@@ -404,11 +398,12 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const vo
     float *target_logit = ws.take<float>(plan.target / 4);
     Stat *stats = ws.take<Stat>(plan.stats / sizeof(Stat));
     if (type == DKZ_BF16) {
-        const ProductPlan p = whole_plan(rows, classes, inputs);
+        Matrix x{static_cast<const __bf16 *>(input), inputs}, w{static_cast<const __bf16 *>(weights), inputs};
+        if (!few_rows(rows)) DKZ_TRY(pack(x, rows, w, classes, inputs, ws));
+        const ProductPlan p = plan_product(rows, classes, inputs, true, false, operands_direct(x.p, x.ld, w.p, w.ld));
         const uint32_t parts = (uint32_t)p.row_parts(classes);
         const StatEpilogue epi{biases, targets, stats, target_logit, parts};
-        DKZ_TRY((run_product<false, false>(kName, static_cast<const __bf16 *>(input), inputs, static_cast<const __bf16 *>(weights), inputs,
-                                           rows, classes, inputs, p, nullptr, epi)));
+        DKZ_TRY((run_product<false, false>(kName, x.p, x.ld, w.p, w.ld, rows, classes, inputs, p, nullptr, epi)));
         return launch("linear_cross_entropy_merge", merge_stats_kernel, dim3((uint32_t)rows), dim3(kBlock), stats, parts, targets,
                       target_logit, (uint32_t)classes, loss, lse);
     }
@@ -458,31 +453,37 @@ int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16
     __bf16 *d = ws.take<__bf16>(plan.d / 2);
     float *sums = ws.take<float>(plan.sums / 4), *accumulate = ws.take<float>(plan.accumulate / 4);
     float *partial = ws.take<float>(plan.partial / 4);
+    Matrix x{input, inputs}, all{weights, inputs};
+    if (rows != 0) DKZ_TRY(pack(x, rows, all, classes, inputs, ws));
     for (uint64_t first = 0; first < classes; first += plan.piece) {
+        const __bf16 *w = all.p + first * all.ld;
         const uint64_t n = std::min(plan.piece, classes - first), ldd = round_up(n, 8);
-        const ProductPlan p = whole_plan(rows, n, inputs);
+        const ProductPlan p =
+            plan_product(rows, n, inputs, true, false, operands_direct(x.p, x.ld, w, all.ld));
         const uint64_t chunks = p.column_parts(rows);
-        const __bf16 *w = weights + first * inputs;
         const GradientEpilogue epi{biases != nullptr ? biases + first : nullptr, grad, d, (uint32_t)ldd, (uint32_t)first,
                                             bias_updates != nullptr ? sums : nullptr};
-        DKZ_TRY((run_product<false, false>("linear_cross_entropy_gradient", input, inputs, w, inputs, rows, n, inputs, p, nullptr, epi)));
+        DKZ_TRY((run_product<false, false>("linear_cross_entropy_gradient", x.p, x.ld, w, all.ld, rows, n, inputs, p, nullptr, epi)));
         if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
         if (weight_updates != nullptr)
-            DKZ_TRY((run_product<true, true>(kWeights, d, ldd, input, inputs, n, inputs, rows, plan_product(n, inputs, rows, false, true), partial,
-                                             store_epilogue<__bf16>(weight_updates + first * inputs, nullptr, inputs, beta))));
+            DKZ_TRY((run_product<true, true>(kWeights, d, ldd, x.p, x.ld, n, inputs, rows,
+                                             plan_product(n, inputs, rows, false, true,
+                                                          operands_direct(d, ldd, x.p, x.ld)),
+                                             partial, store_epilogue<__bf16>(weight_updates + first * inputs, nullptr, inputs, beta))));
         if (input_delta == nullptr) continue;
-        const ProductPlan pi = plan_product(rows, inputs, n, false, true);
+        const ProductPlan pi =
+            plan_product(rows, inputs, n, false, true, operands_direct(d, ldd, w, all.ld));
         if (n == classes) {
-            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial,
-                                              store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f), true)));
+            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, all.ld, rows, inputs, n, pi, partial,
+                                              store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f))));
         } else {
             PieceEpilogue e;
             e.sum = accumulate;
             e.out = first + n == classes ? input_delta : nullptr;
             e.ld = (uint32_t)inputs;
             e.begin = first == 0;
-            e.vec = eights(inputs, accumulate, e.out);
-            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, inputs, rows, inputs, n, pi, partial, e, true)));
+            e.words = e.out == nullptr || rows_in_words<__bf16>(inputs, e.out);
+            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, all.ld, rows, inputs, n, pi, partial, e)));
         }
     }
     return 0;
@@ -564,7 +565,7 @@ int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classe
         if (type == DKZ_F32)
             return run_f32<kRowMajor, kColMajor>(kInput, (const float *)nullptr, 0, (const float *)nullptr, k, 0.0f,
                                                  static_cast<float *>(input_delta), k, m, k, 0, nullptr);
-        return run_product<false, true>(kInput, nullptr, 0, nullptr, k, m, k, 0, plan_product(m, k, 0, false, true), nullptr,
+        return run_product<false, true>(kInput, nullptr, 0, nullptr, k, m, k, 0, plan_product(m, k, 0, false, false, true), nullptr,
                                         store_epilogue<__bf16>(input_delta, nullptr, k, 0.0f));
     }
     if (type == DKZ_F32)

@@ -28,15 +28,18 @@ template <class T>
 __device__ __forceinline__ void store1(T *p, uint64_t i, float v) {
     p[i] = (T)v;
 }
-// Eight consecutive elements on a 16-byte boundary.
+// Eight consecutive elements, at any alignment of theirs (16-byte accesses need none).
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
 template <class T>
 __device__ __forceinline__ void load8(const T *p, uint64_t i, float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4 *>(p + i)[0], b = reinterpret_cast<const float4 *>(p + i)[1];
+        const f32x4u a = reinterpret_cast<const f32x4u *>(p + i)[0], b = reinterpret_cast<const f32x4u *>(p + i)[1];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] = lane(x < 4 ? a : b, x & 3);
+        for (int x = 0; x < 8; ++x) v[x] = x < 4 ? a[x & 3] : b[x & 3];
     } else {
-        const bf16x8 a = *reinterpret_cast<const bf16x8 *>(p + i);
+        const bf16x8u a = *reinterpret_cast<const bf16x8u *>(p + i);
 #pragma unroll
         for (int x = 0; x < 8; ++x) v[x] = (float)a[x];
     }
@@ -44,13 +47,37 @@ __device__ __forceinline__ void load8(const T *p, uint64_t i, float (&v)[8]) {
 template <class T>
 __device__ __forceinline__ void store8(T *p, uint64_t i, const float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4 *>(p + i)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4 *>(p + i)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        reinterpret_cast<f32x4u *>(p + i)[0] = f32x4u{v[0], v[1], v[2], v[3]};
+        reinterpret_cast<f32x4u *>(p + i)[1] = f32x4u{v[4], v[5], v[6], v[7]};
     } else {
-        typedef float f32x8 __attribute__((ext_vector_type(8)));
         const f32x8 f = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-        *reinterpret_cast<bf16x8 *>(p + i) = __builtin_convertvector(f, bf16x8);
+        *reinterpret_cast<bf16x8u *>(p + i) = __builtin_convertvector(f, bf16x8);
     }
+}
+
+// N elements from p[i] on, `step` apart (N == 8 and step 1: eight at once), of which the first n exist.
+template <class T, int N>
+__device__ __forceinline__ void load_n(const T *p, uint64_t i, uint64_t step, uint32_t n, float (&v)[N]) {
+    if constexpr (N == 8) {
+        if (step == 1 && n == 8) {
+            load8(p, i, v);
+            return;
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < N; ++x) v[x] = x < (int)n ? load1(p, i + x * step) : 0.0f;
+}
+template <class T, int N>
+__device__ __forceinline__ void store_n(T *p, uint64_t i, uint64_t step, uint32_t n, const float (&v)[N]) {
+    if constexpr (N == 8) {
+        if (step == 1 && n == 8) {
+            store8(p, i, v);
+            return;
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < N; ++x)
+        if (x < (int)n) store1(p, i + x * step, v[x]);
 }
 
 inline bool type_ok(int type) { return type == DKZ_F32 || type == DKZ_BF16; }
@@ -108,6 +135,16 @@ struct Draws {
     __device__ __forceinline__ float apply(float v, uint64_t i) const {
         v *= scale;
         return limit != 0 && dropped(i) ? 0.0f : v;
+    }
+    // Elements i, i + step, ..
+    template <int N>
+    __device__ __forceinline__ void apply(float (&v)[N], uint64_t i, uint64_t step) const {
+        if (step == 1) {
+            apply(v, i);
+        } else {
+#pragma unroll
+            for (int x = 0; x < N; ++x) v[x] = apply(v[x], i + x * step);
+        }
     }
     // Elements i .. i + N - 1.
     template <int N>

@@ -1,6 +1,5 @@
 // epilogue.hpp -- what becomes of a product's elements: epilogues of both
-// product kernels (put: one element; quad: four of a row), and the column sums
-// behind the bias gradients.
+// product kernels, and the column sums behind the bias gradients.
 #pragma once
 
 #include "dense_internal.hpp"
@@ -13,14 +12,32 @@ constexpr bool uses_exp(int act) {
     return act == kLogistic || act == kLoggy || act == kElu || act == kSelu || act == kTanh;
 }
 
-// The activation `act` of n values: EXP, one of those that take an exponential; else one of the others.
-template <bool EXP, int N>
+// An activation with an exponential for a bf16 result: activate<A>'s formula with
+// expf_cw, under one ulp of fp32 off, in place of the host's bits, and a
+// reciprocal instruction (one ulp) in place of the rounded division: 2^-21
+// relative to the larger of 1 and the value, where a bf16 has 2^-9.
+template <int A>
+__device__ __forceinline__ float activate_bf16(float x) {
+    if constexpr (A == kLogistic) return __builtin_amdgcn_rcpf(1.0f + expf_cw(-x));
+    else if constexpr (A == kLoggy) return 2.0f * __builtin_amdgcn_rcpf(1.0f + expf_cw(-x)) - 1.0f;
+    else if constexpr (A == kElu) return x >= 0.0f ? x : expf_cw(x) - 1.0f;
+    else if constexpr (A == kSelu) return x >= 0.0f ? 1.0507f * x : 1.75803124f * (expf_cw(x) - 1.0f);
+    else if constexpr (A == kTanh) {
+        const float e = expf_cw(2.0f * x);
+        return x >= 40.0f ? 1.0f : (e - 1.0f) * __builtin_amdgcn_rcpf(e + 1.0f);  // e is infinite from 44 on
+    } else return activate<A>(x);
+}
+
+// The activation `act` of N values for a result of type T (fp32 ones are
+// activate_array's). EXP: `act` is one of those with an exponential; else one of the others.
+template <class T, bool EXP, int N>
 __device__ __forceinline__ void activate_all(int act, float (&x)[N]) {
-#define DKZ_ACT(A)                                                      \
-    case A:                                                             \
-        if constexpr (uses_exp(A) == EXP) {                             \
-            _Pragma("unroll") for (int i = 0; i < N; ++i) x[i] = activate<A>(x[i]); \
-        }                                                               \
+#define DKZ_ACT(A)                                                                                                  \
+    case A:                                                                                                         \
+        if constexpr (uses_exp(A) == EXP) {                                                                         \
+            _Pragma("unroll") for (int i = 0; i < N; ++i)                                                           \
+                x[i] = sizeof(T) == 2 ? activate_bf16<A>(x[i]) : activate<A>(x[i]);                                 \
+        }                                                                                                           \
         break;
     switch (act) {
         DKZ_ACT(kLogistic) DKZ_ACT(kRelu) DKZ_ACT(kRelie) DKZ_ACT(kRamp) DKZ_ACT(kTanh) DKZ_ACT(kPlse) DKZ_ACT(kLeaky)
@@ -54,45 +71,33 @@ struct LinearEpilogue : TileEpilogue<LinearEpilogue<T, EXP>> {
     T *activated, *output;
     uint32_t ld;
     int act;
-    bool vec;
+    bool words;
     Draws draws;
 
-    struct Columns {
-        float bias[8];
-    };
-    __device__ __forceinline__ bool whole() const { return vec; }
-    __device__ __forceinline__ Columns columns(uint32_t c) const {
-        Columns s = {};
-        if (vec && biases != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s.bias[i] = biases[c + i];
-        }
-        return s;
-    }
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
-        const uint64_t at = (uint64_t)r * ld + c;
-        float a[1] = {biases != nullptr ? z + biases[c] : z};
-        activate_all<EXP>(act, a);
-        if (activated != nullptr) store1(activated, at, a[0]);
-        draws.apply(a, at);
-        store1(output, at, residual != nullptr ? a[0] + load1(residual, at) : a[0]);
-    }
-    __device__ __forceinline__ void row(const Columns &s, uint32_t r, uint32_t c, float (&a)[8]) const {
-        const uint64_t at = (uint64_t)r * ld + c;
-        float add[8] = {};
-        if (residual != nullptr) load8(residual, at, add);
+    __device__ __forceinline__ float bias(uint32_t c) const { return biases != nullptr ? biases[c] : 0.0f; }
+    __device__ __forceinline__ bool in_words() const { return words; }
+    template <bool STEP_ROW, int N>
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, uint32_t n, const float (&bias)[N], float (&a)[N]) const {
+        const uint64_t at = (uint64_t)r * ld + c, step = STEP_ROW ? ld : 1;
+        float add[N] = {};
+        if (residual != nullptr) load_n(residual, at, step, n, add);
         if (biases != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] += s.bias[i];
+            for (int i = 0; i < N; ++i) a[i] += bias[i];
         }
-        activate_all<EXP>(act, a);
-        if (activated != nullptr) store8(activated, at, a);
-        draws.apply(a, at);
+        activate_all<T, EXP>(act, a);
+        if (activated != nullptr) store_n(activated, at, step, n, a);
+        draws.apply(a, at, step);
         if (residual != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] += add[i];
+            for (int i = 0; i < N; ++i) a[i] += add[i];
         }
-        store8(output, at, a);
+        store_n(output, at, step, n, a);
+    }
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
+        const float b[1] = {bias(c)};
+        float v[1] = {z};
+        put<true>(r, c, 1, b, v);
     }
 };
 
@@ -103,36 +108,37 @@ struct StoreEpilogue : TileEpilogue<StoreEpilogue<T>> {
     const T *add;
     uint32_t ld;
     float beta;
-    bool vec;
+    bool words;
 
-    struct Columns {};
-    __device__ __forceinline__ bool whole() const { return vec; }
-    __device__ __forceinline__ Columns columns(uint32_t) const { return {}; }
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
-        const uint64_t at = (uint64_t)r * ld + c;
-        if (beta != 0.0f) z += beta * load1(out, at);
-        store1(out, at, add != nullptr ? z + load1(add, at) : z);
-    }
-    __device__ __forceinline__ void row(const Columns &, uint32_t r, uint32_t c, float (&z)[8]) const {
-        const uint64_t at = (uint64_t)r * ld + c;
-        float x[8];
+    __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
+    __device__ __forceinline__ bool in_words() const { return words; }
+    template <bool STEP_ROW, int N>
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, uint32_t n, const float (&)[N], float (&z)[N]) const {
+        const uint64_t at = (uint64_t)r * ld + c, step = STEP_ROW ? ld : 1;
+        float x[N];
         if (beta != 0.0f) {
-            load8(out, at, x);
+            load_n(out, at, step, n, x);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] += beta * x[i];
+            for (int i = 0; i < N; ++i) z[i] += beta * x[i];
         }
         if (add != nullptr) {
-            load8(add, at, x);
+            load_n(add, at, step, n, x);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] += x[i];
+            for (int i = 0; i < N; ++i) z[i] += x[i];
         }
-        store8(out, at, z);
+        store_n(out, at, step, n, z);
+    }
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
+        const float b[1] = {};
+        float v[1] = {z};
+        put<true>(r, c, 1, b, v);
     }
 };
 
-// Whether matrices with rows of ld elements may be moved eight at a time.
-inline bool eights(uint64_t ld, const void *a, const void *b = nullptr, const void *c = nullptr) {
-    return ld % 8 == 0 && aligned16(a) && aligned16(b) && aligned16(c);
+// Whether rows of ld elements of these tensors start on 4-byte boundaries.
+template <class T>
+bool rows_in_words(uint64_t ld, const void *a, const void *b = nullptr, const void *c = nullptr) {
+    return ld * sizeof(T) % 4 == 0 && (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 3) == 0;
 }
 
 template <class T>
@@ -142,7 +148,7 @@ StoreEpilogue<T> store_epilogue(void *out, const void *add, uint64_t ld, float b
     e.add = static_cast<const T *>(add);
     e.ld = (uint32_t)ld;
     e.beta = beta;
-    e.vec = eights(ld, out, add);
+    e.words = rows_in_words<T>(ld, out, add);
     return e;
 }
 

@@ -18,7 +18,7 @@ LinearEpilogue<T, EXP> linear_epilogue(uint64_t outputs, int act, const Draws &d
     e.output = static_cast<T *>(output);
     e.ld = (uint32_t)outputs;
     e.act = act;
-    e.vec = eights(outputs, residual, activated, output);
+    e.words = rows_in_words<T>(outputs, residual, activated, output);
     e.draws = draws;
     return e;
 }
@@ -34,16 +34,18 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act,
                                              outputs, inputs, partial,
                                              linear_epilogue<float, EXP>(outputs, act, draws, biases, residual, activated, output));
     }
-    const ProductPlan p = plan_product(rows, outputs, inputs, true, true);
+    Matrix x{static_cast<const __bf16 *>(input), inputs}, w{static_cast<const __bf16 *>(weights), inputs};
+    if (!few_rows(rows)) DKZ_TRY(pack(x, rows, w, outputs, inputs, ws));
+    const ProductPlan p = plan_product(rows, outputs, inputs, true, true, operands_direct(x.p, x.ld, w.p, w.ld));
     float *partial = ws.take<float>(p.partial_bytes(rows, outputs) / 4);
-    return run_product<false, false>(kName, static_cast<const __bf16 *>(input), inputs, static_cast<const __bf16 *>(weights),
-                                     inputs, rows, outputs, inputs, p, partial,
+    return run_product<false, false>(kName, x.p, x.ld, w.p, w.ld, rows, outputs, inputs, p, partial,
                                      linear_epilogue<__bf16, EXP>(outputs, act, draws, biases, residual, activated, output));
 }
 
 uint64_t forward_bytes(int type, uint64_t rows, uint64_t inputs, uint64_t outputs) {
     if (type == DKZ_F32) return f32_partial_bytes(rows, outputs, inputs);
-    return plan_product(rows, outputs, inputs, true, true).partial_bytes(rows, outputs);
+    const uint64_t packed = few_rows(rows) ? 0 : packed_bytes(rows, inputs) + packed_bytes(outputs, inputs);
+    return packed + most_partial_bytes(rows, outputs, inputs, true);
 }
 
 // ---- backward ----
@@ -52,8 +54,8 @@ constexpr uint32_t kDeltaRows = 64;  // rows a workgroup of delta_kernel takes
 
 // d = dropout(delta) * gradient(activated), stored to d (null: not) in rows of
 // ldd, and the sums of kDeltaRows rows' columns to partial (null: not). Bound by
-// memory: a thread takes W columns (eight where rows start on 16-byte
-// boundaries) of eight rows, all of its loads issued before the first is used;
+// memory: a thread takes W columns (eight where rows are whole
+// eights) of eight rows, all of its loads issued before the first is used;
 // the eight sums of a column's threads are added in row order.
 template <class T, int W>
 __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *activated, uint32_t rows, uint32_t cols, int act,
@@ -108,7 +110,7 @@ int run_delta(const T *delta, const T *activated, uint64_t rows, uint64_t cols, 
               float *partial) {
     constexpr const char *kName = "linear_backward_delta";
     const dim3 block(kBlock);
-    if (eights(cols, delta, act != kLinear ? activated : nullptr))
+    if (cols % 8 == 0)
         return launch(kName, delta_kernel<T, 8>, dim3(div_up(cols, 32 * 8), div_up(rows, kDeltaRows)), block, delta, activated,
                       (uint32_t)rows, (uint32_t)cols, act, draws, d, (uint32_t)ldd, partial);
     return launch(kName, delta_kernel<T, 1>, dim3(div_up(ldd, 32), div_up(rows, kDeltaRows)), block, delta, activated, (uint32_t)rows,
@@ -119,18 +121,18 @@ int run_delta(const T *delta, const T *activated, uint64_t rows, uint64_t cols, 
 inline uint64_t delta_ld(int type, uint64_t outputs) { return round_up(outputs, type == DKZ_F32 ? 4 : 8); }
 
 struct BackwardPlan {
-    uint64_t d_bytes, sum_bytes, partial_bytes;
-    uint64_t total() const { return d_bytes + sum_bytes + partial_bytes; }
+    uint64_t d_bytes, sum_bytes, packed, partial_bytes;
+    uint64_t total() const { return d_bytes + sum_bytes + packed + partial_bytes; }
 };
 BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t outputs) {
     BackwardPlan p;
     p.d_bytes = padded(rows * delta_ld(type, outputs) * type_size(type));
     p.sum_bytes = padded(4 * outputs * div_up(rows, kDeltaRows));
+    p.packed = type == DKZ_F32 || rows == 0 ? 0 : packed_bytes(rows, inputs) + packed_bytes(outputs, inputs);
     if (type == DKZ_F32)
         p.partial_bytes = std::max(f32_partial_bytes(rows, inputs, outputs), f32_partial_bytes(outputs, inputs, rows));
     else
-        p.partial_bytes = std::max(plan_product(rows, inputs, outputs, false, true).partial_bytes(rows, inputs),
-                                   plan_product(outputs, inputs, rows, false, true).partial_bytes(outputs, inputs));
+        p.partial_bytes = std::max(most_partial_bytes(rows, inputs, outputs, false), most_partial_bytes(outputs, inputs, rows, false));
     return p;
 }
 
@@ -143,8 +145,8 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
     float *sums = ws.take<float>(plan.sum_bytes / 4), *partial = ws.take<float>(plan.partial_bytes / 4);
     uint64_t ldd = delta_ld(type, outputs);
     const bool products = weight_updates != nullptr || input_delta != nullptr;
-    // The delta itself where nothing changes it.
-    const bool same = act == kLinear && draws.limit == 0 && draws.scale == 1.0f;
+    // The delta itself where nothing changes it and its rows lie on 16-byte boundaries.
+    const bool same = act == kLinear && draws.limit == 0 && draws.scale == 1.0f && ldd == outputs && aligned16(delta);
     if (same || !products) {
         d = nullptr;
         ldd = outputs;
@@ -154,9 +156,9 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
                           bias_updates != nullptr ? sums : nullptr));
     if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, div_up(rows, kDeltaRows), outputs, beta, bias_updates));
     const T *dd = d != nullptr ? d : static_cast<const T *>(delta);
-    const T *x = static_cast<const T *>(input), *w = static_cast<const T *>(weights);
     constexpr const char *kWeights = "linear_backward_weights", *kInput = "linear_backward_input";
     if constexpr (sizeof(T) == 4) {
+        const T *x = static_cast<const T *>(input), *w = static_cast<const T *>(weights);
         if (weight_updates != nullptr)
             DKZ_TRY((run_f32<kColMajor, kColMajor>(kWeights, dd, ldd, x, inputs, beta, static_cast<float *>(weight_updates),
                                                    inputs, outputs, inputs, rows, partial)));
@@ -164,14 +166,19 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
             DKZ_TRY((run_f32<kRowMajor, kColMajor>(kInput, dd, ldd, w, inputs, 0.0f, (float *)nullptr, inputs, rows, inputs,
                                                    outputs, partial, store_epilogue<T>(input_delta, input_residual, inputs, 0.0f))));
     } else {
+        Matrix x{weight_updates != nullptr ? static_cast<const T *>(input) : nullptr, inputs};
+        Matrix w{input_delta != nullptr ? static_cast<const T *>(weights) : nullptr, inputs};
+        if (rows != 0) DKZ_TRY(pack(x, rows, w, outputs, inputs, ws));
         if (weight_updates != nullptr)
-            DKZ_TRY((run_product<true, true>(kWeights, dd, ldd, x, inputs, outputs, inputs, rows,
-                                             plan_product(outputs, inputs, rows, false, true), partial,
-                                             store_epilogue<T>(weight_updates, nullptr, inputs, beta))));
+            DKZ_TRY((run_product<true, true>(
+                kWeights, dd, ldd, x.p, x.ld, outputs, inputs, rows,
+                plan_product(outputs, inputs, rows, false, true, operands_direct(dd, ldd, x.p, x.ld)), partial,
+                store_epilogue<T>(weight_updates, nullptr, inputs, beta))));
         if (input_delta != nullptr)
-            DKZ_TRY((run_product<false, true>(kInput, dd, ldd, w, inputs, rows, inputs, outputs,
-                                              plan_product(rows, inputs, outputs, false, true), partial,
-                                              store_epilogue<T>(input_delta, input_residual, inputs, 0.0f), d != nullptr)));
+            DKZ_TRY((run_product<false, true>(
+                kInput, dd, ldd, w.p, w.ld, rows, inputs, outputs,
+                plan_product(rows, inputs, outputs, false, true, operands_direct(dd, ldd, w.p, w.ld)), partial,
+                store_epilogue<T>(input_delta, input_residual, inputs, 0.0f))));
     }
     return 0;
 }
@@ -210,6 +217,8 @@ int dkz_linear_forward(int type, int rows, int inputs, int outputs, int activati
     DKZ_REQUIRE(disjoint(writes, reads));
     const Draws draws = make_draws(prob, scale, seed, first);
     const Workspace ws{static_cast<char *>(workspace), need};
+    // Activations with an exponential are kernels of their own: in one kernel they cost the others too (8192x4096x16384
+    // with leaky and dropout 1000 us alone, 1590 beside them).
     return uses_exp(activation)
                ? forward<true>(type, m, k, n, activation, draws, input, weights, biases, residual, activated, output, ws)
                : forward<false>(type, m, k, n, activation, draws, input, weights, biases, residual, activated, output, ws);

@@ -25,6 +25,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -58,6 +60,18 @@ __device__ __forceinline__ void tile_of(uint32_t t, uint32_t tiles_r, uint32_t t
     const uint32_t in_group = t % per_group, size = min(tiles_r - first, 8u);
     tr = first + in_group % size;
     tc = in_group / size;
+}
+
+// Eight elements at any alignment of theirs: the whole words that hold them,
+// shifted (a 16-byte load at an odd element is taken apart by the hardware).
+__device__ __forceinline__ s16x8 load_shifted(const short *p) {
+    const uint32_t *q = reinterpret_cast<const uint32_t *>((uintptr_t)p & ~(uintptr_t)3);
+    const uint32_t odd = (uint32_t)(uintptr_t)p >> 1 & 1;
+    const u32x4u x = *reinterpret_cast<const u32x4u *>(q);
+    const uint32_t end = q[3 + odd];
+    const u32x4 y = {__builtin_amdgcn_alignbit(x.y, x.x, 16 * odd), __builtin_amdgcn_alignbit(x.z, x.y, 16 * odd),
+                     __builtin_amdgcn_alignbit(x.w, x.z, 16 * odd), __builtin_amdgcn_alignbit(end, x.w, 16 * odd)};
+    return __builtin_bit_cast(s16x8, y);
 }
 
 // A slab of R rows of an operand on its way to LDS through registers, whatever
@@ -172,10 +186,12 @@ __device__ __forceinline__ void await_loads() {
 }
 
 // Epilogues that treat every element by itself derive from this and give
-//   put(r, c, z)            one element;
-//   whole()                 whether rows are whole eights of columns on 16-byte
-//                           boundaries, to be moved as
-//   row(state, r, c, z[8])  with state = columns(c), what the columns share (biases).
+//   bias(c)                 what is added to column c (0: nothing);
+//   in_words()              whether rows start on 4-byte boundaries;
+//   put<STEP_ROW>(r, c, n, bias, z)
+//                           elements z[0 .. n - 1] from (r, c) on, of one column
+//                           (STEP_ROW) or one row, their biases in bias[0 .. n - 1];
+//                           n a compile-time constant 8 or less in a variable.
 // A wave passes its part of the tile through LDS, 32 rows at a time: there a
 // lane wrote four columns of its row at once, here it takes eight of one of
 // four rows, so that rows are read and written in whole lines and the columns a
@@ -189,7 +205,11 @@ struct TileEpilogue {
     // Few rows (product_skinny.hpp): one element, if it is there.
     template <int COLS>
     __device__ __forceinline__ void skinny(uint32_t r, uint32_t c, float z, uint32_t rows, uint32_t cols, uint32_t) const {
-        if (r < rows && c < cols) static_cast<const Self *>(this)->put(r, c, z);
+        if (r >= rows || c >= cols) return;
+        const Self &self = *static_cast<const Self *>(this);
+        const float bias[1] = {self.bias(c)};
+        float v[1] = {z};
+        self.template put<true>(r, c, 1, bias, v);
     }
     template <int TR, int TC, int WR, int WC>
     __device__ __forceinline__ void tile(const f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
@@ -199,8 +219,10 @@ struct TileEpilogue {
         const uint32_t lane = threadIdx.x & 63;
         float4 *part = reinterpret_cast<float4 *>(lds) + (threadIdx.x >> 6) * (32 * kCols / 4);
         const uint32_t c = c0 + wc0 + lane % kLanes * 8;
-        const bool whole = self.whole();
-        const auto state = self.columns(whole ? min(c, cols - 8) : 0);
+        const bool words = self.in_words();
+        float bias[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bias[i] = self.bias(min(words ? c + i : c0 + wc0 + lane % kCols, cols - 1));
 #pragma unroll
         for (int j = 0; j < TR; ++j) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -214,24 +236,39 @@ struct TileEpilogue {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             const uint32_t top = r0 + wr0 + 32 * j;
-            if (whole) {
+            if (words) {
+                if (c >= cols) continue;
 #pragma unroll 2
                 for (uint32_t x = lane / kLanes; x < 32; x += kStep) {
-                    const uint32_t at = x * (kCols / 4), chunk = lane % kLanes * 2;
+                    const uint32_t at = x * (kCols / 4), chunk = lane % kLanes * 2, r = top + x;
                     const float4 a = part[at + (chunk ^ (x & kMask))], b = part[at + ((chunk + 1) ^ (x & kMask))];
                     float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                    if (top + x < rows && c < cols) self.row(state, top + x, c, z);
+                    if (r >= rows) break;
+                    self.template put<false>(r, c, min(cols - c, 8u), bias, z);
                 }
-            } else {  // a lane a column
-                const uint32_t r_end = rows > top ? min(rows - top, 32u) : 0;
-                for (uint32_t y = lane; y < kCols; y += kWave) {
-                    if (c0 + wc0 + y >= cols) break;
-#pragma unroll 4
-                    for (uint32_t x = 0; x < r_end; ++x) {
-                        const float4 &q = part[x * (kCols / 4) + ((y / 4) ^ (x & kMask))];
-                        self.put(top + x, c0 + wc0 + y, reinterpret_cast<const float *>(&q)[y % 4]);
+                continue;
+            }
+            // Rows that start inside a word: a lane a column, eight rows at a time.
+#pragma unroll
+            for (uint32_t y = 0; y < kCols; y += kWave) {
+                const uint32_t col = y + lane, at = c0 + wc0 + col;
+                if (y != 0) {  // the second half of 128 columns
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) bias[i] = self.bias(min(at, cols - 1));
+                }
+                if (col < kCols && at < cols)
+#pragma unroll 1
+                    for (uint32_t x = 0; x < 32 && top + x < rows; x += 8) {
+                        float z[8];
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; ++i)
+                            z[i] = reinterpret_cast<const float *>(part)[((x + i) * (kCols / 4) + ((col / 4) ^ ((x + i) & kMask))) * 4 + col % 4];
+                        self.template put<true>(top + x, at, min(rows - top - x, 8u), bias, z);
                     }
-                }
+            }
+            if constexpr (kCols > kWave) {  // back to the first half's
+#pragma unroll
+                for (int i = 0; i < 8; ++i) bias[i] = self.bias(min(c0 + wc0 + lane, cols - 1));
             }
         }
     }
@@ -242,18 +279,14 @@ struct PartialEpilogue : TileEpilogue<PartialEpilogue> {
     float *out;
     uint32_t ld;  // a multiple of eight
     __device__ __forceinline__ PartialEpilogue(float *out, uint32_t ld) : out(out), ld(ld) {}
-    struct Columns {};
-    __device__ __forceinline__ Columns columns(uint32_t) const { return {}; }
-    __device__ __forceinline__ bool whole() const { return true; }
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const { out[(uint64_t)r * ld + c] = z; }
-    __device__ __forceinline__ void row(const Columns &, uint32_t r, uint32_t c, const float (&z)[8]) const {
-        float4 *to = reinterpret_cast<float4 *>(out + (uint64_t)r * ld + c);
-        to[0] = make_float4(z[0], z[1], z[2], z[3]);
-        to[1] = make_float4(z[4], z[5], z[6], z[7]);
+    __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
+    __device__ __forceinline__ bool in_words() const { return true; }
+    template <bool STEP_ROW, int N>
+    __device__ __forceinline__ void put(uint32_t r, uint32_t c, uint32_t, const float (&)[N], float (&z)[N]) const {
+        store8(out, (uint64_t)r * ld + c, z);  // also past the last column: ld is whole eights
     }
 };
 
-// acc[i][j][e] is (r, c) = (32 * j + lane % 32, 32 * i + 8 * (e / 4) + 4 * (lane / 32) + e % 4) of the wave's part.
 // Tile: its rows and columns, the waves that share them, the slab's depth and how many slabs LDS holds.
 template <int BR_, int BC_, int WR_, int WC_, int BK_, int STAGES_>
 struct Tile {
@@ -381,34 +414,45 @@ __global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs g, 
             await_loads<0>();  // LDS is the epilogue's now
         }
     } else {
-        Staged<BR, BK, VMC, kThreads> sv;
-        Staged<BC, BK, UMC, kThreads> su;
+        // Two slabs of LDS and two in registers: a slab's loads are issued two
+        // slabs ahead and stored to LDS one ahead.
         if (kbeg < kend) {
-            sv.load(g.v, g.ldv, r0, g.rows, kbeg, kend);
-            su.load(g.u, g.ldu, c0, g.cols, kbeg, kend);
-            sv.store(lds);
-            su.store(lds + kV);
+            struct Slab {
+                Staged<BR, BK, VMC, kThreads> v;
+                Staged<BC, BK, UMC, kThreads> u;
+            };
+            auto load = [&](Slab &s, uint32_t k0) __attribute__((always_inline)) {
+                if (k0 >= kend) return;
+                s.v.load(g.v, g.ldv, r0, g.rows, k0, kend);
+                s.u.load(g.u, g.ldu, c0, g.cols, k0, kend);
+            };
+            auto store = [&](const Slab &s, uint32_t stage) __attribute__((always_inline)) {
+                s.v.store(lds + stage * kStage);
+                s.u.store(lds + stage * kStage + kV);
+            };
+            Slab a, b;
+            load(a, kbeg);
+            load(b, kbeg + BK);
+            store(a, 0);
             __syncthreads();
-            uint32_t stage = 0;
-#pragma unroll 1
-            for (uint32_t k0 = kbeg; k0 < kend; k0 += BK) {
-                const bool more = k0 + BK < kend;
-                if (more) {
-                    sv.load(g.v, g.ldv, r0, g.rows, k0 + BK, kend);
-                    su.load(g.u, g.ldu, c0, g.cols, k0 + BK, kend);
-                }
+            // Slab k0 is in LDS and the next one in `next`; the one after goes to `after`.
+            auto slab = [&](uint32_t k0, uint32_t stage, Slab &after, const Slab &next) __attribute__((always_inline)) {
+                load(after, k0 + 2 * BK);
+                __builtin_amdgcn_sched_barrier(0);
                 Fragments f;
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) {
                     read(f, stage, s);
                     multiply(f);
                 }
-                stage ^= 1;
-                if (more) {
-                    sv.store(lds + stage * kStage);
-                    su.store(lds + stage * kStage + kV);
-                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (k0 + BK < kend) store(next, stage ^ 1);
                 __syncthreads();
+            };
+#pragma unroll 1
+            for (uint32_t k0 = kbeg; k0 < kend; k0 += 2 * BK) {
+                slab(k0, 0, a, b);
+                if (k0 + BK < kend) slab(k0 + BK, 1, b, a);
             }
         }
     }
@@ -438,13 +482,10 @@ __global__ __launch_bounds__(kBlock) void join_kernel(ProductArgs g, Epi epi) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)s[i];
-    if (epi.whole() && c + 8 <= g.cols) {
-        epi.row(epi.columns(c), r, c, v);
-    } else {
+    float bias[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < g.cols) epi.put(r, c + i, v[i]);
-    }
+    for (int i = 0; i < 8; ++i) bias[i] = epi.bias(min(c + i, g.cols - 1));
+    epi.template put<false>(r, c, min(g.cols - c, 8u), bias, v);
 }
 
 }  // namespace

@@ -35,6 +35,7 @@ constexpr uint32_t kComputeUnits = 256;
 // ranges of k_chunk. br 0: the kernel for few rows.
 struct ProductPlan {
     uint32_t br, bc, wr, wc, splits, k_chunk;
+    bool direct;  // operands straight to LDS
     bool skinny() const { return br == 0; }
     uint64_t partial_bytes(uint64_t rows, uint64_t cols) const {
         return splits > 1 ? padded(4 * (uint64_t)splits * rows * round_up(cols, 8)) : 0;
@@ -44,17 +45,25 @@ struct ProductPlan {
     uint64_t column_parts(uint64_t rows) const { return skinny() ? rows : (uint64_t)div_up(rows, br) * wr; }
 };
 
-// nt: both operands with k contiguous. The least time over the kinds of tile and
+// Whether an operand's rows start on 16-byte boundaries and are within the
+// loads' 32-bit offsets of each other. (Rows longer than k end in zeros, all of
+// them the workspace's.)
+inline bool direct_ok(const void *p, uint64_t ld) { return aligned16(p) && ld % 8 == 0 && ld < (1u << 22); }
+inline bool operands_direct(const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu) { return direct_ok(v, ldv) && direct_ok(u, ldu); }
+
+// nt: both operands with k contiguous; direct: operands_direct. The least time over the kinds of tile and
 // the ways to cut K, each range at least four slabs long: rounds of the chip x
 // slabs x a slab's time; ranges add their partials' way out and back and the
 // launch that joins them.
-inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool nt, bool may_split) {
-    if (nt && rows <= kSkinnyRows) return {0, 0, 0, 0, 1, 0};
+inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool nt, bool may_split, bool direct) {
+    if (nt && few_rows(rows)) return {0, 0, 0, 0, 1, 0, false};
     const uint64_t slabs = (k + 63) / 64;
     constexpr uint32_t kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
     ProductPlan best{};
     float least = 1e30f;
     for (const TileKind &t : kTileKinds) {
+        if (!direct && t.br != t.bc) continue;  // the kernel that goes through registers has two kinds
+        if (!direct && t.br == 256) continue;
         const uint64_t tiles = (uint64_t)div_up(rows, t.br) * div_up(cols, t.bc), slots = (uint64_t)kComputeUnits * t.occupancy;
         for (const uint32_t want : kSplits) {
             const uint64_t chunk = std::max<uint64_t>((slabs + want - 1) / want, 1), splits = std::max<uint64_t>((slabs + chunk - 1) / chunk, 1);
@@ -66,32 +75,78 @@ inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool n
             if (splits > 1) us += 3.0f + 8e-6f * (float)(splits * rows * cols) / 4.0f;
             if (us < least) {
                 least = us;
-                best = {t.br, t.bc, t.wr, t.wc, (uint32_t)splits, (uint32_t)(chunk * 64)};
+                best = {t.br, t.bc, t.wr, t.wc, (uint32_t)splits, (uint32_t)(chunk * 64), direct};
             }
         }
     }
     return best;
 }
 
-// Whether an operand's rows start on 16-byte boundaries and are within the
-// loads' 32-bit offsets of each other. A k-contiguous one is whole chunks long
-// (`k` of them, or zeros to the end of the last).
-template <bool MC>
-inline bool direct_ok(const void *p, uint64_t ld, uint64_t k, bool zeros) {
-    return aligned16(p) && ld % 8 == 0 && ld < (1u << 22) && (MC || k % 8 == 0 || zeros);
+// ---- rows that are no whole chunks ----
+//
+// Matrices with k contiguous and k % 8 != 0 are copied to the workspace in rows
+// of whole chunks that end in zeros, for the products that read them once a
+// tile: 777x1001x2503 takes ... us by copies, 86 us through registers, where
+// loads at odd elements and the shifts at rows' ends hold up the products.
+
+inline uint64_t packed_ld(uint64_t k) { return round_up(k, 8); }
+inline uint64_t packed_bytes(uint64_t rows, uint64_t k) { return k % 8 == 0 ? 0 : padded(2 * rows * packed_ld(k)); }
+
+// A thread a chunk of the copies of a (rows_a) and b (rows_b).
+__global__ __launch_bounds__(kBlock) void pack_kernel(const __bf16 *a, uint32_t rows_a, __bf16 *to_a, const __bf16 *b, uint32_t rows_b,
+                                                     __bf16 *to_b, uint32_t k, FastDiv chunks) {
+    uint32_t at = blockIdx.x * kBlock + threadIdx.x;
+    const uint32_t end_a = rows_a * chunks.d;
+    if (at >= end_a + rows_b * chunks.d) return;
+    const __bf16 *from = at < end_a ? a : b;
+    __bf16 *to = at < end_a ? to_a : to_b;
+    at -= at < end_a ? 0 : end_a;
+    const uint32_t row = fdiv(at, chunks), c = (at - row * chunks.d) * 8;
+    const short *p = reinterpret_cast<const short *>(from) + (uint64_t)row * k + c;
+    s16x8 v = {};
+    if (c + 8 <= k) {
+        v = load_shifted(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (c + i < k) v[i] = p[i];
+    }
+    reinterpret_cast<s16x8 *>(to)[at] = v;
 }
 
-template <class T, bool VMC, bool UMC, class Epi>
-int launch_product(const char *name, dim3 grid, bool aligned, const ProductArgs &g, const Epi &epi) {
-    const dim3 block(T::kThreads);
-    if (aligned) return launch(name, product_kernel<T, VMC, UMC, true, Epi>, grid, block, g, epi);
-    return launch(name, product_kernel<T, VMC, UMC, false, Epi>, grid, block, g, epi);
+// A matrix as the products take it.
+struct Matrix {
+    const __bf16 *p;
+    uint64_t ld;
+};
+
+// Copies a and b (null: left out) to the workspace where their rows are no whole chunks.
+inline int pack(Matrix &a, uint64_t rows_a, Matrix &b, uint64_t rows_b, uint64_t k, Workspace &ws) {
+    if (k % 8 == 0) return 0;
+    const uint64_t ld = packed_ld(k), na = a.p != nullptr ? rows_a : 0, nb = b.p != nullptr ? rows_b : 0;
+    __bf16 *to_a = ws.take<__bf16>(packed_bytes(rows_a, k) / 2), *to_b = ws.take<__bf16>(packed_bytes(rows_b, k) / 2);
+    const uint64_t chunks = (na + nb) * (ld / 8);
+    if (chunks != 0)
+        DKZ_TRY(launch("pack", pack_kernel, dim3(div_up(chunks, kBlock)), dim3(kBlock), a.p, (uint32_t)na, to_a, b.p, (uint32_t)nb, to_b,
+                       (uint32_t)k, make_fastdiv((uint32_t)(ld / 8))));
+    if (na) a = {to_a, ld};
+    if (nb) b = {to_b, ld};
+    return 0;
 }
 
-// zeros: rows of v end in zeros up to a whole chunk. `partial` has the plan's partial_bytes.
+// A size that a workspace is planned by, whatever the alignment of the operands.
+template <class F>
+inline uint64_t most_of_plans(uint64_t rows, uint64_t cols, uint64_t k, bool nt, bool may_split, F f) {
+    return std::max<uint64_t>(f(plan_product(rows, cols, k, nt, may_split, true)), f(plan_product(rows, cols, k, nt, may_split, false)));
+}
+inline uint64_t most_partial_bytes(uint64_t rows, uint64_t cols, uint64_t k, bool nt) {
+    return most_of_plans(rows, cols, k, nt, true, [&](const ProductPlan &p) { return p.partial_bytes(rows, cols); });
+}
+
+// `partial` has the plan's partial_bytes.
 template <bool VMC, bool UMC, class Epi>
 int run_product(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu, uint64_t rows, uint64_t cols,
-                uint64_t k, const ProductPlan &p, float *partial, const Epi &epi, bool zeros = false) {
+                uint64_t k, const ProductPlan &p, float *partial, const Epi &epi) {
     if (rows == 0 || cols == 0) return 0;
     if constexpr (!VMC && !UMC)
         if (p.skinny()) return run_skinny(name, v, ldv, u, ldu, rows, cols, k, epi);
@@ -99,12 +154,19 @@ int run_product(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u
                   div_up(cols, p.bc), p.splits, p.k_chunk, partial, (uint32_t)round_up(cols, 8)};
     const uint64_t groups = (uint64_t)g.tiles_r * g.tiles_c * g.splits;
     DKZ_REQUIRE(groups <= 0x7fffffffull);
-    const dim3 grid((uint32_t)groups);
-    const bool aligned = direct_ok<VMC>(v, ldv, k, zeros) && direct_ok<UMC>(u, ldu, k, false);
-    if (p.br == 256) DKZ_TRY((launch_product<Tile256, VMC, UMC>(name, grid, aligned, g, epi)));
-    else if (p.br == 128) DKZ_TRY((launch_product<Tile128, VMC, UMC>(name, grid, aligned, g, epi)));
-    else if (p.bc == 128) DKZ_TRY((launch_product<Tile64x128, VMC, UMC>(name, grid, aligned, g, epi)));
-    else DKZ_TRY((launch_product<Tile64, VMC, UMC>(name, grid, aligned, g, epi)));
+    const dim3 grid((uint32_t)groups), four(256);
+    if (!p.direct) {
+        if (p.br == 128) DKZ_TRY(launch(name, product_kernel<Tile128, VMC, UMC, false, Epi>, grid, four, g, epi));
+        else DKZ_TRY(launch(name, product_kernel<Tile64, VMC, UMC, false, Epi>, grid, four, g, epi));
+    } else if (p.br == 256) {
+        DKZ_TRY(launch(name, product_kernel<Tile256, VMC, UMC, true, Epi>, grid, dim3(Tile256::kThreads), g, epi));
+    } else if (p.br == 128) {
+        DKZ_TRY(launch(name, product_kernel<Tile128, VMC, UMC, true, Epi>, grid, four, g, epi));
+    } else if (p.bc == 128) {
+        DKZ_TRY(launch(name, product_kernel<Tile64x128, VMC, UMC, true, Epi>, grid, four, g, epi));
+    } else {
+        DKZ_TRY(launch(name, product_kernel<Tile64, VMC, UMC, true, Epi>, grid, four, g, epi));
+    }
     if constexpr (Epi::kElementwise)
         if (g.splits > 1)
             return launch(name, join_kernel<Epi>, dim3(div_up((uint64_t)g.rows * (g.ldp / 8), kBlock)), dim3(kBlock), g, epi);

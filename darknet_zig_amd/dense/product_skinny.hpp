@@ -3,8 +3,7 @@
 // the weights' way from memory.
 //
 // A workgroup takes 16 * CT columns and all rows, its waves a share of K each:
-// no LDS on the way, a lane loads eight k of a weight row (16 bytes at any
-// alignment) straight into an operand of v_mfma_f32_16x16x32_bf16 and eight of
+// no LDS on the way, a lane loads eight k of a weight row straight into an operand of v_mfma_f32_16x16x32_bf16 and eight of
 // an input row, which the caches hold, into the other. Each wave keeps two
 // steps of 64 k in flight beside the one it multiplies. The waves' sums meet in
 // LDS in wave order, and the epilogue takes them from there.
@@ -16,13 +15,16 @@
 namespace dkz {
 namespace {
 
+typedef short s16x8w __attribute__((ext_vector_type(8), aligned(4)));
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kSkinnyRows = 64;  // rows at most
+// Rows at most.
+constexpr uint32_t kSkinnyRows = 64;
+inline bool few_rows(uint64_t rows) { return rows <= kSkinnyRows; }
 
-template <int RT, int CT, int WAVES, bool UMC, class Epi>
+// ODD: rows may start inside a 4-byte word.
+template <int RT, int CT, int WAVES, bool ODD, class Epi>
 __global__ __launch_bounds__(64 * WAVES) void skinny_kernel(ProductArgs g, Epi epi) {
-    static_assert(!UMC, "weights with k contiguous");
     constexpr int kCols = 16 * CT, kRows = 16 * RT, kPitch = kCols + 4;
     __shared__ __align__(16) float sums[WAVES][kRows][kPitch];
     // In a scalar, so that what depends on it is a branch: matrix instructions take no notice of masked lanes.
@@ -46,14 +48,18 @@ __global__ __launch_bounds__(64 * WAVES) void skinny_kernel(ProductArgs g, Epi e
     struct Step {
         s16x8 u[CT][2], v[RT][2];
     };
+    auto eight = [&](const short *p) __attribute__((always_inline)) {
+        if constexpr (ODD) return load_shifted(p);
+        else return (s16x8)*reinterpret_cast<const s16x8w *>(p);
+    };
     auto load = [&](Step &s, uint32_t step) __attribute__((always_inline)) {
         const uint32_t k = step * 64;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int i = 0; i < CT; ++i) s.u[i][h] = *reinterpret_cast<const s16x8u *>(pu[i] + k + 8 * h);
+            for (int i = 0; i < CT; ++i) s.u[i][h] = eight(pu[i] + k + 8 * h);
 #pragma unroll
-            for (int j = 0; j < RT; ++j) s.v[j][h] = *reinterpret_cast<const s16x8u *>(pv[j] + k + 8 * h);
+            for (int j = 0; j < RT; ++j) s.v[j][h] = eight(pv[j] + k + 8 * h);
         }
     };
     auto load_end = [&](Step &s, uint32_t step) __attribute__((always_inline)) {  // k past the end read as 0
@@ -120,6 +126,13 @@ __global__ __launch_bounds__(64 * WAVES) void skinny_kernel(ProductArgs g, Epi e
 // Columns of a workgroup: 32 where that fills the chip, else 16.
 inline uint32_t skinny_columns(uint64_t cols) { return cols >= 32 * 512 ? 32 : 16; }
 
+template <int RT, int CT, int WAVES, class Epi>
+int launch_skinny(const char *name, dim3 grid, const ProductArgs &g, const Epi &epi) {
+    const bool odd = ((g.ldv | g.ldu) & 1) != 0 || (((uintptr_t)g.v | (uintptr_t)g.u) & 3) != 0;
+    if (odd) return launch(name, skinny_kernel<RT, CT, WAVES, true, Epi>, grid, dim3(64 * WAVES), g, epi);
+    return launch(name, skinny_kernel<RT, CT, WAVES, false, Epi>, grid, dim3(64 * WAVES), g, epi);
+}
+
 template <class Epi>
 int run_skinny(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu, uint64_t rows, uint64_t cols, uint64_t k,
                const Epi &epi) {
@@ -134,13 +147,13 @@ int run_skinny(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u,
     const uint32_t width = skinny_columns(cols);
     const dim3 grid(div_up(cols, width));
     if (width == 32) {
-        if (rows <= 16) return launch(name, skinny_kernel<1, 2, 4, false, Epi>, grid, dim3(256), g, epi);
-        if (rows <= 32) return launch(name, skinny_kernel<2, 2, 4, false, Epi>, grid, dim3(256), g, epi);
-        return launch(name, skinny_kernel<4, 2, 4, false, Epi>, grid, dim3(256), g, epi);
+        if (rows <= 16) return launch_skinny<1, 2, 4>(name, grid, g, epi);
+        if (rows <= 32) return launch_skinny<2, 2, 4>(name, grid, g, epi);
+        return launch_skinny<4, 2, 4>(name, grid, g, epi);
     }
-    if (rows <= 16) return launch(name, skinny_kernel<1, 1, 8, false, Epi>, grid, dim3(512), g, epi);
-    if (rows <= 32) return launch(name, skinny_kernel<2, 1, 8, false, Epi>, grid, dim3(512), g, epi);
-    return launch(name, skinny_kernel<4, 1, 8, false, Epi>, grid, dim3(512), g, epi);
+    if (rows <= 16) return launch_skinny<1, 1, 8>(name, grid, g, epi);
+    if (rows <= 32) return launch_skinny<2, 1, 8>(name, grid, g, epi);
+    return launch_skinny<4, 1, 8>(name, grid, g, epi);
 }
 
 }  // namespace
