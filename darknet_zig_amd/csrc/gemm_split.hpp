@@ -603,8 +603,10 @@ constexpr int min_waves() { return BM * BN >= 128 * 128 ? 2 : BM * BN >= 128 * 6
 // registers; a 128x128 tile's would take 128), each a part of the g.tile_bm x
 // g.tile_bn tile whose pieces it adds up, or the 32x128 ones.
 //
-// Epi: none, and C is alpha * the product + beta * C; or one object, whose
-// put(row, col, value) takes every element of the product instead.
+// Epi: none, and C is alpha * the product + beta * C; or one object that takes
+// the product's elements instead: block(row, rows, col, v[16]) those of column
+// col that a lane holds of a 32x32 block (rows row + 8 * (x / 4) + x % 4), and
+// where partials are joined row(row, col, cols, v[N]) N of a row.
 template <int BM, int BN, Operand AK, Operand BK, bool ORDERED = false, class... Epi>
 __global__ __launch_bounds__(kBlock, (min_waves<BM, BN>() - (ORDERED ? 2 : 0))) void gemm_split_kernel(SplitArgs g, Epi... epi) {
     constexpr int kRowsOfWaves = BM == 32 ? 1 : 2;  // 32-row tiles: four waves side by side
@@ -908,9 +910,10 @@ __global__ __launch_bounds__(kBlock, (min_waves<BM, BN>() - (ORDERED ? 2 : 0))) 
             float out[16];
             if constexpr (sizeof...(Epi) != 0) {
                 if (!part) {
+                    float v[16];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (row(r) < g.m) (epi.put(row(r), j, big[ti][tj][r]), ...);
+                    for (int r = 0; r < 16; ++r) v[r] = big[ti][tj][r];
+                    (epi.block(i0, g.m, j, v), ...);
                     continue;
                 }
             }
@@ -987,8 +990,10 @@ __global__ __launch_bounds__(kBlock) void split_reduce_kernel(SplitArgs g, Epi..
     if (!in) return;
     const uint32_t e = v * kW, i = e / g.n, j = e - i * g.n;
     if constexpr (sizeof...(Epi) != 0) {
+        float out[kW];
 #pragma unroll
-        for (uint32_t x = 0; x < kW; ++x) (epi.put(i, j + x, (float)s[x]), ...);
+        for (uint32_t x = 0; x < kW; ++x) out[x] = (float)s[x];
+        (epi.row(i, j, g.n, out), ...);
         return;
     }
     float *cp = c_column(g.c, j, g, 0, 0) + (size_t)i * g.ldc;
@@ -1026,9 +1031,10 @@ __global__ __launch_bounds__(kBlock) void stream_reduce_kernel(SplitArgs g, Epi.
             for (int x = 0; x < 4; ++x) s[x] += b + u <= last ? (double)::dkz::lane(p[u], x) : 0.0;
     }
     if constexpr (sizeof...(Epi) != 0) {
+        float out[4];
 #pragma unroll
-        for (uint32_t x = 0; x < 4; ++x)
-            if (j + x < g.n) (epi.put(i, j + x, (float)s[x]), ...);
+        for (uint32_t x = 0; x < 4; ++x) out[x] = (float)s[x];
+        (epi.row(i, j, g.n, out), ...);
         return;
     }
     if constexpr (V4) {

@@ -57,34 +57,51 @@ struct StatEpilogue {
     template <int TR, int TC, int WR, int WC>
     __device__ __forceinline__ void tile(f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
                                          uint32_t rows, uint32_t cols, uint32_t, uint32_t tc, char *) const {
-        const uint32_t lane = threadIdx.x & 63, wave_c = (threadIdx.x >> 6) % WC;
-        const uint32_t cl = c0 + wc0 + 4 * (lane >> 5);
-#pragma unroll
-        for (int j = 0; j < TR; ++j) {
-            const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
-            const uint32_t t = r < rows ? (uint32_t)targets[r] : ~0u;
-            float m = neg_inf();
+        constexpr uint32_t kCols = TC * 32;
+        const uint32_t lane = threadIdx.x & 63, wave_c = (threadIdx.x >> 6) % WC, first = c0 + wc0;
+        const uint32_t cl = first + 4 * (lane >> 5);  // this lane's columns: cl + 8 * n + 0 .. 3
+        const auto column = [](int i, int e) { return (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3)); };
+        const bool edge = first + kCols > cols;
+        // Bias and edge first: a wave's usual part, inside and without a bias, is left alone.
+        if (biases != nullptr || edge) {
 #pragma unroll
             for (int i = 0; i < TC; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const uint32_t c = cl + 32 * i + 8 * (e >> 2) + (e & 3);
-                    float z = acc[i][j][e];
-                    if (biases != nullptr && c < cols) z += biases[c];
-                    if (c >= cols) z = neg_inf();
-                    else if (c == t) target_logit[r] = z;
-                    acc[i][j][e] = z;
-                    m = fmaxf(m, z);
+                    const uint32_t c = cl + column(i, e);
+                    const float b = c >= cols ? neg_inf() : biases != nullptr ? biases[c] : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < TR; ++j) acc[i][j][e] = c < cols ? acc[i][j][e] + b : neg_inf();
                 }
-            m = fmaxf(m, __shfl_xor(m, 32));
-            const float base = m == neg_inf() ? 0.0f : m;
-            float s = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < TR; ++j) {
+            const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
+            float m = neg_inf();
 #pragma unroll
             for (int i = 0; i < TC; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s += exp_fast(acc[i][j][e] - base);
-            s += __shfl_xor(s, 32);
-            if (r < rows && lane < 32) stats[(uint64_t)r * parts + tc * WC + wave_c] = {m, s};
+                for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float base = m == neg_inf() ? 0.0f : m;
+            float s[2] = {};
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e & 1] += exp_fast(acc[i][j][e] - base);
+            s[0] += s[1];
+            s[0] += __shfl_xor(s[0], 32);
+            if (r < rows && lane < 32) stats[(uint64_t)r * parts + tc * WC + wave_c] = {m, s[0]};
+            // The target's logit, where it is one of this wave's columns: seldom.
+            const uint32_t t = r < rows ? (uint32_t)targets[r] : ~0u, o = t - cl;
+            if (o < kCols && t < cols && (o & 4) == 0) {
+                float z = 0.0f;
+#pragma unroll
+                for (int i = 0; i < TC; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) z = o == column(i, e) ? acc[i][j][e] : z;
+                target_logit[r] = z;
+            }
         }
     }
     // Few rows: COLS lanes hold a row's part.
@@ -164,9 +181,13 @@ struct GradientEpilogue {
         const uint32_t c = c0 + wc0 + lane % kLanes * 8;
         float bias[8], sum[8] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) bias[i] = c + i >= cols ? neg_inf() : biases != nullptr ? biases[c + i] : 0.0f;
+        for (int i = 0; i < 8; ++i) bias[i] = biases != nullptr ? biases[min(c + i, cols - 1)] : 0.0f;
 #pragma unroll
         for (int j = 0; j < TR; ++j) {
+            // Lane x has the values of row x of the 32.
+            uint32_t target_of = ~0u;
+            float s_of = 0.0f, l_of = 0.0f;
+            if (const uint32_t r = r0 + wr0 + 32 * j + (lane & 31); r < rows) rows_of.row(r, target_of, s_of, l_of);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -180,20 +201,18 @@ struct GradientEpilogue {
 #pragma unroll 2
             for (uint32_t x = lane / kLanes; x < 32; x += kStep) {
                 const uint32_t r = r0 + wr0 + 32 * j + x, at = x * (kCols / 4), chunk = lane % kLanes * 2;
-                if (r >= rows) break;
                 const float4 a = part[at + (chunk ^ (x & kMask))], b = part[at + ((chunk + 1) ^ (x & kMask))];
-                uint32_t target;
-                float s, l;
-                rows_of.row(r, target, s, l);
+                const uint32_t target = __shfl(target_of, x), hot = target - first - c;
+                const float s = __shfl(s_of, x), l = __shfl(l_of, x);
                 float v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    // A column past the last class: exp(-infinity), and no target. NaN logits stay in rows that have a gradient.
-                    const float p = c + i < cols ? exp_fast(::dkz::lane(i < 4 ? a : b, i & 3) + bias[i] - l) : 0.0f;
-                    v[i] = target == ~0u ? 0.0f : s * ((target == first + c + i ? 1.0f : 0.0f) - p);
+                    const float p = exp_fast(::dkz::lane(i < 4 ? a : b, i & 3) + bias[i] - l);
+                    // NaN logits stay in rows that have a gradient, those past the last class out of it.
+                    v[i] = target == ~0u || c + i >= cols ? 0.0f : s * ((hot == (uint32_t)i ? 1.0f : 0.0f) - p);
                     sum[i] += v[i];
                 }
-                if (c < ldd) store8(d, (uint64_t)r * ldd + c, v);
+                if (r < rows && c < ldd) store8(d, (uint64_t)r * ldd + c, v);
             }
         }
         if (sums == nullptr) return;
@@ -224,34 +243,52 @@ struct GradientEpilogue {
 // ---- fp32 ----
 
 // Logits with their bias, to the workspace.
-struct LogitEpilogue {
+struct LogitEpilogue : TileEpilogue<LogitEpilogue> {
     const float *biases;
     float *out;
     uint32_t ld;
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
-        out[(uint64_t)r * ld + c] = biases != nullptr ? z + biases[c] : z;
+    LogitEpilogue(const float *biases, float *out, uint64_t ld) : biases(biases), out(out), ld((uint32_t)ld) {}
+    __device__ __forceinline__ float bias(uint32_t c) const { return biases != nullptr ? biases[c] : 0.0f; }
+    template <class E, int N>
+    __device__ __forceinline__ void put(const E &e, const float (&bias)[N], float (&z)[N]) const {
+        if (biases != nullptr) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) z[i] += bias[i];
+        }
+        store_n(out, e, z);
     }
 };
 
-// A workgroup a row: the pair of a piece's logits merged into the row's; the last piece finishes the row.
-__global__ __launch_bounds__(kBlock) void row_stats_kernel(const float *z, uint32_t ld, uint32_t cols, uint32_t first, uint32_t classes,
-                                                          const int *targets, Stat *run, float *target_logit, float *loss,
-                                                          float *lse) {
-    __shared__ Stat waves[kBlock / kWave];
+constexpr uint32_t kStatThreads = 512, kStatEach = 8;
+
+// A workgroup a row: the pair of a piece's logits, in one pass with the running
+// maximum, merged into the row's; the last piece finishes the row. A thread
+// takes eight logits at a time, a workgroup's width apart.
+__global__ __launch_bounds__(kStatThreads) void row_stats_kernel(const float *z, uint32_t ld, uint32_t cols, uint32_t first, uint32_t classes,
+                                                                const int *targets, Stat *run, float *target_logit, float *loss,
+                                                                float *lse) {
+    __shared__ Stat waves[kStatThreads / kWave];
     const uint32_t r = blockIdx.x;
     const float *row = z + (uint64_t)r * ld;
-    float m = neg_inf();
-    for (uint32_t c = threadIdx.x; c < cols; c += kBlock) m = fmaxf(m, row[c]);
-    const float base = m == neg_inf() ? 0.0f : m;
-    float s = 0.0f;
-    for (uint32_t c = threadIdx.x; c < cols; c += kBlock) s += expf_cw(row[c] - base);
-    Stat t{m, s};
+    Stat t{neg_inf(), 0.0f};
+    for (uint32_t c = threadIdx.x; c < cols; c += kStatEach * kStatThreads) {
+        float v[kStatEach], m = t.m;
+#pragma unroll
+        for (uint32_t i = 0; i < kStatEach; ++i) v[i] = row[min(c + i * kStatThreads, cols - 1)];
+#pragma unroll
+        for (uint32_t i = 0; i < kStatEach; ++i) m = fmaxf(m, v[i]);
+        const float base = m == neg_inf() ? 0.0f : m;
+        t.s *= expf_cw(t.m - base);
+#pragma unroll
+        for (uint32_t i = 0; i < kStatEach; ++i) t.s += c + i * kStatThreads < cols ? expf_cw(v[i] - base) : 0.0f;
+        t.m = m;
+    }
 #pragma unroll
     for (int x = 1; x < kWave; x *= 2) t = merge(t, {__shfl_xor(t.m, x), __shfl_xor(t.s, x)});
     if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = t;
     __syncthreads();
     if (threadIdx.x != 0) return;
-    for (int w = 1; w < kBlock / kWave; ++w) t = merge(t, waves[w]);
+    for (uint32_t w = 1; w < kStatThreads / kWave; ++w) t = merge(t, waves[w]);
     if (first != 0) t = merge(run[r], t);
     const uint32_t target = (uint32_t)targets[r];
     if (target - first < cols) target_logit[r] = row[target - first];
@@ -261,23 +298,49 @@ __global__ __launch_bounds__(kBlock) void row_stats_kernel(const float *z, uint3
 
 constexpr uint32_t kGradRows = 64;  // rows a workgroup of logit_gradient_kernel takes
 
-// A piece's logits become d; a thread a column, and its sum of kGradRows rows to `sums`.
+// A piece's logits become d, and the sums of kGradRows rows' columns go to
+// `sums` (null: not). A thread takes four columns of eight rows, its loads
+// issued before the first is used; a column's eight threads are added in row
+// order. Rows are ld logits long, a multiple of four.
 __global__ __launch_bounds__(kBlock) void logit_gradient_kernel(float *z, uint32_t ld, uint32_t rows, uint32_t cols, uint32_t first,
                                                                RowGradient rows_of, float *sums) {
-    const uint32_t c = blockIdx.x * kBlock + threadIdx.x, r0 = blockIdx.y * kGradRows;
-    if (c >= cols) return;
-    float sum = 0.0f;
-    for (uint32_t r = r0; r < min(r0 + kGradRows, rows); ++r) {
-        uint32_t target;
-        float s, l;
-        rows_of.row(r, target, s, l);
-        float *at = z + (uint64_t)r * ld + c;
-        const float p = expf_cw(*at - l);
-        const float g = target == ~0u ? 0.0f : s * ((target == first + c ? 1.0f : 0.0f) - p);
-        *at = g;
-        sum += g;
+    constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes, kEach = kGradRows / kGroups;
+    __shared__ float part[kGroups][kLanes * 4 + 4];
+    const uint32_t x = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const uint32_t c = (blockIdx.x * kLanes + x) * 4, r0 = blockIdx.y * kGradRows + group * kEach;
+    float4 v[kEach];
+    uint32_t target[kEach];
+    float s[kEach], l[kEach], sum[4] = {};
+    if (c < ld) {
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t r = min(r0 + i, rows - 1);
+            v[i] = *reinterpret_cast<const float4 *>(z + (uint64_t)r * ld + c);
+            rows_of.row(r, target[i], s[i], l[i]);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            if (r0 + i >= rows) break;
+#pragma unroll
+            for (uint32_t w = 0; w < 4; ++w) {
+                float &g = ::dkz::lane(v[i], w);
+                const float p = expf_cw(g - l[i]);
+                g = target[i] == ~0u || c + w >= cols ? 0.0f : s[i] * ((target[i] == first + c + w ? 1.0f : 0.0f) - p);
+                sum[w] += g;
+            }
+            *reinterpret_cast<float4 *>(z + (uint64_t)(r0 + i) * ld + c) = v[i];
+        }
     }
-    if (sums != nullptr) sums[(uint64_t)blockIdx.y * cols + c] = sum;
+    if (sums == nullptr) return;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) part[group][x * 4 + w] = sum[w];
+    __syncthreads();
+    if (threadIdx.x >= kLanes * 4) return;
+    float t = part[0][threadIdx.x];
+#pragma unroll
+    for (uint32_t i = 1; i < kGroups; ++i) t += part[i][threadIdx.x];
+    const uint32_t column = blockIdx.x * kLanes * 4 + threadIdx.x;
+    if (column < cols) sums[(uint64_t)blockIdx.y * cols + column] = t;
 }
 
 // Rows whose classes are none: lse -infinity, no target, no loss.
@@ -376,17 +439,16 @@ struct PieceEpilogue : TileEpilogue<PieceEpilogue> {
     bool begin, words;
     __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
     __device__ __forceinline__ bool in_words() const { return words; }
-    template <bool STEP_ROW, int N>
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, uint32_t n, const float (&)[N], float (&z)[N]) const {
-        const uint64_t at = (uint64_t)r * ld + c, step = STEP_ROW ? ld : 1;
+    template <class E, int N>
+    __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N]) const {
         if (!begin) {
             float o[N];
-            load_n(sum, at, step, n, o);
+            load_n(sum, e, o);
 #pragma unroll
             for (int i = 0; i < N; ++i) z[i] += o[i];
         }
-        if (out != nullptr) store_n(out, at, step, n, z);
-        else store_n(sum, at, step, n, z);
+        if (out != nullptr) store_n(out, e, z);
+        else store_n(sum, e, z);
     }
 };
 
@@ -409,12 +471,12 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const vo
     }
     float *logits = ws.take<float>(plan.logits / 4), *partial = ws.take<float>(plan.partial / 4);
     for (uint64_t first = 0; first < classes; first += plan.piece) {
-        const uint64_t n = std::min(plan.piece, classes - first);
-        const LogitEpilogue epi{biases != nullptr ? biases + first : nullptr, logits, (uint32_t)n};
+        const uint64_t n = std::min(plan.piece, classes - first), ld = round_up(n, 4);
+        const LogitEpilogue epi(biases != nullptr ? biases + first : nullptr, logits, ld);
         DKZ_TRY((run_f32<kRowMajor, kRowMajor>(kName, static_cast<const float *>(input), inputs,
-                                               static_cast<const float *>(weights) + first * inputs, inputs, 0.0f, (float *)nullptr, n,
+                                               static_cast<const float *>(weights) + first * inputs, inputs, 0.0f, (float *)nullptr, ld,
                                                rows, n, inputs, partial, epi)));
-        DKZ_TRY(launch("linear_cross_entropy_stats", row_stats_kernel, dim3((uint32_t)rows), dim3(kBlock), logits, (uint32_t)n, (uint32_t)n,
+        DKZ_TRY(launch("linear_cross_entropy_stats", row_stats_kernel, dim3((uint32_t)rows), dim3(kStatThreads), logits, (uint32_t)ld, (uint32_t)n,
                        (uint32_t)first, (uint32_t)classes, targets, stats, target_logit, loss, lse));
     }
     return 0;
@@ -427,21 +489,21 @@ int backward_f32(uint64_t rows, uint64_t inputs, uint64_t classes, const float *
                  const BackwardPlan &plan, Workspace ws) {
     float *d = ws.take<float>(plan.d / 4), *sums = ws.take<float>(plan.sums / 4), *partial = ws.take<float>(plan.partial / 4);
     for (uint64_t first = 0; first < classes; first += plan.piece) {
-        const uint64_t n = std::min(plan.piece, classes - first), chunks = div_up(rows, kGradRows);
+        const uint64_t n = std::min(plan.piece, classes - first), ld = round_up(n, 4), chunks = div_up(rows, kGradRows);
         const float *w = weights + first * inputs;
         if (rows != 0) {
-            const LogitEpilogue epi{biases != nullptr ? biases + first : nullptr, d, (uint32_t)n};
-            DKZ_TRY((run_f32<kRowMajor, kRowMajor>("linear_cross_entropy_logits", input, inputs, w, inputs, 0.0f, (float *)nullptr, n, rows,
+            const LogitEpilogue epi(biases != nullptr ? biases + first : nullptr, d, ld);
+            DKZ_TRY((run_f32<kRowMajor, kRowMajor>("linear_cross_entropy_logits", input, inputs, w, inputs, 0.0f, (float *)nullptr, ld, rows,
                                                    n, inputs, partial, epi)));
-            DKZ_TRY(launch("linear_cross_entropy_gradient", logit_gradient_kernel, dim3(div_up(n, kBlock), (uint32_t)chunks), dim3(kBlock),
-                           d, (uint32_t)n, (uint32_t)rows, (uint32_t)n, (uint32_t)first, grad, bias_updates != nullptr ? sums : nullptr));
+            DKZ_TRY(launch("linear_cross_entropy_gradient", logit_gradient_kernel, dim3(div_up(ld, 128), (uint32_t)chunks), dim3(kBlock),
+                           d, (uint32_t)ld, (uint32_t)rows, (uint32_t)n, (uint32_t)first, grad, bias_updates != nullptr ? sums : nullptr));
         }
         if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
         if (weight_updates != nullptr)
-            DKZ_TRY((run_f32<kColMajor, kColMajor>(kWeights, d, n, input, inputs, beta, weight_updates + first * inputs, inputs, n, inputs,
+            DKZ_TRY((run_f32<kColMajor, kColMajor>(kWeights, d, ld, input, inputs, beta, weight_updates + first * inputs, inputs, n, inputs,
                                                    rows, partial)));
         if (input_delta != nullptr)
-            DKZ_TRY((run_f32<kRowMajor, kColMajor>(kInput, d, n, w, inputs, first == 0 ? 0.0f : 1.0f, input_delta, inputs, rows, inputs, n,
+            DKZ_TRY((run_f32<kRowMajor, kColMajor>(kInput, d, ld, w, inputs, first == 0 ? 0.0f : 1.0f, input_delta, inputs, rows, inputs, n,
                                                    partial)));
     }
     return 0;

@@ -55,29 +55,54 @@ __device__ __forceinline__ void store8(T *p, uint64_t i, const float (&v)[8]) {
     }
 }
 
-// N elements from p[i] on, `step` apart (N == 8 and step 1: eight at once), of which the first n exist.
-template <class T, int N>
-__device__ __forceinline__ void load_n(const T *p, uint64_t i, uint64_t step, uint32_t n, float (&v)[N]) {
-    if constexpr (N == 8) {
-        if (step == 1 && n == 8) {
-            load8(p, i, v);
+// ---- the elements of a matrix that a thread treats together: N of them, element
+// x at index at(x), there if in(x) ----
+
+struct RowRun {  // of one row, next to each other
+    uint64_t first;
+    uint32_t n;
+    static constexpr bool kRow = true;
+    __device__ __forceinline__ uint64_t at(int x) const { return first + x; }
+    __device__ __forceinline__ bool in(int x) const { return x < (int)n; }
+};
+struct ColumnRun {  // of one column, in rows next to each other
+    uint64_t first;
+    uint32_t ld, n;
+    static constexpr bool kRow = false;
+    __device__ __forceinline__ uint64_t at(int x) const { return first + (uint64_t)x * ld; }
+    __device__ __forceinline__ bool in(int x) const { return x < (int)n; }
+};
+struct BlockColumn {  // of one column, in the rows of a 32x32 block that one lane holds: four, every eight
+    uint64_t first;
+    uint32_t ld, n;  // n: rows from the first on that exist
+    static constexpr bool kRow = false;
+    static __device__ __forceinline__ int row(int x) { return (x >> 2) * 8 + (x & 3); }
+    __device__ __forceinline__ uint64_t at(int x) const { return first + (uint64_t)row(x) * ld; }
+    __device__ __forceinline__ bool in(int x) const { return row(x) < (int)n; }
+};
+
+template <class T, class E, int N>
+__device__ __forceinline__ void load_n(const T *p, const E &e, float (&v)[N]) {
+    if constexpr (E::kRow && N == 8) {
+        if (e.n == 8) {
+            load8(p, e.first, v);
             return;
         }
     }
 #pragma unroll
-    for (int x = 0; x < N; ++x) v[x] = x < (int)n ? load1(p, i + x * step) : 0.0f;
+    for (int x = 0; x < N; ++x) v[x] = e.in(x) ? load1(p, e.at(x)) : 0.0f;
 }
-template <class T, int N>
-__device__ __forceinline__ void store_n(T *p, uint64_t i, uint64_t step, uint32_t n, const float (&v)[N]) {
-    if constexpr (N == 8) {
-        if (step == 1 && n == 8) {
-            store8(p, i, v);
+template <class T, class E, int N>
+__device__ __forceinline__ void store_n(T *p, const E &e, const float (&v)[N]) {
+    if constexpr (E::kRow && N == 8) {
+        if (e.n == 8) {
+            store8(p, e.first, v);
             return;
         }
     }
 #pragma unroll
     for (int x = 0; x < N; ++x)
-        if (x < (int)n) store1(p, i + x * step, v[x]);
+        if (e.in(x)) store1(p, e.at(x), v[x]);
 }
 
 inline bool type_ok(int type) { return type == DKZ_F32 || type == DKZ_BF16; }
@@ -136,19 +161,18 @@ struct Draws {
         v *= scale;
         return limit != 0 && dropped(i) ? 0.0f : v;
     }
-    // Elements i, i + step, ..
-    template <int N>
-    __device__ __forceinline__ void apply(float (&v)[N], uint64_t i, uint64_t step) const {
-        if (step == 1) {
-            apply(v, i);
+    template <class E, int N>
+    __device__ __forceinline__ void apply(float (&v)[N], const E &e) const {
+        if constexpr (E::kRow) {
+            run(v, e.first);
         } else {
 #pragma unroll
-            for (int x = 0; x < N; ++x) v[x] = apply(v[x], i + x * step);
+            for (int x = 0; x < N; ++x) v[x] = apply(v[x], e.at(x));
         }
     }
     // Elements i .. i + N - 1.
     template <int N>
-    __device__ __forceinline__ void apply(float (&v)[N], uint64_t i) const {
+    __device__ __forceinline__ void run(float (&v)[N], uint64_t i) const {
 #pragma unroll
         for (int x = 0; x < N; ++x) v[x] *= scale;
         if (limit == 0) return;

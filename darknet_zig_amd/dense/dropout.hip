@@ -38,7 +38,7 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(const X *x, const Y *re
             for (uint32_t e = i; e < n; ++e) one(x, residual, y, e, draws);
             break;
         }
-        draws.apply(v[u], i);
+        draws.run(v[u], i);
         if (residual != nullptr) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[u][e] += add[u][e];

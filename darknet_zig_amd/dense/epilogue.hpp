@@ -76,28 +76,22 @@ struct LinearEpilogue : TileEpilogue<LinearEpilogue<T, EXP>> {
 
     __device__ __forceinline__ float bias(uint32_t c) const { return biases != nullptr ? biases[c] : 0.0f; }
     __device__ __forceinline__ bool in_words() const { return words; }
-    template <bool STEP_ROW, int N>
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, uint32_t n, const float (&bias)[N], float (&a)[N]) const {
-        const uint64_t at = (uint64_t)r * ld + c, step = STEP_ROW ? ld : 1;
+    template <class E, int N>
+    __device__ __forceinline__ void put(const E &e, const float (&bias)[N], float (&a)[N]) const {
         float add[N] = {};
-        if (residual != nullptr) load_n(residual, at, step, n, add);
+        if (residual != nullptr) load_n(residual, e, add);
         if (biases != nullptr) {
 #pragma unroll
             for (int i = 0; i < N; ++i) a[i] += bias[i];
         }
         activate_all<T, EXP>(act, a);
-        if (activated != nullptr) store_n(activated, at, step, n, a);
-        draws.apply(a, at, step);
+        if (activated != nullptr) store_n(activated, e, a);
+        draws.apply(a, e);
         if (residual != nullptr) {
 #pragma unroll
             for (int i = 0; i < N; ++i) a[i] += add[i];
         }
-        store_n(output, at, step, n, a);
-    }
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
-        const float b[1] = {bias(c)};
-        float v[1] = {z};
-        put<true>(r, c, 1, b, v);
+        store_n(output, e, a);
     }
 };
 
@@ -112,26 +106,20 @@ struct StoreEpilogue : TileEpilogue<StoreEpilogue<T>> {
 
     __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
     __device__ __forceinline__ bool in_words() const { return words; }
-    template <bool STEP_ROW, int N>
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, uint32_t n, const float (&)[N], float (&z)[N]) const {
-        const uint64_t at = (uint64_t)r * ld + c, step = STEP_ROW ? ld : 1;
+    template <class E, int N>
+    __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N]) const {
         float x[N];
         if (beta != 0.0f) {
-            load_n(out, at, step, n, x);
+            load_n(out, e, x);
 #pragma unroll
             for (int i = 0; i < N; ++i) z[i] += beta * x[i];
         }
         if (add != nullptr) {
-            load_n(add, at, step, n, x);
+            load_n(add, e, x);
 #pragma unroll
             for (int i = 0; i < N; ++i) z[i] += x[i];
         }
-        store_n(out, at, step, n, z);
-    }
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, float z) const {
-        const float b[1] = {};
-        float v[1] = {z};
-        put<true>(r, c, 1, b, v);
+        store_n(out, e, z);
     }
 };
 

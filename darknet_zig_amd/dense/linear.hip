@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *
     for (uint32_t i = 0; i < kEach; ++i) {
         const uint32_t r = r0 + i;
         if (r >= rows) break;
-        draws.apply(v[i], (uint64_t)r * cols + c);
+        draws.run(v[i], (uint64_t)r * cols + c);
         if (act != kLinear) gradient_all(act, y[i], v[i]);
 #pragma unroll
         for (int w = 0; w < W; ++w) {

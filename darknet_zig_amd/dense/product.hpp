@@ -186,12 +186,10 @@ __device__ __forceinline__ void await_loads() {
 }
 
 // Epilogues that treat every element by itself derive from this and give
+//   ld                      the matrix's columns, and the step from row to row;
 //   bias(c)                 what is added to column c (0: nothing);
 //   in_words()              whether rows start on 4-byte boundaries;
-//   put<STEP_ROW>(r, c, n, bias, z)
-//                           elements z[0 .. n - 1] from (r, c) on, of one column
-//                           (STEP_ROW) or one row, their biases in bias[0 .. n - 1];
-//                           n a compile-time constant 8 or less in a variable.
+//   put(elements, bias, z)  takes z[x] for element x, its bias in bias[x].
 // A wave passes its part of the tile through LDS, 32 rows at a time: there a
 // lane wrote four columns of its row at once, here it takes eight of one of
 // four rows, so that rows are read and written in whole lines and the columns a
@@ -202,14 +200,33 @@ __device__ __forceinline__ void await_loads() {
 template <class Self>
 struct TileEpilogue {
     static constexpr bool kElementwise = true;  // the K of a product may be cut, and the pieces joined
+    __device__ __forceinline__ void one(uint32_t r, uint32_t c, float z) const {
+        const Self &self = *static_cast<const Self *>(this);
+        const float bias[1] = {self.bias(c)};
+        float v[1] = {z};
+        self.put(RowRun{(uint64_t)r * self.ld + c, 1}, bias, v);
+    }
+    // The fp32 kernel's: rows of a 32x32 block, and some of a row.
+    __device__ __forceinline__ void block(uint32_t r, uint32_t rows, uint32_t c, float (&z)[16]) const {
+        if (r >= rows) return;
+        const Self &self = *static_cast<const Self *>(this);
+        const float b = self.bias(c);
+        const float bias[16] = {b, b, b, b, b, b, b, b, b, b, b, b, b, b, b, b};
+        self.put(BlockColumn{(uint64_t)r * self.ld + c, self.ld, rows - r}, bias, z);
+    }
+    template <int N>
+    __device__ __forceinline__ void row(uint32_t r, uint32_t c, uint32_t cols, float (&z)[N]) const {
+        const Self &self = *static_cast<const Self *>(this);
+        float bias[N];
+#pragma unroll
+        for (int x = 0; x < N; ++x) bias[x] = self.bias(min(c + x, cols - 1));
+        self.put(RowRun{(uint64_t)r * self.ld + c, min(cols - c, (uint32_t)N)}, bias, z);
+    }
     // Few rows (product_skinny.hpp): one element, if it is there.
     template <int COLS>
     __device__ __forceinline__ void skinny(uint32_t r, uint32_t c, float z, uint32_t rows, uint32_t cols, uint32_t) const {
         if (r >= rows || c >= cols) return;
-        const Self &self = *static_cast<const Self *>(this);
-        const float bias[1] = {self.bias(c)};
-        float v[1] = {z};
-        self.template put<true>(r, c, 1, bias, v);
+        one(r, c, z);
     }
     template <int TR, int TC, int WR, int WC>
     __device__ __forceinline__ void tile(const f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
@@ -244,7 +261,7 @@ struct TileEpilogue {
                     const float4 a = part[at + (chunk ^ (x & kMask))], b = part[at + ((chunk + 1) ^ (x & kMask))];
                     float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
                     if (r >= rows) break;
-                    self.template put<false>(r, c, min(cols - c, 8u), bias, z);
+                    self.put(RowRun{(uint64_t)r * self.ld + c, min(cols - c, 8u)}, bias, z);
                 }
                 continue;
             }
@@ -263,7 +280,7 @@ struct TileEpilogue {
 #pragma unroll
                         for (uint32_t i = 0; i < 8; ++i)
                             z[i] = reinterpret_cast<const float *>(part)[((x + i) * (kCols / 4) + ((col / 4) ^ ((x + i) & kMask))) * 4 + col % 4];
-                        self.template put<true>(top + x, at, min(rows - top - x, 8u), bias, z);
+                        self.put(ColumnRun{(uint64_t)(top + x) * self.ld + at, self.ld, min(rows - top - x, 8u)}, bias, z);
                     }
             }
             if constexpr (kCols > kWave) {  // back to the first half's
@@ -281,9 +298,9 @@ struct PartialEpilogue : TileEpilogue<PartialEpilogue> {
     __device__ __forceinline__ PartialEpilogue(float *out, uint32_t ld) : out(out), ld(ld) {}
     __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
     __device__ __forceinline__ bool in_words() const { return true; }
-    template <bool STEP_ROW, int N>
-    __device__ __forceinline__ void put(uint32_t r, uint32_t c, uint32_t, const float (&)[N], float (&z)[N]) const {
-        store8(out, (uint64_t)r * ld + c, z);  // also past the last column: ld is whole eights
+    template <class E, int N>
+    __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N]) const {
+        if constexpr (N == 8) store8(out, e.first, z);  // also past the last column: ld is whole eights
     }
 };
 
@@ -482,10 +499,7 @@ __global__ __launch_bounds__(kBlock) void join_kernel(ProductArgs g, Epi epi) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)s[i];
-    float bias[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bias[i] = epi.bias(min(c + i, g.cols - 1));
-    epi.template put<false>(r, c, min(g.cols - c, 8u), bias, v);
+    epi.row(r, c, g.cols, v);
 }
 
 }  // namespace
