@@ -482,20 +482,39 @@ __global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs g, 
     epi.template tile<kTR, kTC, WR, WC>(acc, r0, c0, wr0, wc0, g.rows, g.cols, tr, tc, lds);
 }
 
-// The join of a split product: adds eight columns' partials in split order, in f64, and passes them to the epilogue.
-template <class Epi>
+// The join of a split product: adds eight columns' partials in f64 and passes
+// them to the epilogue. GROUPS threads share them, each taking every GROUPSth
+// split, and are added in order: one thread up to four splits, eight beyond
+// (5x368 of 24 splits 9.7 us with one).
+template <int GROUPS, class Epi>
 __global__ __launch_bounds__(kBlock) void join_kernel(ProductArgs g, Epi epi) {
-    const uint32_t eights = g.ldp / 8, e = blockIdx.x * kBlock + threadIdx.x;
-    if (e >= g.rows * eights) return;
+    constexpr uint32_t kItems = kBlock / GROUPS;
+    const uint32_t eights = g.ldp / 8, group = threadIdx.x / kItems, e = blockIdx.x * kItems + threadIdx.x % kItems;
+    const bool in = e < g.rows * eights;
     const uint32_t r = e / eights, c = (e - r * eights) * 8;
-    const float *from = g.partial + (uint64_t)r * g.ldp + c;
     double s[8] = {};
-    for (uint32_t p = 0; p < g.splits; ++p) {
-        const float4 *at = reinterpret_cast<const float4 *>(from + (uint64_t)p * g.rows * g.ldp);
-        const float4 x = at[0], y = at[1];
+    if (in) {
+        const float *from = g.partial + (uint64_t)r * g.ldp + c;
+#pragma unroll 4
+        for (uint32_t p = group; p < g.splits; p += GROUPS) {
+            const float4 *at = reinterpret_cast<const float4 *>(from + (uint64_t)p * g.rows * g.ldp);
+            const float4 x = at[0], y = at[1];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] += (double)lane(i < 4 ? x : y, i & 3);
+            for (int i = 0; i < 8; ++i) s[i] += (double)lane(i < 4 ? x : y, i & 3);
+        }
     }
+    if constexpr (GROUPS > 1) {
+        __shared__ double sums[GROUPS][8][kItems];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[group][i][threadIdx.x % kItems] = s[i];
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int p = 1; p < GROUPS; ++p)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += sums[p][i][threadIdx.x];
+    }
+    if (!in) return;
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)s[i];

@@ -20,15 +20,16 @@ typedef Tile<64, 64, 2, 2, 64, 3> Tile64;
 // units at work: measured over K 4096 at 4096^2 (256x256: 108 us), 1024x4096
 // (128x128: 36.5; two slabs in LDS and two a compute unit are 4 us slower),
 // 512x4096 and 1024x4096 (64x128: 24.5 and 41.6), 256x4096 .. 1024x4096 (64x64:
-// 19.0, 26.7, 51.6).
+// 19.0, 26.7, 51.6). `fixed`: a round's first loads and its stores.
 struct TileKind {
     uint32_t br, bc, wr, wc, occupancy;
     float slab[3], fixed;
 };
-constexpr TileKind kTileKinds[] = {{256, 256, 4, 2, 1, {1.62f}, 6.0f},
-                                   {128, 128, 2, 2, 1, {0.52f}, 4.0f},
-                                   {64, 128, 2, 2, 2, {0.32f, 0.59f}, 4.0f},
-                                   {64, 64, 2, 2, 3, {0.24f, 0.37f, 0.55f}, 4.0f}};
+constexpr TileKind kTileKinds[] = {{256, 256, 4, 2, 1, {1.62f}, 4.0f},
+                                   {128, 128, 2, 2, 1, {0.52f}, 1.2f},
+                                   {64, 128, 2, 2, 2, {0.32f, 0.59f}, 1.0f},
+                                   {64, 64, 2, 2, 3, {0.24f, 0.37f, 0.55f}, 1.0f}};
+constexpr float kLaunchUs = 3.0f;
 constexpr uint32_t kComputeUnits = 256;
 
 // How a product is cut: tiles of br x bc, each by wr x wc waves; K in `splits`
@@ -72,7 +73,7 @@ inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool n
             const uint64_t rounds = groups / slots, rest = groups % slots;
             float us = (float)rounds * ((float)chunk * t.slab[t.occupancy - 1] + t.fixed);
             if (rest) us += (float)chunk * t.slab[(rest - 1) / kComputeUnits] + t.fixed;
-            if (splits > 1) us += 3.0f + 8e-6f * (float)(splits * rows * cols) / 4.0f;
+            if (splits > 1) us += kLaunchUs + 8e-6f * (float)(splits * rows * cols) / 4.0f;
             if (us < least) {
                 least = us;
                 best = {t.br, t.bc, t.wr, t.wc, (uint32_t)splits, (uint32_t)(chunk * 64), direct};
@@ -167,9 +168,11 @@ int run_product(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u
     } else {
         DKZ_TRY(launch(name, product_kernel<Tile64, VMC, UMC, true, Epi>, grid, four, g, epi));
     }
-    if constexpr (Epi::kElementwise)
-        if (g.splits > 1)
-            return launch(name, join_kernel<Epi>, dim3(div_up((uint64_t)g.rows * (g.ldp / 8), kBlock)), dim3(kBlock), g, epi);
+    if constexpr (Epi::kElementwise) {
+        const uint64_t eights = (uint64_t)g.rows * (g.ldp / 8);
+        if (g.splits > 4) return launch(name, join_kernel<8, Epi>, dim3(div_up(eights, kBlock / 8)), dim3(kBlock), g, epi);
+        if (g.splits > 1) return launch(name, join_kernel<1, Epi>, dim3(div_up(eights, kBlock)), dim3(kBlock), g, epi);
+    }
     return 0;
 }
 

@@ -88,18 +88,29 @@ __global__ __launch_bounds__(64 * WAVES) void skinny_kernel(ProductArgs g, Epi e
     const bool ragged = last == steps && first < last && g.k % 64 != 0;
     const uint32_t whole = last - ragged;
     if (first < whole) {
-        constexpr int kAhead = RT * CT >= 4 ? 2 : 4;  // steps in flight
+        constexpr uint32_t kAhead = RT * CT >= 4 ? 2 : 4;  // steps in flight
         Step s[kAhead];
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) load(s[a], min(first + a, whole - 1));
+        for (uint32_t a = 0; a < kAhead; ++a)
+            if (first + a < whole) load(s[a], first + a);
+        uint32_t step = first;
 #pragma unroll 1
-        for (uint32_t step = first; step < whole; step += kAhead) {
+        for (; step + 2 * kAhead <= whole; step += kAhead) {
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
-                if (step + a < whole) multiply(s[a]);
-                load(s[a], min(step + a + kAhead, whole - 1));  // past the end: the last one again, not multiplied
+            for (uint32_t a = 0; a < kAhead; ++a) {
+                multiply(s[a]);
+                load(s[a], step + a + kAhead);
             }
         }
+        // Fewer than two rounds are left.
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            if (step + a < whole) multiply(s[a]);
+            if (step + a + kAhead < whole) load(s[a], step + a + kAhead);
+        }
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a)
+            if (step + a + kAhead < whole) multiply(s[a]);
     }
     if (ragged) {
         Step s;
@@ -151,7 +162,7 @@ int run_skinny(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u,
         if (rows <= 32) return launch_skinny<2, 2, 4>(name, grid, g, epi);
         return launch_skinny<4, 2, 4>(name, grid, g, epi);
     }
-    if (rows <= 16) return launch_skinny<1, 1, 8>(name, grid, g, epi);
+    if (rows <= 16) return k < 1024 ? launch_skinny<1, 1, 4>(name, grid, g, epi) : launch_skinny<1, 1, 8>(name, grid, g, epi);
     if (rows <= 32) return launch_skinny<2, 1, 8>(name, grid, g, epi);
     return launch_skinny<4, 1, 8>(name, grid, g, epi);
 }
