@@ -239,7 +239,7 @@ struct TileEpilogue {
         const bool words = self.in_words();
         float bias[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) bias[i] = self.bias(min(words ? c + i : c0 + wc0 + lane % kCols, cols - 1));
+        for (int i = 0; i < 8; ++i) bias[i] = self.bias(min(c + i, cols - 1));
 #pragma unroll
         for (int j = 0; j < TR; ++j) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -265,27 +265,21 @@ struct TileEpilogue {
                 }
                 continue;
             }
-            // Rows that start inside a word: a lane a column, eight rows at a time.
+            // Rows that start inside a word: a lane a column, sixteen rows at a time.
 #pragma unroll
             for (uint32_t y = 0; y < kCols; y += kWave) {
                 const uint32_t col = y + lane, at = c0 + wc0 + col;
-                if (y != 0) {  // the second half of 128 columns
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) bias[i] = self.bias(min(at, cols - 1));
-                }
-                if (col < kCols && at < cols)
+                if (col >= kCols || at >= cols) break;
+                const float b = self.bias(at);
+                const float same[16] = {b, b, b, b, b, b, b, b, b, b, b, b, b, b, b, b};
 #pragma unroll 1
-                    for (uint32_t x = 0; x < 32 && top + x < rows; x += 8) {
-                        float z[8];
+                for (uint32_t x = 0; x < 32 && top + x < rows; x += 16) {
+                    float z[16];
 #pragma unroll
-                        for (uint32_t i = 0; i < 8; ++i)
-                            z[i] = reinterpret_cast<const float *>(part)[((x + i) * (kCols / 4) + ((col / 4) ^ ((x + i) & kMask))) * 4 + col % 4];
-                        self.put(ColumnRun{(uint64_t)(top + x) * self.ld + at, self.ld, min(rows - top - x, 8u)}, bias, z);
-                    }
-            }
-            if constexpr (kCols > kWave) {  // back to the first half's
-#pragma unroll
-                for (int i = 0; i < 8; ++i) bias[i] = self.bias(min(c0 + wc0 + lane, cols - 1));
+                    for (uint32_t i = 0; i < 16; ++i)
+                        z[i] = reinterpret_cast<const float *>(part)[((x + i) * (kCols / 4) + ((col / 4) ^ ((x + i) & kMask))) * 4 + col % 4];
+                    self.put(ColumnRun{(uint64_t)(top + x) * self.ld + at, self.ld, min(rows - top - x, 16u)}, same, z);
+                }
             }
         }
     }

@@ -4,7 +4,9 @@ what it refuses before any HIP call (no GPU needed)."""
 from __future__ import annotations
 
 import ctypes as C
+import inspect
 import re
+import shutil
 import subprocess
 
 import pytest
@@ -161,3 +163,92 @@ def test_cross_entropy_workspaces(type, rows, inputs, classes):
 ])
 def test_workspace_queries_refuse(call):
     assert call(C.byref(C.c_size_t(0))) == INVALID
+
+
+# ---- the other hosts' bindings ----
+
+ZIG = ROOT / "darknet_zig_amd" / "zig" / "dkz_dense.zig"
+WRAPPERS = ["seededDropout", "linearForwardWorkspace", "linearForward", "linearBackwardWorkspace", "linearBackward",
+            "linearCrossEntropyForwardWorkspace", "linearCrossEntropyForward", "linearCrossEntropyBackwardWorkspace",
+            "linearCrossEntropyBackward"]
+
+
+def header_params() -> dict[str, list[tuple[str, str]]]:
+    text = re.sub(r"/\*.*?\*/", "", HEADER.read_text(), flags=re.S)
+    out = {}
+    for name, params in re.findall(r"(dkz_\w+)\s*\(([^)]*)\)\s*;", text):
+        ps = [] if params.strip() == "void" else [" ".join(p.split()) for p in params.split(",")]
+        out[name] = [re.match(r"(.*?)(\w+)$", p).groups() for p in ps]
+    return out
+
+
+def zig_type(ctype: str) -> str:
+    base = ctype.replace("const ", "").replace(" ", "")
+    return {"int": "c_int", "float": "f32", "unsignedint": "c_uint", "unsignedlonglong": "c_ulonglong", "size_t": "usize",
+            "size_t*": "*usize"}.get(base, "?*anyopaque")
+
+
+def test_zig_externs_follow_the_header():
+    externs = re.findall(r"^pub extern fn (dkz_\w+)\((.*)\) (.+);$", ZIG.read_text(), flags=re.M)
+    params = header_params()
+    assert [e[0] for e in externs] == list(params) == header_symbols()
+    for name, ps, ret in externs:
+        got = [tuple(p.split(": ", 1)) for p in ps.split(", ")] if ps else []
+        assert got == [(n, zig_type(t)) for t, n in params[name]], name
+        assert ret == ("[*:0]const u8" if name.endswith("context") else "Status")
+
+
+def test_zig_wrappers_pass_every_argument_in_order():
+    text = ZIG.read_text()
+    params = header_params()
+    for name in WRAPPERS:
+        m = re.search(r"^pub fn " + name + r"\((.*?)\) [\w.]+ \{\n(.*?)^\}", text, flags=re.M | re.S)
+        assert m, name
+        body = m.group(2)
+        assert body.strip().startswith("if (!gpu.enabled) unreachable;")
+        call = re.search(r"must\((dkz_\w+)\((.*)\), \"", body)
+        args = re.sub(r"\bci\((\w+)\)", r"\1", call.group(2)).split(", ")
+        assert len(args) == len(params[call.group(1)]), name
+        for arg, (_, want) in zip(args, params[call.group(1)]):
+            bare = re.sub(r"^&need(\.)?|\.ptr$", "", arg)
+            assert bare in (want, "", "type_code" if want == "type" else want) or arg == "bytes(workspace)" and want == "workspace_bytes", (
+                name, arg, want)
+
+
+@pytest.mark.parametrize("name", WRAPPERS)
+def test_python_and_cpp_wrappers_take_the_same_arguments(name):
+    cpp = (ROOT / "darknet_zig_amd" / "host" / "dkz_dense.hpp").read_text()
+    m = re.search(r"inline [\w:]+ " + name + r"\((.*?)\) \{", cpp, flags=re.S)
+    assert [p.split()[-1] for p in m.group(1).split(",")] == list(inspect.signature(getattr(gpu, name)).parameters)
+
+
+def test_cpp_mirror_compiles_links_and_refuses(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    src = tmp_path / "dense.cpp"
+    src.write_text('''#include <cstdio>
+#include "dkz_dense.hpp"
+using namespace dkz::gpu;
+int main() {
+    if (linearForwardWorkspace(DKZ_F32, 256, 4096, 4096) == 0) return 1;
+    const Workspaces w = linearCrossEntropyBackwardWorkspace(DKZ_BF16, 64, 128, 5000);
+    if (w.least == 0 || w.best < w.least) return 2;
+    seededDropout(0, DKZ_F32, Buf{}, Buf{}, 0.5f, 2.0f, 1, 0, DKZ_F32, Buf{});
+    try {
+        linearForward(DKZ_BF16, 4, 8, 6, 99, 0.0f, 1.0f, 0, 0, Buf{}, Buf{}, Buf{}, Buf{}, Buf{}, Buf{}, Buf{});
+        return 3;
+    } catch (const Error &e) {
+        std::puts(e.what());
+        return e.code() == 1 ? 0 : 4;
+    }
+}
+''')
+    lib = LIB.parent
+    exe = tmp_path / "dense"
+    proc = subprocess.run([gxx, "-std=c++17", "-Wall", "-Wextra", "-Werror", f"-I{ROOT / 'include'}", f"-I{lib / 'host'}", str(src), "-o",
+                           str(exe), f"-L{lib}", "-ldkz_dense", "-ldkz", f"-Wl,-rpath,{lib}", "-Wl,-rpath-link,/opt/rocm/lib"],
+                          capture_output=True, text=True)
+    assert proc.returncode == 0, proc.stderr
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and "dkz_linear_forward" in run.stdout, (run.returncode, run.stdout)
