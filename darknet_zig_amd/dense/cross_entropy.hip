@@ -8,6 +8,7 @@
 // products for the gradients then read. fp32: the logits of a piece are written
 // to the workspace and reduced, or replaced by d, there.
 #include <algorithm>
+#include <type_traits>
 
 #include "dense_internal.hpp"
 #include "epilogue.hpp"
@@ -55,52 +56,51 @@ struct StatEpilogue {
     uint32_t parts;
 
     template <int TR, int TC, int WR, int WC>
-    __device__ __forceinline__ void tile(f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
+    __device__ __forceinline__ void tile(const f32x16 (&acc)[TC][TR], uint32_t r0, uint32_t c0, uint32_t wr0, uint32_t wc0,
                                          uint32_t rows, uint32_t cols, uint32_t, uint32_t tc, char *) const {
         constexpr uint32_t kCols = TC * 32;
         const uint32_t lane = threadIdx.x & 63, wave_c = (threadIdx.x >> 6) % WC, first = c0 + wc0;
         const uint32_t cl = first + 4 * (lane >> 5);  // this lane's columns: cl + 8 * n + 0 .. 3
         const auto column = [](int i, int e) { return (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3)); };
         const bool edge = first + kCols > cols;
-        // Bias and edge first: a wave's usual part, inside and without a bias, is left alone.
-        if (biases != nullptr || edge) {
-#pragma unroll
-            for (int i = 0; i < TC; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const uint32_t c = cl + column(i, e);
-                    const float b = c >= cols ? neg_inf() : biases != nullptr ? biases[c] : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < TR; ++j) acc[i][j][e] = c < cols ? acc[i][j][e] + b : neg_inf();
-                }
-        }
-#pragma unroll
-        for (int j = 0; j < TR; ++j) {
-            const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
+        // A wave's usual part, inside and without a bias, is taken as it is. (Adding the bias into the accumulators first
+        // costs a copy of all 128.)
+        const bool plain = biases == nullptr && !edge;
+        const auto logit = [&](auto usual, int i, int j, int e) __attribute__((always_inline)) {
+            if constexpr (decltype(usual)::value) return acc[i][j][e];
+            const uint32_t c = cl + column(i, e);
+            return c >= cols ? neg_inf() : biases != nullptr ? acc[i][j][e] + biases[c] : acc[i][j][e];
+        };
+        const auto part = [&](auto usual, int j) __attribute__((always_inline)) {
             float m = neg_inf();
 #pragma unroll
             for (int i = 0; i < TC; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
+                for (int e = 0; e < 16; ++e) m = fmaxf(m, logit(usual, i, j, e));
             m = fmaxf(m, __shfl_xor(m, 32));
             const float base = m == neg_inf() ? 0.0f : m;
             float s[2] = {};
 #pragma unroll
             for (int i = 0; i < TC; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e & 1] += exp_fast(acc[i][j][e] - base);
+                for (int e = 0; e < 16; ++e) s[e & 1] += exp_fast(logit(usual, i, j, e) - base);
             s[0] += s[1];
-            s[0] += __shfl_xor(s[0], 32);
-            if (r < rows && lane < 32) stats[(uint64_t)r * parts + tc * WC + wave_c] = {m, s[0]};
+            return Stat{m, s[0] + __shfl_xor(s[0], 32)};
+        };
+#pragma unroll
+        for (int j = 0; j < TR; ++j) {
+            const uint32_t r = r0 + wr0 + 32 * j + (lane & 31);
+            const Stat t = plain ? part(std::true_type{}, j) : part(std::false_type{}, j);
+            if (r < rows && lane < 32) stats[(uint64_t)r * parts + tc * WC + wave_c] = t;
             // The target's logit, where it is one of this wave's columns: seldom.
-            const uint32_t t = r < rows ? (uint32_t)targets[r] : ~0u, o = t - cl;
-            if (o < kCols && t < cols && (o & 4) == 0) {
+            const uint32_t target = r < rows ? (uint32_t)targets[r] : ~0u, o = target - cl;
+            if (o < kCols && target < cols && (o & 4) == 0) {
                 float z = 0.0f;
 #pragma unroll
                 for (int i = 0; i < TC; ++i)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) z = o == column(i, e) ? acc[i][j][e] : z;
-                target_logit[r] = z;
+                target_logit[r] = biases != nullptr ? z + biases[target] : z;
             }
         }
     }
@@ -182,7 +182,7 @@ struct GradientEpilogue {
         float bias[8], sum[8] = {};
 #pragma unroll
         for (int i = 0; i < 8; ++i) bias[i] = biases != nullptr ? biases[min(c + i, cols - 1)] : 0.0f;
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < TR; ++j) {
             // Lane x has the values of row x of the 32.
             uint32_t target_of = ~0u;
@@ -190,12 +190,7 @@ struct GradientEpilogue {
             if (const uint32_t r = r0 + wr0 + 32 * j + (lane & 31); r < rows) rows_of.row(r, target_of, s_of, l_of);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int i = 0; i < TC; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    part[(lane & 31) * (kCols / 4) + ((8 * i + 2 * q + (lane >> 5)) ^ (lane & 31 & kMask))] =
-                        make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+            block_to_lds<TR, TC>(acc, j, part);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 2
@@ -249,8 +244,12 @@ struct LogitEpilogue : TileEpilogue<LogitEpilogue> {
     uint32_t ld;
     LogitEpilogue(const float *biases, float *out, uint64_t ld) : biases(biases), out(out), ld((uint32_t)ld) {}
     __device__ __forceinline__ float bias(uint32_t c) const { return biases != nullptr ? biases[c] : 0.0f; }
+    template <int N>
+    struct Before {};
+    template <int N, class E>
+    __device__ __forceinline__ Before<N> before(const E &) const { return {}; }
     template <class E, int N>
-    __device__ __forceinline__ void put(const E &e, const float (&bias)[N], float (&z)[N]) const {
+    __device__ __forceinline__ void put(const E &e, const float (&bias)[N], float (&z)[N], const Before<N> &) const {
         if (biases != nullptr) {
 #pragma unroll
             for (int i = 0; i < N; ++i) z[i] += bias[i];
@@ -439,11 +438,17 @@ struct PieceEpilogue : TileEpilogue<PieceEpilogue> {
     bool begin, words;
     __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
     __device__ __forceinline__ bool in_words() const { return words; }
+    template <int N>
+    using Before = Raw<float, N>;
+    template <int N, class E>
+    __device__ __forceinline__ Before<N> before(const E &e) const {
+        Before<N> o = {};
+        if (!begin) load_raw<float, E, N>(sum, e, o);
+        return o;
+    }
     template <class E, int N>
-    __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N]) const {
+    __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N], const Before<N> &o) const {
         if (!begin) {
-            float o[N];
-            load_n(sum, e, o);
 #pragma unroll
             for (int i = 0; i < N; ++i) z[i] += o[i];
         }

@@ -81,16 +81,25 @@ struct BlockColumn {  // of one column, in the rows of a 32x32 block that one la
     __device__ __forceinline__ bool in(int x) const { return row(x) < (int)n; }
 };
 
+// The elements as they are loaded: kept like this, they are waited for where
+// they are used and not where they are loaded.
+template <class T, int N>
+using Raw = T __attribute__((ext_vector_type(N)));
 template <class T, class E, int N>
-__device__ __forceinline__ void load_n(const T *p, const E &e, float (&v)[N]) {
+__device__ __forceinline__ void load_raw(const T *p, const E &e, Raw<T, N> &v) {
     if constexpr (E::kRow && N == 8) {
         if (e.n == 8) {
-            load8(p, e.first, v);
+            if constexpr (sizeof(T) == 4) {
+                const f32x4u a = reinterpret_cast<const f32x4u *>(p + e.first)[0], b = reinterpret_cast<const f32x4u *>(p + e.first)[1];
+                v = __builtin_shufflevector((f32x4)a, (f32x4)b, 0, 1, 2, 3, 4, 5, 6, 7);
+            } else {
+                v = *reinterpret_cast<const bf16x8u *>(p + e.first);
+            }
             return;
         }
     }
 #pragma unroll
-    for (int x = 0; x < N; ++x) v[x] = e.in(x) ? load1(p, e.at(x)) : 0.0f;
+    for (int x = 0; x < N; ++x) v[x] = e.in(x) ? p[e.at(x)] : (T)0.0f;
 }
 template <class T, class E, int N>
 __device__ __forceinline__ void store_n(T *p, const E &e, const float (&v)[N]) {

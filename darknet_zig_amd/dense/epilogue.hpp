@@ -76,10 +76,16 @@ struct LinearEpilogue : TileEpilogue<LinearEpilogue<T, EXP>> {
 
     __device__ __forceinline__ float bias(uint32_t c) const { return biases != nullptr ? biases[c] : 0.0f; }
     __device__ __forceinline__ bool in_words() const { return words; }
+    template <int N>
+    using Before = Raw<T, N>;
+    template <int N, class E>
+    __device__ __forceinline__ Before<N> before(const E &e) const {
+        Before<N> add = {};
+        if (residual != nullptr) load_raw<T, E, N>(residual, e, add);
+        return add;
+    }
     template <class E, int N>
-    __device__ __forceinline__ void put(const E &e, const float (&bias)[N], float (&a)[N]) const {
-        float add[N] = {};
-        if (residual != nullptr) load_n(residual, e, add);
+    __device__ __forceinline__ void put(const E &e, const float (&bias)[N], float (&a)[N], const Before<N> &add) const {
         if (biases != nullptr) {
 #pragma unroll
             for (int i = 0; i < N; ++i) a[i] += bias[i];
@@ -89,7 +95,7 @@ struct LinearEpilogue : TileEpilogue<LinearEpilogue<T, EXP>> {
         draws.apply(a, e);
         if (residual != nullptr) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) a[i] += add[i];
+            for (int i = 0; i < N; ++i) a[i] += (float)add[i];
         }
         store_n(output, e, a);
     }
@@ -106,18 +112,26 @@ struct StoreEpilogue : TileEpilogue<StoreEpilogue<T>> {
 
     __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
     __device__ __forceinline__ bool in_words() const { return words; }
+    template <int N>
+    struct Before {
+        Raw<T, N> old, add;
+    };
+    template <int N, class E>
+    __device__ __forceinline__ Before<N> before(const E &e) const {
+        Before<N> b = {};
+        if (beta != 0.0f) load_raw<T, E, N>(out, e, b.old);
+        if (add != nullptr) load_raw<T, E, N>(add, e, b.add);
+        return b;
+    }
     template <class E, int N>
-    __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N]) const {
-        float x[N];
+    __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N], const Before<N> &b) const {
         if (beta != 0.0f) {
-            load_n(out, e, x);
 #pragma unroll
-            for (int i = 0; i < N; ++i) z[i] += beta * x[i];
+            for (int i = 0; i < N; ++i) z[i] += beta * (float)b.old[i];
         }
         if (add != nullptr) {
-            load_n(add, e, x);
 #pragma unroll
-            for (int i = 0; i < N; ++i) z[i] += x[i];
+            for (int i = 0; i < N; ++i) z[i] += (float)b.add[i];
         }
         store_n(out, e, z);
     }

@@ -173,8 +173,7 @@ struct Direct {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                      :
                      : "s"(to + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024 + i * THREADS * 16),
-                       "v"(k[i] < left ? off[i] : kOutside), "s"(buf)
-                     : "m0");
+                       "v"(k[i] < left ? off[i] : kOutside), "s"(buf));
     }
 };
 
@@ -185,11 +184,31 @@ __device__ __forceinline__ void await_loads() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// A wave's block of 32 rows, j of its part, to LDS: a row's chunk of four columns
+// at chunk ^ row. (The writes of every block are there once, behind a branch on j,
+// which is the same in all lanes.)
+template <int TR, int TC>
+__device__ __forceinline__ void block_to_lds(const f32x16 (&acc)[TC][TR], int j, float4 *part) {
+    constexpr uint32_t kChunks = TC * 8, kMask = kChunks - 1;
+    const uint32_t lane = threadIdx.x & 63, row = lane & 31;
+#pragma unroll
+    for (int b = 0; b < TR; ++b)
+        if (b == j)
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    part[row * kChunks + ((8 * i + 2 * q + (lane >> 5)) ^ (row & kMask))] =
+                        make_float4(acc[i][b][4 * q], acc[i][b][4 * q + 1], acc[i][b][4 * q + 2], acc[i][b][4 * q + 3]);
+}
+
 // Epilogues that treat every element by itself derive from this and give
 //   ld                      the matrix's columns, and the step from row to row;
 //   bias(c)                 what is added to column c (0: nothing);
 //   in_words()              whether rows start on 4-byte boundaries;
-//   put(elements, bias, z)  takes z[x] for element x, its bias in bias[x].
+//   before<N>(elements)     what the elements' put reads of memory, loaded ahead of it;
+//   put(elements, bias, z, before)
+//                           takes z[x] for element x, its bias in bias[x].
 // A wave passes its part of the tile through LDS, 32 rows at a time: there a
 // lane wrote four columns of its row at once, here it takes eight of one of
 // four rows, so that rows are read and written in whole lines and the columns a
@@ -204,7 +223,8 @@ struct TileEpilogue {
         const Self &self = *static_cast<const Self *>(this);
         const float bias[1] = {self.bias(c)};
         float v[1] = {z};
-        self.put(RowRun{(uint64_t)r * self.ld + c, 1}, bias, v);
+        const RowRun e{(uint64_t)r * self.ld + c, 1};
+        self.put(e, bias, v, self.template before<1>(e));
     }
     // The fp32 kernel's: rows of a 32x32 block, and some of a row.
     __device__ __forceinline__ void block(uint32_t r, uint32_t rows, uint32_t c, float (&z)[16]) const {
@@ -212,7 +232,8 @@ struct TileEpilogue {
         const Self &self = *static_cast<const Self *>(this);
         const float b = self.bias(c);
         const float bias[16] = {b, b, b, b, b, b, b, b, b, b, b, b, b, b, b, b};
-        self.put(BlockColumn{(uint64_t)r * self.ld + c, self.ld, rows - r}, bias, z);
+        const BlockColumn e{(uint64_t)r * self.ld + c, self.ld, rows - r};
+        self.put(e, bias, z, self.template before<16>(e));
     }
     template <int N>
     __device__ __forceinline__ void row(uint32_t r, uint32_t c, uint32_t cols, float (&z)[N]) const {
@@ -220,7 +241,8 @@ struct TileEpilogue {
         float bias[N];
 #pragma unroll
         for (int x = 0; x < N; ++x) bias[x] = self.bias(min(c + x, cols - 1));
-        self.put(RowRun{(uint64_t)r * self.ld + c, min(cols - c, (uint32_t)N)}, bias, z);
+        const RowRun e{(uint64_t)r * self.ld + c, min(cols - c, (uint32_t)N)};
+        self.put(e, bias, z, self.template before<N>(e));
     }
     // Few rows (product_skinny.hpp): one element, if it is there.
     template <int COLS>
@@ -240,45 +262,61 @@ struct TileEpilogue {
         float bias[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) bias[i] = self.bias(min(c + i, cols - 1));
-#pragma unroll
+        // One copy of the code for all blocks of rows; only the writes to LDS name registers.
+#pragma unroll 1
         for (int j = 0; j < TR; ++j) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int i = 0; i < TC; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    part[(lane & 31) * (kCols / 4) + ((8 * i + 2 * q + (lane >> 5)) ^ (lane & 31 & kMask))] =
-                        make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
             const uint32_t top = r0 + wr0 + 32 * j;
+            // A few rows of eights at a time (kStep rows apart), what they read of memory first; the first ones' before the
+            // passage through LDS.
+            constexpr uint32_t kRows = TC * TR > 4 ? 2 : 4;  // by the registers that the tile leaves
+            using Eight = typename Self::template Before<8>;
+            const auto eight = [&](uint32_t x) { return RowRun{(uint64_t)(top + x) * self.ld + c, cols - c < 8u ? cols - c : 8u}; };
+            const auto ahead = [&](Eight(&to)[kRows], uint32_t x) __attribute__((always_inline)) {
+#pragma unroll
+                for (uint32_t g = 0; g < kRows; ++g)
+                    if (top + x + g * kStep < rows) to[g] = self.template before<8>(eight(x + g * kStep));
+            };
+            Eight before[kRows] = {};
+            if (words && c < cols) ahead(before, lane / kLanes);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            block_to_lds<TR, TC>(acc, j, part);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
             if (words) {
                 if (c >= cols) continue;
-#pragma unroll 2
-                for (uint32_t x = lane / kLanes; x < 32; x += kStep) {
-                    const uint32_t at = x * (kCols / 4), chunk = lane % kLanes * 2, r = top + x;
-                    const float4 a = part[at + (chunk ^ (x & kMask))], b = part[at + ((chunk + 1) ^ (x & kMask))];
-                    float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                    if (r >= rows) break;
-                    self.put(RowRun{(uint64_t)r * self.ld + c, min(cols - c, 8u)}, bias, z);
+#pragma unroll 1
+                for (uint32_t x = lane / kLanes; x < 32; x += kRows * kStep) {
+                    if (x >= kRows * kStep) ahead(before, x);
+#pragma unroll
+                    for (uint32_t g = 0; g < kRows; ++g) {
+                        const uint32_t y = x + g * kStep, at = y * (kCols / 4), chunk = lane % kLanes * 2;
+                        if (y >= 32 || top + y >= rows) break;
+                        const float4 a = part[at + (chunk ^ (y & kMask))], b = part[at + ((chunk + 1) ^ (y & kMask))];
+                        float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                        self.put(eight(y), bias, z, before[g]);
+                    }
                 }
                 continue;
             }
             // Rows that start inside a word: a lane a column, sixteen rows at a time.
-#pragma unroll
-            for (uint32_t y = 0; y < kCols; y += kWave) {
-                const uint32_t col = y + lane, at = c0 + wc0 + col;
-                if (col >= kCols || at >= cols) break;
+#pragma unroll 1
+            for (uint32_t col = lane; col < kCols; col += kWave) {
+                const uint32_t at = c0 + wc0 + col;
+                if (at >= cols) break;
                 const float b = self.bias(at);
                 const float same[16] = {b, b, b, b, b, b, b, b, b, b, b, b, b, b, b, b};
+                const auto sixteen = [&](uint32_t x) {
+                    return ColumnRun{(uint64_t)(top + x) * self.ld + at, self.ld, top + x + 16 <= rows ? 16u : top + x < rows ? rows - top - x : 0u};
+                };
+                const auto first = self.template before<16>(sixteen(0)), second = self.template before<16>(sixteen(16));
 #pragma unroll 1
-                for (uint32_t x = 0; x < 32 && top + x < rows; x += 16) {
+                for (uint32_t x = 0; x < 32; x += 16) {
                     float z[16];
 #pragma unroll
                     for (uint32_t i = 0; i < 16; ++i)
                         z[i] = reinterpret_cast<const float *>(part)[((x + i) * (kCols / 4) + ((col / 4) ^ ((x + i) & kMask))) * 4 + col % 4];
-                    self.put(ColumnRun{(uint64_t)(top + x) * self.ld + at, self.ld, min(rows - top - x, 16u)}, same, z);
+                    self.put(sixteen(x), same, z, x == 0 ? first : second);
                 }
             }
         }
@@ -292,8 +330,12 @@ struct PartialEpilogue : TileEpilogue<PartialEpilogue> {
     __device__ __forceinline__ PartialEpilogue(float *out, uint32_t ld) : out(out), ld(ld) {}
     __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
     __device__ __forceinline__ bool in_words() const { return true; }
+    template <int N>
+    struct Before {};
+    template <int N, class E>
+    __device__ __forceinline__ Before<N> before(const E &) const { return {}; }
     template <class E, int N>
-    __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N]) const {
+    __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N], const Before<N> &) const {
         if constexpr (N == 8) store8(out, e.first, z);  // also past the last column: ld is whole eights
     }
 };
