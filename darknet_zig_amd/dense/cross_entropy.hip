@@ -118,30 +118,37 @@ struct StatEpilogue {
     }
 };
 
+// Workgroups of the kernels that take a row at a time; beyond, a workgroup takes several.
+constexpr uint32_t kRowGroups = 1u << 18;
+
 // A workgroup a row: merges its parts.
 __global__ __launch_bounds__(kBlock) void merge_stats_kernel(const Stat *stats, uint32_t parts, const int *targets,
-                                                            const float *target_logit, uint32_t classes, float *loss, float *lse) {
+                                                            const float *target_logit, uint32_t rows, uint32_t classes, float *loss,
+                                                            float *lse) {
     __shared__ Stat waves[kBlock / kWave];
-    const uint32_t r = blockIdx.x;
-    const Stat *row = stats + (uint64_t)r * parts;
-    Stat t{neg_inf(), 0.0f};
-    for (uint32_t i = threadIdx.x; i < parts; i += 4 * kBlock) {
-        Stat next[4];
+    for (uint32_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const Stat *row = stats + (uint64_t)r * parts;
+        Stat t{neg_inf(), 0.0f};
+        for (uint32_t i = threadIdx.x; i < parts; i += 4 * kBlock) {
+            Stat next[4];
 #pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) next[u] = row[min(i + u * kBlock, parts - 1)];
+            for (uint32_t u = 0; u < 4; ++u) next[u] = row[min(i + u * kBlock, parts - 1)];
 #pragma unroll
-        for (uint32_t u = 0; u < 4; ++u)
-            if (i + u * kBlock < parts) t = merge(t, next[u]);
+            for (uint32_t u = 0; u < 4; ++u)
+                if (i + u * kBlock < parts) t = merge(t, next[u]);
+        }
+#pragma unroll
+        for (int x = 1; x < kWave; x *= 2) t = merge(t, {__shfl_xor(t.m, x), __shfl_xor(t.s, x)});
+        if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = t;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int w = 1; w < kBlock / kWave; ++w) t = merge(t, waves[w]);
+            const bool target = (uint32_t)targets[r] < classes;
+            finish_row(t, target, target ? target_logit[r] : 0.0f, loss + r, lse + r);
+        }
+        __syncthreads();
     }
-#pragma unroll
-    for (int x = 1; x < kWave; x *= 2) t = merge(t, {__shfl_xor(t.m, x), __shfl_xor(t.s, x)});
-    if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = t;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-#pragma unroll
-    for (int w = 1; w < kBlock / kWave; ++w) t = merge(t, waves[w]);
-    const bool target = (uint32_t)targets[r] < classes;
-    finish_row(t, target, target ? target_logit[r] : 0.0f, loss + r, lse + r);
 }
 
 // ---- the gradient of a logit ----
@@ -263,36 +270,40 @@ constexpr uint32_t kStatThreads = 512, kStatEach = 8;
 // A workgroup a row: the pair of a piece's logits, in one pass with the running
 // maximum, merged into the row's; the last piece finishes the row. A thread
 // takes eight logits at a time, a workgroup's width apart.
-__global__ __launch_bounds__(kStatThreads) void row_stats_kernel(const float *z, uint32_t ld, uint32_t cols, uint32_t first, uint32_t classes,
-                                                                const int *targets, Stat *run, float *target_logit, float *loss,
-                                                                float *lse) {
+__global__ __launch_bounds__(kStatThreads) void row_stats_kernel(const float *z, uint32_t ld, uint32_t rows, uint32_t cols, uint32_t first,
+                                                                uint32_t classes, const int *targets, Stat *run, float *target_logit,
+                                                                float *loss, float *lse) {
     __shared__ Stat waves[kStatThreads / kWave];
-    const uint32_t r = blockIdx.x;
-    const float *row = z + (uint64_t)r * ld;
-    Stat t{neg_inf(), 0.0f};
-    for (uint32_t c = threadIdx.x; c < cols; c += kStatEach * kStatThreads) {
-        float v[kStatEach], m = t.m;
+    for (uint32_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const float *row = z + (uint64_t)r * ld;
+        Stat t{neg_inf(), 0.0f};
+        for (uint32_t c = threadIdx.x; c < cols; c += kStatEach * kStatThreads) {
+            float v[kStatEach], m = t.m;
 #pragma unroll
-        for (uint32_t i = 0; i < kStatEach; ++i) v[i] = row[min(c + i * kStatThreads, cols - 1)];
+            for (uint32_t i = 0; i < kStatEach; ++i) v[i] = row[min(c + i * kStatThreads, cols - 1)];
 #pragma unroll
-        for (uint32_t i = 0; i < kStatEach; ++i) m = fmaxf(m, v[i]);
-        const float base = m == neg_inf() ? 0.0f : m;
-        t.s *= expf_cw(t.m - base);
+            for (uint32_t i = 0; i < kStatEach; ++i) m = fmaxf(m, v[i]);
+            const float base = m == neg_inf() ? 0.0f : m;
+            t.s *= expf_cw(t.m - base);
 #pragma unroll
-        for (uint32_t i = 0; i < kStatEach; ++i) t.s += c + i * kStatThreads < cols ? expf_cw(v[i] - base) : 0.0f;
-        t.m = m;
+            for (uint32_t i = 0; i < kStatEach; ++i) t.s += c + i * kStatThreads < cols ? expf_cw(v[i] - base) : 0.0f;
+            t.m = m;
+        }
+#pragma unroll
+        for (int x = 1; x < kWave; x *= 2) t = merge(t, {__shfl_xor(t.m, x), __shfl_xor(t.s, x)});
+        if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = t;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (uint32_t w = 1; w < kStatThreads / kWave; ++w) t = merge(t, waves[w]);
+            if (first != 0) t = merge(run[r], t);
+            const uint32_t target = (uint32_t)targets[r];
+            if (target - first < cols) target_logit[r] = row[target - first];
+            run[r] = t;
+            if (first + cols == classes)
+                finish_row(t, target < classes, target < classes ? target_logit[r] : 0.0f, loss + r, lse + r);
+        }
+        __syncthreads();
     }
-#pragma unroll
-    for (int x = 1; x < kWave; x *= 2) t = merge(t, {__shfl_xor(t.m, x), __shfl_xor(t.s, x)});
-    if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = t;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (uint32_t w = 1; w < kStatThreads / kWave; ++w) t = merge(t, waves[w]);
-    if (first != 0) t = merge(run[r], t);
-    const uint32_t target = (uint32_t)targets[r];
-    if (target - first < cols) target_logit[r] = row[target - first];
-    run[r] = t;
-    if (first + cols == classes) finish_row(t, target < classes, target < classes ? target_logit[r] : 0.0f, loss + r, lse + r);
 }
 
 constexpr uint32_t kGradRows = 64;  // rows a workgroup of logit_gradient_kernel takes
@@ -302,11 +313,12 @@ constexpr uint32_t kGradRows = 64;  // rows a workgroup of logit_gradient_kernel
 // issued before the first is used; a column's eight threads are added in row
 // order. Rows are ld logits long, a multiple of four.
 __global__ __launch_bounds__(kBlock) void logit_gradient_kernel(float *z, uint32_t ld, uint32_t rows, uint32_t cols, uint32_t first,
-                                                               RowGradient rows_of, float *sums) {
+                                                               uint32_t blocks_c, RowGradient rows_of, float *sums) {
     constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes, kEach = kGradRows / kGroups;
     __shared__ float part[kGroups][kLanes * 4 + 4];
     const uint32_t x = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const uint32_t c = (blockIdx.x * kLanes + x) * 4, r0 = blockIdx.y * kGradRows + group * kEach;
+    const uint32_t block_r = blockIdx.x / blocks_c, block_c = blockIdx.x - block_r * blocks_c;
+    const uint32_t c = (block_c * kLanes + x) * 4, r0 = block_r * kGradRows + group * kEach;
     float4 v[kEach];
     uint32_t target[kEach];
     float s[kEach], l[kEach], sum[4] = {};
@@ -338,8 +350,8 @@ __global__ __launch_bounds__(kBlock) void logit_gradient_kernel(float *z, uint32
     float t = part[0][threadIdx.x];
 #pragma unroll
     for (uint32_t i = 1; i < kGroups; ++i) t += part[i][threadIdx.x];
-    const uint32_t column = blockIdx.x * kLanes * 4 + threadIdx.x;
-    if (column < cols) sums[(uint64_t)blockIdx.y * cols + column] = t;
+    const uint32_t column = block_c * kLanes * 4 + threadIdx.x;
+    if (column < cols) sums[(uint64_t)block_r * cols + column] = t;
 }
 
 // Rows whose classes are none: lse -infinity, no target, no loss.
@@ -471,8 +483,8 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const vo
         const uint32_t parts = (uint32_t)p.row_parts(classes);
         const StatEpilogue epi{biases, targets, stats, target_logit, parts};
         DKZ_TRY((run_product<false, false>(kName, x.p, x.ld, w.p, w.ld, rows, classes, inputs, p, nullptr, epi)));
-        return launch("linear_cross_entropy_merge", merge_stats_kernel, dim3((uint32_t)rows), dim3(kBlock), stats, parts, targets,
-                      target_logit, (uint32_t)classes, loss, lse);
+        return launch("linear_cross_entropy_merge", merge_stats_kernel, dim3(std::min((uint32_t)rows, kRowGroups)), dim3(kBlock), stats,
+                      parts, targets, target_logit, (uint32_t)rows, (uint32_t)classes, loss, lse);
     }
     float *logits = ws.take<float>(plan.logits / 4), *partial = ws.take<float>(plan.partial / 4);
     for (uint64_t first = 0; first < classes; first += plan.piece) {
@@ -481,8 +493,8 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const vo
         DKZ_TRY((run_f32<kRowMajor, kRowMajor>(kName, static_cast<const float *>(input), inputs,
                                                static_cast<const float *>(weights) + first * inputs, inputs, 0.0f, (float *)nullptr, ld,
                                                rows, n, inputs, partial, epi)));
-        DKZ_TRY(launch("linear_cross_entropy_stats", row_stats_kernel, dim3((uint32_t)rows), dim3(kStatThreads), logits, (uint32_t)ld, (uint32_t)n,
-                       (uint32_t)first, (uint32_t)classes, targets, stats, target_logit, loss, lse));
+        DKZ_TRY(launch("linear_cross_entropy_stats", row_stats_kernel, dim3(std::min((uint32_t)rows, kRowGroups)), dim3(kStatThreads), logits,
+                       (uint32_t)ld, (uint32_t)rows, (uint32_t)n, (uint32_t)first, (uint32_t)classes, targets, stats, target_logit, loss, lse));
     }
     return 0;
 }
@@ -500,8 +512,8 @@ int backward_f32(uint64_t rows, uint64_t inputs, uint64_t classes, const float *
             const LogitEpilogue epi(biases != nullptr ? biases + first : nullptr, d, ld);
             DKZ_TRY((run_f32<kRowMajor, kRowMajor>("linear_cross_entropy_logits", input, inputs, w, inputs, 0.0f, (float *)nullptr, ld, rows,
                                                    n, inputs, partial, epi)));
-            DKZ_TRY(launch("linear_cross_entropy_gradient", logit_gradient_kernel, dim3(div_up(ld, 128), (uint32_t)chunks), dim3(kBlock),
-                           d, (uint32_t)ld, (uint32_t)rows, (uint32_t)n, (uint32_t)first, grad, bias_updates != nullptr ? sums : nullptr));
+            DKZ_TRY(launch("linear_cross_entropy_gradient", logit_gradient_kernel, dim3(div_up(ld, 128) * (uint32_t)chunks), dim3(kBlock),
+                           d, (uint32_t)ld, (uint32_t)rows, (uint32_t)n, (uint32_t)first, div_up(ld, 128), grad, bias_updates != nullptr ? sums : nullptr));
         }
         if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
         if (weight_updates != nullptr)
@@ -565,6 +577,9 @@ extern "C" {
 
 int dkz_linear_cross_entropy_forward_workspace(int type, int rows, int inputs, int classes, size_t *least, size_t *best) {
     DKZ_REQUIRE(least != nullptr && best != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
+    DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(classes);
+    DKZ_REQUIRE((uint64_t)rows * (uint64_t)classes <= 1ull << 38);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(classes, inputs);
     const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes;
@@ -577,6 +592,9 @@ int dkz_linear_cross_entropy_forward(int type, int rows, int inputs, int classes
                                      const float *biases, const int *targets, float *loss, float *lse, void *workspace,
                                      size_t workspace_bytes) {
     DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
+    DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(classes);
+    DKZ_REQUIRE((uint64_t)rows * (uint64_t)classes <= 1ull << 38);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(classes, inputs);
     if (rows == 0) return 0;
@@ -596,6 +614,9 @@ int dkz_linear_cross_entropy_forward(int type, int rows, int inputs, int classes
 
 int dkz_linear_cross_entropy_backward_workspace(int type, int rows, int inputs, int classes, size_t *least, size_t *best) {
     DKZ_REQUIRE(least != nullptr && best != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
+    DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(classes);
+    DKZ_REQUIRE((uint64_t)rows * (uint64_t)classes <= 1ull << 38);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(classes, inputs);
     const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes;
@@ -609,6 +630,9 @@ int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classe
                                       float scale, float beta, float *bias_updates, void *weight_updates, void *input_delta,
                                       void *workspace, size_t workspace_bytes) {
     DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
+    DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(classes);
+    DKZ_REQUIRE((uint64_t)rows * (uint64_t)classes <= 1ull << 38);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(classes, inputs);
     const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes, size = type_size(type);

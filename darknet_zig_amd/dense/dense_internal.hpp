@@ -230,6 +230,9 @@ inline uint64_t round_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * t
 // Matrices past the ABI's largest element count (less what rounds a load up) are refused.
 #define DKZ_REQUIRE_ELEMS(a, b) DKZ_REQUIRE((uint64_t)(a) * (uint64_t)(b) + 3 <= kMaxElems)
 
+// A launch counts its threads in 32 bits; sides up to here keep all of them well below.
+#define DKZ_REQUIRE_SIDE(n) DKZ_REQUIRE((n) <= 1 << 26)
+
 // A call's workspace: `need` bytes at a 16-byte boundary.
 #define DKZ_REQUIRE_WORKSPACE(need) \
     DKZ_REQUIRE((need) == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= (need)))

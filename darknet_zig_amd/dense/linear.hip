@@ -59,38 +59,40 @@ constexpr uint32_t kDeltaRows = 64;  // rows a workgroup of delta_kernel takes
 // the eight sums of a column's threads are added in row order.
 template <class T, int W>
 __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *activated, uint32_t rows, uint32_t cols, int act,
-                                                      Draws draws, T *d, uint32_t ldd, float *partial) {
+                                                      Draws draws, T *d, uint32_t ldd, uint32_t blocks_c, float *partial) {
     constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes, kEach = kDeltaRows / kGroups;
     __shared__ float sums[kGroups][kLanes * W + 4];
     const uint32_t x = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const uint32_t c = (blockIdx.x * kLanes + x) * W, r0 = blockIdx.y * kDeltaRows + group * kEach;
+    const uint32_t block_r = blockIdx.x / blocks_c, block_c = blockIdx.x - block_r * blocks_c;
+    const uint32_t c = (block_c * kLanes + x) * W, r0 = block_r * kDeltaRows + group * kEach;
     const bool in = c < cols;  // W == 8: cols is a multiple of it, and ldd is cols
-    float v[kEach][W], y[kEach][W], s[W] = {};
+    Raw<T, W> v[kEach], y[kEach];
+    float s[W] = {};
 #pragma unroll
     for (uint32_t i = 0; i < kEach; ++i) {
-        const uint64_t at = (uint64_t)min(r0 + i, rows - 1) * cols + (in ? c : 0);
-        if constexpr (W == 8) load8(delta, at, v[i]);
-        else v[i][0] = load1(delta, at);
-        if (act != kLinear) {
-            if constexpr (W == 8) load8(activated, at, y[i]);
-            else y[i][0] = load1(activated, at);
-        }
+        const RowRun e{(uint64_t)min(r0 + i, rows - 1) * cols + (in ? c : 0), W};
+        load_raw<T, RowRun, W>(delta, e, v[i]);
+        if (act != kLinear) load_raw<T, RowRun, W>(activated, e, y[i]);
     }
 #pragma unroll
     for (uint32_t i = 0; i < kEach; ++i) {
         const uint32_t r = r0 + i;
         if (r >= rows) break;
-        draws.run(v[i], (uint64_t)r * cols + c);
-        if (act != kLinear) gradient_all(act, y[i], v[i]);
+        float g[W], a[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) g[w] = (float)v[i][w];
+        draws.run(g, (uint64_t)r * cols + c);
+        if (act != kLinear) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) a[w] = (float)y[i][w];
+            gradient_all(act, a, g);
+        }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            if (!in) v[i][w] = 0.0f;  // the rows' padding
-            s[w] += v[i][w];
+            if (!in) g[w] = 0.0f;  // the rows' padding
+            s[w] += g[w];
         }
-        if (d != nullptr && c < ldd) {
-            if constexpr (W == 8) store8(d, (uint64_t)r * ldd + c, v[i]);
-            else store1(d, (uint64_t)r * ldd + c, v[i][0]);
-        }
+        if (d != nullptr && c < ldd) store_n(d, RowRun{(uint64_t)r * ldd + c, W}, g);
     }
     if (partial == nullptr) return;
 #pragma unroll
@@ -100,8 +102,8 @@ __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *
         float t = sums[0][e];
 #pragma unroll
         for (uint32_t i = 1; i < kGroups; ++i) t += sums[i][e];
-        const uint32_t column = blockIdx.x * kLanes * W + e;
-        if (column < cols) partial[(uint64_t)blockIdx.y * cols + column] = t;
+        const uint32_t column = block_c * kLanes * W + e;
+        if (column < cols) partial[(uint64_t)block_r * cols + column] = t;
     }
 }
 
@@ -109,12 +111,13 @@ template <class T>
 int run_delta(const T *delta, const T *activated, uint64_t rows, uint64_t cols, int act, const Draws &draws, T *d, uint64_t ldd,
               float *partial) {
     constexpr const char *kName = "linear_backward_delta";
-    const dim3 block(kBlock);
-    if (cols % 8 == 0)
-        return launch(kName, delta_kernel<T, 8>, dim3(div_up(cols, 32 * 8), div_up(rows, kDeltaRows)), block, delta, activated,
-                      (uint32_t)rows, (uint32_t)cols, act, draws, d, (uint32_t)ldd, partial);
-    return launch(kName, delta_kernel<T, 1>, dim3(div_up(ldd, 32), div_up(rows, kDeltaRows)), block, delta, activated, (uint32_t)rows,
-                  (uint32_t)cols, act, draws, d, (uint32_t)ldd, partial);
+    const bool eights = cols % 8 == 0;
+    const uint32_t blocks_c = div_up(eights ? cols : ldd, eights ? 32 * 8 : 32);
+    const dim3 grid(blocks_c * div_up(rows, kDeltaRows)), block(kBlock);
+    return eights ? launch(kName, delta_kernel<T, 8>, grid, block, delta, activated, (uint32_t)rows, (uint32_t)cols, act, draws, d,
+                           (uint32_t)ldd, blocks_c, partial)
+                  : launch(kName, delta_kernel<T, 1>, grid, block, delta, activated, (uint32_t)rows, (uint32_t)cols, act, draws, d,
+                           (uint32_t)ldd, blocks_c, partial);
 }
 
 // Leading dimension of d in the workspace: whole 16-byte chunks.
@@ -192,6 +195,8 @@ extern "C" {
 
 int dkz_linear_forward_workspace(int type, int rows, int inputs, int outputs, size_t *bytes) {
     DKZ_REQUIRE(bytes != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
+    DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(outputs);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(outputs, inputs);
     DKZ_REQUIRE_ELEMS(rows, outputs);
@@ -204,6 +209,8 @@ int dkz_linear_forward(int type, int rows, int inputs, int outputs, int activati
                        const void *residual, void *activated, void *output, void *workspace, size_t workspace_bytes) {
     DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
     DKZ_REQUIRE(activation >= 0 && activation < kActCount);
+    DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(outputs);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(outputs, inputs);
     DKZ_REQUIRE_ELEMS(rows, outputs);
@@ -226,6 +233,8 @@ int dkz_linear_forward(int type, int rows, int inputs, int outputs, int activati
 
 int dkz_linear_backward_workspace(int type, int rows, int inputs, int outputs, size_t *bytes) {
     DKZ_REQUIRE(bytes != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
+    DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(outputs);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(outputs, inputs);
     DKZ_REQUIRE_ELEMS(rows, outputs);
@@ -239,6 +248,8 @@ int dkz_linear_backward(int type, int rows, int inputs, int outputs, int activat
                         void *input_delta, void *workspace, size_t workspace_bytes) {
     DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
     DKZ_REQUIRE(activation >= 0 && activation < kActCount);
+    DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(outputs);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(outputs, inputs);
     DKZ_REQUIRE_ELEMS(rows, outputs);

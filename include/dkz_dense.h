@@ -20,7 +20,8 @@
  *   - Matrices are row-major without gaps: input [rows, inputs], weights
  *     [outputs, inputs], output [rows, outputs]. Any size and element
  *     alignment will do; sizes that are multiples of eight, on 16-byte
- *     boundaries, run fastest. A tensor holds at most 2^31 - 4 elements.
+ *     boundaries, run fastest. A tensor holds at most 2^31 - 4 elements; rows,
+ *     outputs and classes are 2^26 at most, and rows * classes 2^38.
  *   - A negative size, an unknown type or activation, a null pointer where
  *     elements must be touched or a workspace that is too small returns
  *     hipErrorInvalidValue (1) and launches nothing. An output may not overlap

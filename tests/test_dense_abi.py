@@ -81,6 +81,7 @@ def forward(L, type=BF16, rows=4, inputs=8, outputs=6, act=RELU, x=X, w=W, b=B, 
     (dict(x=None), INVALID), (dict(w=None), INVALID), (dict(y=None), INVALID), (dict(y=X), INVALID), (dict(y=W), INVALID),
     (dict(y=B), INVALID), (dict(a=Y), INVALID), (dict(a=R, r=R), INVALID), (dict(r=C.c_void_p(Y.value + 2)), INVALID), (dict(a=X), INVALID),
     (dict(rows=65536, inputs=8, outputs=32768), INVALID), (dict(rows=1 << 30, inputs=2, outputs=1), INVALID),
+    (dict(rows=1, inputs=1, outputs=(1 << 26) + 1), INVALID), (dict(rows=(1 << 26) + 1, inputs=1, outputs=1), INVALID),
 ], ids=str)
 def test_linear_forward_refusals(kw, want):
     assert forward(_lib.load_dense(), **kw) == want
@@ -122,6 +123,7 @@ def loss(L, type=BF16, rows=4, inputs=8, classes=600, x=X, w=W, b=B, t=A, l=Y, l
     (dict(x=None), INVALID), (dict(w=None), INVALID), (dict(t=None), INVALID), (dict(l=None), INVALID), (dict(lse=None), INVALID),
     (dict(l=Z), INVALID), (dict(l=A), INVALID), (dict(ws=None), INVALID), (dict(ws_bytes=64), INVALID), (dict(ws=W), INVALID),
     (dict(ws=C.c_void_p(WS.value + 4)), INVALID), (dict(inputs=1 << 16, classes=1 << 16), INVALID),
+    (dict(inputs=1, classes=(1 << 26) + 1), INVALID), (dict(rows=1 << 20, inputs=1, classes=1 << 19), INVALID),
 ], ids=str)
 @pytest.mark.parametrize("type", [F32, BF16])
 def test_cross_entropy_forward_refusals(kw, want, type):

@@ -263,3 +263,9 @@ def test_same_call_same_bits(pool, kind):
     again = [d.raw().copy() for d in run(pool, kind, x, w, b, t)]
     for p, q in zip(first, again):
         assert (p.view(np.uint8) == q.view(np.uint8)).all()
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_more_rows_than_workgroups(pool, kind):
+    """Kernels that take a row a workgroup take several beyond 2^18 rows."""
+    run(pool, kind, *make(kind, (1 << 18) + 77, 2, 3), backward=False)

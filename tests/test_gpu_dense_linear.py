@@ -286,3 +286,22 @@ def test_backward_is_the_forward_s_derivative(pool, kind):
             num[i] = (loss(*args[:which], up, *args[which + 1 :]) - loss(*args[:which], down, *args[which + 1 :])) / (2 * h)
         mags = {2: np.abs(g).sum(0), 1: np.abs(g).T @ np.abs(x64), 0: np.abs(g) @ np.abs(w64)}[which] * scale
         assert_within(got, num, tol * mags + 1e-7 * size, ("input", "weights", "biases")[which])
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_more_rows_than_a_grid_side(pool, kind):
+    """Workgroups of 64 rows: 65537 of them and more. Values -1, 0 and 1: every sum is a whole number below 2^24, exact in
+    fp32, so that only the rounding to the result's type is left."""
+    rows, k, n = 4194304 + 65, 2, 3
+    r = np.random.default_rng(1)
+    x, w, d = (r.integers(-1, 2, s).astype(np.float32) for s in ((rows, k), (n, k), (rows, n)))
+    dx, dw, dd = pool(x, kind), pool(w, kind), pool(d, kind)
+    y, gx, gb, gw = pool(kind=kind, n=(rows, n)), pool(kind=kind, n=(rows, k)), pool(n=n), pool(kind=kind, n=(n, k))
+    ws = pool.work(max(gpu.linearForwardWorkspace(kind, rows, k, n), gpu.linearBackwardWorkspace(kind, rows, k, n)))
+    gpu.linearForward(kind, rows, k, n, LINEAR, 0.0, 1.0, 0, 0, dx.buf, dw.buf, None, None, None, y.buf, buf(ws))
+    gpu.linearBackward(kind, rows, k, n, LINEAR, 0.0, 1.0, 0, 0, dx.buf, dw.buf, None, dd.buf, None, 0.0, gb.buf, gw.buf, gx.buf, buf(ws))
+    x64, w64, d64 = x.astype(np.float64), w.astype(np.float64), d.astype(np.float64)
+    assert (y.get() == ref.rounded(x64 @ w64.T, kind)).all()
+    assert (gx.get() == ref.rounded(d64 @ w64, kind)).all()
+    assert (gb.get() == d64.sum(0)).all()
+    assert (gw.get() == ref.rounded(d64.T @ x64, kind)).all()
