@@ -29,7 +29,7 @@ constexpr TileKind kTileKinds[] = {{256, 256, 4, 2, 1, {1.62f}, 4.0f},
                                    {128, 128, 2, 2, 1, {0.52f}, 1.2f},
                                    {64, 128, 2, 2, 2, {0.32f, 0.59f}, 1.0f},
                                    {64, 64, 2, 2, 3, {0.24f, 0.37f, 0.55f}, 1.0f}};
-constexpr float kLaunchUs = 3.0f;
+constexpr float kLaunchUs = 3.0f, kPartialBytesUs = 4e6f;  // a launch, and bytes of partials a us
 constexpr uint32_t kComputeUnits = 256;
 
 // How a product is cut: tiles of br x bc, each by wr x wc waves; K in `splits`
@@ -52,8 +52,8 @@ struct ProductPlan {
 inline bool direct_ok(const void *p, uint64_t ld) { return aligned16(p) && ld % 8 == 0 && ld < (1u << 22); }
 inline bool operands_direct(const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu) { return direct_ok(v, ldv) && direct_ok(u, ldu); }
 
-// nt: both operands with k contiguous; direct: operands_direct. The least time over the kinds of tile and
-// the ways to cut K, each range at least four slabs long: rounds of the chip x
+// nt: both operands with k contiguous; direct: operands_direct. The least time
+// over the kinds of tile and the ways to cut K, each range at least four slabs long: rounds of the chip x
 // slabs x a slab's time; ranges add their partials' way out and back and the
 // launch that joins them.
 inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool nt, bool may_split, bool direct) {
@@ -63,8 +63,7 @@ inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool n
     ProductPlan best{};
     float least = 1e30f;
     for (const TileKind &t : kTileKinds) {
-        if (!direct && t.br != t.bc) continue;  // the kernel that goes through registers has two kinds
-        if (!direct && t.br == 256) continue;
+        if (!direct && (t.br != t.bc || t.br == 256)) continue;  // the kernel that goes through registers has two kinds
         const uint64_t tiles = (uint64_t)div_up(rows, t.br) * div_up(cols, t.bc), slots = (uint64_t)kComputeUnits * t.occupancy;
         for (const uint32_t want : kSplits) {
             const uint64_t chunk = std::max<uint64_t>((slabs + want - 1) / want, 1), splits = std::max<uint64_t>((slabs + chunk - 1) / chunk, 1);
@@ -73,7 +72,7 @@ inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool n
             const uint64_t rounds = groups / slots, rest = groups % slots;
             float us = (float)rounds * ((float)chunk * t.slab[t.occupancy - 1] + t.fixed);
             if (rest) us += (float)chunk * t.slab[(rest - 1) / kComputeUnits] + t.fixed;
-            if (splits > 1) us += kLaunchUs + 8e-6f * (float)(splits * rows * cols) / 4.0f;
+            if (splits > 1) us += kLaunchUs + 2 * 4.0f / kPartialBytesUs * (float)(splits * rows * cols);
             if (us < least) {
                 least = us;
                 best = {t.br, t.bc, t.wr, t.wc, (uint32_t)splits, (uint32_t)(chunk * 64), direct};
@@ -87,8 +86,10 @@ inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool n
 //
 // Matrices with k contiguous and k % 8 != 0 are copied to the workspace in rows
 // of whole chunks that end in zeros, for the products that read them once a
-// tile: 777x1001x2503 takes ... us by copies, 86 us through registers, where
-// loads at odd elements and the shifts at rows' ends hold up the products.
+// tile: 777x1001x2503 with its epilogue took 86 us through registers, where loads
+// at odd elements and the shifts at rows' ends hold up the products, and 44 us
+// by copies (5 us of them). Operands whose rows are whole chunks and whose base
+// is off a 16-byte boundary go through registers (4096^3 270 us).
 
 inline uint64_t packed_ld(uint64_t k) { return round_up(k, 8); }
 inline uint64_t packed_bytes(uint64_t rows, uint64_t k) { return k % 8 == 0 ? 0 : padded(2 * rows * packed_ld(k)); }
