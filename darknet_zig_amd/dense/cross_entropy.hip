@@ -442,6 +442,17 @@ bool fit_plan(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int typ
     }
 }
 
+// The bytes of the smallest of these plans (not always the one with the smallest pieces: one piece needs no fp32 sums of
+// the input gradient).
+template <class Plan>
+uint64_t least_plan(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int type, uint64_t rows, uint64_t inputs, uint64_t classes) {
+    uint64_t least = ~0ull;
+    for (uint64_t most = kPieceBytes;; most /= 2) {
+        least = std::min(least, make(type, rows, inputs, classes, most).total());
+        if (most == 0) return least;
+    }
+}
+
 // The input gradient of one of several pieces: added up in fp32, the last one rounded to out.
 struct PieceEpilogue : TileEpilogue<PieceEpilogue> {
     float *sum;
@@ -578,12 +589,13 @@ extern "C" {
 int dkz_linear_cross_entropy_forward_workspace(int type, int rows, int inputs, int classes, size_t *least, size_t *best) {
     DKZ_REQUIRE(least != nullptr && best != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
     DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(inputs);
     DKZ_REQUIRE_SIDE(classes);
     DKZ_REQUIRE((uint64_t)rows * (uint64_t)classes <= 1ull << 38);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(classes, inputs);
     const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes;
-    *least = m == 0 || n == 0 ? 0 : (size_t)forward_plan(type, m, k, n, 0).total();
+    *least = m == 0 || n == 0 ? 0 : (size_t)least_plan(forward_plan, type, m, k, n);
     *best = m == 0 || n == 0 ? 0 : (size_t)forward_plan(type, m, k, n, kPieceBytes).total();
     return 0;
 }
@@ -593,6 +605,7 @@ int dkz_linear_cross_entropy_forward(int type, int rows, int inputs, int classes
                                      size_t workspace_bytes) {
     DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
     DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(inputs);
     DKZ_REQUIRE_SIDE(classes);
     DKZ_REQUIRE((uint64_t)rows * (uint64_t)classes <= 1ull << 38);
     DKZ_REQUIRE_ELEMS(rows, inputs);
@@ -615,12 +628,13 @@ int dkz_linear_cross_entropy_forward(int type, int rows, int inputs, int classes
 int dkz_linear_cross_entropy_backward_workspace(int type, int rows, int inputs, int classes, size_t *least, size_t *best) {
     DKZ_REQUIRE(least != nullptr && best != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
     DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(inputs);
     DKZ_REQUIRE_SIDE(classes);
     DKZ_REQUIRE((uint64_t)rows * (uint64_t)classes <= 1ull << 38);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(classes, inputs);
     const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes;
-    *least = n == 0 ? 0 : (size_t)backward_plan(type, m, k, n, 0).total();
+    *least = n == 0 ? 0 : (size_t)least_plan(backward_plan, type, m, k, n);
     *best = n == 0 ? 0 : (size_t)backward_plan(type, m, k, n, kPieceBytes).total();
     return 0;
 }
@@ -631,6 +645,7 @@ int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classe
                                       void *workspace, size_t workspace_bytes) {
     DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && classes >= 0);
     DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(inputs);
     DKZ_REQUIRE_SIDE(classes);
     DKZ_REQUIRE((uint64_t)rows * (uint64_t)classes <= 1ull << 38);
     DKZ_REQUIRE_ELEMS(rows, inputs);
@@ -643,7 +658,7 @@ int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classe
     }
     BackwardPlan plan{};
     if (n != 0) {
-        DKZ_REQUIRE(backward_plan(type, m, k, n, 0).total() == 0 || (workspace != nullptr && aligned16(workspace)));
+        DKZ_REQUIRE(least_plan(backward_plan, type, m, k, n) == 0 || (workspace != nullptr && aligned16(workspace)));
         DKZ_REQUIRE(fit_plan(backward_plan, type, m, k, n, workspace_bytes, plan));
     }
     const Span writes[] = {{bias_updates, 4 * n}, {weight_updates, n * k * size}, {input_delta, m * k * size}, {workspace, plan.total()}};

@@ -147,7 +147,7 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
     T *d = ws.take<T>(plan.d_bytes / sizeof(T));
     float *sums = ws.take<float>(plan.sum_bytes / 4), *partial = ws.take<float>(plan.partial_bytes / 4);
     uint64_t ldd = delta_ld(type, outputs);
-    const bool products = weight_updates != nullptr || input_delta != nullptr;
+    const bool products = inputs != 0 && (weight_updates != nullptr || input_delta != nullptr);
     // The delta itself where nothing changes it and its rows lie on 16-byte boundaries.
     const bool same = act == kLinear && draws.limit == 0 && draws.scale == 1.0f && ldd == outputs && aligned16(delta);
     if (same || !products) {
@@ -196,6 +196,7 @@ extern "C" {
 int dkz_linear_forward_workspace(int type, int rows, int inputs, int outputs, size_t *bytes) {
     DKZ_REQUIRE(bytes != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
     DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(inputs);
     DKZ_REQUIRE_SIDE(outputs);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(outputs, inputs);
@@ -210,6 +211,7 @@ int dkz_linear_forward(int type, int rows, int inputs, int outputs, int activati
     DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
     DKZ_REQUIRE(activation >= 0 && activation < kActCount);
     DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(inputs);
     DKZ_REQUIRE_SIDE(outputs);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(outputs, inputs);
@@ -234,6 +236,7 @@ int dkz_linear_forward(int type, int rows, int inputs, int outputs, int activati
 int dkz_linear_backward_workspace(int type, int rows, int inputs, int outputs, size_t *bytes) {
     DKZ_REQUIRE(bytes != nullptr && type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
     DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(inputs);
     DKZ_REQUIRE_SIDE(outputs);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(outputs, inputs);
@@ -249,6 +252,7 @@ int dkz_linear_backward(int type, int rows, int inputs, int outputs, int activat
     DKZ_REQUIRE(type_ok(type) && rows >= 0 && inputs >= 0 && outputs >= 0);
     DKZ_REQUIRE(activation >= 0 && activation < kActCount);
     DKZ_REQUIRE_SIDE(rows);
+    DKZ_REQUIRE_SIDE(inputs);
     DKZ_REQUIRE_SIDE(outputs);
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(outputs, inputs);

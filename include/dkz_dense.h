@@ -21,7 +21,7 @@
  *     [outputs, inputs], output [rows, outputs]. Any size and element
  *     alignment will do; sizes that are multiples of eight, on 16-byte
  *     boundaries, run fastest. A tensor holds at most 2^31 - 4 elements; rows,
- *     outputs and classes are 2^26 at most, and rows * classes 2^38.
+ *     inputs, outputs and classes are 2^26 at most, and rows * classes 2^38.
  *   - A negative size, an unknown type or activation, a null pointer where
  *     elements must be touched or a workspace that is too small returns
  *     hipErrorInvalidValue (1) and launches nothing. An output may not overlap
@@ -32,8 +32,8 @@
  *     may overlap on any streams, host threads and captured graphs. Nothing is
  *     allocated, copied to the host or waited for, and every op may be captured
  *     in a graph. Pointers belong to the current device.
- *   - Sums are taken in an order that depends on sizes and the workspace's size
- *     alone: the same call gives the same bits.
+ *   - Sums are taken in an order that depends on sizes, the tensors' alignment and
+ *     the workspace's size alone: the same call gives the same bits.
  */
 #ifndef DKZ_DENSE_H
 #define DKZ_DENSE_H
@@ -118,7 +118,8 @@ int dkz_linear_backward(int type, int rows, int inputs, int outputs, int activat
  * A target outside 0 .. classes - 1 (-1, say) is none: the row's loss is 0 and
  * it has no gradient. A class whose bias is -infinity has probability 0; a row
  * with no class left has lse -infinity, loss +infinity if it has a target, and
- * no gradient. A row with a NaN or +infinity logit has NaN results.
+ * no gradient. A row with a NaN or +infinity logit has lse NaN, and with a target
+ * NaN loss and gradient.
  *
  * The classes are taken in pieces, as many at a time as the workspace has room
  * for: *best is what the fastest way takes, *least what any call of this shape

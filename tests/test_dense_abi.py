@@ -82,6 +82,7 @@ def forward(L, type=BF16, rows=4, inputs=8, outputs=6, act=RELU, x=X, w=W, b=B, 
     (dict(y=B), INVALID), (dict(a=Y), INVALID), (dict(a=R, r=R), INVALID), (dict(r=C.c_void_p(Y.value + 2)), INVALID), (dict(a=X), INVALID),
     (dict(rows=65536, inputs=8, outputs=32768), INVALID), (dict(rows=1 << 30, inputs=2, outputs=1), INVALID),
     (dict(rows=1, inputs=1, outputs=(1 << 26) + 1), INVALID), (dict(rows=(1 << 26) + 1, inputs=1, outputs=1), INVALID),
+    (dict(rows=1, inputs=(1 << 26) + 1, outputs=1), INVALID),
 ], ids=str)
 def test_linear_forward_refusals(kw, want):
     assert forward(_lib.load_dense(), **kw) == want
@@ -153,6 +154,18 @@ def test_cross_entropy_workspaces(type, rows, inputs, classes):
         least, best = f(type, rows, inputs, classes)
         assert 0 < least <= best
         assert best < (1 << 30) + 64 * rows * inputs + rows * classes // 4
+
+
+@pytest.mark.parametrize("type", [F32, BF16])
+@pytest.mark.parametrize("rows,inputs,classes", [(1, 1 << 20, 300), (40, 8, 300), (500, 2000, 300), (64, 1 << 18, 1000)])
+def test_the_least_workspace_is_the_least(type, rows, inputs, classes):
+    """Also where one piece of all classes takes less than several, which add up the input's gradient in fp32."""
+    for f in (gpu.linearCrossEntropyForwardWorkspace, gpu.linearCrossEntropyBackwardWorkspace):
+        least, best = f(type, rows, inputs, classes)
+        assert least <= best
+    L = _lib.load_dense()
+    args = dict(type=type, rows=rows, inputs=inputs, classes=classes)
+    assert grad(L, **args, ws_bytes=least - 256) == INVALID
 
 
 @pytest.mark.parametrize("call", [

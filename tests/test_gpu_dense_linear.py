@@ -252,6 +252,17 @@ def test_backward_without_rows_keeps_beta_of_the_updates(pool, kind):
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("outputs", [6, 8])
+def test_backward_without_inputs_touches_no_delta_unless_for_the_bias(pool, kind, outputs):
+    """No inputs: weights and input gradients are empty, whatever their pointers, and delta is read for the bias alone."""
+    rows, some = 5, pool(np.zeros(8, np.float32))
+    ws = pool.work(gpu.linearBackwardWorkspace(kind, rows, 0, outputs))
+    gpu.linearBackward(kind, rows, 0, outputs, RELU, 0.5, 2.0, 0, 0, None, None, None, None, None, 0.0, None, some.buf, some.buf, buf(ws))
+    assert (some.get() == 0).all()
+    run_backward(pool, kind, rows, 0, outputs, RELU, 0.5, False, want=(1, 0, 0))
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
 def test_backward_is_the_forward_s_derivative(pool, kind):
     """Differences: the gradients of L = sum(g * output) by weights, biases and input, against central differences of
     the 64-bit forward with the GPU's own draws."""
