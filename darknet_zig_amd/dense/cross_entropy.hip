@@ -493,7 +493,7 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const vo
         const ProductPlan p = plan_product(rows, classes, inputs, true, false, operands_direct(x.p, x.ld, w.p, w.ld));
         const uint32_t parts = (uint32_t)p.row_parts(classes);
         const StatEpilogue epi{biases, targets, stats, target_logit, parts};
-        DKZ_TRY((run_product<false, false>(kName, x.p, x.ld, w.p, w.ld, rows, classes, inputs, p, nullptr, epi)));
+        DKZ_TRY((run_product<false, false>(kName, {x.p, x.ld, w.p, w.ld, rows, classes, inputs}, p, nullptr, epi)));
         return launch("linear_cross_entropy_merge", merge_stats_kernel, dim3(std::min((uint32_t)rows, kRowGroups)), dim3(kBlock), stats,
                       parts, targets, target_logit, (uint32_t)rows, (uint32_t)classes, loss, lse);
     }
@@ -553,27 +553,22 @@ int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16
         const uint64_t chunks = p.column_parts(rows);
         const GradientEpilogue epi{biases != nullptr ? biases + first : nullptr, grad, d, (uint32_t)ldd, (uint32_t)first,
                                             bias_updates != nullptr ? sums : nullptr};
-        DKZ_TRY((run_product<false, false>("linear_cross_entropy_gradient", x.p, x.ld, w, all.ld, rows, n, inputs, p, nullptr, epi)));
+        DKZ_TRY((run_product<false, false>("linear_cross_entropy_gradient", {x.p, x.ld, w, all.ld, rows, n, inputs}, p, nullptr, epi)));
         if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
-        if (weight_updates != nullptr)
-            DKZ_TRY((run_product<true, true>(kWeights, d, ldd, x.p, x.ld, n, inputs, rows,
-                                             plan_product(n, inputs, rows, false, true,
-                                                          operands_direct(d, ldd, x.p, x.ld)),
-                                             partial, store_epilogue<__bf16>(weight_updates + first * inputs, nullptr, inputs, beta))));
-        if (input_delta == nullptr) continue;
-        const ProductPlan pi =
-            plan_product(rows, inputs, n, false, true, operands_direct(d, ldd, w, all.ld));
-        if (n == classes) {
-            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, all.ld, rows, inputs, n, pi, partial,
-                                              store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f))));
-        } else {
+        const Product to_input{d, ldd, w, all.ld, rows, inputs, n}, to_weights{d, ldd, x.p, x.ld, n, inputs, rows};
+        __bf16 *updates = weight_updates != nullptr ? weight_updates + first * inputs : nullptr;
+        const auto epi_weights = store_epilogue<__bf16>(updates, nullptr, inputs, beta);
+        const bool one = n == classes;
+        DKZ_TRY(run_gradients(kInput, one && input_delta != nullptr ? &to_input : nullptr, store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f),
+                              kWeights, updates != nullptr ? &to_weights : nullptr, epi_weights, partial));
+        if (!one && input_delta != nullptr) {
             PieceEpilogue e;
             e.sum = accumulate;
             e.out = first + n == classes ? input_delta : nullptr;
             e.ld = (uint32_t)inputs;
             e.begin = first == 0;
             e.words = e.out == nullptr || rows_in_words<__bf16>(inputs, e.out);
-            DKZ_TRY((run_product<false, true>(kInput, d, ldd, w, all.ld, rows, inputs, n, pi, partial, e)));
+            DKZ_TRY((run_product<false, true>(kInput, to_input, plan_product(rows, inputs, n, false, true, to_input.direct()), partial, e)));
         }
     }
     return 0;
@@ -671,7 +666,7 @@ int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classe
         if (type == DKZ_F32)
             return run_f32<kRowMajor, kColMajor>(kInput, (const float *)nullptr, 0, (const float *)nullptr, k, 0.0f,
                                                  static_cast<float *>(input_delta), k, m, k, 0, nullptr);
-        return run_product<false, true>(kInput, nullptr, 0, nullptr, k, m, k, 0, plan_product(m, k, 0, false, false, true), nullptr,
+        return run_product<false, true>(kInput, {nullptr, 0, nullptr, k, m, k, 0}, plan_product(m, k, 0, false, false, true), nullptr,
                                         store_epilogue<__bf16>(input_delta, nullptr, k, 0.0f));
     }
     if (type == DKZ_F32)

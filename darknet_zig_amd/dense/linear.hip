@@ -38,7 +38,7 @@ int forward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act,
     if (!few_rows(rows)) DKZ_TRY(pack(x, rows, w, outputs, inputs, ws));
     const ProductPlan p = plan_product(rows, outputs, inputs, true, true, operands_direct(x.p, x.ld, w.p, w.ld));
     float *partial = ws.take<float>(p.partial_bytes(rows, outputs) / 4);
-    return run_product<false, false>(kName, x.p, x.ld, w.p, w.ld, rows, outputs, inputs, p, partial,
+    return run_product<false, false>(kName, {x.p, x.ld, w.p, w.ld, rows, outputs, inputs}, p, partial,
                                      linear_epilogue<__bf16, EXP>(outputs, act, draws, biases, residual, activated, output));
 }
 
@@ -50,74 +50,96 @@ uint64_t forward_bytes(int type, uint64_t rows, uint64_t inputs, uint64_t output
 
 // ---- backward ----
 
-constexpr uint32_t kDeltaRows = 64;  // rows a workgroup of delta_kernel takes
+constexpr uint32_t kDeltaRows = 64;   // rows a workgroup of delta_kernel takes at once
+constexpr uint32_t kDeltaWhole = 128;  // rows up to which it takes all of its columns'
+constexpr uint32_t kDeltaFill = 128;   // workgroups that are enough for eight columns a thread
 
 // d = dropout(delta) * gradient(activated), stored to d (null: not) in rows of
-// ldd, and the sums of kDeltaRows rows' columns to partial (null: not). Bound by
-// memory: a thread takes W columns (eight where rows are whole
-// eights) of eight rows, all of its loads issued before the first is used;
-// the eight sums of a column's threads are added in row order.
-template <class T, int W>
+// ldd, and the sums of kDeltaRows rows' columns to `to` (null: not). Bound by
+// memory: a thread takes W columns of eight rows, all of its loads issued before
+// the first is used; the eight sums of a column's threads are added in row order.
+// W is eight where rows are whole eights and that leaves workgroups for the chip
+// (8192x4096 48 us), else one (250x1024 with leaky and dropout: the backward pass 16
+// us, 33 with eight). WHOLE: a workgroup takes all rows, adds their sums in f64 and
+// `to` is bias_updates itself: a launch less where there are few rows.
+template <class T, int W, bool WHOLE>
 __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *activated, uint32_t rows, uint32_t cols, int act,
-                                                      Draws draws, T *d, uint32_t ldd, uint32_t blocks_c, float *partial) {
+                                                      Draws draws, T *d, uint32_t ldd, uint32_t blocks_c, float beta, float *to) {
     constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes, kEach = kDeltaRows / kGroups;
     __shared__ float sums[kGroups][kLanes * W + 4];
     const uint32_t x = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
     const uint32_t block_r = blockIdx.x / blocks_c, block_c = blockIdx.x - block_r * blocks_c;
-    const uint32_t c = (block_c * kLanes + x) * W, r0 = block_r * kDeltaRows + group * kEach;
+    const uint32_t c = (block_c * kLanes + x) * W;
     const bool in = c < cols;  // W == 8: cols is a multiple of it, and ldd is cols
-    Raw<T, W> v[kEach], y[kEach];
-    float s[W] = {};
+    const uint32_t column = block_c * kLanes * W + threadIdx.x;  // whose sum this thread stores
+    const bool stores = threadIdx.x < kLanes * W && column < cols;
+    static_assert(kLanes * W <= kBlock, "a thread a column");
+    double total = 0.0;
+    for (uint32_t top = WHOLE ? 0 : block_r * kDeltaRows; top < rows; top += kDeltaRows) {
+        const uint32_t r0 = top + group * kEach;
+        Raw<T, W> v[kEach], y[kEach];
+        float s[W] = {};
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-        const RowRun e{(uint64_t)min(r0 + i, rows - 1) * cols + (in ? c : 0), W};
-        load_raw<T, RowRun, W>(delta, e, v[i]);
-        if (act != kLinear) load_raw<T, RowRun, W>(activated, e, y[i]);
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-        const uint32_t r = r0 + i;
-        if (r >= rows) break;
-        float g[W], a[W];
-#pragma unroll
-        for (int w = 0; w < W; ++w) g[w] = (float)v[i][w];
-        draws.run(g, (uint64_t)r * cols + c);
-        if (act != kLinear) {
-#pragma unroll
-            for (int w = 0; w < W; ++w) a[w] = (float)y[i][w];
-            gradient_all(act, a, g);
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const RowRun e{(uint64_t)min(r0 + i, rows - 1) * cols + (in ? c : 0), W};
+            load_raw<T, RowRun, W>(delta, e, v[i]);
+            if (act != kLinear) load_raw<T, RowRun, W>(activated, e, y[i]);
         }
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (!in) g[w] = 0.0f;  // the rows' padding
-            s[w] += g[w];
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t r = r0 + i;
+            if (r >= rows) break;
+            float g[W], a[W];
+#pragma unroll
+            for (int w = 0; w < W; ++w) g[w] = (float)v[i][w];
+            draws.run(g, (uint64_t)r * cols + c);
+            if (act != kLinear) {
+#pragma unroll
+                for (int w = 0; w < W; ++w) a[w] = (float)y[i][w];
+                gradient_all(act, a, g);
+            }
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (!in) g[w] = 0.0f;  // the rows' padding
+                s[w] += g[w];
+            }
+            if (d != nullptr && c < ldd) store_n(d, RowRun{(uint64_t)r * ldd + c, W}, g);
         }
-        if (d != nullptr && c < ldd) store_n(d, RowRun{(uint64_t)r * ldd + c, W}, g);
-    }
-    if (partial == nullptr) return;
+        if (to != nullptr) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) sums[group][x * W + w] = s[w];
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < kLanes * W; e += kBlock) {
-        float t = sums[0][e];
+            for (int w = 0; w < W; ++w) sums[group][x * W + w] = s[w];
+            __syncthreads();
+            if (stores) {
+                float t = sums[0][threadIdx.x];
 #pragma unroll
-        for (uint32_t i = 1; i < kGroups; ++i) t += sums[i][e];
-        const uint32_t column = block_c * kLanes * W + e;
-        if (column < cols) partial[(uint64_t)block_r * cols + column] = t;
+                for (uint32_t i = 1; i < kGroups; ++i) t += sums[i][threadIdx.x];
+                if constexpr (WHOLE) total += (double)t;
+                else to[(uint64_t)block_r * cols + column] = t;
+            }
+            if constexpr (WHOLE) __syncthreads();
+        }
+        if constexpr (!WHOLE) break;
     }
+    if (WHOLE && to != nullptr && stores) to[column] = beta == 0.0f ? (float)total : beta * to[column] + (float)total;
 }
 
+// bias_updates null: not wanted; sums: room for the sums of every kDeltaRows rows.
 template <class T>
 int run_delta(const T *delta, const T *activated, uint64_t rows, uint64_t cols, int act, const Draws &draws, T *d, uint64_t ldd,
-              float *partial) {
+              float *sums, float beta, float *bias_updates) {
     constexpr const char *kName = "linear_backward_delta";
-    const bool eights = cols % 8 == 0;
+    const bool whole = rows <= kDeltaWhole;
+    const uint32_t blocks_r = whole ? 1 : div_up(rows, kDeltaRows);
+    const bool eights = cols % 8 == 0 && div_up(cols, 32 * 8) * blocks_r >= kDeltaFill;
     const uint32_t blocks_c = div_up(eights ? cols : ldd, eights ? 32 * 8 : 32);
-    const dim3 grid(blocks_c * div_up(rows, kDeltaRows)), block(kBlock);
-    return eights ? launch(kName, delta_kernel<T, 8>, grid, block, delta, activated, (uint32_t)rows, (uint32_t)cols, act, draws, d,
-                           (uint32_t)ldd, blocks_c, partial)
-                  : launch(kName, delta_kernel<T, 1>, grid, block, delta, activated, (uint32_t)rows, (uint32_t)cols, act, draws, d,
-                           (uint32_t)ldd, blocks_c, partial);
+    const dim3 grid(blocks_c * blocks_r), block(kBlock);
+    const auto run = [&](auto kernel) {
+        return launch(kName, kernel, grid, block, delta, activated, (uint32_t)rows, (uint32_t)cols, act, draws, d, (uint32_t)ldd, blocks_c, beta,
+                      bias_updates == nullptr ? nullptr : whole ? bias_updates : sums);
+    };
+    if (whole) return eights ? run(delta_kernel<T, 8, true>) : run(delta_kernel<T, 1, true>);
+    DKZ_TRY(eights ? run(delta_kernel<T, 8, false>) : run(delta_kernel<T, 1, false>));
+    return bias_updates != nullptr ? add_column_sums(sums, div_up(rows, kDeltaRows), cols, beta, bias_updates) : 0;
 }
 
 // Leading dimension of d in the workspace: whole 16-byte chunks.
@@ -155,9 +177,10 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
         ldd = outputs;
     }
     if (rows != 0 && outputs != 0 && (bias_updates != nullptr || d != nullptr))
-        DKZ_TRY(run_delta(static_cast<const T *>(delta), static_cast<const T *>(activated), rows, outputs, act, draws, d, ldd,
-                          bias_updates != nullptr ? sums : nullptr));
-    if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, div_up(rows, kDeltaRows), outputs, beta, bias_updates));
+        DKZ_TRY(run_delta(static_cast<const T *>(delta), static_cast<const T *>(activated), rows, outputs, act, draws, d, ldd, sums, beta,
+                          bias_updates));
+    else if (bias_updates != nullptr)
+        DKZ_TRY(add_column_sums(sums, 0, outputs, beta, bias_updates));  // no rows: beta * bias_updates
     const T *dd = d != nullptr ? d : static_cast<const T *>(delta);
     constexpr const char *kWeights = "linear_backward_weights", *kInput = "linear_backward_input";
     if constexpr (sizeof(T) == 4) {
@@ -172,16 +195,11 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
         Matrix x{weight_updates != nullptr ? static_cast<const T *>(input) : nullptr, inputs};
         Matrix w{input_delta != nullptr ? static_cast<const T *>(weights) : nullptr, inputs};
         if (rows != 0) DKZ_TRY(pack(x, rows, w, outputs, inputs, ws));
-        if (weight_updates != nullptr)
-            DKZ_TRY((run_product<true, true>(
-                kWeights, dd, ldd, x.p, x.ld, outputs, inputs, rows,
-                plan_product(outputs, inputs, rows, false, true, operands_direct(dd, ldd, x.p, x.ld)), partial,
-                store_epilogue<T>(weight_updates, nullptr, inputs, beta))));
-        if (input_delta != nullptr)
-            DKZ_TRY((run_product<false, true>(
-                kInput, dd, ldd, w.p, w.ld, rows, inputs, outputs,
-                plan_product(rows, inputs, outputs, false, true, operands_direct(dd, ldd, w.p, w.ld)), partial,
-                store_epilogue<T>(input_delta, input_residual, inputs, 0.0f))));
+        const Product to_input{dd, ldd, w.p, w.ld, rows, inputs, outputs}, to_weights{dd, ldd, x.p, x.ld, outputs, inputs, rows};
+        const auto epi_input = store_epilogue<T>(input_delta, input_residual, inputs, 0.0f);
+        const auto epi_weights = store_epilogue<T>(weight_updates, nullptr, inputs, beta);
+        DKZ_TRY(run_gradients(kInput, input_delta != nullptr ? &to_input : nullptr, epi_input, kWeights,
+                              weight_updates != nullptr ? &to_weights : nullptr, epi_weights, partial));
     }
     return 0;
 }

@@ -351,16 +351,22 @@ struct Tile {
     static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_, BK = BK_, STAGES = STAGES_, kThreads = 64 * WR * WC;
 };
 
+// LDS of a kernel of these tiles: the slabs, in whose place the epilogue's blocks of 32 rows come after the product.
+template <class T, bool ALIGNED>
+constexpr uint32_t lds_bytes() {
+    constexpr uint32_t slabs = (ALIGNED ? T::STAGES : 2) * (T::BR + T::BC) * T::BK * 2, blocks = T::WR * 32 * T::BC * 4;
+    return slabs > blocks ? slabs : blocks;
+}
+
+// Workgroup `block` of a product's.
 template <class T, bool VMC, bool UMC, bool ALIGNED, class Epi>
-__global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs g, Epi epi) {
+__device__ __forceinline__ void product_tile(const ProductArgs &g, const Epi &epi, uint32_t block, char *lds) {
     constexpr int BR = T::BR, BC = T::BC, WR = T::WR, WC = T::WC, BK = T::BK, kThreads = T::kThreads;
     constexpr int kTR = BR / WR / 32, kTC = BC / WC / 32, kSteps = BK / 16, kStages = ALIGNED ? T::STAGES : 2;
     constexpr uint32_t kV = BR * BK * 2, kStage = kV + BC * BK * 2;
-    constexpr uint32_t kEpilogue = WR * WC * 32 * (kTC * 32) * 4;
-    __shared__ __align__(1024) char lds[kStages * kStage > kEpilogue ? kStages * kStage : kEpilogue];
     const uint32_t wave = threadIdx.x >> 6;
     const uint32_t tiles = g.tiles_r * g.tiles_c;
-    const uint32_t w = xcd_run(blockIdx.x, tiles * g.splits), split = w / tiles;
+    const uint32_t w = xcd_run(block, tiles * g.splits), split = w / tiles;
     uint32_t tr, tc;
     tile_of(w - split * tiles, g.tiles_r, g.tiles_c, tr, tc);
     const uint32_t r0 = tr * BR, c0 = tc * BC, wr0 = wave / WC * (BR / WR), wc0 = wave % WC * (BC / WC);
@@ -521,6 +527,23 @@ __global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs g, 
         return;
     }
     epi.template tile<kTR, kTC, WR, WC>(acc, r0, c0, wr0, wc0, g.rows, g.cols, tr, tc, lds);
+}
+
+template <class T, bool VMC, bool UMC, bool ALIGNED, class Epi>
+__global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs g, Epi epi) {
+    __shared__ __align__(1024) char lds[lds_bytes<T, ALIGNED>()];
+    product_tile<T, VMC, UMC, ALIGNED>(g, epi, blockIdx.x, lds);
+}
+
+// A backward pass's two products in one launch: a's tiles (u row-contiguous
+// alone) and b's (both operands), a's in the first workgroups or in the last.
+template <class T, class Epi>
+__global__ __launch_bounds__(T::kThreads, 2) void product_pair_kernel(ProductArgs a, Epi epi_a, ProductArgs b, Epi epi_b, uint32_t tiles_a,
+                                                                     bool a_first) {
+    __shared__ __align__(1024) char lds[lds_bytes<T, true>()];
+    const uint32_t first = a_first ? tiles_a : gridDim.x - tiles_a, block = blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
+    if ((blockIdx.x < first) == a_first) product_tile<T, false, true, true>(a, epi_a, block, lds);
+    else product_tile<T, true, true, true>(b, epi_b, block, lds);
 }
 
 // The join of a split product: adds eight columns' partials in f64 and passes

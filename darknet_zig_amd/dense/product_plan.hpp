@@ -37,6 +37,7 @@ constexpr uint32_t kComputeUnits = 256;
 struct ProductPlan {
     uint32_t br, bc, wr, wc, splits, k_chunk;
     bool direct;  // operands straight to LDS
+    float us;     // its time, without a launch
     bool skinny() const { return br == 0; }
     uint64_t partial_bytes(uint64_t rows, uint64_t cols) const {
         return splits > 1 ? padded(4 * (uint64_t)splits * rows * round_up(cols, 8)) : 0;
@@ -57,7 +58,7 @@ inline bool operands_direct(const __bf16 *v, uint64_t ldv, const __bf16 *u, uint
 // slabs x a slab's time; ranges add their partials' way out and back and the
 // launch that joins them.
 inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool nt, bool may_split, bool direct) {
-    if (nt && few_rows(rows)) return {0, 0, 0, 0, 1, 0, false};
+    if (nt && few_rows(rows)) return {0, 0, 0, 0, 1, 0, false, 0.0f};
     const uint64_t slabs = (k + 63) / 64;
     constexpr uint32_t kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
     ProductPlan best{};
@@ -75,7 +76,7 @@ inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool n
             if (splits > 1) us += kLaunchUs + 2 * 4.0f / kPartialBytesUs * (float)(splits * rows * cols);
             if (us < least) {
                 least = us;
-                best = {t.br, t.bc, t.wr, t.wc, (uint32_t)splits, (uint32_t)(chunk * 64), direct};
+                best = {t.br, t.bc, t.wr, t.wc, (uint32_t)splits, (uint32_t)(chunk * 64), direct, us};
             }
         }
     }
@@ -145,15 +146,27 @@ inline uint64_t most_partial_bytes(uint64_t rows, uint64_t cols, uint64_t k, boo
     return most_of_plans(rows, cols, k, nt, true, [&](const ProductPlan &p) { return p.partial_bytes(rows, cols); });
 }
 
+// A bf16 product's operands and sizes.
+struct Product {
+    const __bf16 *v;
+    uint64_t ldv;
+    const __bf16 *u;
+    uint64_t ldu, rows, cols, k;
+    bool direct() const { return operands_direct(v, ldv, u, ldu); }
+};
+
+inline ProductArgs product_args(const Product &x, const ProductPlan &p, float *partial) {
+    return {x.v, x.u, (uint32_t)x.ldv, (uint32_t)x.ldu, (uint32_t)x.rows, (uint32_t)x.cols, (uint32_t)x.k, div_up(x.rows, p.br),
+            div_up(x.cols, p.bc), p.splits, p.k_chunk, partial, (uint32_t)round_up(x.cols, 8)};
+}
+
 // `partial` has the plan's partial_bytes.
 template <bool VMC, bool UMC, class Epi>
-int run_product(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu, uint64_t rows, uint64_t cols,
-                uint64_t k, const ProductPlan &p, float *partial, const Epi &epi) {
-    if (rows == 0 || cols == 0) return 0;
+int run_product(const char *name, const Product &x, const ProductPlan &p, float *partial, const Epi &epi) {
+    if (x.rows == 0 || x.cols == 0) return 0;
     if constexpr (!VMC && !UMC)
-        if (p.skinny()) return run_skinny(name, v, ldv, u, ldu, rows, cols, k, epi);
-    ProductArgs g{v, u, (uint32_t)ldv, (uint32_t)ldu, (uint32_t)rows, (uint32_t)cols, (uint32_t)k, div_up(rows, p.br),
-                  div_up(cols, p.bc), p.splits, p.k_chunk, partial, (uint32_t)round_up(cols, 8)};
+        if (p.skinny()) return run_skinny(name, x.v, x.ldv, x.u, x.ldu, x.rows, x.cols, x.k, epi);
+    const ProductArgs g = product_args(x, p, partial);
     const uint64_t groups = (uint64_t)g.tiles_r * g.tiles_c * g.splits;
     DKZ_REQUIRE(groups <= 0x7fffffffull);
     const dim3 grid((uint32_t)groups), four(256);
@@ -175,6 +188,63 @@ int run_product(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u
         if (g.splits > 1) return launch(name, join_kernel<1, Epi>, dim3(div_up(eights, kBlock)), dim3(kBlock), g, epi);
     }
     return 0;
+}
+
+// The two products of a backward pass, one for the input gradient (u
+// row-contiguous) and one for the weights' (both operands), in one launch of one
+// kind of tile where that takes less: it saves a launch, and the chip's emptying
+// and filling between them. The longer tiles start first. Estimated as the
+// longest tile, or all tiles' share of the chip and half a shorter one's for the
+// uneven end. Not for products whose K is cut (they fill the chip, 64x4096x4096 is
+// 1 us slower paired) nor kinds of which a compute unit holds one (nothing runs
+// beside them). A whole backward pass, apart and paired: 64x1024x1024 17.3 and 11.5
+// us, 128x4096x1000 18.8 and 13.9, 768x768x3000 31.4 and 25.6, 1536^3 37.2 and 32.4.
+inline bool plan_pair(const Product &a, const Product &b, ProductPlan &pa, ProductPlan &pb) {
+    float least = pa.us + pb.us + kLaunchUs;
+    bool found = false;
+    if (pa.splits != 1 || pb.splits != 1 || !a.direct() || !b.direct() || a.rows == 0 || a.cols == 0 || b.rows == 0 || b.cols == 0) return false;
+    for (const TileKind &t : kTileKinds) {
+        if (t.occupancy == 1) continue;
+        const uint64_t slabs_a = (a.k + 63) / 64, slabs_b = (b.k + 63) / 64;
+        const uint64_t tiles_a = (uint64_t)div_up(a.rows, t.br) * div_up(a.cols, t.bc), tiles_b = (uint64_t)div_up(b.rows, t.br) * div_up(b.cols, t.bc);
+        const uint64_t each = std::min<uint64_t>((tiles_a + tiles_b + kComputeUnits - 1) / kComputeUnits, t.occupancy);
+        const float us_a = (float)slabs_a * t.slab[each - 1] + t.fixed, us_b = (float)slabs_b * t.slab[each - 1] + t.fixed;
+        const float all = ((float)tiles_a * us_a + (float)tiles_b * us_b) / (float)(kComputeUnits * each);
+        // A product's tile takes as long as beside the others of its kind.
+        const auto alone = [&](uint64_t slabs, uint64_t tiles) {
+            return (float)slabs * t.slab[std::min<uint64_t>((tiles + kComputeUnits - 1) / kComputeUnits, t.occupancy) - 1] + t.fixed;
+        };
+        const float us = std::max(std::max(alone(slabs_a, tiles_a), alone(slabs_b, tiles_b)), all + 0.5f * std::min(us_a, us_b));
+        if (us >= least || tiles_a + tiles_b > 0x7fffffffull) continue;
+        least = us;
+        pa = {t.br, t.bc, t.wr, t.wc, 1, (uint32_t)(slabs_a * 64), true, us};
+        pb = {t.br, t.bc, t.wr, t.wc, 1, (uint32_t)(slabs_b * 64), true, us};
+        found = true;
+    }
+    return found;
+}
+
+template <class T, class Epi>
+int launch_pair(const char *name, const ProductArgs &a, const Epi &epi_a, const ProductArgs &b, const Epi &epi_b) {
+    const uint32_t tiles_a = a.tiles_r * a.tiles_c, tiles_b = b.tiles_r * b.tiles_c;
+    return launch(name, product_pair_kernel<T, Epi>, dim3(tiles_a + tiles_b), dim3(T::kThreads), a, epi_a, b, epi_b, tiles_a, a.k >= b.k);
+}
+
+// The products of a backward pass, each null if it is not wanted.
+template <class Epi>
+int run_gradients(const char *name_a, const Product *to_input, const Epi &epi_a, const char *name_b, const Product *to_weights, const Epi &epi_b,
+                  float *partial) {
+    ProductPlan pa{}, pb{};
+    if (to_input != nullptr) pa = plan_product(to_input->rows, to_input->cols, to_input->k, false, true, to_input->direct());
+    if (to_weights != nullptr) pb = plan_product(to_weights->rows, to_weights->cols, to_weights->k, false, true, to_weights->direct());
+    if (to_input == nullptr || to_weights == nullptr || !plan_pair(*to_input, *to_weights, pa, pb)) {
+        if (to_weights != nullptr) DKZ_TRY((run_product<true, true>(name_b, *to_weights, pb, partial, epi_b)));
+        return to_input == nullptr ? 0 : run_product<false, true>(name_a, *to_input, pa, partial, epi_a);
+    }
+    const Product &a = *to_input, &b = *to_weights;
+    const ProductArgs ga = product_args(a, pa, nullptr), gb = product_args(b, pb, nullptr);
+    if (pa.bc == 128) return launch_pair<Tile64x128>(name_a, ga, epi_a, gb, epi_b);
+    return launch_pair<Tile64>(name_a, ga, epi_a, gb, epi_b);
 }
 
 }  // namespace

@@ -219,6 +219,13 @@ def test_backward_shapes_and_alignments(pool, kind, shape, shift):
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("shape", [(1024, 1000, 1024), (100, 8, 32768), (4096, 16, 512), (64, 24, 40), (129, 30, 33)], ids=str)
+def test_backward_many_and_few_rows(pool, kind, shape):
+    """Bias sums in one launch and in two, eight columns a thread and one, both products in one launch."""
+    run_backward(pool, kind, *shape, RELU, 0.5, False, beta=0.5)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
 @pytest.mark.parametrize("act", [LOGISTIC, RELU, LINEAR, TANH, ELU, SELU])
 @pytest.mark.parametrize("prob", [0.0, 0.5])
 def test_backward_activations(pool, kind, act, prob):
