@@ -33,7 +33,7 @@ constexpr float kLaunchUs = 3.0f, kPartialBytesUs = 4e6f;  // a launch, and byte
 constexpr uint32_t kComputeUnits = 256;
 
 // How a product is cut: tiles of br x bc, each by wr x wc waves; K in `splits`
-// ranges of k_chunk. br 0: the kernel for few rows.
+// ranges of k_chunk. br 0: the kernel for few rows, bc its columns a workgroup.
 struct ProductPlan {
     uint32_t br, bc, wr, wc, splits, k_chunk;
     bool direct;  // operands straight to LDS
@@ -43,7 +43,7 @@ struct ProductPlan {
         return splits > 1 ? padded(4 * (uint64_t)splits * rows * round_up(cols, 8)) : 0;
     }
     // How many parts of a row, and of a column, an epilogue sees one at a time.
-    uint64_t row_parts(uint64_t cols) const { return skinny() ? div_up(cols, skinny_columns(cols)) : (uint64_t)div_up(cols, bc) * wc; }
+    uint64_t row_parts(uint64_t cols) const { return (uint64_t)div_up(cols, bc) * (skinny() ? 1 : wc); }
     uint64_t column_parts(uint64_t rows) const { return skinny() ? rows : (uint64_t)div_up(rows, br) * wr; }
 };
 
@@ -58,7 +58,7 @@ inline bool operands_direct(const __bf16 *v, uint64_t ldv, const __bf16 *u, uint
 // slabs x a slab's time; ranges add their partials' way out and back and the
 // launch that joins them.
 inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool nt, bool may_split, bool direct) {
-    if (nt && few_rows(rows)) return {0, 0, 0, 0, 1, 0, false, 0.0f};
+    if (nt && few_rows(rows)) return {0, skinny_columns(rows, cols, k), 0, 0, 1, 0, false, 0.0f};
     const uint64_t slabs = (k + 63) / 64;
     constexpr uint32_t kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
     ProductPlan best{};
@@ -165,7 +165,7 @@ template <bool VMC, bool UMC, class Epi>
 int run_product(const char *name, const Product &x, const ProductPlan &p, float *partial, const Epi &epi) {
     if (x.rows == 0 || x.cols == 0) return 0;
     if constexpr (!VMC && !UMC)
-        if (p.skinny()) return run_skinny(name, x.v, x.ldv, x.u, x.ldu, x.rows, x.cols, x.k, epi);
+        if (p.skinny()) return run_skinny(name, x.v, x.ldv, x.u, x.ldu, x.rows, x.cols, x.k, p.bc, epi);
     const ProductArgs g = product_args(x, p, partial);
     const uint64_t groups = (uint64_t)g.tiles_r * g.tiles_c * g.splits;
     DKZ_REQUIRE(groups <= 0x7fffffffull);

@@ -3,10 +3,11 @@
 // the weights' way from memory.
 //
 // A workgroup takes 16 * CT columns and all rows, its waves a share of K each:
-// no LDS on the way, a lane loads eight k of a weight row straight into an operand of v_mfma_f32_16x16x32_bf16 and eight of
-// an input row, which the caches hold, into the other. Each wave keeps two
-// steps of 64 k in flight beside the one it multiplies. The waves' sums meet in
-// LDS in wave order, and the epilogue takes them from there.
+// no LDS on the way, a lane loads eight k of a weight row straight into an operand
+// of v_mfma_f32_16x16x32_bf16 and eight of an input row, which the caches hold,
+// into the other. Each wave keeps two or four steps of 64 k in flight. The waves'
+// sums meet in LDS in wave order, and the epilogue takes them from there. One row
+// of 4096 to 16384 outputs 25.1 us (5.3 TB/s), 32768 47.8, 4096 9.
 #pragma once
 
 #include "dense_internal.hpp"
@@ -21,19 +22,20 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 // Rows at most: 4096x4096 weights take 7.8 us at one row, 9.8 at 16 and 13.2 at 32,
 // where tiles take 13.6 (at 64 they take no more, this kernel 20.4).
 constexpr uint32_t kSkinnyRows = 32;
+constexpr int kSkinnyWaves = 4;
 inline bool few_rows(uint64_t rows) { return rows <= kSkinnyRows; }
 
 // ODD: rows may start inside a 4-byte word.
-template <int RT, int CT, int WAVES, bool ODD, class Epi>
-__global__ __launch_bounds__(64 * WAVES) void skinny_kernel(ProductArgs g, Epi epi) {
-    constexpr int kCols = 16 * CT, kRows = 16 * RT, kPitch = kCols + 4;
-    __shared__ __align__(16) float sums[WAVES][kRows][kPitch];
+template <int RT, int CT, bool ODD, class Epi>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(ProductArgs g, Epi epi) {
+    constexpr int kCols = 16 * CT, kRows = 16 * RT, kPitch = kCols + 4, kWaves = kSkinnyWaves;
+    __shared__ __align__(16) float sums[kWaves][kRows][kPitch];
     // In a scalar, so that what depends on it is a branch: matrix instructions take no notice of masked lanes.
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, group = lane >> 4;
     const uint32_t c0 = xcd_run(blockIdx.x, gridDim.x) * kCols;
     // This wave's K: whole steps of 64 but for the last wave's end.
-    const uint32_t steps = (g.k + 63) / 64, per = (steps + WAVES - 1) / WAVES;
+    const uint32_t steps = (g.k + 63) / 64, per = (steps + kWaves - 1) / kWaves;
     const uint32_t first = min(wave * per, steps), last = min(first + per, steps);
 
     f32x4v acc[CT][RT] = {};
@@ -126,28 +128,39 @@ __global__ __launch_bounds__(64 * WAVES) void skinny_kernel(ProductArgs g, Epi e
             *reinterpret_cast<f32x4v *>(&sums[wave][16 * j + l16][16 * i + 4 * group]) = acc[i][j];
     __syncthreads();
     // A thread an element, the columns along the lanes.
-    for (uint32_t e = threadIdx.x; e < kRows * kCols; e += 64 * WAVES) {
+    for (uint32_t e = threadIdx.x; e < kRows * kCols; e += 64 * kWaves) {
         const uint32_t r = e / kCols, c = e % kCols;
         float z = sums[0][r][c];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) z += sums[w][r][c];
+        for (int w = 1; w < kWaves; ++w) z += sums[w][r][c];
         epi.template skinny<kCols>(r, c0 + c, z, g.rows, g.cols, c0 / kCols);
     }
 }
 
-// Columns of a workgroup: 32 where that fills the chip, else 16.
-inline uint32_t skinny_columns(uint64_t cols) { return cols >= 32 * 512 ? 32 : 16; }
+// Columns of a workgroup, 16 or 32. (Eight waves and 16 columns take as long as four
+// or, 1x16384x4096, a third longer.) Up to 16 rows: what gives the compute
+// units as many workgroups each, as far as it can, 32 where both do; but 16 where K
+// is long (us for 32 and 16 columns at K 4096: 8192 columns 13.6 and 15.0, 18432
+// 31.4 and 26.7, 24576 35.6 and 38.7; 8192x8192 30.9 and 28.4). More rows: 32 unless
+// that leaves compute units without (20 rows, K 4096: 4096 columns 16.4 and 12.3, 6144
+// 16.6 and 21.1, 16384 32.0 and 43.1).
+inline uint32_t skinny_columns(uint64_t rows, uint64_t cols, uint64_t k) {
+    constexpr uint64_t kUnits = 256;
+    if (rows > 16) return cols > 16 * kUnits ? 32 : 16;
+    const auto rounded = [&](uint64_t width) { return round_up((cols + width - 1) / width, kUnits) * width; };
+    return k < 8192 && rounded(32) <= rounded(16) ? 32 : 16;
+}
 
-template <int RT, int CT, int WAVES, class Epi>
+template <int RT, int CT, class Epi>
 int launch_skinny(const char *name, dim3 grid, const ProductArgs &g, const Epi &epi) {
     const bool odd = ((g.ldv | g.ldu) & 1) != 0 || (((uintptr_t)g.v | (uintptr_t)g.u) & 3) != 0;
-    if (odd) return launch(name, skinny_kernel<RT, CT, WAVES, true, Epi>, grid, dim3(64 * WAVES), g, epi);
-    return launch(name, skinny_kernel<RT, CT, WAVES, false, Epi>, grid, dim3(64 * WAVES), g, epi);
+    if (odd) return launch(name, skinny_kernel<RT, CT, true, Epi>, grid, dim3(64 * kSkinnyWaves), g, epi);
+    return launch(name, skinny_kernel<RT, CT, false, Epi>, grid, dim3(64 * kSkinnyWaves), g, epi);
 }
 
 template <class Epi>
 int run_skinny(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu, uint64_t rows, uint64_t cols, uint64_t k,
-               const Epi &epi) {
+               uint32_t width, const Epi &epi) {
     ProductArgs g{};
     g.v = v;
     g.u = u;
@@ -156,14 +169,9 @@ int run_skinny(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u,
     g.rows = (uint32_t)rows;
     g.cols = (uint32_t)cols;
     g.k = (uint32_t)k;
-    const uint32_t width = skinny_columns(cols);
     const dim3 grid(div_up(cols, width));
-    if (width == 32) {
-        if (rows <= 16) return launch_skinny<1, 2, 4>(name, grid, g, epi);
-        return launch_skinny<2, 2, 4>(name, grid, g, epi);
-    }
-    if (rows <= 16) return k < 1024 ? launch_skinny<1, 1, 4>(name, grid, g, epi) : launch_skinny<1, 1, 8>(name, grid, g, epi);
-    return launch_skinny<2, 1, 8>(name, grid, g, epi);
+    if (rows <= 16) return width == 32 ? launch_skinny<1, 2>(name, grid, g, epi) : launch_skinny<1, 1>(name, grid, g, epi);
+    return width == 32 ? launch_skinny<2, 2>(name, grid, g, epi) : launch_skinny<2, 1>(name, grid, g, epi);
 }
 
 }  // namespace

@@ -72,6 +72,12 @@ def test_forward_shapes_and_alignments(pool, kind, shape, shift):
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("shape", [(1, 70, 8192), (16, 129, 8190), (3, 8200, 9000), (17, 64, 5001), (32, 200, 4097)], ids=str)
+def test_forward_few_rows_of_many_outputs(pool, kind, shape):
+    run_forward(pool, kind, *shape, RELU, 0.2, True, True, True)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
 @pytest.mark.parametrize("act", [LOGISTIC, RELU, LINEAR, TANH, LEAKY, ELU, SELU])
 @pytest.mark.parametrize("extras", [(0.0, False, False, False), (0.5, False, True, True), (0.0, True, False, True)], ids=str)
 def test_forward_activations_and_operands(pool, kind, act, extras):
