@@ -480,39 +480,40 @@ struct PieceEpilogue : TileEpilogue<PieceEpilogue> {
     }
 };
 
-int forward(int type, uint64_t rows, uint64_t inputs, uint64_t classes, const void *input, const void *weights,
+int forward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint64_t classes, const void *input, const void *weights,
             const float *biases, const int *targets, float *loss, float *lse, const ForwardPlan &plan, Workspace ws) {
     constexpr const char *kName = "linear_cross_entropy";
     if (classes == 0)
-        return launch("linear_cross_entropy_none", no_classes_kernel, dim3(div_up(rows, kBlock)), dim3(kBlock), (uint32_t)rows, loss, lse);
+        return launch_on(stream, "linear_cross_entropy_none", no_classes_kernel, dim3(div_up(rows, kBlock)), dim3(kBlock), (uint32_t)rows, loss, lse);
     float *target_logit = ws.take<float>(plan.target / 4);
     Stat *stats = ws.take<Stat>(plan.stats / sizeof(Stat));
     if (type == DKZ_BF16) {
         Matrix x{static_cast<const __bf16 *>(input), inputs}, w{static_cast<const __bf16 *>(weights), inputs};
-        if (!few_rows(rows)) DKZ_TRY(pack(x, rows, w, classes, inputs, ws));
+        if (!few_rows(rows)) DKZ_TRY(pack(stream, x, rows, w, classes, inputs, ws));
         const ProductPlan p = plan_product(rows, classes, inputs, true, false, operands_direct(x.p, x.ld, w.p, w.ld));
         const uint32_t parts = (uint32_t)p.row_parts(classes);
         const StatEpilogue epi{biases, targets, stats, target_logit, parts};
-        DKZ_TRY((run_product<false, false>(kName, {x.p, x.ld, w.p, w.ld, rows, classes, inputs}, p, nullptr, epi)));
-        return launch("linear_cross_entropy_merge", merge_stats_kernel, dim3(std::min((uint32_t)rows, kRowGroups)), dim3(kBlock), stats,
+        DKZ_TRY((run_product<false, false>(stream, kName, {x.p, x.ld, w.p, w.ld, rows, classes, inputs}, p, nullptr, epi)));
+        return launch_on(stream, "linear_cross_entropy_merge", merge_stats_kernel, dim3(std::min((uint32_t)rows, kRowGroups)), dim3(kBlock), stats,
                       parts, targets, target_logit, (uint32_t)rows, (uint32_t)classes, loss, lse);
     }
     float *logits = ws.take<float>(plan.logits / 4), *partial = ws.take<float>(plan.partial / 4);
     for (uint64_t first = 0; first < classes; first += plan.piece) {
         const uint64_t n = std::min(plan.piece, classes - first), ld = round_up(n, 4);
         const LogitEpilogue epi(biases != nullptr ? biases + first : nullptr, logits, ld);
-        DKZ_TRY((run_f32<kRowMajor, kRowMajor>(kName, static_cast<const float *>(input), inputs,
+        DKZ_TRY((run_f32<kRowMajor, kRowMajor>(stream, kName, static_cast<const float *>(input), inputs,
                                                static_cast<const float *>(weights) + first * inputs, inputs, 0.0f, (float *)nullptr, ld,
                                                rows, n, inputs, partial, epi)));
-        DKZ_TRY(launch("linear_cross_entropy_stats", row_stats_kernel, dim3(std::min((uint32_t)rows, kRowGroups)), dim3(kStatThreads), logits,
-                       (uint32_t)ld, (uint32_t)rows, (uint32_t)n, (uint32_t)first, (uint32_t)classes, targets, stats, target_logit, loss, lse));
+        DKZ_TRY(launch_on(stream, "linear_cross_entropy_stats", row_stats_kernel, dim3(std::min((uint32_t)rows, kRowGroups)),
+                          dim3(kStatThreads), logits, (uint32_t)ld, (uint32_t)rows, (uint32_t)n, (uint32_t)first, (uint32_t)classes, targets,
+                          stats, target_logit, loss, lse));
     }
     return 0;
 }
 
 constexpr const char *kWeights = "linear_cross_entropy_weights", *kInput = "linear_cross_entropy_input";
 
-int backward_f32(uint64_t rows, uint64_t inputs, uint64_t classes, const float *input, const float *weights, const float *biases,
+int backward_f32(hipStream_t stream, uint64_t rows, uint64_t inputs, uint64_t classes, const float *input, const float *weights, const float *biases,
                  const RowGradient &grad, float beta, float *bias_updates, float *weight_updates, float *input_delta,
                  const BackwardPlan &plan, Workspace ws) {
     float *d = ws.take<float>(plan.d / 4), *sums = ws.take<float>(plan.sums / 4), *partial = ws.take<float>(plan.partial / 4);
@@ -521,30 +522,31 @@ int backward_f32(uint64_t rows, uint64_t inputs, uint64_t classes, const float *
         const float *w = weights + first * inputs;
         if (rows != 0) {
             const LogitEpilogue epi(biases != nullptr ? biases + first : nullptr, d, ld);
-            DKZ_TRY((run_f32<kRowMajor, kRowMajor>("linear_cross_entropy_logits", input, inputs, w, inputs, 0.0f, (float *)nullptr, ld, rows,
+            DKZ_TRY((run_f32<kRowMajor, kRowMajor>(stream, "linear_cross_entropy_logits", input, inputs, w, inputs, 0.0f, (float *)nullptr, ld, rows,
                                                    n, inputs, partial, epi)));
-            DKZ_TRY(launch("linear_cross_entropy_gradient", logit_gradient_kernel, dim3(div_up(ld, 128) * (uint32_t)chunks), dim3(kBlock),
-                           d, (uint32_t)ld, (uint32_t)rows, (uint32_t)n, (uint32_t)first, div_up(ld, 128), grad, bias_updates != nullptr ? sums : nullptr));
+            DKZ_TRY(launch_on(stream, "linear_cross_entropy_gradient", logit_gradient_kernel, dim3(div_up(ld, 128) * (uint32_t)chunks), dim3(kBlock),
+                              d, (uint32_t)ld, (uint32_t)rows, (uint32_t)n, (uint32_t)first, div_up(ld, 128), grad,
+                              bias_updates != nullptr ? sums : nullptr));
         }
-        if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
+        if (bias_updates != nullptr) DKZ_TRY(add_column_sums(stream, sums, chunks, n, beta, bias_updates + first));
         if (weight_updates != nullptr)
-            DKZ_TRY((run_f32<kColMajor, kColMajor>(kWeights, d, ld, input, inputs, beta, weight_updates + first * inputs, inputs, n, inputs,
+            DKZ_TRY((run_f32<kColMajor, kColMajor>(stream, kWeights, d, ld, input, inputs, beta, weight_updates + first * inputs, inputs, n, inputs,
                                                    rows, partial)));
         if (input_delta != nullptr)
-            DKZ_TRY((run_f32<kRowMajor, kColMajor>(kInput, d, ld, w, inputs, first == 0 ? 0.0f : 1.0f, input_delta, inputs, rows, inputs, n,
+            DKZ_TRY((run_f32<kRowMajor, kColMajor>(stream, kInput, d, ld, w, inputs, first == 0 ? 0.0f : 1.0f, input_delta, inputs, rows, inputs, n,
                                                    partial)));
     }
     return 0;
 }
 
-int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16 *input, const __bf16 *weights, const float *biases,
-                  const RowGradient &grad, float beta, float *bias_updates, __bf16 *weight_updates, __bf16 *input_delta,
-                  const BackwardPlan &plan, Workspace ws) {
+int backward_bf16(hipStream_t stream, uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16 *input, const __bf16 *weights,
+                  const float *biases, const RowGradient &grad, float beta, float *bias_updates, __bf16 *weight_updates,
+                  __bf16 *input_delta, const BackwardPlan &plan, Workspace ws) {
     __bf16 *d = ws.take<__bf16>(plan.d / 2);
     float *sums = ws.take<float>(plan.sums / 4), *accumulate = ws.take<float>(plan.accumulate / 4);
     float *partial = ws.take<float>(plan.partial / 4);
     Matrix x{input, inputs}, all{weights, inputs};
-    if (rows != 0) DKZ_TRY(pack(x, rows, all, classes, inputs, ws));
+    if (rows != 0) DKZ_TRY(pack(stream, x, rows, all, classes, inputs, ws));
     for (uint64_t first = 0; first < classes; first += plan.piece) {
         const __bf16 *w = all.p + first * all.ld;
         const uint64_t n = std::min(plan.piece, classes - first), ldd = round_up(n, 8);
@@ -553,14 +555,14 @@ int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16
         const uint64_t chunks = p.column_parts(rows);
         const GradientEpilogue epi{biases != nullptr ? biases + first : nullptr, grad, d, (uint32_t)ldd, (uint32_t)first,
                                             bias_updates != nullptr ? sums : nullptr};
-        DKZ_TRY((run_product<false, false>("linear_cross_entropy_gradient", {x.p, x.ld, w, all.ld, rows, n, inputs}, p, nullptr, epi)));
-        if (bias_updates != nullptr) DKZ_TRY(add_column_sums(sums, chunks, n, beta, bias_updates + first));
+        DKZ_TRY((run_product<false, false>(stream, "linear_cross_entropy_gradient", {x.p, x.ld, w, all.ld, rows, n, inputs}, p, nullptr, epi)));
+        if (bias_updates != nullptr) DKZ_TRY(add_column_sums(stream, sums, chunks, n, beta, bias_updates + first));
         const Product to_input{d, ldd, w, all.ld, rows, inputs, n}, to_weights{d, ldd, x.p, x.ld, n, inputs, rows};
         __bf16 *updates = weight_updates != nullptr ? weight_updates + first * inputs : nullptr;
         const auto epi_weights = store_epilogue<__bf16>(updates, nullptr, inputs, beta);
         const bool one = n == classes;
-        DKZ_TRY(run_gradients(kInput, one && input_delta != nullptr ? &to_input : nullptr, store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f),
-                              kWeights, updates != nullptr ? &to_weights : nullptr, epi_weights, partial));
+        DKZ_TRY(run_gradients(stream, kInput, one && input_delta != nullptr ? &to_input : nullptr,
+                              store_epilogue<__bf16>(input_delta, nullptr, inputs, 0.0f), kWeights, updates != nullptr ? &to_weights : nullptr, epi_weights, partial));
         if (!one && input_delta != nullptr) {
             PieceEpilogue e;
             e.sum = accumulate;
@@ -568,7 +570,7 @@ int backward_bf16(uint64_t rows, uint64_t inputs, uint64_t classes, const __bf16
             e.ld = (uint32_t)inputs;
             e.begin = first == 0;
             e.words = e.out == nullptr || rows_in_words<__bf16>(inputs, e.out);
-            DKZ_TRY((run_product<false, true>(kInput, to_input, plan_product(rows, inputs, n, false, true, to_input.direct()), partial, e)));
+            DKZ_TRY((run_product<false, true>(stream, kInput, to_input, plan_product(rows, inputs, n, false, true, to_input.direct()), partial, e)));
         }
     }
     return 0;
@@ -617,7 +619,7 @@ int dkz_linear_cross_entropy_forward(int type, int rows, int inputs, int classes
     const Span writes[] = {{loss, 4 * m}, {lse, 4 * m}, {workspace, plan.total()}};
     const Span reads[] = {{input, m * k * size}, {weights, n * k * size}, {biases, 4 * n}, {targets, 4 * m}};
     DKZ_REQUIRE(disjoint(writes, reads));
-    return forward(type, m, k, n, input, weights, biases, targets, loss, lse, plan, {static_cast<char *>(workspace), plan.total()});
+    return forward(current_stream(), type, m, k, n, input, weights, biases, targets, loss, lse, plan, {static_cast<char *>(workspace), plan.total()});
 }
 
 int dkz_linear_cross_entropy_backward_workspace(int type, int rows, int inputs, int classes, size_t *least, size_t *best) {
@@ -661,18 +663,19 @@ int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classe
     DKZ_REQUIRE(disjoint(writes, reads));
     const RowGradient grad{targets, lse, row_scales, scale, (uint32_t)n};
     const Workspace ws{static_cast<char *>(workspace), plan.total()};
+    const hipStream_t stream = current_stream();
     if (n == 0) {  // no class pulls at the input
         if (input_delta == nullptr || m * k == 0) return 0;
         if (type == DKZ_F32)
-            return run_f32<kRowMajor, kColMajor>(kInput, (const float *)nullptr, 0, (const float *)nullptr, k, 0.0f,
+            return run_f32<kRowMajor, kColMajor>(stream, kInput, (const float *)nullptr, 0, (const float *)nullptr, k, 0.0f,
                                                  static_cast<float *>(input_delta), k, m, k, 0, nullptr);
-        return run_product<false, true>(kInput, {nullptr, 0, nullptr, k, m, k, 0}, plan_product(m, k, 0, false, false, true), nullptr,
+        return run_product<false, true>(stream, kInput, {nullptr, 0, nullptr, k, m, k, 0}, plan_product(m, k, 0, false, false, true), nullptr,
                                         store_epilogue<__bf16>(input_delta, nullptr, k, 0.0f));
     }
     if (type == DKZ_F32)
-        return backward_f32(m, k, n, static_cast<const float *>(input), static_cast<const float *>(weights), biases, grad, beta,
+        return backward_f32(stream, m, k, n, static_cast<const float *>(input), static_cast<const float *>(weights), biases, grad, beta,
                             bias_updates, static_cast<float *>(weight_updates), static_cast<float *>(input_delta), plan, ws);
-    return backward_bf16(m, k, n, static_cast<const __bf16 *>(input), static_cast<const __bf16 *>(weights), biases, grad, beta, bias_updates,
+    return backward_bf16(stream, m, k, n, static_cast<const __bf16 *>(input), static_cast<const __bf16 *>(weights), biases, grad, beta, bias_updates,
                          static_cast<__bf16 *>(weight_updates), static_cast<__bf16 *>(input_delta), plan, ws);
 }
 

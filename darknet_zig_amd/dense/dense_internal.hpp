@@ -1,7 +1,9 @@
 // dense_internal.hpp -- what the sources of libdkz_dense.so share: the element
 // types, the argument checks and the caller's workspace. The stream, the
 // sync-after-launch switch and the launch helper are dkz_internal.hpp's, over
-// libdkz.so's own state (runtime.hip).
+// libdkz.so's own state (runtime.hip). The stream is the process's and another host
+// thread may set it at any time: an op reads it once and passes it on, so that
+// launches that wait for each other are on one stream.
 #pragma once
 
 #include <hip/hip_runtime.h>

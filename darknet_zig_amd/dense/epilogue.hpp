@@ -175,10 +175,10 @@ __global__ __launch_bounds__(kBlock) void column_sums_kernel(const float *partia
     updates[c] = beta == 0.0f ? (float)s : beta * updates[c] + (float)s;
 }
 
-inline int add_column_sums(const float *partial, uint64_t chunks, uint64_t cols, float beta, float *updates) {
+inline int add_column_sums(hipStream_t stream, const float *partial, uint64_t chunks, uint64_t cols, float beta, float *updates) {
     if (cols == 0) return 0;
-    return launch("bias_updates", column_sums_kernel, dim3(div_up(cols, 32)), dim3(kBlock), partial, (uint32_t)chunks, (uint32_t)cols, beta,
-                  updates);
+    return launch_on(stream, "bias_updates", column_sums_kernel, dim3(div_up(cols, 32)), dim3(kBlock), partial, (uint32_t)chunks,
+                     (uint32_t)cols, beta, updates);
 }
 
 }  // namespace

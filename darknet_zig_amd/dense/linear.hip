@@ -24,21 +24,21 @@ LinearEpilogue<T, EXP> linear_epilogue(uint64_t outputs, int act, const Draws &d
 }
 
 template <bool EXP>
-int forward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act, const Draws &draws, const void *input,
+int forward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act, const Draws &draws, const void *input,
             const void *weights, const float *biases, const void *residual, void *activated, void *output, Workspace ws) {
     constexpr const char *kName = "linear_forward";
     if (type == DKZ_F32) {
         float *partial = ws.take<float>(f32_partial_bytes(rows, outputs, inputs) / 4);
-        return run_f32<kRowMajor, kRowMajor>(kName, static_cast<const float *>(input), inputs,
+        return run_f32<kRowMajor, kRowMajor>(stream, kName, static_cast<const float *>(input), inputs,
                                              static_cast<const float *>(weights), inputs, 0.0f, (float *)nullptr, outputs, rows,
                                              outputs, inputs, partial,
                                              linear_epilogue<float, EXP>(outputs, act, draws, biases, residual, activated, output));
     }
     Matrix x{static_cast<const __bf16 *>(input), inputs}, w{static_cast<const __bf16 *>(weights), inputs};
-    if (!few_rows(rows)) DKZ_TRY(pack(x, rows, w, outputs, inputs, ws));
+    if (!few_rows(rows)) DKZ_TRY(pack(stream, x, rows, w, outputs, inputs, ws));
     const ProductPlan p = plan_product(rows, outputs, inputs, true, true, operands_direct(x.p, x.ld, w.p, w.ld));
     float *partial = ws.take<float>(p.partial_bytes(rows, outputs) / 4);
-    return run_product<false, false>(kName, {x.p, x.ld, w.p, w.ld, rows, outputs, inputs}, p, partial,
+    return run_product<false, false>(stream, kName, {x.p, x.ld, w.p, w.ld, rows, outputs, inputs}, p, partial,
                                      linear_epilogue<__bf16, EXP>(outputs, act, draws, biases, residual, activated, output));
 }
 
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *
 
 // bias_updates null: not wanted; sums: room for the sums of every kDeltaRows rows.
 template <class T>
-int run_delta(const T *delta, const T *activated, uint64_t rows, uint64_t cols, int act, const Draws &draws, T *d, uint64_t ldd,
+int run_delta(hipStream_t stream, const T *delta, const T *activated, uint64_t rows, uint64_t cols, int act, const Draws &draws, T *d, uint64_t ldd,
               float *sums, float beta, float *bias_updates) {
     constexpr const char *kName = "linear_backward_delta";
     const bool whole = rows <= kDeltaWhole;
@@ -134,12 +134,12 @@ int run_delta(const T *delta, const T *activated, uint64_t rows, uint64_t cols, 
     const uint32_t blocks_c = div_up(eights ? cols : ldd, eights ? 32 * 8 : 32);
     const dim3 grid(blocks_c * blocks_r), block(kBlock);
     const auto run = [&](auto kernel) {
-        return launch(kName, kernel, grid, block, delta, activated, (uint32_t)rows, (uint32_t)cols, act, draws, d, (uint32_t)ldd, blocks_c, beta,
-                      bias_updates == nullptr ? nullptr : whole ? bias_updates : sums);
+        return launch_on(stream, kName, kernel, grid, block, delta, activated, (uint32_t)rows, (uint32_t)cols, act, draws, d, (uint32_t)ldd,
+                         blocks_c, beta, bias_updates == nullptr ? nullptr : whole ? bias_updates : sums);
     };
     if (whole) return eights ? run(delta_kernel<T, 8, true>) : run(delta_kernel<T, 1, true>);
     DKZ_TRY(eights ? run(delta_kernel<T, 8, false>) : run(delta_kernel<T, 1, false>));
-    return bias_updates != nullptr ? add_column_sums(sums, div_up(rows, kDeltaRows), cols, beta, bias_updates) : 0;
+    return bias_updates != nullptr ? add_column_sums(stream, sums, div_up(rows, kDeltaRows), cols, beta, bias_updates) : 0;
 }
 
 // Leading dimension of d in the workspace: whole 16-byte chunks.
@@ -162,7 +162,7 @@ BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t ou
 }
 
 template <class T>
-int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act, const Draws &draws, const void *input,
+int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act, const Draws &draws, const void *input,
              const void *weights, const void *activated, const void *delta, const void *input_residual, float beta,
              float *bias_updates, void *weight_updates, void *input_delta, Workspace ws) {
     const BackwardPlan plan = backward_plan(type, rows, inputs, outputs);
@@ -177,28 +177,28 @@ int backward(int type, uint64_t rows, uint64_t inputs, uint64_t outputs, int act
         ldd = outputs;
     }
     if (rows != 0 && outputs != 0 && (bias_updates != nullptr || d != nullptr))
-        DKZ_TRY(run_delta(static_cast<const T *>(delta), static_cast<const T *>(activated), rows, outputs, act, draws, d, ldd, sums, beta,
+        DKZ_TRY(run_delta(stream, static_cast<const T *>(delta), static_cast<const T *>(activated), rows, outputs, act, draws, d, ldd, sums, beta,
                           bias_updates));
     else if (bias_updates != nullptr)
-        DKZ_TRY(add_column_sums(sums, 0, outputs, beta, bias_updates));  // no rows: beta * bias_updates
+        DKZ_TRY(add_column_sums(stream, sums, 0, outputs, beta, bias_updates));  // no rows: beta * bias_updates
     const T *dd = d != nullptr ? d : static_cast<const T *>(delta);
     constexpr const char *kWeights = "linear_backward_weights", *kInput = "linear_backward_input";
     if constexpr (sizeof(T) == 4) {
         const T *x = static_cast<const T *>(input), *w = static_cast<const T *>(weights);
         if (weight_updates != nullptr)
-            DKZ_TRY((run_f32<kColMajor, kColMajor>(kWeights, dd, ldd, x, inputs, beta, static_cast<float *>(weight_updates),
+            DKZ_TRY((run_f32<kColMajor, kColMajor>(stream, kWeights, dd, ldd, x, inputs, beta, static_cast<float *>(weight_updates),
                                                    inputs, outputs, inputs, rows, partial)));
         if (input_delta != nullptr)
-            DKZ_TRY((run_f32<kRowMajor, kColMajor>(kInput, dd, ldd, w, inputs, 0.0f, (float *)nullptr, inputs, rows, inputs,
+            DKZ_TRY((run_f32<kRowMajor, kColMajor>(stream, kInput, dd, ldd, w, inputs, 0.0f, (float *)nullptr, inputs, rows, inputs,
                                                    outputs, partial, store_epilogue<T>(input_delta, input_residual, inputs, 0.0f))));
     } else {
         Matrix x{weight_updates != nullptr ? static_cast<const T *>(input) : nullptr, inputs};
         Matrix w{input_delta != nullptr ? static_cast<const T *>(weights) : nullptr, inputs};
-        if (rows != 0) DKZ_TRY(pack(x, rows, w, outputs, inputs, ws));
+        if (rows != 0) DKZ_TRY(pack(stream, x, rows, w, outputs, inputs, ws));
         const Product to_input{dd, ldd, w.p, w.ld, rows, inputs, outputs}, to_weights{dd, ldd, x.p, x.ld, outputs, inputs, rows};
         const auto epi_input = store_epilogue<T>(input_delta, input_residual, inputs, 0.0f);
         const auto epi_weights = store_epilogue<T>(weight_updates, nullptr, inputs, beta);
-        DKZ_TRY(run_gradients(kInput, input_delta != nullptr ? &to_input : nullptr, epi_input, kWeights,
+        DKZ_TRY(run_gradients(stream, kInput, input_delta != nullptr ? &to_input : nullptr, epi_input, kWeights,
                               weight_updates != nullptr ? &to_weights : nullptr, epi_weights, partial));
     }
     return 0;
@@ -244,11 +244,12 @@ int dkz_linear_forward(int type, int rows, int inputs, int outputs, int activati
     DKZ_REQUIRE(disjoint(writes, reads));
     const Draws draws = make_draws(prob, scale, seed, first);
     const Workspace ws{static_cast<char *>(workspace), need};
+    const hipStream_t stream = current_stream();
     // Activations with an exponential are kernels of their own: in one kernel they cost the others too (8192x4096x16384
     // with leaky and dropout 1000 us alone, 1590 beside them).
     return uses_exp(activation)
-               ? forward<true>(type, m, k, n, activation, draws, input, weights, biases, residual, activated, output, ws)
-               : forward<false>(type, m, k, n, activation, draws, input, weights, biases, residual, activated, output, ws);
+               ? forward<true>(stream, type, m, k, n, activation, draws, input, weights, biases, residual, activated, output, ws)
+               : forward<false>(stream, type, m, k, n, activation, draws, input, weights, biases, residual, activated, output, ws);
 }
 
 int dkz_linear_backward_workspace(int type, int rows, int inputs, int outputs, size_t *bytes) {
@@ -291,10 +292,11 @@ int dkz_linear_backward(int type, int rows, int inputs, int outputs, int activat
     DKZ_REQUIRE(disjoint(writes, reads));
     const Draws draws = make_draws(prob, scale, seed, first);
     const Workspace ws{static_cast<char *>(workspace), need};
+    const hipStream_t stream = current_stream();
     if (type == DKZ_F32)
-        return backward<float>(type, m, k, n, activation, draws, input, weights, activated, delta, input_residual, beta,
+        return backward<float>(stream, type, m, k, n, activation, draws, input, weights, activated, delta, input_residual, beta,
                                bias_updates, weight_updates, input_delta, ws);
-    return backward<__bf16>(type, m, k, n, activation, draws, input, weights, activated, delta, input_residual, beta,
+    return backward<__bf16>(stream, type, m, k, n, activation, draws, input, weights, activated, delta, input_residual, beta,
                             bias_updates, weight_updates, input_delta, ws);
 }
 

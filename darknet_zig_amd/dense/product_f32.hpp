@@ -27,19 +27,19 @@ inline uint64_t f32_partial_bytes(uint64_t m, uint64_t n, uint64_t k) {
 }
 
 template <Operand AK, Operand BK, class... Epi>
-int launch_f32_tiles(const char *name, const Tiling &t, dim3 grid, const SplitArgs &g, const Epi &...epi) {
+int launch_f32_tiles(hipStream_t stream, const char *name, const Tiling &t, dim3 grid, const SplitArgs &g, const Epi &...epi) {
     const dim3 block(kBlock);
-    if (t.bm == 128 && t.bn == 128) return launch(name, gemm_split_kernel<128, 128, AK, BK, false, Epi...>, grid, block, g, epi...);
-    if (t.bm == 128) return launch(name, gemm_split_kernel<128, 64, AK, BK, false, Epi...>, grid, block, g, epi...);
-    if (t.bm == 64 && t.bn == 128) return launch(name, gemm_split_kernel<64, 128, AK, BK, false, Epi...>, grid, block, g, epi...);
-    if (t.bm == 32) return launch(name, gemm_split_kernel<32, 128, AK, BK, false, Epi...>, grid, block, g, epi...);
-    return launch(name, gemm_split_kernel<64, 64, AK, BK, false, Epi...>, grid, block, g, epi...);
+    if (t.bm == 128 && t.bn == 128) return launch_on(stream, name, gemm_split_kernel<128, 128, AK, BK, false, Epi...>, grid, block, g, epi...);
+    if (t.bm == 128) return launch_on(stream, name, gemm_split_kernel<128, 64, AK, BK, false, Epi...>, grid, block, g, epi...);
+    if (t.bm == 64 && t.bn == 128) return launch_on(stream, name, gemm_split_kernel<64, 128, AK, BK, false, Epi...>, grid, block, g, epi...);
+    if (t.bm == 32) return launch_on(stream, name, gemm_split_kernel<32, 128, AK, BK, false, Epi...>, grid, block, g, epi...);
+    return launch_on(stream, name, gemm_split_kernel<64, 64, AK, BK, false, Epi...>, grid, block, g, epi...);
 }
 
 // C (m x n, leading dimension ldc) = beta * C + op(A) op(B), or every element of the product to `epi`.
 // kRowMajor: A is m x k, B n x k; kColMajor: A is k x m, B k x n. `partial` has f32_partial_bytes.
 template <Operand AK, Operand BK, class... Epi>
-int run_f32(const char *name, const float *a, uint64_t lda, const float *b, uint64_t ldb, float beta, float *c, uint64_t ldc,
+int run_f32(hipStream_t stream, const char *name, const float *a, uint64_t lda, const float *b, uint64_t ldb, float beta, float *c, uint64_t ldc,
             uint64_t m, uint64_t n, uint64_t k, float *partial, const Epi &...epi) {
     if (m == 0 || n == 0) return 0;
     const Tiling t = plan_f32(m, n, k);
@@ -74,22 +74,22 @@ int run_f32(const char *name, const float *a, uint64_t lda, const float *b, uint
         total = t.full_tiles + g.runs;
     }
     DKZ_REQUIRE(total <= 0x7fffffffull);
-    DKZ_TRY((launch_f32_tiles<AK, BK, Epi...>(name, t, dim3((uint32_t)total), g, epi...)));
+    DKZ_TRY((launch_f32_tiles<AK, BK, Epi...>(stream, name, t, dim3((uint32_t)total), g, epi...)));
     const bool v4 = n % 4 == 0 && ldc % 4 == 0 && aligned16(c);
     const dim3 block(kBlock);
     if (t.stream) {
         const dim3 blocks(streamed * (t.bm * t.bn / 4 / kBlock));
-        return v4 ? launch(name, stream_reduce_kernel<true, Epi...>, blocks, block, g, epi...)
-                  : launch(name, stream_reduce_kernel<false, Epi...>, blocks, block, g, epi...);
+        return v4 ? launch_on(stream, name, stream_reduce_kernel<true, Epi...>, blocks, block, g, epi...)
+                  : launch_on(stream, name, stream_reduce_kernel<false, Epi...>, blocks, block, g, epi...);
     }
     if (g.splits == 1) return 0;
     const bool many = g.splits > 32;
     const dim3 blocks(div_up(m * n / (v4 ? 4 : 1), many ? kBlock / 16 : kBlock));
     if (v4)
-        return many ? launch(name, split_reduce_kernel<true, 16, Epi...>, blocks, block, g, epi...)
-                    : launch(name, split_reduce_kernel<true, 1, Epi...>, blocks, block, g, epi...);
-    return many ? launch(name, split_reduce_kernel<false, 16, Epi...>, blocks, block, g, epi...)
-                : launch(name, split_reduce_kernel<false, 1, Epi...>, blocks, block, g, epi...);
+        return many ? launch_on(stream, name, split_reduce_kernel<true, 16, Epi...>, blocks, block, g, epi...)
+                    : launch_on(stream, name, split_reduce_kernel<true, 1, Epi...>, blocks, block, g, epi...);
+    return many ? launch_on(stream, name, split_reduce_kernel<false, 16, Epi...>, blocks, block, g, epi...)
+                : launch_on(stream, name, split_reduce_kernel<false, 1, Epi...>, blocks, block, g, epi...);
 }
 
 }  // namespace

@@ -124,14 +124,14 @@ struct Matrix {
 };
 
 // Copies a and b (null: left out) to the workspace where their rows are no whole chunks.
-inline int pack(Matrix &a, uint64_t rows_a, Matrix &b, uint64_t rows_b, uint64_t k, Workspace &ws) {
+inline int pack(hipStream_t stream, Matrix &a, uint64_t rows_a, Matrix &b, uint64_t rows_b, uint64_t k, Workspace &ws) {
     if (k % 8 == 0) return 0;
     const uint64_t ld = packed_ld(k), na = a.p != nullptr ? rows_a : 0, nb = b.p != nullptr ? rows_b : 0;
     __bf16 *to_a = ws.take<__bf16>(packed_bytes(rows_a, k) / 2), *to_b = ws.take<__bf16>(packed_bytes(rows_b, k) / 2);
     const uint64_t chunks = (na + nb) * (ld / 8);
     if (chunks != 0)
-        DKZ_TRY(launch("pack", pack_kernel, dim3(div_up(chunks, kBlock)), dim3(kBlock), a.p, (uint32_t)na, to_a, b.p, (uint32_t)nb, to_b,
-                       (uint32_t)k, make_fastdiv((uint32_t)(ld / 8))));
+        DKZ_TRY(launch_on(stream, "pack", pack_kernel, dim3(div_up(chunks, kBlock)), dim3(kBlock), a.p, (uint32_t)na, to_a, b.p, (uint32_t)nb, to_b,
+                          (uint32_t)k, make_fastdiv((uint32_t)(ld / 8))));
     if (na) a = {to_a, ld};
     if (nb) b = {to_b, ld};
     return 0;
@@ -162,30 +162,30 @@ inline ProductArgs product_args(const Product &x, const ProductPlan &p, float *p
 
 // `partial` has the plan's partial_bytes.
 template <bool VMC, bool UMC, class Epi>
-int run_product(const char *name, const Product &x, const ProductPlan &p, float *partial, const Epi &epi) {
+int run_product(hipStream_t stream, const char *name, const Product &x, const ProductPlan &p, float *partial, const Epi &epi) {
     if (x.rows == 0 || x.cols == 0) return 0;
     if constexpr (!VMC && !UMC)
-        if (p.skinny()) return run_skinny(name, x.v, x.ldv, x.u, x.ldu, x.rows, x.cols, x.k, p.bc, epi);
+        if (p.skinny()) return run_skinny(stream, name, x.v, x.ldv, x.u, x.ldu, x.rows, x.cols, x.k, p.bc, epi);
     const ProductArgs g = product_args(x, p, partial);
     const uint64_t groups = (uint64_t)g.tiles_r * g.tiles_c * g.splits;
     DKZ_REQUIRE(groups <= 0x7fffffffull);
     const dim3 grid((uint32_t)groups), four(256);
     if (!p.direct) {
-        if (p.br == 128) DKZ_TRY(launch(name, product_kernel<Tile128, VMC, UMC, false, Epi>, grid, four, g, epi));
-        else DKZ_TRY(launch(name, product_kernel<Tile64, VMC, UMC, false, Epi>, grid, four, g, epi));
+        if (p.br == 128) DKZ_TRY(launch_on(stream, name, product_kernel<Tile128, VMC, UMC, false, Epi>, grid, four, g, epi));
+        else DKZ_TRY(launch_on(stream, name, product_kernel<Tile64, VMC, UMC, false, Epi>, grid, four, g, epi));
     } else if (p.br == 256) {
-        DKZ_TRY(launch(name, product_kernel<Tile256, VMC, UMC, true, Epi>, grid, dim3(Tile256::kThreads), g, epi));
+        DKZ_TRY(launch_on(stream, name, product_kernel<Tile256, VMC, UMC, true, Epi>, grid, dim3(Tile256::kThreads), g, epi));
     } else if (p.br == 128) {
-        DKZ_TRY(launch(name, product_kernel<Tile128, VMC, UMC, true, Epi>, grid, four, g, epi));
+        DKZ_TRY(launch_on(stream, name, product_kernel<Tile128, VMC, UMC, true, Epi>, grid, four, g, epi));
     } else if (p.bc == 128) {
-        DKZ_TRY(launch(name, product_kernel<Tile64x128, VMC, UMC, true, Epi>, grid, four, g, epi));
+        DKZ_TRY(launch_on(stream, name, product_kernel<Tile64x128, VMC, UMC, true, Epi>, grid, four, g, epi));
     } else {
-        DKZ_TRY(launch(name, product_kernel<Tile64, VMC, UMC, true, Epi>, grid, four, g, epi));
+        DKZ_TRY(launch_on(stream, name, product_kernel<Tile64, VMC, UMC, true, Epi>, grid, four, g, epi));
     }
     if constexpr (Epi::kElementwise) {
         const uint64_t eights = (uint64_t)g.rows * (g.ldp / 8);
-        if (g.splits > 4) return launch(name, join_kernel<8, Epi>, dim3(div_up(eights, kBlock / 8)), dim3(kBlock), g, epi);
-        if (g.splits > 1) return launch(name, join_kernel<1, Epi>, dim3(div_up(eights, kBlock)), dim3(kBlock), g, epi);
+        if (g.splits > 4) return launch_on(stream, name, join_kernel<8, Epi>, dim3(div_up(eights, kBlock / 8)), dim3(kBlock), g, epi);
+        if (g.splits > 1) return launch_on(stream, name, join_kernel<1, Epi>, dim3(div_up(eights, kBlock)), dim3(kBlock), g, epi);
     }
     return 0;
 }
@@ -225,26 +225,26 @@ inline bool plan_pair(const Product &a, const Product &b, ProductPlan &pa, Produ
 }
 
 template <class T, class Epi>
-int launch_pair(const char *name, const ProductArgs &a, const Epi &epi_a, const ProductArgs &b, const Epi &epi_b) {
+int launch_pair(hipStream_t stream, const char *name, const ProductArgs &a, const Epi &epi_a, const ProductArgs &b, const Epi &epi_b) {
     const uint32_t tiles_a = a.tiles_r * a.tiles_c, tiles_b = b.tiles_r * b.tiles_c;
-    return launch(name, product_pair_kernel<T, Epi>, dim3(tiles_a + tiles_b), dim3(T::kThreads), a, epi_a, b, epi_b, tiles_a, a.k >= b.k);
+    return launch_on(stream, name, product_pair_kernel<T, Epi>, dim3(tiles_a + tiles_b), dim3(T::kThreads), a, epi_a, b, epi_b, tiles_a, a.k >= b.k);
 }
 
 // The products of a backward pass, each null if it is not wanted.
 template <class Epi>
-int run_gradients(const char *name_a, const Product *to_input, const Epi &epi_a, const char *name_b, const Product *to_weights, const Epi &epi_b,
-                  float *partial) {
+int run_gradients(hipStream_t stream, const char *name_a, const Product *to_input, const Epi &epi_a, const char *name_b,
+                  const Product *to_weights, const Epi &epi_b, float *partial) {
     ProductPlan pa{}, pb{};
     if (to_input != nullptr) pa = plan_product(to_input->rows, to_input->cols, to_input->k, false, true, to_input->direct());
     if (to_weights != nullptr) pb = plan_product(to_weights->rows, to_weights->cols, to_weights->k, false, true, to_weights->direct());
     if (to_input == nullptr || to_weights == nullptr || !plan_pair(*to_input, *to_weights, pa, pb)) {
-        if (to_weights != nullptr) DKZ_TRY((run_product<true, true>(name_b, *to_weights, pb, partial, epi_b)));
-        return to_input == nullptr ? 0 : run_product<false, true>(name_a, *to_input, pa, partial, epi_a);
+        if (to_weights != nullptr) DKZ_TRY((run_product<true, true>(stream, name_b, *to_weights, pb, partial, epi_b)));
+        return to_input == nullptr ? 0 : run_product<false, true>(stream, name_a, *to_input, pa, partial, epi_a);
     }
     const Product &a = *to_input, &b = *to_weights;
     const ProductArgs ga = product_args(a, pa, nullptr), gb = product_args(b, pb, nullptr);
-    if (pa.bc == 128) return launch_pair<Tile64x128>(name_a, ga, epi_a, gb, epi_b);
-    return launch_pair<Tile64>(name_a, ga, epi_a, gb, epi_b);
+    if (pa.bc == 128) return launch_pair<Tile64x128>(stream, name_a, ga, epi_a, gb, epi_b);
+    return launch_pair<Tile64>(stream, name_a, ga, epi_a, gb, epi_b);
 }
 
 }  // namespace

@@ -152,15 +152,15 @@ inline uint32_t skinny_columns(uint64_t rows, uint64_t cols, uint64_t k) {
 }
 
 template <int RT, int CT, class Epi>
-int launch_skinny(const char *name, dim3 grid, const ProductArgs &g, const Epi &epi) {
+int launch_skinny(hipStream_t stream, const char *name, dim3 grid, const ProductArgs &g, const Epi &epi) {
     const bool odd = ((g.ldv | g.ldu) & 1) != 0 || (((uintptr_t)g.v | (uintptr_t)g.u) & 3) != 0;
-    if (odd) return launch(name, skinny_kernel<RT, CT, true, Epi>, grid, dim3(64 * kSkinnyWaves), g, epi);
-    return launch(name, skinny_kernel<RT, CT, false, Epi>, grid, dim3(64 * kSkinnyWaves), g, epi);
+    if (odd) return launch_on(stream, name, skinny_kernel<RT, CT, true, Epi>, grid, dim3(64 * kSkinnyWaves), g, epi);
+    return launch_on(stream, name, skinny_kernel<RT, CT, false, Epi>, grid, dim3(64 * kSkinnyWaves), g, epi);
 }
 
 template <class Epi>
-int run_skinny(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu, uint64_t rows, uint64_t cols, uint64_t k,
-               uint32_t width, const Epi &epi) {
+int run_skinny(hipStream_t stream, const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u, uint64_t ldu, uint64_t rows,
+               uint64_t cols, uint64_t k, uint32_t width, const Epi &epi) {
     ProductArgs g{};
     g.v = v;
     g.u = u;
@@ -170,8 +170,8 @@ int run_skinny(const char *name, const __bf16 *v, uint64_t ldv, const __bf16 *u,
     g.cols = (uint32_t)cols;
     g.k = (uint32_t)k;
     const dim3 grid(div_up(cols, width));
-    if (rows <= 16) return width == 32 ? launch_skinny<1, 2>(name, grid, g, epi) : launch_skinny<1, 1>(name, grid, g, epi);
-    return width == 32 ? launch_skinny<2, 2>(name, grid, g, epi) : launch_skinny<2, 1>(name, grid, g, epi);
+    if (rows <= 16) return width == 32 ? launch_skinny<1, 2>(stream, name, grid, g, epi) : launch_skinny<1, 1>(stream, name, grid, g, epi);
+    return width == 32 ? launch_skinny<2, 2>(stream, name, grid, g, epi) : launch_skinny<2, 1>(stream, name, grid, g, epi);
 }
 
 }  // namespace

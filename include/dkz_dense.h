@@ -3,10 +3,11 @@
  * layers with their bias, activation, dropout and residual, and a softmax
  * cross-entropy over many classes) as fused gfx950 kernels over fp32 or bf16
  * tensors. A companion of libdkz.so (dkz_ops.h), beside which it is installed
- * and which it loads: ops are issued on dkz_set_stream's stream, wait for their
- * kernels under dkz_set_sync_after_launch, and return 0 or a hipError_t that
- * dkz_error_string decodes. dkz_dense_last_error_context has the text of the
- * last nonzero return of this library's calls on this host thread.
+ * and which it loads: ops are issued on dkz_set_stream's stream -- all launches
+ * of a call on the one that is set as it begins --, wait for their kernels under
+ * dkz_set_sync_after_launch, and return 0 or a hipError_t that dkz_error_string
+ * decodes. dkz_dense_last_error_context has the text of the last nonzero return
+ * of this library's calls on this host thread.
  *
  * The reference runs these as separate ops: a connected layer's gemm, addBias
  * and activateArray, randUniform + dropout with the draws kept for the backward
@@ -29,9 +30,11 @@
  *   - The ops keep no scratch of their own: what they need is the caller's
  *     workspace (16-byte aligned device memory, contents irrelevant before and
  *     after; null where 0 bytes are needed). Calls with workspaces of their own
- *     may overlap on any streams, host threads and captured graphs. Nothing is
- *     allocated, copied to the host or waited for, and every op may be captured
- *     in a graph. Pointers belong to the current device.
+ *     may overlap on any streams, host threads and captured graphs. (The stream is
+ *     the process's: host threads that set streams of their own take a lock from
+ *     dkz_set_stream to the call's return.) Nothing is allocated, copied to the
+ *     host or waited for, and every op may be captured in a graph. Pointers belong
+ *     to the current device.
  *   - Sums are taken in an order that depends on sizes, the tensors' alignment and
  *     the workspace's size alone: the same call gives the same bits.
  */

@@ -34,6 +34,8 @@ def _ensure_built() -> None:
         native_build.build()
     if not native_build.GPUTEST.exists():
         native_build.build_gputest()
+    if not native_build.LAUNCHES.exists():
+        native_build.build_launches()
 
 
 _ensure_built()

@@ -5,7 +5,9 @@
   inside libdkz.so; the host half is built for x86-64-v3 (AVX2 + FMA);
 * tests/native/gputest, gputest.zig's CPU-vs-GPU check written against the
   C++ host mirror (darknet_zig_amd/host/dkz_gpu.hpp), linked with libdkz.so
-  and the CPU oracle. It needs both built first.
+  and the CPU oracle. It needs both built first;
+* tests/native/liblaunches.so, which stands in for the HIP runtime's launches
+  (launches.cpp) in the CPU tests of what the libraries launch.
 """
 
 from __future__ import annotations
@@ -23,6 +25,8 @@ SRC = HERE / "dkz_checks.hip"
 LIB = HERE / "libdkz_checks.so"
 GPUTEST_SRC = HERE / "gputest.cpp"
 GPUTEST = HERE / "gputest"
+LAUNCHES_SRC = HERE / "launches.cpp"
+LAUNCHES = HERE / "liblaunches.so"
 ROOT = HERE.parents[1]
 
 
@@ -35,6 +39,7 @@ def build() -> Path:
         raise RuntimeError(f"building {LIB.name} failed:\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, LIB)
     build_gputest()
+    build_launches()
     return LIB
 
 
@@ -50,6 +55,16 @@ def build_gputest() -> Path:
         raise RuntimeError(f"building {GPUTEST.name} failed:\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, GPUTEST)
     return GPUTEST
+
+
+def build_launches() -> Path:
+    tmp = LAUNCHES.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", "-shared", "-fPIC", str(LAUNCHES_SRC), "-o", str(tmp)]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"building {LAUNCHES.name} failed:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, LAUNCHES)
+    return LAUNCHES
 
 
 if __name__ == "__main__":

@@ -1,0 +1,66 @@
+"""What the dense operators launch, on the CPU (tests/launches.py): kernels, grids and streams."""
+
+from __future__ import annotations
+
+import pytest
+
+from tests import launches
+from tests.launches import buf, in_child, recorded
+
+F32, BF16, LEAKY = 0, 1, 7
+
+
+def forward(kind, rows, inputs, outputs, shift=0):
+    from darknet_zig_amd import gpu
+
+    gpu.linearForward(kind, rows, inputs, outputs, LEAKY, 0.5, 2.0, 1, 0, buf(1, shift), buf(2, shift), buf(3), buf(4, shift), buf(5, shift),
+                      buf(6, shift), buf(7))
+
+
+def backward(kind, rows, inputs, outputs, shift=0):
+    from darknet_zig_amd import gpu
+
+    gpu.linearBackward(kind, rows, inputs, outputs, LEAKY, 0.5, 2.0, 1, 0, buf(1, shift), buf(2, shift), buf(3, shift), buf(4, shift),
+                       buf(5, shift), 0.5, buf(6), buf(7, shift), buf(8, shift), buf(9))
+
+
+def loss(kind, rows, inputs, classes, least=False, shift=0):
+    from darknet_zig_amd import gpu
+
+    ws = gpu.Buf(buf(7).ptr, gpu.linearCrossEntropyForwardWorkspace(kind, rows, inputs, classes)[0 if least else 1] // 4)
+    gpu.linearCrossEntropyForward(kind, rows, inputs, classes, buf(1, shift), buf(2, shift), buf(3), buf(4), buf(5), buf(6), ws)
+
+
+def gradients(kind, rows, inputs, classes, least=False, shift=0):
+    from darknet_zig_amd import gpu
+
+    ws = gpu.Buf(buf(10).ptr, gpu.linearCrossEntropyBackwardWorkspace(kind, rows, inputs, classes)[0 if least else 1] // 4)
+    gpu.linearCrossEntropyBackward(kind, rows, inputs, classes, buf(1, shift), buf(2, shift), buf(3), buf(4), buf(5), buf(6), 1.0, 0.5, buf(7),
+                                   buf(8, shift), buf(9, shift), ws)
+
+
+CALLS = {"forward": forward, "backward": backward, "loss": loss, "gradients": gradients}
+
+
+# ---- streams ----
+
+# Ops of several launches each: packing, ranges of K and their join, delta and its sums, pieces of the classes.
+SEVERAL = [("forward", BF16, 40, 4097, 100), ("forward", F32, 256, 4096, 4096), ("backward", BF16, 300, 129, 200),
+           ("backward", BF16, 8192, 4096, 4096), ("backward", F32, 300, 129, 200), ("loss", BF16, 200, 65, 1000),
+           ("loss", F32, 200, 65, 1000, True), ("gradients", BF16, 200, 65, 1000, True), ("gradients", F32, 200, 65, 1000, True),
+           ("gradients", BF16, 128, 4096, 1000)]
+
+
+def streams_of(name, *args):
+    """The streams of a call's launches, another host thread setting another stream behind each."""
+    from darknet_zig_amd import _lib
+
+    lib = _lib.load()
+    lib.dkz_set_stream(0x1000)
+    return [x.stream for x in recorded(lambda: CALLS[name](*args), after=lambda: lib.dkz_set_stream(0x2000))]
+
+
+@pytest.mark.parametrize("call", SEVERAL, ids=str)
+def test_an_op_s_launches_are_of_one_stream(call):
+    streams = in_child("tests.test_dense_launches:streams_of", *call)
+    assert len(streams) > 1 and set(streams) == {0x1000}, streams
