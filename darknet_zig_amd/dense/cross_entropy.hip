@@ -381,11 +381,11 @@ struct ForwardPlan {
     uint64_t logits, stats, target, packed, partial;
     uint64_t total() const { return logits + stats + target + packed + partial; }
 };
-ForwardPlan forward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t classes, uint64_t piece_bytes) {
+ForwardPlan forward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t classes, uint64_t piece) {
     ForwardPlan p{};
     p.target = padded(4 * rows);
     if (type == DKZ_F32) {
-        p.piece = piece_of(classes, piece_bytes, 4 * rows);
+        p.piece = piece;
         p.logits = padded(4 * rows * p.piece);
         p.stats = padded(sizeof(Stat) * rows);
         const uint64_t last = classes % p.piece;
@@ -403,10 +403,10 @@ struct BackwardPlan {
     uint64_t piece, d, sums, accumulate, packed, partial;
     uint64_t total() const { return d + sums + accumulate + packed + partial; }
 };
-BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t classes, uint64_t piece_bytes) {
+BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t classes, uint64_t piece) {
     BackwardPlan p{};
     const uint64_t size = type_size(type);
-    p.piece = piece_of(classes, piece_bytes, size * rows);
+    p.piece = piece;
     p.d = padded(size * rows * p.piece);
     const uint64_t last = classes % p.piece, whole = classes >= p.piece ? p.piece : 0;
     if (type == DKZ_F32) {
@@ -431,26 +431,41 @@ BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t cl
     return p;
 }
 
-// The plan with the largest piece, of powers of two of kPieceBytes, that `bytes` has room for.
-template <class Plan>
-bool fit_plan(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int type, uint64_t rows, uint64_t inputs, uint64_t classes,
-              uint64_t bytes, Plan &plan) {
+// Calls f with the plans of pieces of at most kPieceBytes, half of that, and so on, the largest first, until it returns
+// true; whether it did. Most halvings leave a piece as it is, bounded at both ends: each piece is planned once, as planning
+// costs the host microseconds (1x432x8493 fp32: all 31 halvings 60 us, the first plan 4).
+template <class Plan, class F>
+bool each_plan(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int type, uint64_t rows, uint64_t inputs, uint64_t classes, F f) {
+    uint64_t last = ~0ull;
     for (uint64_t most = kPieceBytes;; most /= 2) {
-        plan = make(type, rows, inputs, classes, most);
-        if (plan.total() <= bytes) return true;
+        const uint64_t piece = piece_of(classes, most, type_size(type) * rows);
+        if (piece != last && f(make(type, rows, inputs, classes, piece))) return true;
         if (most == 0) return false;
+        last = piece;
     }
 }
 
-// The bytes of the smallest of these plans (not always the one with the smallest pieces: one piece needs no fp32 sums of
-// the input gradient).
+// The first of these plans that `bytes` has room for.
 template <class Plan>
-uint64_t least_plan(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int type, uint64_t rows, uint64_t inputs, uint64_t classes) {
-    uint64_t least = ~0ull;
-    for (uint64_t most = kPieceBytes;; most /= 2) {
-        least = std::min(least, make(type, rows, inputs, classes, most).total());
-        if (most == 0) return least;
-    }
+bool fit_plan(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int type, uint64_t rows, uint64_t inputs, uint64_t classes,
+              uint64_t bytes, Plan &plan) {
+    return each_plan(make, type, rows, inputs, classes, [&](const Plan &p) {
+        plan = p;
+        return p.total() <= bytes;
+    });
+}
+
+// The bytes of the smallest of these plans (not always the one with the smallest pieces: one piece needs no fp32 sums of
+// the input gradient), and of the first.
+template <class Plan>
+void plan_bytes(Plan (*make)(int, uint64_t, uint64_t, uint64_t, uint64_t), int type, uint64_t rows, uint64_t inputs, uint64_t classes,
+                size_t *least, size_t *best) {
+    *least = *best = 0;
+    each_plan(make, type, rows, inputs, classes, [&](const Plan &p) {
+        if (*best == 0) *least = *best = (size_t)p.total();
+        *least = std::min(*least, (size_t)p.total());
+        return false;
+    });
 }
 
 // The input gradient of one of several pieces: added up in fp32, the last one rounded to out.
@@ -592,8 +607,8 @@ int dkz_linear_cross_entropy_forward_workspace(int type, int rows, int inputs, i
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(classes, inputs);
     const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes;
-    *least = m == 0 || n == 0 ? 0 : (size_t)least_plan(forward_plan, type, m, k, n);
-    *best = m == 0 || n == 0 ? 0 : (size_t)forward_plan(type, m, k, n, kPieceBytes).total();
+    *least = *best = 0;
+    if (m != 0 && n != 0) plan_bytes(forward_plan, type, m, k, n, least, best);
     return 0;
 }
 
@@ -631,8 +646,8 @@ int dkz_linear_cross_entropy_backward_workspace(int type, int rows, int inputs, 
     DKZ_REQUIRE_ELEMS(rows, inputs);
     DKZ_REQUIRE_ELEMS(classes, inputs);
     const uint64_t m = (uint64_t)rows, k = (uint64_t)inputs, n = (uint64_t)classes;
-    *least = n == 0 ? 0 : (size_t)least_plan(backward_plan, type, m, k, n);
-    *best = n == 0 ? 0 : (size_t)backward_plan(type, m, k, n, kPieceBytes).total();
+    *least = *best = 0;
+    if (n != 0) plan_bytes(backward_plan, type, m, k, n, least, best);
     return 0;
 }
 
@@ -655,8 +670,8 @@ int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classe
     }
     BackwardPlan plan{};
     if (n != 0) {
-        DKZ_REQUIRE(least_plan(backward_plan, type, m, k, n) == 0 || (workspace != nullptr && aligned16(workspace)));
         DKZ_REQUIRE(fit_plan(backward_plan, type, m, k, n, workspace_bytes, plan));
+        DKZ_REQUIRE(plan.total() == 0 || (workspace != nullptr && aligned16(workspace)));
     }
     const Span writes[] = {{bias_updates, 4 * n}, {weight_updates, n * k * size}, {input_delta, m * k * size}, {workspace, plan.total()}};
     const Span reads[] = {{input, m * k * size}, {weights, n * k * size}, {biases, 4 * n}, {targets, 4 * m}, {lse, 4 * m}, {row_scales, 4 * m}};

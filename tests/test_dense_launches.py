@@ -64,3 +64,42 @@ def streams_of(name, *args):
 def test_an_op_s_launches_are_of_one_stream(call):
     streams = in_child("tests.test_dense_launches:streams_of", *call)
     assert len(streams) > 1 and set(streams) == {0x1000}, streams
+
+
+# ---- the host's part of a call ----
+
+
+def host_time(shapes):
+    """us of the host in a call of the loss and of its gradients, nothing being launched: the least of many."""
+    from time import perf_counter
+
+    from darknet_zig_amd import _lib, gpu
+
+    lib, out = _lib.load_dense(), []
+    p = [buf(i).ptr for i in range(12)]
+    for kind, rows, inputs, classes, least in shapes:
+        need = [f(kind, rows, inputs, classes)[0 if least else 1]
+                for f in (gpu.linearCrossEntropyForwardWorkspace, gpu.linearCrossEntropyBackwardWorkspace)]
+        ends = []
+        for call in (lambda: lib.dkz_linear_cross_entropy_forward(kind, rows, inputs, classes, p[1], p[2], p[3], p[4], p[5], p[6], p[7], need[0]),
+                     lambda: lib.dkz_linear_cross_entropy_backward(kind, rows, inputs, classes, p[1], p[2], p[3], p[4], p[6], None, 1.0, 0.0,
+                                                                   p[8], p[9], p[10], p[11], need[1])):
+            best = 1.0
+            for _ in range(30):
+                t = perf_counter()
+                for _ in range(20):
+                    assert call() == 0
+                best = min(best, (perf_counter() - t) / 20)
+            ends.append(best * 1e6)
+        out.append(ends)
+    return out
+
+
+def test_the_gradients_are_planned_as_often_as_they_are_needed():
+    """A backward pass is at most three products where a forward pass is one, so its host time is a few times the forward's;
+    it was 15 to 30 times that when every call searched for the smallest workspace."""
+    shapes = [(kind, *shape, least) for kind in (F32, BF16) for shape in ((1, 432, 8493), (8, 1024, 1000), (128, 4096, 1000))
+              for least in (False, True)]
+    for shape, (forth, back) in zip(shapes, in_child("tests.test_dense_launches:host_time", shapes)):
+        print(shape, round(forth, 1), round(back, 1))
+        assert shape[-1] or back < 6 * forth + 4, (shape, forth, back)
