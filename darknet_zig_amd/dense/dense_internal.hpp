@@ -232,7 +232,8 @@ inline uint64_t round_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * t
 // Matrices past the ABI's largest element count (less what rounds a load up) are refused.
 #define DKZ_REQUIRE_ELEMS(a, b) DKZ_REQUIRE((uint64_t)(a) * (uint64_t)(b) + 3 <= kMaxElems)
 
-// A launch counts its threads in 32 bits; sides up to here keep all of them well below.
+// A launch counts its threads in 32 bits. Sides up to here keep the kernels that go over rows, columns or a tensor's
+// elements below that; products of more workgroups than a launch has room for take several (run_product).
 #define DKZ_REQUIRE_SIDE(n) DKZ_REQUIRE((n) <= 1 << 26)
 
 // A call's workspace: `need` bytes at a 16-byte boundary.

@@ -51,6 +51,7 @@ struct ProductArgs {
     uint32_t tiles_r, tiles_c, splits, k_chunk;  // k_chunk: a split's K, a multiple of the slab's depth
     float *partial;                              // splits > 1: [splits][rows][ldp]
     uint32_t ldp;
+    uint32_t first_block;  // the launch's first workgroup among the product's
 };
 
 // Consecutive workgroups go round the 8 XCDs: gives each XCD a run of neighbours.
@@ -532,7 +533,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs &g, const Epi &ep
 template <class T, bool VMC, bool UMC, bool ALIGNED, class Epi>
 __global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs g, Epi epi) {
     __shared__ __align__(1024) char lds[lds_bytes<T, ALIGNED>()];
-    product_tile<T, VMC, UMC, ALIGNED>(g, epi, blockIdx.x, lds);
+    product_tile<T, VMC, UMC, ALIGNED>(g, epi, g.first_block + blockIdx.x, lds);
 }
 
 // A backward pass's two products in one launch: a's tiles (u row-contiguous

@@ -157,8 +157,12 @@ struct Product {
 
 inline ProductArgs product_args(const Product &x, const ProductPlan &p, float *partial) {
     return {x.v, x.u, (uint32_t)x.ldv, (uint32_t)x.ldu, (uint32_t)x.rows, (uint32_t)x.cols, (uint32_t)x.k, div_up(x.rows, p.br),
-            div_up(x.cols, p.bc), p.splits, p.k_chunk, partial, (uint32_t)round_up(x.cols, 8)};
+            div_up(x.cols, p.bc), p.splits, p.k_chunk, partial, (uint32_t)round_up(x.cols, 8), 0};
 }
+
+// Workgroups of a launch at most: its threads are counted in 32 bits, and 2^38 logits in tiles of 128x128 are 2^24
+// workgroups of 256. A product of more takes several launches. (A multiple of the XCDs, so that xcd_run goes on as it was.)
+constexpr uint64_t kMostGroups = 1ull << 22;
 
 // `partial` has the plan's partial_bytes.
 template <bool VMC, bool UMC, class Epi>
@@ -166,21 +170,25 @@ int run_product(hipStream_t stream, const char *name, const Product &x, const Pr
     if (x.rows == 0 || x.cols == 0) return 0;
     if constexpr (!VMC && !UMC)
         if (p.skinny()) return run_skinny(stream, name, x.v, x.ldv, x.u, x.ldu, x.rows, x.cols, x.k, p.bc, epi);
-    const ProductArgs g = product_args(x, p, partial);
+    ProductArgs g = product_args(x, p, partial);
     const uint64_t groups = (uint64_t)g.tiles_r * g.tiles_c * g.splits;
     DKZ_REQUIRE(groups <= 0x7fffffffull);
-    const dim3 grid((uint32_t)groups), four(256);
-    if (!p.direct) {
-        if (p.br == 128) DKZ_TRY(launch_on(stream, name, product_kernel<Tile128, VMC, UMC, false, Epi>, grid, four, g, epi));
-        else DKZ_TRY(launch_on(stream, name, product_kernel<Tile64, VMC, UMC, false, Epi>, grid, four, g, epi));
-    } else if (p.br == 256) {
-        DKZ_TRY(launch_on(stream, name, product_kernel<Tile256, VMC, UMC, true, Epi>, grid, dim3(Tile256::kThreads), g, epi));
-    } else if (p.br == 128) {
-        DKZ_TRY(launch_on(stream, name, product_kernel<Tile128, VMC, UMC, true, Epi>, grid, four, g, epi));
-    } else if (p.bc == 128) {
-        DKZ_TRY(launch_on(stream, name, product_kernel<Tile64x128, VMC, UMC, true, Epi>, grid, four, g, epi));
-    } else {
-        DKZ_TRY(launch_on(stream, name, product_kernel<Tile64, VMC, UMC, true, Epi>, grid, four, g, epi));
+    const dim3 four(256);
+    for (uint64_t first = 0; first < groups; first += kMostGroups) {
+        g.first_block = (uint32_t)first;
+        const dim3 grid((uint32_t)std::min(groups - first, kMostGroups));
+        if (!p.direct) {
+            if (p.br == 128) DKZ_TRY(launch_on(stream, name, product_kernel<Tile128, VMC, UMC, false, Epi>, grid, four, g, epi));
+            else DKZ_TRY(launch_on(stream, name, product_kernel<Tile64, VMC, UMC, false, Epi>, grid, four, g, epi));
+        } else if (p.br == 256) {
+            DKZ_TRY(launch_on(stream, name, product_kernel<Tile256, VMC, UMC, true, Epi>, grid, dim3(Tile256::kThreads), g, epi));
+        } else if (p.br == 128) {
+            DKZ_TRY(launch_on(stream, name, product_kernel<Tile128, VMC, UMC, true, Epi>, grid, four, g, epi));
+        } else if (p.bc == 128) {
+            DKZ_TRY(launch_on(stream, name, product_kernel<Tile64x128, VMC, UMC, true, Epi>, grid, four, g, epi));
+        } else {
+            DKZ_TRY(launch_on(stream, name, product_kernel<Tile64, VMC, UMC, true, Epi>, grid, four, g, epi));
+        }
     }
     if constexpr (Epi::kElementwise) {
         const uint64_t eights = (uint64_t)g.rows * (g.ldp / 8);

@@ -103,3 +103,30 @@ def test_the_gradients_are_planned_as_often_as_they_are_needed():
     for shape, (forth, back) in zip(shapes, in_child("tests.test_dense_launches:host_time", shapes)):
         print(shape, round(forth, 1), round(back, 1))
         assert shape[-1] or back < 6 * forth + 4, (shape, forth, back)
+
+
+# ---- grids ----
+
+# The most logits that a loss takes (2^38), in products through registers (the inputs' base off a 16-byte boundary, which are not
+# copied to the workspace: their rows are whole eights), and tensors of the most rows and columns.
+LARGEST = [("loss", BF16, 4096, 8, 1 << 26, False, 2), ("loss", BF16, 4096, 8, 1 << 26), ("loss", BF16, 1 << 26, 8, 4096, False, 2),
+           ("loss", F32, 4096, 8, 1 << 26), ("gradients", BF16, 4096, 8, 1 << 26, False, 2), ("gradients", F32, 4096, 8, 1 << 26),
+           ("gradients", BF16, 1 << 26, 8, 4096, False, 2), ("gradients", F32, 1 << 26, 8, 4096), ("forward", BF16, 1 << 26, 8, 31, 2),
+           ("forward", F32, 1 << 26, 31, 31), ("forward", BF16, 1, 31, 1 << 26, 2), ("backward", BF16, 1 << 26, 31, 31, 2),
+           ("backward", F32, 1 << 26, 31, 31), ("backward", BF16, 31, 31, 1 << 26, 2), ("backward", BF16, 31, 1 << 26, 31),
+           ("forward", BF16, 46340, 8, 46340, 2), ("backward", BF16, 46340, 8, 46340, 2)]
+
+
+def grids_of(name, *args):
+    seen = recorded(lambda: CALLS[name](*args))
+    # Few are looked at: the largest of each kernel.
+    most: dict[str, int] = {}
+    for x in seen:
+        most[x.kernel] = max(most.get(x.kernel, 0), x.threads)
+    return most
+
+
+@pytest.mark.parametrize("call", LARGEST, ids=str)
+def test_a_launch_has_fewer_than_2_to_the_32_threads(call):
+    most = in_child("tests.test_dense_launches:grids_of", *call)
+    assert most and all(0 < threads < 2**32 for threads in most.values()), most
