@@ -172,14 +172,18 @@ struct Direct {
     // Load i of a slab to LDS address `to` (the slab's). p: element (r0, k0);
     // left: k from k0 to the end, 0 past it. In asm, so that the compiler does
     // not make every later read of LDS wait for it: the loop below waits itself
-    // (await_loads).
+    // (await_loads). (The address in LDS is in m0, which the load may read two wait
+    // states after. Scalars that a vector instruction wrote would need five, which
+    // cost 0.5% in every load; in the code as it is built there are none, and a test
+    // looks.)
     __device__ __forceinline__ void load(int i, const __bf16 *p, uint32_t left, uint32_t to) const {
         const uint64_t at = (uint64_t)p;
         const i32x4 buf = {(int)(uint32_t)at, (int)(uint32_t)(at >> 32), (int)kOutside, 0x00020000};
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                      :
                      : "s"(to + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024 + i * THREADS * 16),
-                       "v"(k[i] < left ? off[i] : kOutside), "s"(buf));
+                       "v"(k[i] < left ? off[i] : kOutside), "s"(buf)
+                     : "m0");
     }
 };
 

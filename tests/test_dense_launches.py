@@ -2,6 +2,11 @@
 
 from __future__ import annotations
 
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
 import pytest
 
 from tests import launches
@@ -130,3 +135,48 @@ def grids_of(name, *args):
 def test_a_launch_has_fewer_than_2_to_the_32_threads(call):
     most = in_child("tests.test_dense_launches:grids_of", *call)
     assert most and all(0 < threads < 2**32 for threads in most.values()), most
+
+
+# ---- what the compiler is told ----
+
+
+def test_asm_names_the_registers_that_it_writes():
+    """m0 is no operand: an asm that writes it has to say so, or the compiler may keep a value there."""
+    for path in sorted((launches.ROOT / "darknet_zig_amd").rglob("*.h*")):
+        for text in re.findall(r"\basm\b[^;]*;", path.read_text()):
+            if re.search(r"\bs_\w+ m0,", text):
+                assert re.search(r':[^:]*"m0"[^:]*\)\s*;$', text), (path.name, text)
+
+
+def _scalars(operand):
+    m = re.fullmatch(r"s\[(\d+):(\d+)\]|s(\d+)", operand)
+    return set() if m is None else {int(m[3])} if m[3] else set(range(int(m[1]), int(m[2]) + 1))
+
+
+def test_loads_to_lds_wait_for_the_scalars_of_vector_instructions(tmp_path):
+    """A vector memory instruction may read a scalar register that a vector instruction wrote five wait states before, not sooner. The
+    compiler sees to that but inside an asm, where the loads to LDS are: in the code that it built none of their scalars comes so late."""
+    objdump = Path("/opt/rocm/llvm/bin/llvm-objdump")
+    if not objdump.exists():
+        pytest.skip("no llvm-objdump")
+    lib = shutil.copy(launches.ROOT / "darknet_zig_amd" / "libdkz_dense.so", tmp_path)
+    subprocess.run([objdump, "--offloading", lib], capture_output=True, check=True, cwd=tmp_path)
+    loads = 0
+    for code in sorted(tmp_path.glob("*gfx950")):
+        text = subprocess.run([objdump, "-d", "--no-show-raw-insn", code], capture_output=True, text=True, check=True).stdout
+        before: list[tuple[set[int], int, str]] = []  # the last instructions: scalars that a vector one wrote, wait states, text
+        for line in text.splitlines():
+            m = re.match(r"\s+([a-z]\w+)(.*?)\s*//", line)
+            if not m:
+                continue
+            op, args = m[1], [x.strip() for x in m[2].split(",")]
+            if op == "buffer_load_dwordx4" and "lds" in m[2]:
+                loads += 1
+                need, waited = _scalars(args[1]), 0
+                assert len(need) == 4, line
+                for written, states, what in reversed(before):
+                    assert waited >= 5 or not written & need, (what, line)
+                    waited += states
+            written = set().union(*(_scalars(a) for a in args[:2 if "_co_" in op else 1])) if op.startswith("v_") else set()
+            before = before[-8:] + [(written, int(args[0], 0) + 1 if op == "s_nop" else 1, line)]
+    assert loads > 500, loads
