@@ -9,23 +9,24 @@ from pathlib import Path
 
 import pytest
 
+from tests import dense_cases as cases
 from tests import launches
 from tests.launches import buf, in_child, recorded
 
 F32, BF16, LEAKY = 0, 1, 7
 
 
-def forward(kind, rows, inputs, outputs, shift=0):
+def forward(kind, rows, inputs, outputs, shift=0, act=LEAKY):
     from darknet_zig_amd import gpu
 
-    gpu.linearForward(kind, rows, inputs, outputs, LEAKY, 0.5, 2.0, 1, 0, buf(1, shift), buf(2, shift), buf(3), buf(4, shift), buf(5, shift),
+    gpu.linearForward(kind, rows, inputs, outputs, act, 0.5, 2.0, 1, 0, buf(1, shift), buf(2, shift), buf(3), buf(4, shift), buf(5, shift),
                       buf(6, shift), buf(7))
 
 
-def backward(kind, rows, inputs, outputs, shift=0):
+def backward(kind, rows, inputs, outputs, shift=0, act=LEAKY):
     from darknet_zig_amd import gpu
 
-    gpu.linearBackward(kind, rows, inputs, outputs, LEAKY, 0.5, 2.0, 1, 0, buf(1, shift), buf(2, shift), buf(3, shift), buf(4, shift),
+    gpu.linearBackward(kind, rows, inputs, outputs, act, 0.5, 2.0, 1, 0, buf(1, shift), buf(2, shift), buf(3, shift), buf(4, shift),
                        buf(5, shift), 0.5, buf(6), buf(7, shift), buf(8, shift), buf(9))
 
 
@@ -36,10 +37,11 @@ def loss(kind, rows, inputs, classes, least=False, shift=0):
     gpu.linearCrossEntropyForward(kind, rows, inputs, classes, buf(1, shift), buf(2, shift), buf(3), buf(4), buf(5), buf(6), ws)
 
 
-def gradients(kind, rows, inputs, classes, least=False, shift=0):
+def gradients(kind, rows, inputs, classes, least=False, shift=0, between=False):
     from darknet_zig_amd import gpu
 
-    ws = gpu.Buf(buf(10).ptr, gpu.linearCrossEntropyBackwardWorkspace(kind, rows, inputs, classes)[0 if least else 1] // 4)
+    sizes = gpu.linearCrossEntropyBackwardWorkspace(kind, rows, inputs, classes)
+    ws = gpu.Buf(buf(10).ptr, (cases.between(sizes) if between else sizes[0 if least else 1]) // 4)
     gpu.linearCrossEntropyBackward(kind, rows, inputs, classes, buf(1, shift), buf(2, shift), buf(3), buf(4), buf(5), buf(6), 1.0, 0.5, buf(7),
                                    buf(8, shift), buf(9, shift), ws)
 
@@ -108,6 +110,37 @@ def test_the_gradients_are_planned_as_often_as_they_are_needed():
     for shape, (forth, back) in zip(shapes, in_child("tests.test_dense_launches:host_time", shapes)):
         print(shape, round(forth, 1), round(back, 1))
         assert shape[-1] or back < 6 * forth + 4, (shape, forth, back)
+
+
+# ---- kernels ----
+
+
+def kernels_of_the_cases():
+    """The kernels that the cases launch of those that the library has, and those that none does."""
+    from darknet_zig_amd import gpu
+
+    seen = []
+    for kind, rows, inputs, outputs, act, shift in cases.FORWARD:
+        seen += recorded(lambda: forward(kind, rows, inputs, outputs, shift * (4 if kind == F32 else 2), act))
+    for kind, rows, inputs, outputs, act, shift in cases.BACKWARD:
+        seen += recorded(lambda: backward(kind, rows, inputs, outputs, shift * (4 if kind == F32 else 2), act))
+    for kind, rows, inputs, classes, least, shift in cases.LOSS:
+        for f in (loss, gradients):
+            seen += recorded(lambda: f(kind, rows, inputs, classes, least, shift * (4 if kind == F32 else 2)))
+    for shape in cases.PIECES:
+        seen += recorded(lambda: gradients(BF16, *shape, between=True))
+    for x, y in ((F32, F32), (F32, BF16), (BF16, F32), (BF16, BF16)):  # all of them in the tests of dropout
+        seen += recorded(lambda: gpu.seededDropout(100, x, buf(1), None, 0.5, 2.0, 1, 0, y, buf(2)))
+    seen += recorded(lambda: gpu.linearCrossEntropyForward(F32, 5, 8, 0, None, None, None, buf(1), buf(2), buf(3), None))
+    names = {x.kernel for x in seen}
+    return sorted(names), sorted(set(launches.dense_kernels) - names)
+
+
+def test_the_cases_run_every_kernel():
+    """So that no change of the rules leaves one without a GPU test (test_gpu_dense_kernels.py)."""
+    seen, missing = in_child("tests.test_dense_launches:kernels_of_the_cases")
+    assert not missing, missing
+    assert len(seen) > 180
 
 
 # ---- grids ----
