@@ -101,13 +101,13 @@ struct LinearEpilogue : TileEpilogue<LinearEpilogue<T, EXP>> {
     }
 };
 
-// out = z + beta * old + add, old being out's own value. beta 0 does not read it.
+// out = alpha * z + beta * old + add, old being out's own value. beta 0 does not read it.
 template <class T>
 struct StoreEpilogue : TileEpilogue<StoreEpilogue<T>> {
     T *out;
     const T *add;
     uint32_t ld;
-    float beta;
+    float alpha, beta;
     bool words;
 
     __device__ __forceinline__ float bias(uint32_t) const { return 0.0f; }
@@ -125,6 +125,8 @@ struct StoreEpilogue : TileEpilogue<StoreEpilogue<T>> {
     }
     template <class E, int N>
     __device__ __forceinline__ void put(const E &e, const float (&)[N], float (&z)[N], const Before<N> &b) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] *= alpha;
         if (beta != 0.0f) {
 #pragma unroll
             for (int i = 0; i < N; ++i) z[i] += beta * (float)b.old[i];
@@ -144,11 +146,12 @@ bool rows_in_words(uint64_t ld, const void *a, const void *b = nullptr, const vo
 }
 
 template <class T>
-StoreEpilogue<T> store_epilogue(void *out, const void *add, uint64_t ld, float beta) {
+StoreEpilogue<T> store_epilogue(void *out, const void *add, uint64_t ld, float beta, float alpha = 1.0f) {
     StoreEpilogue<T> e;
     e.out = static_cast<T *>(out);
     e.add = static_cast<const T *>(add);
     e.ld = (uint32_t)ld;
+    e.alpha = alpha;
     e.beta = beta;
     e.words = rows_in_words<T>(ld, out, add);
     return e;

@@ -1,5 +1,9 @@
 // linear.hip -- a connected layer with its epilogue in the product (bias,
 // activation, dropout, residual), and its backward pass.
+#include <math.h>
+
+#include <utility>
+
 #include "dense_internal.hpp"
 #include "epilogue.hpp"
 #include "product_plan.hpp"
@@ -55,7 +59,7 @@ constexpr uint32_t kDeltaWhole = 128;  // rows up to which it takes all of its c
 constexpr uint32_t kDeltaFill = 128;   // workgroups that are enough for eight columns a thread
 
 // d = dropout(delta) * gradient(activated), stored to d (null: not) in rows of
-// ldd, and the sums of kDeltaRows rows' columns to `to` (null: not). Bound by
+// ldd, and sum_scale times the sums of kDeltaRows rows' columns to `to` (null: not). Bound by
 // memory: a thread takes W columns of eight rows, all of its loads issued before
 // the first is used; the eight sums of a column's threads are added in row order.
 // W is eight where rows are whole eights and that leaves workgroups for the chip
@@ -64,7 +68,8 @@ constexpr uint32_t kDeltaFill = 128;   // workgroups that are enough for eight c
 // `to` is bias_updates itself: a launch less where there are few rows.
 template <class T, int W, bool WHOLE>
 __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *activated, uint32_t rows, uint32_t cols, int act,
-                                                      Draws draws, T *d, uint32_t ldd, uint32_t blocks_c, float beta, float *to) {
+                                                      Draws draws, T *d, uint32_t ldd, uint32_t blocks_c, float sum_scale, float beta,
+                                                      float *to) {
     constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes, kEach = kDeltaRows / kGroups;
     __shared__ float sums[kGroups][kLanes * W + 4];
     const uint32_t x = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
@@ -113,6 +118,7 @@ __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *
                 float t = sums[0][threadIdx.x];
 #pragma unroll
                 for (uint32_t i = 1; i < kGroups; ++i) t += sums[i][threadIdx.x];
+                t *= sum_scale;
                 if constexpr (WHOLE) total += (double)t;
                 else to[(uint64_t)block_r * cols + column] = t;
             }
@@ -125,8 +131,8 @@ __global__ __launch_bounds__(kBlock) void delta_kernel(const T *delta, const T *
 
 // bias_updates null: not wanted; sums: room for the sums of every kDeltaRows rows.
 template <class T>
-int run_delta(hipStream_t stream, const T *delta, const T *activated, uint64_t rows, uint64_t cols, int act, const Draws &draws, T *d, uint64_t ldd,
-              float *sums, float beta, float *bias_updates) {
+int run_delta(hipStream_t stream, const T *delta, const T *activated, uint64_t rows, uint64_t cols, int act, const Draws &draws,
+              T *d, uint64_t ldd, float sum_scale, float *sums, float beta, float *bias_updates) {
     constexpr const char *kName = "linear_backward_delta";
     const bool whole = rows <= kDeltaWhole;
     const uint32_t blocks_r = whole ? 1 : div_up(rows, kDeltaRows);
@@ -135,7 +141,7 @@ int run_delta(hipStream_t stream, const T *delta, const T *activated, uint64_t r
     const dim3 grid(blocks_c * blocks_r), block(kBlock);
     const auto run = [&](auto kernel) {
         return launch_on(stream, kName, kernel, grid, block, delta, activated, (uint32_t)rows, (uint32_t)cols, act, draws, d, (uint32_t)ldd,
-                         blocks_c, beta, bias_updates == nullptr ? nullptr : whole ? bias_updates : sums);
+                         blocks_c, sum_scale, beta, bias_updates == nullptr ? nullptr : whole ? bias_updates : sums);
     };
     if (whole) return eights ? run(delta_kernel<T, 8, true>) : run(delta_kernel<T, 1, true>);
     DKZ_TRY(eights ? run(delta_kernel<T, 8, false>) : run(delta_kernel<T, 1, false>));
@@ -170,15 +176,23 @@ int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint6
     float *sums = ws.take<float>(plan.sum_bytes / 4), *partial = ws.take<float>(plan.partial_bytes / 4);
     uint64_t ldd = delta_ld(type, outputs);
     const bool products = inputs != 0 && (weight_updates != nullptr || input_delta != nullptr);
+    // bf16 products take d / scale, and their results are multiplied by the scale in fp32: where the gradient is 0 or 1 (linear, relu)
+    // d / scale is a delta or 0 and needs no rounding, and an input or weight gradient is off by its own rounding alone (8192x4096x4096
+    // with dropout, distance from 64 bits: 0.0024 with d rounded, 0.0017 so). Other gradients' d is rounded to bf16, as any operand of
+    // a bf16 product has to be. A scale far from 1 stays with d: the sums might overflow without it, and an infinite one (all dropped)
+    // times sums of 0 is no 0.
+    Draws inner = draws;
+    float alpha = 1.0f;
+    if (sizeof(T) == 2 && fabsf(draws.scale) >= 0x1p-20f && fabsf(draws.scale) <= 0x1p20f) std::swap(alpha, inner.scale);
     // The delta itself where nothing changes it and its rows lie on 16-byte boundaries.
-    const bool same = act == kLinear && draws.limit == 0 && draws.scale == 1.0f && ldd == outputs && aligned16(delta);
+    const bool same = act == kLinear && inner.limit == 0 && inner.scale == 1.0f && ldd == outputs && aligned16(delta);
     if (same || !products) {
         d = nullptr;
         ldd = outputs;
     }
     if (rows != 0 && outputs != 0 && (bias_updates != nullptr || d != nullptr))
-        DKZ_TRY(run_delta(stream, static_cast<const T *>(delta), static_cast<const T *>(activated), rows, outputs, act, draws, d, ldd, sums, beta,
-                          bias_updates));
+        DKZ_TRY(run_delta(stream, static_cast<const T *>(delta), static_cast<const T *>(activated), rows, outputs, act, inner, d, ldd,
+                          alpha, sums, beta, bias_updates));
     else if (bias_updates != nullptr)
         DKZ_TRY(add_column_sums(stream, sums, 0, outputs, beta, bias_updates));  // no rows: beta * bias_updates
     const T *dd = d != nullptr ? d : static_cast<const T *>(delta);
@@ -196,8 +210,8 @@ int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint6
         Matrix w{input_delta != nullptr ? static_cast<const T *>(weights) : nullptr, inputs};
         if (rows != 0) DKZ_TRY(pack(stream, x, rows, w, outputs, inputs, ws));
         const Product to_input{dd, ldd, w.p, w.ld, rows, inputs, outputs}, to_weights{dd, ldd, x.p, x.ld, outputs, inputs, rows};
-        const auto epi_input = store_epilogue<T>(input_delta, input_residual, inputs, 0.0f);
-        const auto epi_weights = store_epilogue<T>(weight_updates, nullptr, inputs, beta);
+        const auto epi_input = store_epilogue<T>(input_delta, input_residual, inputs, 0.0f, alpha);
+        const auto epi_weights = store_epilogue<T>(weight_updates, nullptr, inputs, beta, alpha);
         DKZ_TRY(run_gradients(stream, kInput, input_delta != nullptr ? &to_input : nullptr, epi_input, kWeights,
                               weight_updates != nullptr ? &to_weights : nullptr, epi_weights, partial));
     }

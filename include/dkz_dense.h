@@ -102,8 +102,10 @@ int dkz_linear_forward(int type, int rows, int inputs, int outputs, int activati
  * does not read the updates. Each of the three results may be NULL: it is not
  * computed. activated may be NULL for the linear activation; input_residual (a
  * second path's delta, or input_delta itself to add to it) may be NULL. A bf16
- * pass takes d rounded to bf16 into the two products (the bias sums take it
- * unrounded). */
+ * pass takes d / scale rounded to bf16 into the two products, and multiplies
+ * their sums by the scale: exact where the gradient is 0 or 1, else the results
+ * are off by this rounding and their own (for a scale of 2^-20 to 2^20; beyond, d
+ * itself is rounded). The bias sums take d unrounded. */
 int dkz_linear_backward_workspace(int type, int rows, int inputs, int outputs, size_t *bytes);
 int dkz_linear_backward(int type, int rows, int inputs, int outputs, int activation, float prob, float scale,
                         unsigned int seed, unsigned long long first, const void *input, const void *weights,
@@ -139,7 +141,8 @@ int dkz_linear_cross_entropy_forward(int type, int rows, int inputs, int classes
  *     d(r, c) = s(r) * ((c == targets[r]) - p(r, c))
  * -- the delta truth - probability, as dkz_softmax_cross_entropy's -- and
  * bias_updates, weight_updates and input_delta follow from d as in
- * dkz_linear_backward, without an input_residual. */
+ * dkz_linear_backward, without an input_residual. A bf16 pass takes d rounded to
+ * bf16 into the two products, the bias sums take it unrounded. */
 int dkz_linear_cross_entropy_backward_workspace(int type, int rows, int inputs, int classes, size_t *least,
                                                 size_t *best);
 int dkz_linear_cross_entropy_backward(int type, int rows, int inputs, int classes, const void *input,

@@ -37,6 +37,43 @@ def test_backward(pool, case):
     linear.run_backward(pool, kind, rows, inputs, outputs, act, 0.25, True, beta=0.5, shift=shift)
 
 
+@pytest.mark.parametrize("act", [ref.LINEAR, ref.RELU])
+@pytest.mark.parametrize("shape,prob", [((300, 136, 200), 0.1), ((70, 41, 53), 0.3), ((3400, 72, 264), 0.1), ((64, 64, 64), 0.0)], ids=str)
+def test_backward_rounds_no_delta_that_is_kept_or_dropped(pool, act, shape, prob):
+    """Where the gradient is 0 or 1, d is the scale times a bf16 delta or 0: the products take it unrounded, and their results
+    are off by their own rounding alone."""
+    rows, inputs, outputs = shape
+    r = np.random.default_rng(rows + inputs)
+    x, w, delta, a = (ref.rounded(r.normal(size=s), BF16) for s in ((rows, inputs), (outputs, inputs), (rows, outputs), (rows, outputs)))
+    scale, seed = 1 / (1 - prob) if prob else 1.7, 11
+    dx, dw, dd, da = (pool(v, BF16) for v in (x, w, delta, a))
+    gb, gw, gx = pool(n=outputs), pool(kind=BF16, n=(outputs, inputs)), pool(kind=BF16, n=(rows, inputs))
+    ws = pool.work(gpu.linearBackwardWorkspace(BF16, rows, inputs, outputs))
+    gpu.linearBackward(BF16, rows, inputs, outputs, act, prob, scale, seed, 0, dx.buf, dw.buf, da.buf if act != ref.LINEAR else None, dd.buf, None,
+                       0.0, gb.buf, gw.buf, gx.buf, ws.buf)
+    drop = ref.dropped(rows * outputs, prob, seed, 0).reshape(rows, outputs)
+    d = np.where(drop, 0.0, delta.astype(np.float64) * float(np.float32(scale))) * ref.gradient(act, a.astype(np.float64))
+    for got, p, q, what in ((gw, d.T, x, "weight_updates"), (gx, d, w, "input_delta")):
+        q = q.astype(np.float64)
+        y, err = p @ q, ref.product_error(p, q) * 1.01
+        err = err + 2.0**-24 * np.abs(y)  # the scale
+        ref.assert_within(got.get(), y, err + ref.HALF[BF16] * (np.abs(y) + err), what)
+    total = d.sum(0)  # 64 rows in fp32, each element off by its scaling's rounding at most, then 64 bits and two roundings
+    ref.assert_within(gb.get(), total, (65 * np.abs(d).sum(0) + 3 * np.abs(total)) * 2.0**-24, "bias_updates")
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_backward_of_everything_dropped(pool, kind):
+    """prob 1: the scale 1 / (1 - prob) is infinite and no element is kept, so every d is 0, and no gradient a NaN."""
+    rows, inputs, outputs = 70, 40, 48
+    x, w, d = (pool(np.ones(s, np.float32), kind) for s in ((rows, inputs), (outputs, inputs), (rows, outputs)))
+    gb, gw, gx = pool(n=outputs), pool(kind=kind, n=(outputs, inputs)), pool(kind=kind, n=(rows, inputs))
+    ws = pool.work(gpu.linearBackwardWorkspace(kind, rows, inputs, outputs))
+    gpu.linearBackward(kind, rows, inputs, outputs, ref.LINEAR, 1.0, float("inf"), 1, 0, x.buf, w.buf, None, d.buf, None, 0.0, gb.buf, gw.buf,
+                       gx.buf, ws.buf)
+    assert not gb.get().any() and not gw.get().any() and not gx.get().any()
+
+
 def many_classes(plain, kind, classes):
     """lse_error where a row is more than a few parts. Pairs are merged in at most five roundings, fp32 logits added in at
     most ten for every eight; all terms are positive. bf16: parts of at least 16 classes, a thread merging every 256th, then 9 among
