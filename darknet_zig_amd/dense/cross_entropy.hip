@@ -364,9 +364,11 @@ __global__ __launch_bounds__(kBlock) void no_classes_kernel(uint32_t rows, float
 
 // ---- plans ----
 
-// Bytes of a piece's logits or d at most where the workspace has room for it:
-// enough rows and columns for whole rounds of tiles, and little beside the
-// weights of a class count that needs it.
+// Bytes of a piece's logits or d where the workspace has room for it: enough rows
+// and columns for whole rounds of tiles, and little beside the weights of a class
+// count that needs it. A piece has kLeastPiece classes all the same, so that from 2^20
+// bf16 rows (2^19 fp32) on it takes more: the products would read all rows' inputs for
+// a few columns of tiles each time. bf16's forward pass needs no logits, and no pieces.
 constexpr uint64_t kPieceBytes = 512ull << 20;
 constexpr uint64_t kLeastPiece = 256;  // classes
 

@@ -128,7 +128,10 @@ int dkz_linear_backward(int type, int rows, int inputs, int outputs, int activat
  *
  * The classes are taken in pieces, as many at a time as the workspace has room
  * for: *best is what the fastest way takes, *least what any call of this shape
- * needs. */
+ * needs. A piece holds its logits, or the deltas d below, in the tensors' type: half a
+ * gigabyte of them at most, but at least 256 classes (256 * rows elements). A bf16
+ * forward pass takes all classes at once: a pair of floats for every 16 to 128
+ * classes of a row, *least and *best the same. */
 int dkz_linear_cross_entropy_forward_workspace(int type, int rows, int inputs, int classes, size_t *least,
                                                size_t *best);
 int dkz_linear_cross_entropy_forward(int type, int rows, int inputs, int classes, const void *input,
