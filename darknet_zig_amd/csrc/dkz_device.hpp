@@ -434,4 +434,15 @@ __device__ __forceinline__ float gradient(float y) {
     else return 1.0f;
 }
 
+// The hash of the draws (darknet_kernels.hip:168-183), Wellons' "lowbias32":
+// rand_uniform's and seeded dropout's, which take the same draws.
+__device__ __forceinline__ uint32_t hash_u32(uint32_t x) {
+    x ^= x >> 16;
+    x *= 0x7feb352du;
+    x ^= x >> 15;
+    x *= 0x846ca68bu;
+    x ^= x >> 16;
+    return x;
+}
+
 }  // namespace dkz

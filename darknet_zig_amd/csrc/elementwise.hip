@@ -255,16 +255,7 @@ struct AdamOp {
 };
 
 // darknet_kernels.hip:168-183: element i of a rand_uniform draw is the top 24
-// bits of hash(seed ^ hash(i)), scaled into [0, 1) (every value exact). The
-// hash is Wellons' "lowbias32".
-__device__ __forceinline__ uint32_t hash_u32(uint32_t x) {
-    x ^= x >> 16;
-    x *= 0x7feb352du;
-    x ^= x >> 15;
-    x *= 0x846ca68bu;
-    x ^= x >> 16;
-    return x;
-}
+// bits of hash(seed ^ hash(i)) (hash_u32), scaled into [0, 1) (every value exact).
 __device__ __forceinline__ float uniform_at(uint32_t seed, uint32_t i) {
     return (float)(hash_u32(seed ^ hash_u32(i)) >> 8) * (1.0f / 16777216.0f);
 }

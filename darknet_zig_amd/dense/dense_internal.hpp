@@ -143,15 +143,6 @@ inline bool disjoint(const Span (&writes)[W], const Span (&reads)[R]) {
 
 // ---- draws ----
 
-__device__ __forceinline__ uint32_t draw_hash(uint32_t x) {  // Wellons' lowbias32, as rand_uniform's
-    x ^= x >> 16;
-    x *= 0x7feb352du;
-    x ^= x >> 15;
-    x *= 0x846ca68bu;
-    x ^= x >> 16;
-    return x;
-}
-
 // Element i's draw is the top 24 bits of hash(seed ^ hash(low word of i) ^
 // hash(0x9e3779b9 * high word)), times 2^-24; below 2^32 elements, where the
 // last hash is 0, it is rand_uniform's. A draw is below prob exactly when its
@@ -164,8 +155,8 @@ struct Draws {
     __device__ __forceinline__ bool dropped(uint64_t i) const {
         i += first;
         const uint32_t high = (uint32_t)(i >> 32);
-        const uint32_t key = seed ^ (high ? draw_hash(0x9e3779b9u * high) : 0u);
-        return draw_hash(key ^ draw_hash((uint32_t)i)) >> 8 < limit;
+        const uint32_t key = seed ^ (high ? hash_u32(0x9e3779b9u * high) : 0u);
+        return hash_u32(key ^ hash_u32((uint32_t)i)) >> 8 < limit;
     }
     // A select, not a multiply: a dropped NaN or infinity is 0.
     __device__ __forceinline__ float apply(float v, uint64_t i) const {
@@ -189,10 +180,10 @@ struct Draws {
         if (limit == 0) return;
         i += first;
         const uint32_t low = (uint32_t)i, high = (uint32_t)(i >> 32);
-        const uint32_t key = seed ^ (high ? draw_hash(0x9e3779b9u * high) : 0u);
+        const uint32_t key = seed ^ (high ? hash_u32(0x9e3779b9u * high) : 0u);
         if (low + (N - 1) >= low) {  // one high word
 #pragma unroll
-            for (int x = 0; x < N; ++x) v[x] = draw_hash(key ^ draw_hash(low + x)) >> 8 < limit ? 0.0f : v[x];
+            for (int x = 0; x < N; ++x) v[x] = hash_u32(key ^ hash_u32(low + x)) >> 8 < limit ? 0.0f : v[x];
         } else {
 #pragma unroll
             for (int x = 0; x < N; ++x) v[x] = dropped(i - first + x) ? 0.0f : v[x];
