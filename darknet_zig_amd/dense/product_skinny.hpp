@@ -7,7 +7,8 @@
 // of v_mfma_f32_16x16x32_bf16 and eight of an input row, which the caches hold,
 // into the other. Each wave keeps two or four steps of 64 k in flight. The waves'
 // sums meet in LDS in wave order, and the epilogue takes them from there. One row
-// of 4096 to 16384 outputs 25.1 us (5.3 TB/s), 32768 47.8, 4096 9.
+// of 4096 to 16384 outputs 25.1 us (5.3 TB/s), 32768 47.4 (5.7), 4096 8.5; with weights
+// that the caches hold 21.3, 39.7 and 6.9.
 #pragma once
 
 #include "dense_internal.hpp"
@@ -19,8 +20,8 @@ namespace {
 typedef short s16x8w __attribute__((ext_vector_type(8), aligned(4)));
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 
-// Rows at most: 4096x4096 weights take 7.8 us at one row, 9.8 at 16 and 13.2 at 32,
-// where tiles take 13.6 (at 64 they take no more, this kernel 20.4).
+// Rows at most: 4096x4096 weights in the caches take 6.9 us at one row, 9.6 at 16 and
+// 13.3 at 32, where tiles take 13.6 (at 64 they take no more, this kernel 20.4).
 constexpr uint32_t kSkinnyRows = 32;
 constexpr int kSkinnyWaves = 4;
 inline bool few_rows(uint64_t rows) { return rows <= kSkinnyRows; }
