@@ -179,11 +179,11 @@ int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint6
     // bf16 products take d / scale, and their results are multiplied by the scale in fp32: where the gradient is 0 or 1 (linear, relu)
     // d / scale is a delta or 0 and needs no rounding, and an input or weight gradient is off by its own rounding alone (8192x4096x4096
     // with dropout, distance from 64 bits: 0.0024 with d rounded, 0.0017 so). Other gradients' d is rounded to bf16, as any operand of
-    // a bf16 product has to be. A scale far from 1 stays with d: the sums might overflow without it, and an infinite one (all dropped)
-    // times sums of 0 is no 0.
+    // a bf16 product has to be. A scale far from 1 stays with d: a sum that it keeps below fp32's largest value, or above its smallest,
+    // would not be there without it, and an infinite one (all dropped) times sums of 0 is no 0.
     Draws inner = draws;
     float alpha = 1.0f;
-    if (sizeof(T) == 2 && fabsf(draws.scale) >= 0x1p-20f && fabsf(draws.scale) <= 0x1p20f) std::swap(alpha, inner.scale);
+    if (sizeof(T) == 2 && fabsf(draws.scale) >= 0x1p-8f && fabsf(draws.scale) <= 0x1p8f) std::swap(alpha, inner.scale);
     // The delta itself where nothing changes it and its rows lie on 16-byte boundaries.
     const bool same = act == kLinear && inner.limit == 0 && inner.scale == 1.0f && ldd == outputs && aligned16(delta);
     if (same || !products) {

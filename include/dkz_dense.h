@@ -104,7 +104,7 @@ int dkz_linear_forward(int type, int rows, int inputs, int outputs, int activati
  * second path's delta, or input_delta itself to add to it) may be NULL. A bf16
  * pass takes d / scale rounded to bf16 into the two products, and multiplies
  * their sums by the scale: exact where the gradient is 0 or 1, else the results
- * are off by this rounding and their own (for a scale of 2^-20 to 2^20; beyond, d
+ * are off by this rounding and their own (for a scale of 2^-8 to 2^8; beyond, d
  * itself is rounded). The bias sums take d unrounded. */
 int dkz_linear_backward_workspace(int type, int rows, int inputs, int outputs, size_t *bytes);
 int dkz_linear_backward(int type, int rows, int inputs, int outputs, int activation, float prob, float scale,

@@ -74,6 +74,18 @@ def test_backward_of_everything_dropped(pool, kind):
     assert not gb.get().any() and not gw.get().any() and not gx.get().any()
 
 
+@pytest.mark.parametrize("scale", [2.0**-100, 2.0**100])
+def test_backward_with_an_extreme_scale(pool, scale):
+    """Sums that only the scale keeps in fp32's range: deltas and weights of 2^66, or 2^-66, whose products are 2^132, or 2^-132.
+    All values are powers of two and the sums exact."""
+    rows, inputs, outputs, v = 48, 40, 64, 2.0**66 if scale < 1 else 2.0**-66
+    x, w, d = (pool(np.full(s, v, np.float32), BF16) for s in ((rows, inputs), (outputs, inputs), (rows, outputs)))
+    gw, gx = pool(kind=BF16, n=(outputs, inputs)), pool(kind=BF16, n=(rows, inputs))
+    ws = pool.work(gpu.linearBackwardWorkspace(BF16, rows, inputs, outputs))
+    gpu.linearBackward(BF16, rows, inputs, outputs, ref.LINEAR, 0.0, scale, 1, 0, x.buf, w.buf, None, d.buf, None, 0.0, None, gw.buf, gx.buf, ws.buf)
+    assert (gw.get() == rows * v * v * scale).all() and (gx.get() == outputs * v * v * scale).all()
+
+
 def many_classes(plain, kind, classes):
     """lse_error where a row is more than a few parts. Pairs are merged in at most five roundings, fp32 logits added in at
     most ten for every eight; all terms are positive. bf16: parts of at least 16 classes, a thread merging every 256th, then 9 among
