@@ -1,12 +1,12 @@
 """ctypes binding of libdkz.so, the C ABI declared in include/dkz_ops.h, and of
-its companion libdkz_dense.so (include/dkz_dense.h).
+its companions libdkz_dense.so (include/dkz_dense.h) and libdkz_lm.so (include/dkz_lm.h).
 
 This is the Python-side equivalent of the extern declarations a Zig host would
 write against the same header. Every exported symbol is listed in SIGNATURES;
 tests check the table against the header and the built library.
 
 There is deliberately no fallback: if a library has not been built (or cannot
-be loaded), load() and load_dense() raise and nothing runs.
+be loaded), load(), load_dense() and load_lm() raise and nothing runs.
 """
 
 from __future__ import annotations
@@ -17,6 +17,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libdkz.so"
 DENSE_LIB_NAME = "libdkz_dense.so"
+LM_LIB_NAME = "libdkz_lm.so"
 
 _p = C.c_void_p
 _i = C.c_int
@@ -102,8 +103,23 @@ DENSE_SIGNATURES: dict[str, tuple] = {
     "dkz_linear_cross_entropy_backward": (_i, [_i] * 4 + [_p] * 6 + [_f, _f] + [_p] * 4 + [_sz]),
 }
 
+# The same for include/dkz_lm.h.
+LM_SIGNATURES: dict[str, tuple] = {
+    "dkz_lm_last_error_context": (C.c_char_p, []),
+    "dkz_gated_forward_workspace": (_i, [_i] * 4 + [C.POINTER(_sz)]),
+    "dkz_gated_forward": (_i, [_i] * 5 + [_p] * 6 + [_sz]),
+    "dkz_gated_backward_workspace": (_i, [_i] * 4 + [C.POINTER(_sz)]),
+    "dkz_gated_backward": (_i, [_i] * 5 + [_p] * 5 + [_f] + [_p] * 4 + [_sz]),
+    "dkz_token_log_probs_workspace": (_i, [_i] * 4 + [C.POINTER(_sz)]),
+    "dkz_token_log_probs": (_i, [_i] * 4 + [_p, _f, _i, _p, _i] + [_p] * 6 + [_sz]),
+    "dkz_token_log_probs_backward": (_i, [_i] * 4 + [_p, _f, _i] + [_p] * 5 + [_f, _p]),
+    "dkz_distillation_workspace": (_i, [_i] * 3 + [C.POINTER(_sz)]),
+    "dkz_distillation": (_i, [_i] * 4 + [_p, _f, _i] + [_p] * 3 + [_f] + [_p] * 3 + [_sz]),
+}
+
 _LIB: C.CDLL | None = None
 _DENSE: C.CDLL | None = None
+_LM: C.CDLL | None = None
 
 
 def _open(p: Path, signatures: dict[str, tuple]) -> C.CDLL:
@@ -148,3 +164,12 @@ def load_dense() -> C.CDLL:
         load()
         _DENSE = _open(_path().resolve().parent / DENSE_LIB_NAME, DENSE_SIGNATURES)
     return _DENSE
+
+
+def load_lm() -> C.CDLL:
+    """Loads libdkz_lm.so (once), as load_dense()."""
+    global _LM
+    if _LM is None:
+        load()
+        _LM = _open(_path().resolve().parent / LM_LIB_NAME, LM_SIGNATURES)
+    return _LM

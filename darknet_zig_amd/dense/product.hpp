@@ -55,6 +55,17 @@ struct ProductArgs {
     uint32_t first_block;  // the launch's first workgroup among the product's
 };
 
+// A product's columns are u's rows, or (kPaired of its epilogue) come in eights of two
+// halves in turn, each of `half` rows of u: columns 16 * i + 0 .. 7 are rows 8 * i + 0 .. 7
+// and columns 16 * i + 8 .. 15 the same of the other half, so that a lane that has
+// sixteen columns has eight pairs. Column `c` is there if unit(c) < half.
+template <class Epi>
+constexpr bool kPaired = false;
+struct Pairs {
+    static __device__ __forceinline__ uint32_t unit(uint32_t c) { return c / 16 * 8 + c % 8; }
+    static __device__ __forceinline__ uint32_t row(uint32_t c, uint32_t half) { return (c / 8 & 1) * half + unit(c); }
+};
+
 // Consecutive workgroups go round the 8 XCDs: gives each XCD a run of neighbours.
 __device__ __forceinline__ uint32_t xcd_run(uint32_t w, uint32_t total) {
     const uint32_t x = w & 7, q = total >> 3, rem = total & 7;
@@ -120,6 +131,26 @@ struct Staged {
             }
         }
     }
+    // The same for columns r0 .. r0 + R - 1 in pairs.
+    __device__ __forceinline__ void load_pairs(const __bf16 *p, uint32_t ld, uint32_t r0, uint32_t half, uint32_t k0, uint32_t kend) {
+        static_assert(!MC, "rows of u with k contiguous");
+        const short *base = reinterpret_cast<const short *>(p);
+        const bool inside = r0 + R <= 2 * half && k0 + BK <= kend;
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            const uint32_t c = threadIdx.x + i * THREADS, along = k0 + c % kLine * 8, col = r0 + c / kLine;
+            const short *line = base + (uint64_t)min(Pairs::row(col, half), 2 * half - 1) * ld;
+            if (inside) {
+                v[i] = *reinterpret_cast<const s16x8u *>(line + along);
+            } else {
+                s16x8 x = {};
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (Pairs::unit(col) < half && along + j < kend) x[j] = line[along + j];
+                v[i] = x;
+            }
+        }
+    }
     __device__ __forceinline__ void store(char *lds) const {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
@@ -168,6 +199,17 @@ struct Direct {
             const uint32_t line = c / kLine, chunk = permuted<R, BK, MC>(line, c % kLine);
             k[i] = MC ? line : chunk * 8;
             off[i] = r0 + (MC ? chunk * 8 : line) < rows ? (line * ld + chunk * 8) * 2 : kOutside;
+        }
+    }
+    // The same for columns r0 .. r0 + R - 1 in pairs; p is row r0 / 2.
+    __device__ __forceinline__ void init_pairs(uint32_t ld, uint32_t r0, uint32_t half) {
+        static_assert(!MC && R % 16 == 0, "rows of u with k contiguous");
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t c = threadIdx.x + i * THREADS;
+            const uint32_t line = c / kLine, chunk = permuted<R, BK, MC>(line, c % kLine);
+            k[i] = chunk * 8;
+            off[i] = Pairs::unit(r0 + line) < half ? (Pairs::row(line, half) * ld + chunk * 8) * 2 : kOutside;
         }
     }
     // Load i of a slab to LDS address `to` (the slab's). p: element (r0, k0);
@@ -418,9 +460,11 @@ __device__ __forceinline__ void product_tile(const ProductArgs &g, const Epi &ep
             Direct<BC, BK, UMC, kThreads> du;
             constexpr int kLoads = dv.kLoads + du.kLoads;
             dv.init(g.ldv, r0, g.rows);
-            du.init(g.ldu, c0, g.cols);
+            if constexpr (kPaired<Epi>) du.init_pairs(g.ldu, c0, epi.half);
+            else du.init(g.ldu, c0, g.cols);
             const __bf16 *pv = g.v + (VMC ? (uint64_t)kbeg * g.ldv + r0 : (uint64_t)r0 * g.ldv + kbeg);
-            const __bf16 *pu = g.u + (UMC ? (uint64_t)kbeg * g.ldu + c0 : (uint64_t)c0 * g.ldu + kbeg);
+            const uint32_t u0 = kPaired<Epi> ? c0 / 2 : c0;
+            const __bf16 *pu = g.u + (UMC ? (uint64_t)kbeg * g.ldu + u0 : (uint64_t)u0 * g.ldu + kbeg);
             const uint64_t sv = VMC ? (uint64_t)BK * g.ldv : BK, su = UMC ? (uint64_t)BK * g.ldu : BK;
             const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
             uint32_t left = kend - kbeg, to = base;  // of the slab that is being loaded
@@ -494,7 +538,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs &g, const Epi &ep
             auto load = [&](Slab &s, uint32_t k0) __attribute__((always_inline)) {
                 if (k0 >= kend) return;
                 s.v.load(g.v, g.ldv, r0, g.rows, k0, kend);
-                s.u.load(g.u, g.ldu, c0, g.cols, k0, kend);
+                if constexpr (kPaired<Epi>) s.u.load_pairs(g.u, g.ldu, c0, epi.half, k0, kend);
+                else s.u.load(g.u, g.ldu, c0, g.cols, k0, kend);
             };
             auto store = [&](const Slab &s, uint32_t stage) __attribute__((always_inline)) {
                 s.v.store(lds + stage * kStage);

@@ -42,8 +42,11 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(ProductArgs g
     f32x4v acc[CT][RT] = {};
     const short *pu[CT], *pv[RT];
 #pragma unroll
-    for (int i = 0; i < CT; ++i)  // columns past the end repeat the last one, rows the last row: not stored
-        pu[i] = reinterpret_cast<const short *>(g.u) + (uint64_t)min(c0 + 16 * i + l16, g.cols - 1) * g.ldu + 16 * group;
+    for (int i = 0; i < CT; ++i) {  // columns past the end repeat the last one, rows the last row: not stored
+        uint32_t row = min(c0 + 16 * i + l16, g.cols - 1);
+        if constexpr (kPaired<Epi>) row = min(Pairs::row(row, epi.half), 2 * epi.half - 1);
+        pu[i] = reinterpret_cast<const short *>(g.u) + (uint64_t)row * g.ldu + 16 * group;
+    }
 #pragma unroll
     for (int j = 0; j < RT; ++j)
         pv[j] = reinterpret_cast<const short *>(g.v) + (uint64_t)min(16 * j + l16, g.rows - 1) * g.ldv + 16 * group;
@@ -128,13 +131,27 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(ProductArgs g
         for (int j = 0; j < RT; ++j)
             *reinterpret_cast<f32x4v *>(&sums[wave][16 * j + l16][16 * i + 4 * group]) = acc[i][j];
     __syncthreads();
+    if constexpr (kPaired<Epi>) {
+        // A thread a pair.
+        for (uint32_t e = threadIdx.x; e < kRows * kCols / 2; e += 64 * kWaves) {
+            const uint32_t r = e / (kCols / 2), j = e % (kCols / 2), c = j / 8 * 16 + j % 8;
+            float x = sums[0][r][c], y = sums[0][r][c + 8];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) {
+                x += sums[w][r][c];
+                y += sums[w][r][c + 8];
+            }
+            epi.pair(r, c0 / 2 + j, x, y, g.rows);
+        }
+        return;
+    }
     // A thread an element, the columns along the lanes.
     for (uint32_t e = threadIdx.x; e < kRows * kCols; e += 64 * kWaves) {
         const uint32_t r = e / kCols, c = e % kCols;
         float z = sums[0][r][c];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) z += sums[w][r][c];
-        epi.template skinny<kCols>(r, c0 + c, z, g.rows, g.cols, c0 / kCols);
+        if constexpr (!kPaired<Epi>) epi.template skinny<kCols>(r, c0 + c, z, g.rows, g.cols, c0 / kCols);
     }
 }
 

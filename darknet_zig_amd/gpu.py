@@ -16,7 +16,9 @@ Host arrays are numpy arrays (float32, or int32 for maxpool indexes).
 
 The fused dense operators at the end (`seededDropout`, `linear*`) have no single
 gpu.zig counterpart. They go to libdkz_dense.so and take fp32 or bf16 tensors:
-a bf16 tensor of n elements is a Buf of (n + 1) // 2 four-byte elements.
+a bf16 tensor of n elements is a Buf of (n + 1) // 2 four-byte elements. So do a
+token model's operators after them (`gated*`, `tokenLogProbs*`, `distillation`), which
+go to libdkz_lm.so.
 """
 
 from __future__ import annotations
@@ -638,4 +640,110 @@ def linearCrossEntropyBackward(
             beta, _p(bias_updates), _p(weight_updates), _p(input_delta), _p(workspace), _bytes(workspace),
         ),
         "linear_cross_entropy_backward",
+    )
+
+
+# ---- a token model's operators of libdkz_lm.so (include/dkz_lm.h): gated
+# feed-forward blocks, log probabilities of tokens and distillation from logits.
+# Workspaces as above. ----
+
+SILU, GELU = 14, 15  # a gate's activations beside logistic, relu and linear
+
+
+def _must_lm(code: int, what: str) -> None:
+    if code != 0:
+        raise GpuError(code, what, _lib.load_lm().dkz_lm_last_error_context().decode(errors="replace"))
+
+
+def gatedForwardWorkspace(type: int, rows: int, inputs: int, hidden: int) -> int:
+    need = C.c_size_t(0)
+    _must_lm(_lib.load_lm().dkz_gated_forward_workspace(type, rows, inputs, hidden, C.byref(need)), "gated_forward_workspace")
+    return need.value
+
+
+def gatedForward(
+    type: int, rows: int, inputs: int, hidden: int, activation: int, input: Buf, weights: Buf, biases: Buf | None,
+    sums: Buf | None, output: Buf, workspace: Buf | None,
+) -> None:
+    """output = activation(gate) * up, from weights [2 * hidden, inputs]; both projections to `sums`."""
+    _must_lm(
+        _lib.load_lm().dkz_gated_forward(
+            type, rows, inputs, hidden, int(activation), _p(input), _p(weights), _p(biases), _p(sums), _p(output),
+            _p(workspace), _bytes(workspace),
+        ),
+        "gated_forward",
+    )
+
+
+def gatedBackwardWorkspace(type: int, rows: int, inputs: int, hidden: int) -> int:
+    need = C.c_size_t(0)
+    _must_lm(_lib.load_lm().dkz_gated_backward_workspace(type, rows, inputs, hidden, C.byref(need)), "gated_backward_workspace")
+    return need.value
+
+
+def gatedBackward(
+    type: int, rows: int, inputs: int, hidden: int, activation: int, input: Buf, weights: Buf, sums: Buf, delta: Buf,
+    input_residual: Buf | None, beta: float, bias_updates: Buf | None, weight_updates: Buf | None, input_delta: Buf | None,
+    workspace: Buf | None,
+) -> None:
+    _must_lm(
+        _lib.load_lm().dkz_gated_backward(
+            type, rows, inputs, hidden, int(activation), _p(input), _p(weights), _p(sums), _p(delta), _p(input_residual), beta,
+            _p(bias_updates), _p(weight_updates), _p(input_delta), _p(workspace), _bytes(workspace),
+        ),
+        "gated_backward",
+    )
+
+
+def tokenLogProbsWorkspace(type: int, rows: int, classes: int, top: int) -> int:
+    need = C.c_size_t(0)
+    _must_lm(_lib.load_lm().dkz_token_log_probs_workspace(type, rows, classes, top, C.byref(need)), "token_log_probs_workspace")
+    return need.value
+
+
+def tokenLogProbs(
+    type: int, rows: int, classes: int, pitch: int, logits: Buf, temperature: float, given: int, tokens: Buf | None, top: int,
+    log_probs: Buf | None, entropy: Buf | None, stats: Buf, top_tokens: Buf | None, top_log_probs: Buf | None,
+    workspace: Buf | None,
+) -> None:
+    """Log probabilities of `given` tokens a row, the entropy, and the `top` alternatives in order."""
+    _must_lm(
+        _lib.load_lm().dkz_token_log_probs(
+            type, rows, classes, pitch, _p(logits), temperature, given, _p(tokens), top, _p(log_probs), _p(entropy), _p(stats),
+            _p(top_tokens), _p(top_log_probs), _p(workspace), _bytes(workspace),
+        ),
+        "token_log_probs",
+    )
+
+
+def tokenLogProbsBackward(
+    type: int, rows: int, classes: int, pitch: int, logits: Buf, temperature: float, given: int, tokens: Buf | None,
+    stats: Buf, entropy: Buf | None, log_prob_deltas: Buf | None, entropy_deltas: Buf | None, beta: float, logits_delta: Buf,
+) -> None:
+    _must_lm(
+        _lib.load_lm().dkz_token_log_probs_backward(
+            type, rows, classes, pitch, _p(logits), temperature, given, _p(tokens), _p(stats), _p(entropy), _p(log_prob_deltas),
+            _p(entropy_deltas), beta, _p(logits_delta),
+        ),
+        "token_log_probs_backward",
+    )
+
+
+def distillationWorkspace(type: int, rows: int, classes: int) -> int:
+    need = C.c_size_t(0)
+    _must_lm(_lib.load_lm().dkz_distillation_workspace(type, rows, classes, C.byref(need)), "distillation_workspace")
+    return need.value
+
+
+def distillation(
+    type: int, rows: int, classes: int, pitch: int, logits: Buf, temperature: float, top: int, teacher_tokens: Buf,
+    teacher_logits: Buf, row_scales: Buf | None, scale: float, loss: Buf, logits_delta: Buf | None, workspace: Buf | None,
+) -> None:
+    """The divergence from a teacher's top logits, and the delta of the logits."""
+    _must_lm(
+        _lib.load_lm().dkz_distillation(
+            type, rows, classes, pitch, _p(logits), temperature, top, _p(teacher_tokens), _p(teacher_logits), _p(row_scales),
+            scale, _p(loss), _p(logits_delta), _p(workspace), _bytes(workspace),
+        ),
+        "distillation",
     )
