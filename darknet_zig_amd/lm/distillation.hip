@@ -19,139 +19,212 @@ struct Teacher {
     float *entry_logits;  // [rows][kMostEntries]
 };
 
-// A row's entries in LDS: their classes, and their probabilities, which are 0 for those that are none.
-struct Entries {
+// A row's entries in LDS, for all of its group: their classes (~0: none) and probabilities, which are 0 for those that are
+// none, and the sum that those were divided by: 0 without an entry.
+struct __align__(16) Entries {
     uint32_t token[kMostEntries];
-    float p[kMostEntries];
+    float p[kMostEntries], log_p[kMostEntries], z[kMostEntries];  // log_p, z: for the loss, and their class's logit
+    float mass;
 };
 
-// What a group needs to write its part of a row.
-template <class T, int THREADS>
+// What a group does with a row's entries. Its first wave has them, one a lane and then the next 64: loops over them are kept
+// as loops, since all of this stands beside a row's logits in registers.
+template <class T>
 struct RowOf {
-    static constexpr int kSlots = kMostEntries / THREADS;
-    float z[kSlots], log_p[kSlots];  // of this thread's entries: their class's logit, log p
-    float mass;                      // the sum that p was divided by: 0 without an entry
+    const Logits &g;
+    const Teacher &t;
+    Entries &in;
+    uint32_t row;
+    const T *logits;
+    uint32_t c;  // of the lane's first entry: its class, logit, and its class's logit here
+    float v, z;
 
-    // Reads the entries into `in`: softmax over the entries that are classes.
-    __device__ __forceinline__ void read(const Logits &g, const Teacher &t, uint32_t row, Entries &in, float *lds) {
-        const T *logits = static_cast<const T *>(g.p) + (uint64_t)row * g.pitch;
-        const auto larger = [](float x, float y) { return fmaxf(x, y); };
-        const auto sum = [](float x, float y) { return x + y; };
-        float v[kSlots], m = neg_inf(), s = 0.0f;
-        __syncthreads();  // the last use of `in`
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-            const uint32_t j = threadIdx.x + i * THREADS;
-            const uint64_t at = (uint64_t)row * t.top + j;
-            const uint32_t c = j < t.top ? (uint32_t)t.tokens[at] : ~0u;
-            v[i] = c < g.classes ? t.logits[at] : neg_inf();
-            z[i] = c >= g.classes ? 0.0f : t.entry_logits != nullptr ? t.entry_logits[(uint64_t)row * kMostEntries + j] : load1(logits, c);
-            in.token[j] = c < g.classes ? c : ~0u;
-            m = fmaxf(m, v[i]);
+    __device__ __forceinline__ RowOf(const Logits &g, const Teacher &t, Entries &in, uint32_t row)
+        : g(g), t(t), in(in), row(row), logits(static_cast<const T *>(g.p) + (uint64_t)row * g.pitch) {}
+
+    __device__ __forceinline__ void entry(uint32_t j) {
+        const uint64_t at = (uint64_t)row * t.top + j;
+        c = ~0u;
+        v = neg_inf();
+        if (j < t.top) {
+            c = (uint32_t)t.tokens[at];
+            v = t.logits[at];
         }
-        m = group_reduce<float, THREADS>(m, lds, larger);
+    }
+    __device__ __forceinline__ void class_logit(uint32_t j) {
+        z = 0.0f;
+        if (c >= g.classes) {
+            c = ~0u;
+            v = neg_inf();
+        } else {
+            z = t.entry_logits != nullptr ? t.entry_logits[(uint64_t)row * kMostEntries + j] : load1(logits, c);
+        }
+    }
+    // The first entries' loads, apart so that others are issued between them.
+    __device__ __forceinline__ void begin() { entry(threadIdx.x); }
+    __device__ __forceinline__ void gather() { class_logit(threadIdx.x); }
+    // Softmax over the entries that are classes. A lane looks at its own entries in LDS alone: no barrier. The first entries' z is
+    // on its way and not looked at.
+    __device__ __forceinline__ void finish() {
+        const float first_z = z;
+        float m = v, s = 0.0f;
+        in.token[threadIdx.x] = c;
+        in.log_p[threadIdx.x] = v;
+#pragma unroll 1
+        for (uint32_t j = threadIdx.x + kWave; j - threadIdx.x < t.top; j += kWave) {
+            entry(j);
+            class_logit(j);
+            in.token[j] = c;
+            in.log_p[j] = v;
+            in.z[j] = z;
+            m = fmaxf(m, v);
+        }
+        z = first_z;
+        m = lanes_reduce<kWave>(m, [](float x, float y) { return fmaxf(x, y); });
         const float base = m == neg_inf() ? 0.0f : m;
-        float e[kSlots];
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-            v[i] = (v[i] - base) * g.inv;
-            e[i] = expf_cw(v[i]);
-            s += e[i];
+#pragma unroll 1
+        for (uint32_t j = threadIdx.x; j - threadIdx.x < t.top; j += kWave) {
+            const float y = (in.log_p[j] - base) * g.inv, e = expf_cw(y);
+            in.log_p[j] = y;
+            in.p[j] = e;
+            s += e;
         }
-        s = group_reduce<float, THREADS>(s, lds, sum);
-        mass = s;
-        const float log_s = logf(s);
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-            in.p[threadIdx.x + i * THREADS] = e[i] == 0.0f ? 0.0f : e[i] / s;
-            log_p[i] = v[i] - log_s;
+        s = lanes_reduce<kWave>(s, [](float x, float y) { return x + y; });
+        const float log_s = logf(s), over = 1.0f / s;
+#pragma unroll 1
+        for (uint32_t j = threadIdx.x; j - threadIdx.x < t.top; j += kWave) {
+            in.p[j] = in.p[j] == 0.0f ? 0.0f : in.p[j] * over;
+            in.log_p[j] -= log_s;
         }
-        __syncthreads();
+        if (threadIdx.x == 0) in.mass = s;
+    }
+    __device__ __forceinline__ void read() {
+        begin();
+        gather();
+        finish();
     }
 
-    // The loss, in every thread.
-    __device__ __forceinline__ float loss(const Logits &g, const Teacher &t, const Sums &a, float l, const Entries &in, float *lds) const {
+    // The loss, by the first wave.
+    __device__ __forceinline__ void loss(const Sums &a, float l, bool store = true) const {
         float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-            const float p = in.p[threadIdx.x + i * THREADS];
-            if (p != 0.0f) sum += p * (log_p[i] - log_prob_of(z[i], a.m, l, g.inv));
-        }
-        return t.temperature * (t.temperature * group_reduce<float, THREADS>(sum, lds, [](float x, float y) { return x + y; }));
+        in.z[threadIdx.x] = z;
+#pragma unroll 1
+        for (uint32_t j = threadIdx.x; j < t.top; j += kWave)
+            if (in.p[j] != 0.0f) sum += in.p[j] * (in.log_p[j] - log_prob_of(in.z[j], a.m, l, g.inv));
+        sum = lanes_reduce<kWave>(sum, [](float x, float y) { return x + y; });
+        if (threadIdx.x == 0 && store) t.loss[row] = t.temperature * (t.temperature * sum);
     }
 
-    // Writes a part of the delta.
-    __device__ __forceinline__ void write(const Logits &g, const Teacher &t, const Part<T> &part, uint32_t row, const Sums &a, float l,
-                                          const Entries &in, const Exp<T> &ex) const {
-        constexpr int kEach = kTileVectors;
+    // Writes a part of the delta. vectors(f) calls f(v, logits of vector v) for this thread's vectors of the part.
+    template <int THREADS, class F>
+    __device__ __forceinline__ void write(const Part<T> &part, const Sums &a, float l, const Exp<T> &ex, F vectors) const {
         T *out = static_cast<T *>(t.delta) + (uint64_t)row * g.pitch;
         float factor = t.row_scales != nullptr ? t.scale * t.row_scales[row] : t.scale;
-        const bool none = mass == 0.0f || factor == 0.0f || (a.m == neg_inf() && l == neg_inf());
+        const bool none = in.mass == 0.0f || factor == 0.0f || (a.m == neg_inf() && l == neg_inf());
         factor *= t.temperature;
-        const auto dense = [&](float z) __attribute__((always_inline)) { return none ? 0.0f : -factor * probability<T>(ex.scaled(z - a.m), l); };
-        float fixed[kSlots];
-        bool mine[kSlots];
+        const auto dense = [&](float z) __attribute__((always_inline)) { return none ? 0.0f : -factor * probability<T>(z - a.m, l, ex); };
+        vectors([&](uint32_t v, const u32x4v &raw) __attribute__((always_inline)) {
+            float d[kVec<T>];
+            unpack<T>(raw, d);
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-            const uint32_t j = threadIdx.x + i * THREADS, c = in.token[j];
-            mine[i] = c != ~0u && part.has(c);
-            if (!mine[i]) continue;
-            float p = 0.0f;
-            for (uint32_t k = 0; k < t.top; ++k) {
-                if (in.token[k] != c) continue;
-                if (k < j) mine[i] = false;
-                p += in.p[k];
-            }
-            fixed[i] = none ? 0.0f : factor * p + dense(z[i]);
-        }
-        for (uint32_t v0 = part.v0; v0 < part.v1; v0 += kEach * THREADS) {
-            u32x4v raw[kEach];
-#pragma unroll
-            for (int u = 0; u < kEach; ++u) raw[u] = part.load(v0 + u * THREADS + threadIdx.x);
-#pragma unroll
-            for (int u = 0; u < kEach; ++u) {
-                float d[kVec<T>];
-                unpack<T>(raw[u], d);
-#pragma unroll
-                for (uint32_t i = 0; i < kVec<T>; ++i) d[i] = dense(d[i]);
-                part.store_other(out, v0 + u * THREADS + threadIdx.x, d);
-            }
-        }
+            for (uint32_t i = 0; i < kVec<T>; ++i) d[i] = dense(d[i]);
+            part.store_other(out, v, d);
+        });
+        if (const uint32_t c = part.edge(); c != ~0u) store1(out, c, dense(load1(logits, c)));
+        // The entries' classes are written a second time, when the others have been, by the thread that has a class's first entry.
         __syncthreads();
+#pragma unroll 1
+        for (uint32_t j = threadIdx.x; j < t.top; j += THREADS) {
+            const uint32_t c = in.token[j];
+            if (c == ~0u || !part.has(c)) continue;
+            const Claim own = claim(in.token, in.p, t.top, j, c);
+            if (own.first) store1(out, c, none ? 0.0f : factor * own.sum + dense(in.z[j]));
+        }
+    }
+    // The same, from logits that are read again.
+    template <int THREADS>
+    __device__ __forceinline__ void write_again(const Part<T> &part, const Sums &a, float l, const Exp<T> &ex) const {
+        write<THREADS>(part, a, l, ex, [&](auto f) __attribute__((always_inline)) {
+            constexpr int kEach = kTileVectors;
+            for (uint32_t v0 = part.v0 + threadIdx.x; v0 < part.v1; v0 += kEach * THREADS) {
+                u32x4v raw[kEach];
+                part.load(v0, THREADS, raw);
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i)
-            if (mine[i]) store1(out, in.token[threadIdx.x + i * THREADS], fixed[i]);
+                for (int u = 0; u < kEach; ++u)
+                    if (v0 + u * THREADS < part.v1) f(v0 + u * THREADS, raw[u]);
+            }
+        });
     }
 };
 
 template <class T, int THREADS>
-__device__ __forceinline__ Sums part_sums(const Part<T> &p, const Exp<T> &ex, Sums *lds) {
+__device__ __forceinline__ Sums part_sums(const T *logits, const Part<T> &p, const Exp<T> &ex, Sums *lds) {
     constexpr int kEach = kTileVectors;
     Sums a{neg_inf(), 0.0f, 0.0f};
     for (uint32_t v0 = p.v0; v0 < p.v1; v0 += kEach * THREADS) {
         u32x4v raw[kEach];
-#pragma unroll
-        for (int u = 0; u < kEach; ++u) raw[u] = p.load(v0 + u * THREADS + threadIdx.x);
+        p.load(v0 + threadIdx.x, THREADS, raw);
         add<T, false>(a, raw, ex);
     }
+    const uint32_t edge = p.edge();
+    add_one(a, edge != ~0u ? load1(logits, edge) : neg_inf(), ex);
     return group_reduce<Sums, THREADS>(a, lds, [&](const Sums &x, const Sums &y) { return merge(x, y, ex); });
 }
 
-// A group takes a row: its sums, the loss, and the delta in a second pass.
-template <class T, int THREADS>
-__global__ __launch_bounds__(THREADS) void distillation_kernel(Logits g, Teacher t) {
+// A group takes a row, which it holds in registers, U vectors a thread, from the sums to the delta: every logit is
+// read once.
+template <class T, int THREADS, int U>
+__global__ __launch_bounds__(THREADS, U == 16 ? 4 : U == 8 ? 6 : 8) void distillation_held_kernel(Logits g, Teacher t) {
     __shared__ Sums sums[THREADS / kWave];
-    __shared__ float lds[THREADS / kWave];
+    __shared__ Entries in;
+    const Exp<T> ex(g.inv);
+    const bool first = threadIdx.x < kWave;
+    for (uint32_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
+        const Part<T> p(g, row, 0);
+        RowOf<T> r(g, t, in, row);
+        if (first) r.begin();
+        u32x4v raw[U];
+        p.load(p.v0 + threadIdx.x, THREADS, raw);
+        const uint32_t edge = p.edge();
+        const float at_edge = edge != ~0u ? load1(r.logits, edge) : neg_inf();
+        if (row != blockIdx.x) __syncthreads();  // the last row's use of `in`
+        if (first) {
+            r.gather();
+            r.finish();
+        }
+        Sums a = sums_of<T>(raw, ex);
+        add_one(a, at_edge, ex);
+        a = group_reduce<Sums, THREADS>(a, sums, [&](const Sums &x, const Sums &y) { return merge(x, y, ex); });
+        if constexpr (THREADS == kWave) __syncthreads();  // else the sums' have done it
+        const float l = log_sum(a);
+        if (first) r.loss(a, l);
+        if (t.delta != nullptr)
+            r.template write<THREADS>(p, a, l, ex, [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const uint32_t v = p.v0 + u * THREADS + threadIdx.x;
+                    if (v < p.v1) f(v, raw[u]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            });
+    }
+}
+
+// A group takes a row: its sums, the loss, and the delta in a second pass.
+template <class T>
+__global__ __launch_bounds__(kBlock) void distillation_kernel(Logits g, Teacher t) {
+    __shared__ Sums sums[kBlock / kWave];
     __shared__ Entries in;
     const Exp<T> ex(g.inv);
     for (uint32_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
-        RowOf<T, THREADS> r;
-        r.read(g, t, row, in, lds);
+        RowOf<T> r(g, t, in, row);
+        if (row != blockIdx.x) __syncthreads();  // the last row's use of `in`
+        if (threadIdx.x < kWave) r.read();
         const Part<T> p(g, row, 0);
-        const Sums a = part_sums<T, THREADS>(p, ex, sums);
-        const float l = log_sum(a), loss = r.loss(g, t, a, l, in, lds);
-        if (threadIdx.x == 0) t.loss[row] = loss;
-        if (t.delta != nullptr) r.write(g, t, p, row, a, l, in, ex);
+        const Sums a = part_sums<T, kBlock>(r.logits, p, ex, sums);
+        const float l = log_sum(a);
+        if (threadIdx.x < kWave) r.loss(a, l);
+        if (t.delta != nullptr) r.template write_again<kBlock>(p, a, l, ex);
     }
 }
 
@@ -161,47 +234,58 @@ __global__ __launch_bounds__(kBlock) void distillation_sums_kernel(Logits g, Tea
     __shared__ Sums sums[kBlock / kWave];
     const Exp<T> ex(g.inv);
     const uint32_t row = blockIdx.x / g.parts, part = blockIdx.x - row * g.parts;
-    const Sums a = part_sums<T, kBlock>(Part<T>(g, row, part), ex, sums);
+    const T *logits = static_cast<const T *>(g.p) + (uint64_t)row * g.pitch;
+    const Sums a = part_sums<T, kBlock>(logits, Part<T>(g, row, part), ex, sums);
     if (threadIdx.x == 0) t.part_sums[blockIdx.x] = a;
     if (part == 0 && threadIdx.x < t.top) {
         const uint32_t c = (uint32_t)t.tokens[(uint64_t)row * t.top + threadIdx.x];
-        if (c < g.classes)
-            t.entry_logits[(uint64_t)row * kMostEntries + threadIdx.x] = load1(static_cast<const T *>(g.p) + (uint64_t)row * g.pitch, c);
+        if (c < g.classes) t.entry_logits[(uint64_t)row * kMostEntries + threadIdx.x] = load1(logits, c);
     }
 }
 template <class T>
 __global__ __launch_bounds__(kBlock) void distillation_delta_kernel(Logits g, Teacher t) {
     __shared__ Sums sums[kBlock / kWave];
-    __shared__ float lds[kBlock / kWave];
     __shared__ Entries in;
     const Exp<T> ex(g.inv);
     // Without a delta a group a row suffices.
     const uint32_t parts = t.delta != nullptr ? g.parts : 1, row = blockIdx.x / parts, part = blockIdx.x - row * parts;
-    RowOf<T, kBlock> r;
-    r.read(g, t, row, in, lds);
+    RowOf<T> r(g, t, in, row);
+    if (threadIdx.x < kWave) r.read();
     Sums a{neg_inf(), 0.0f, 0.0f};
     for (uint32_t p = threadIdx.x; p < g.parts; p += kBlock) a = merge(a, t.part_sums[(uint64_t)row * g.parts + p], ex);
     a = group_reduce<Sums, kBlock>(a, sums, [&](const Sums &x, const Sums &y) { return merge(x, y, ex); });
     const float l = log_sum(a);
-    if (part == 0) {
-        const float loss = r.loss(g, t, a, l, in, lds);
-        if (threadIdx.x == 0) t.loss[row] = loss;
-    }
-    if (t.delta != nullptr) r.write(g, t, Part<T>(g, row, part), row, a, l, in, ex);
+    if (threadIdx.x < kWave) r.loss(a, l, part == 0);
+    if (t.delta != nullptr) r.template write_again<kBlock>(Part<T>(g, row, part), a, l, ex);
 }
 
-uint64_t part_bytes(uint64_t rows, const RowPlan &p) {
-    return p.parts == 1 ? 0 : padded(rows * p.parts * sizeof(Sums)) + padded(rows * kMostEntries * 4);
+// How rows are taken: held by groups of `threads` with `vectors` a thread, or (threads 0) as `rows` says.
+struct DistillPlan {
+    uint32_t threads, vectors;
+    RowPlan rows;
+    uint64_t bytes(uint64_t n) const {
+        return threads != 0 || rows.parts == 1 ? 0 : padded(n * rows.parts * sizeof(Sums)) + padded(n * kMostEntries * 4);
+    }
+};
+DistillPlan plan_distillation(int type, uint64_t rows, uint64_t classes) {
+    const uint64_t vectors = classes / (type == DKZ_F32 ? 4 : 8);  // whole ones at most
+    constexpr uint32_t kHeld[][2] = {{64, 4}, {256, 4}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}};
+    for (const auto &h : kHeld)
+        if (vectors <= h[0] * h[1]) return {h[0], h[1], {0, 1, h[0] * h[1]}};
+    return {0, 0, plan_rows(type, rows, classes)};
 }
 
 template <class T>
-int distill(hipStream_t stream, const Logits &g, const RowPlan &plan, const Teacher &t) {
+int distill(hipStream_t stream, const Logits &g, const DistillPlan &plan, const Teacher &t) {
     constexpr const char *kName = "distillation";
-    if (plan.parts == 1) {
-        const dim3 grid(plan.groups(g.rows));
-        if (plan.threads == 64) return launch_on(stream, kName, distillation_kernel<T, 64>, grid, dim3(64), g, t);
-        return launch_on(stream, kName, distillation_kernel<T, kBlock>, grid, dim3(kBlock), g, t);
-    }
+    const dim3 grid(std::min(g.rows, 1u << 20)), block(plan.threads);
+    if (plan.threads == 64) return launch_on(stream, kName, distillation_held_kernel<T, 64, 4>, grid, block, g, t);
+    if (plan.threads == 256 && plan.vectors == 4) return launch_on(stream, kName, distillation_held_kernel<T, 256, 4>, grid, block, g, t);
+    if (plan.threads == 256) return launch_on(stream, kName, distillation_held_kernel<T, 256, 8>, grid, block, g, t);
+    if (plan.threads == 512 && plan.vectors == 8) return launch_on(stream, kName, distillation_held_kernel<T, 512, 8>, grid, block, g, t);
+    if (plan.threads == 512) return launch_on(stream, kName, distillation_held_kernel<T, 512, 16>, grid, block, g, t);
+    if (plan.threads == 1024) return launch_on(stream, kName, distillation_held_kernel<T, 1024, 16>, grid, block, g, t);
+    if (plan.rows.parts == 1) return launch_on(stream, kName, distillation_kernel<T>, grid, dim3(kBlock), g, t);
     DKZ_TRY(launch_on(stream, "distillation_sums", distillation_sums_kernel<T>, dim3(g.rows * g.parts), dim3(kBlock), g, t));
     return launch_on(stream, kName, distillation_delta_kernel<T>, dim3(t.delta != nullptr ? g.rows * g.parts : g.rows), dim3(kBlock), g, t);
 }
@@ -215,7 +299,7 @@ extern "C" {
 
 int dkz_distillation_workspace(int type, int rows, int classes, size_t *bytes) {
     DKZ_REQUIRE(bytes != nullptr && logits_ok(type, rows, classes, classes, 1.0f));
-    *bytes = (size_t)part_bytes((uint64_t)rows, plan_rows(type, rows, classes));
+    *bytes = (size_t)plan_distillation(type, rows, classes).bytes((uint64_t)rows);
     return 0;
 }
 
@@ -228,19 +312,19 @@ int dkz_distillation(int type, int rows, int classes, int pitch, const void *log
     const uint64_t m = (uint64_t)rows, n = m * (uint64_t)top, all = logits_bytes(type, rows, classes, pitch);
     DKZ_REQUIRE(teacher_tokens != nullptr && teacher_logits != nullptr && loss != nullptr && (classes == 0 || logits != nullptr));
     DKZ_REQUIRE(element_aligned(type, logits) && element_aligned(type, logits_delta));
-    const RowPlan plan = plan_rows(type, rows, classes);
-    const uint64_t need = part_bytes(m, plan);
+    const DistillPlan plan = plan_distillation(type, rows, classes);
+    const uint64_t need = plan.bytes(m);
     DKZ_REQUIRE_WORKSPACE(need);
     const Span writes[] = {{loss, 4 * m}, {logits_delta, all}, {workspace, need}};
     const Span reads[] = {{logits == logits_delta ? nullptr : logits, all}, {teacher_tokens, 4 * n}, {teacher_logits, 4 * n}, {row_scales, 4 * m}};
     DKZ_REQUIRE(disjoint(writes, reads));
     Teacher t{teacher_tokens, teacher_logits, row_scales, loss, logits_delta, scale, temperature, (uint32_t)top, nullptr, nullptr};
     Workspace ws{static_cast<char *>(workspace), need};
-    if (plan.parts > 1) {
-        t.part_sums = ws.take<Sums>(m * plan.parts);
+    if (need != 0) {
+        t.part_sums = ws.take<Sums>(m * plan.rows.parts);
         t.entry_logits = ws.take<float>(m * kMostEntries);
     }
-    const Logits g = make_logits(plan, logits, rows, classes, pitch, temperature);
+    const Logits g = make_logits(plan.rows, logits, rows, classes, pitch, temperature);
     const hipStream_t stream = current_stream();
     return type == DKZ_F32 ? distill<float>(stream, g, plan, t) : distill<__bf16>(stream, g, plan, t);
 }

@@ -2,8 +2,8 @@
 // sums of a softmax over a row.
 //
 // A row is read in 16-byte vectors at 16-byte boundaries, whatever its first
-// element's address; the vectors at its ends that reach past it are read element
-// by element. A group of THREADS threads takes a row, or one of its `parts`; a
+// element's address; the few elements before and after them (its edges) are taken one
+// a thread. A group of THREADS threads takes a row, or one of its `parts`; a
 // tile is kEach vectors a thread, loaded together.
 #pragma once
 
@@ -44,70 +44,71 @@ struct Logits {
     float inv;            // 1 / temperature
 };
 
-// A part of a row: vectors [v0, v1) of 16 bytes from `base`, the row's elements in them being [o, end).
+// A part of a row: the whole vectors [v0, v1) from `base`, and where it is the row's first or last part the elements before
+// the first whole vector or after the last one, its edges: at most kEdges, which the group's first threads take.
 template <class T>
 struct Part {
-    const T *base;
-    uint32_t o, end, v0, v1;
+    static constexpr uint32_t kEdges = 2 * kVec<T>;
+    const T *base;  // the vector that holds the row's first element
+    uint32_t o, end, v0, v1;  // the row's elements from base are [o, end)
+    bool first, last;
 
     __device__ __forceinline__ Part(const Logits &g, uint32_t row, uint32_t part) {
-        const T *first = static_cast<const T *>(g.p) + (uint64_t)row * g.pitch;
-        o = (uint32_t)((uintptr_t)first & 15) / sizeof(T);
-        base = first - o;
+        const T *p = static_cast<const T *>(g.p) + (uint64_t)row * g.pitch;
+        o = (uint32_t)((uintptr_t)p & 15) / sizeof(T);
+        base = p - o;
         end = o + g.classes;
-        const uint32_t all = (end + kVec<T> - 1) / kVec<T>;
-        v0 = min(part * g.per, all);
-        v1 = min(v0 + g.per, all);
+        const uint32_t w0 = o != 0, w1 = max(end / kVec<T>, w0);
+        first = part == 0;
+        last = part == g.parts - 1;
+        v0 = min(w0 + part * g.per, w1);
+        v1 = last ? w1 : min(v0 + g.per, w1);
     }
-    __device__ __forceinline__ bool whole(uint32_t v) const { return v * kVec<T> >= o && (v + 1) * kVec<T> <= end; }
-    // Vector v, -infinity in the places outside the row.
+    // Vector v, all of it -infinity past the part's end. (A row is 2^28 bytes at most: a 32-bit offset from an address that
+    // all lanes share.)
     __device__ __forceinline__ u32x4v load(uint32_t v) const {
-        if (whole(v)) return *reinterpret_cast<const u32x4v *>(base + (uint64_t)v * kVec<T>);
-        Raw<T, kVec<T>> x;
+        constexpr uint32_t x = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+        u32x4v raw = {x, x, x, x};
+        if (v < v1) raw = *reinterpret_cast<const u32x4v *>(reinterpret_cast<const char *>(base) + v * 16);
+        return raw;
+    }
+    // Vectors v, v + step ..
+    template <int U>
+    __device__ __forceinline__ void load(uint32_t v, uint32_t step, u32x4v (&raw)[U]) const {
 #pragma unroll
-        for (uint32_t i = 0; i < kVec<T>; ++i) {
-            const uint32_t e = v * kVec<T> + i;
-            x[i] = v < v1 && e >= o && e < end ? base[e] : (T)neg_inf();
-        }
-        return __builtin_bit_cast(u32x4v, x);
+        for (int u = 0; u < U; ++u) raw[u] = load(v + u * step);
+    }
+    // The class of vector v's first element.
+    __device__ __forceinline__ uint32_t class_of(uint32_t v) const { return v * kVec<T> - o; }
+    // The class of this thread's edge, ~0 where it has none.
+    __device__ __forceinline__ uint32_t edge() const {
+        const uint32_t i = threadIdx.x, w0 = (o != 0) * kVec<T>;  // w0: where the whole vectors begin
+        if (first && i < kVec<T> && o + i < min(end, w0)) return i;
+        const uint32_t e = max(end / kVec<T> * kVec<T>, w0) + i - kVec<T>;
+        return last && i >= kVec<T> && i < kEdges && e < end ? e - o : ~0u;
     }
     // Whether class c is one of the part's.
-    __device__ __forceinline__ bool has(uint32_t c) const { return (o + c) / kVec<T> >= v0 && (o + c) / kVec<T> < v1; }
-    // The elements of another tensor's row that are at the places of vector v.
+    __device__ __forceinline__ bool has(uint32_t c) const {
+        const uint32_t v = (o + c) / kVec<T>;
+        return (v >= v0 || first) && (v < v1 || last);
+    }
+    // The elements of another tensor's row at the places of vector v.
     __device__ __forceinline__ void load_other(const T *row, uint32_t v, float (&x)[kVec<T>]) const {
-        if (whole(v)) {
-            const auto raw = *reinterpret_cast<const Unaligned<T> *>(row + class_of(v));
+        const auto raw = *reinterpret_cast<const Unaligned<T> *>(row + class_of(v));
 #pragma unroll
-            for (uint32_t i = 0; i < kVec<T>; ++i) x[i] = (float)raw[i];
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < kVec<T>; ++i) {
-                const uint32_t e = v * kVec<T> + i;
-                x[i] = v < v1 && e >= o && e < end ? load1(row, e - o) : 0.0f;
-            }
-        }
+        for (uint32_t i = 0; i < kVec<T>; ++i) x[i] = (float)raw[i];
     }
     __device__ __forceinline__ void store_other(T *row, uint32_t v, const float (&x)[kVec<T>]) const {
-        if (whole(v)) {
-            Unaligned<T> raw;
-            if constexpr (sizeof(T) == 4) {
+        Unaligned<T> raw;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) raw[i] = x[i];
-            } else {
-                const f32x8 f = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
-                raw = __builtin_convertvector(f, bf16x8);
-            }
-            *reinterpret_cast<Unaligned<T> *>(row + class_of(v)) = raw;
+            for (uint32_t i = 0; i < 4; ++i) raw[i] = x[i];
         } else {
-#pragma unroll
-            for (uint32_t i = 0; i < kVec<T>; ++i) {
-                const uint32_t e = v * kVec<T> + i;
-                if (v < v1 && e >= o && e < end) store1(row, e - o, x[i]);
-            }
+            const f32x8 f = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+            raw = __builtin_convertvector(f, bf16x8);
         }
+        *reinterpret_cast<Unaligned<T> *>(row + class_of(v)) = raw;
     }
-    // The class of vector v's first element; negative, as a 32-bit number, where that lies before the row.
-    __device__ __forceinline__ uint32_t class_of(uint32_t v) const { return v * kVec<T> - o; }
 };
 
 template <class T>
@@ -186,29 +187,127 @@ __device__ __forceinline__ void add(Sums &a, const u32x4v (&raw)[U], const Exp<T
     a.t += t;
 }
 
-// A group's value, in every thread of it. THREADS 64: a wave.
-template <class V, int THREADS, class F>
-__device__ __forceinline__ V group_reduce(V v, V *lds, F merge_two) {
+// Keeps the compiler from carrying the unpacked logits, twice the registers, from here on.
+__device__ __forceinline__ void repacked(u32x4v &raw) { asm volatile("" : "+v"(raw)); }
+
+// The sums of U vectors of logits that stay packed.
+template <class T, int U>
+__device__ __forceinline__ Sums sums_of(u32x4v (&raw)[U], const Exp<T> &ex) {
+    float m = neg_inf(), s = 0.0f;
 #pragma unroll
-    for (int mask = 1; mask < kWave; mask <<= 1) {
-        V o;
-        if constexpr (sizeof(V) == 4) {
-            o = __shfl_xor(v, mask);
-        } else {
-            o = {__shfl_xor(v.m, mask), __shfl_xor(v.s, mask), __shfl_xor(v.t, mask)};
-        }
-        // The lower lane's comes first, so that both lanes have the same bits.
-        v = threadIdx.x & mask ? merge_two(o, v) : merge_two(v, o);
+    for (int u = 0; u < U; ++u) {
+        float z[kVec<T>];
+        unpack<T>(raw[u], z);
+#pragma unroll
+        for (uint32_t i = 0; i < kVec<T>; ++i) m = fmaxf(m, z[i]);
+        repacked(raw[u]);
+        __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (THREADS > kWave) {
-        __syncthreads();  // the last use of lds
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = lds[0];
+    const float base = m == neg_inf() ? 0.0f : m;
 #pragma unroll
-        for (int w = 1; w < THREADS / kWave; ++w) v = merge_two(v, lds[w]);
+    for (int u = 0; u < U; ++u) {
+        float z[kVec<T>];
+        unpack<T>(raw[u], z);
+#pragma unroll
+        for (uint32_t i = 0; i < kVec<T>; ++i) s += Exp<T>::of(ex.scaled(z[i] - base));
+        repacked(raw[u]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    return {m, s, 0.0f};
+}
+
+// Adds one logit, -infinity adding nothing.
+template <class T>
+__device__ __forceinline__ void add_one(Sums &a, float z, const Exp<T> &ex) {
+    a = rebased(a, fmaxf(a.m, z), ex);
+    const float y = ex.scaled(z - (a.m == neg_inf() ? 0.0f : a.m)), e = Exp<T>::of(y);
+    a.s += e;
+    a.t += e * fmaxf(y, -300.0f);
+}
+
+// The value of lane ^ MASK, without LDS: MASK 1, 2, 3, 7, 8 or 15 within sixteen lanes, 4 as 7 ^ 3, 16 and 32 by the
+// instructions that swap rows and halves.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+template <int MASK>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    static_assert(MASK == 1 || MASK == 2 || MASK == 3 || MASK == 4 || MASK == 7 || MASK == 8 || MASK == 15 || MASK == 16 || MASK == 31 ||
+                  MASK == 32 || MASK == 63, "");
+    if constexpr (MASK == 1) return dpp<0xB1>(v);        // quad_perm 1 0 3 2
+    else if constexpr (MASK == 2) return dpp<0x4E>(v);   // quad_perm 2 3 0 1
+    else if constexpr (MASK == 3) return dpp<0x1B>(v);   // quad_perm 3 2 1 0
+    else if constexpr (MASK == 4) return lane_xor<3>(lane_xor<7>(v));
+    else if constexpr (MASK == 7) return dpp<0x141>(v);  // row_half_mirror
+    else if constexpr (MASK == 8) return dpp<0x128>(v);  // row_ror 8
+    else if constexpr (MASK == 15) return dpp<0x140>(v); // row_mirror
+    else if constexpr (MASK == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? r[0] : r[1];
+    } else if constexpr (MASK == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return threadIdx.x & 32 ? r[0] : r[1];
+    } else return lane_xor<MASK - 15>(lane_xor<15>(v));  // 31, 63
+}
+template <>
+__device__ __forceinline__ uint32_t lane_xor<63>(uint32_t v) {
+    return lane_xor<32>(lane_xor<16>(lane_xor<15>(v)));
+}
+template <int MASK>
+__device__ __forceinline__ float other_lane(float v) {
+    return __builtin_bit_cast(float, lane_xor<MASK>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int MASK>
+__device__ __forceinline__ Sums other_lane(const Sums &v) {
+    return {other_lane<MASK>(v.m), other_lane<MASK>(v.s), other_lane<MASK>(v.t)};
+}
+
+// Joins LANES lanes' values, in all of them. The lower lane's comes first, so that every lane has the same bits. (Groups of
+// `mask` lanes have one value, so that mirrors serve as the partners 4 and 8 away.)
+template <int LANES, int MASK = 1, class V, class F>
+__device__ __forceinline__ V lanes_reduce(V v, F merge_two) {
+    if constexpr (MASK < LANES) {
+        const V o = other_lane<MASK == 4 ? 7 : MASK == 8 ? 15 : MASK>(v);
+        v = threadIdx.x & MASK ? merge_two(o, v) : merge_two(v, o);
+        return lanes_reduce<LANES, MASK * 2>(v, merge_two);
     }
     return v;
+}
+// A group's value, in every thread of it. lds: one a wave.
+template <class V, int THREADS, class F>
+__device__ __forceinline__ V group_reduce(V v, V *lds, F merge_two) {
+    constexpr int kWaves = THREADS / kWave;
+    v = lanes_reduce<kWave>(v, merge_two);
+    if constexpr (kWaves > 1) {
+        __syncthreads();  // the last use of lds
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x / kWave] = v;
+        __syncthreads();
+        v = lanes_reduce<kWaves>(lds[threadIdx.x % kWaves], merge_two);
+    }
+    return v;
+}
+
+// Of `n` tokens in LDS: whether the jth, which is c, is the first of its class, and the sum of all that class's values, in
+// order. (Four are read at once; those past n up to a multiple of four are ~0.)
+struct Claim {
+    bool first;
+    float sum;
+};
+__device__ __forceinline__ Claim claim(const uint32_t *tokens, const float *values, uint32_t n, uint32_t j, uint32_t c) {
+    Claim r{true, 0.0f};
+#pragma unroll 4
+    for (uint32_t k = 0; k < n; k += 4) {
+        const u32x4v token = *reinterpret_cast<const u32x4v *>(tokens + k);
+        const float4 value = *reinterpret_cast<const float4 *>(values + k);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const bool same = token[i] == c;
+            r.first &= !(same && k + i < j);
+            r.sum += same ? lane(value, (int)i) : 0.0f;
+        }
+    }
+    return r;
 }
 
 // log of the sum: of a row without a class left -infinity; NaN stays.
@@ -219,10 +318,11 @@ __device__ __forceinline__ float log_prob_of(float z, float m, float l, float in
     return m == neg_inf() && l == neg_inf() ? neg_inf() : (z - m) * inv - l;
 }
 
-// exp(y - l), the probability of a class whose y is in Exp's unit; NaN where l is.
+// exp(d / temperature - l), the probability of a class whose logit is d from the largest; NaN where l is.
 template <class T>
-__device__ __forceinline__ float probability(float y, float l) {
-    return Exp<T>::of(sizeof(T) == 2 ? y - l * 1.44269504088896341f : y - l);
+__device__ __forceinline__ float probability(float d, float l, const Exp<T> &ex) {
+    if constexpr (sizeof(T) == 2) return Exp<T>::of(__builtin_fmaf(d, ex.c, l * -1.44269504088896341f));
+    else return Exp<T>::of(d * ex.inv - l);
 }
 
 // How rows are shared out: groups of `threads` threads, a row in `parts` of `per` vectors.
@@ -236,7 +336,7 @@ constexpr uint32_t kTileVectors = 4;  // vectors a thread and tile
 constexpr uint32_t kFill = 512;       // workgroups that are enough for the chip
 
 inline RowPlan plan_rows(int type, uint64_t rows, uint64_t classes) {
-    const uint64_t vec = type == DKZ_F32 ? 4 : 8, vectors = (classes + 2 * (vec - 1)) / vec;  // at any alignment
+    const uint64_t vec = type == DKZ_F32 ? 4 : 8, vectors = classes / vec;  // whole ones at most
     if (vectors <= kTileVectors * kWave) return {64, 1, (uint32_t)(kTileVectors * kWave)};
     const uint64_t tile = kTileVectors * kBlock, tiles = (vectors + tile - 1) / tile;
     const uint64_t want = std::min<uint64_t>(tiles, rows == 0 ? 1 : (kFill + rows - 1) / rows), each = (tiles + want - 1) / want;

@@ -57,8 +57,7 @@ __global__ __launch_bounds__(THREADS) void log_probs_kernel(Logits g, Answers ou
         TopList top(keys + wave * TopList::kRoom, TOP ? out.top : 1);
         for (uint32_t v0 = p.v0; v0 < p.v1; v0 += kEach * THREADS) {
             u32x4v raw[kEach];
-#pragma unroll
-            for (int u = 0; u < kEach; ++u) raw[u] = p.load(v0 + u * THREADS + threadIdx.x);
+            p.load(v0 + threadIdx.x, THREADS, raw);
             add<T, ENTROPY>(a, raw, ex);
             if constexpr (TOP) {
 #pragma unroll
@@ -71,6 +70,10 @@ __global__ __launch_bounds__(THREADS) void log_probs_kernel(Logits g, Answers ou
                 }
             }
         }
+        const uint32_t edge = p.edge();
+        const float at_edge = edge != ~0u ? load1(static_cast<const T *>(g.p) + (uint64_t)row * g.pitch, edge) : neg_inf();
+        add_one(a, at_edge, ex);
+        if constexpr (TOP) top.offer(key_of(at_edge, edge));
         a = group_reduce<Sums, THREADS>(a, lds, [&](const Sums &x, const Sums &y) { return merge(x, y, ex); });
         uint64_t list = 0;
         if constexpr (TOP) {
@@ -155,8 +158,8 @@ template <class T, int THREADS, bool ENTROPY, bool OLD>
 __global__ __launch_bounds__(THREADS) void log_probs_backward_kernel(Logits g, Deltas in) {
     constexpr int kEach = kTileVectors;
     __shared__ float sums[THREADS / kWave];
-    __shared__ uint32_t tokens[kMostGiven];
-    __shared__ float deltas[kMostGiven];
+    __shared__ __align__(16) uint32_t tokens[kMostGiven];
+    __shared__ __align__(16) float deltas[kMostGiven];
     const Exp<T> ex(g.inv);
     for (uint32_t group = blockIdx.x; group < g.rows * g.parts; group += gridDim.x) {
         const uint32_t row = group / g.parts, part = group - row * g.parts;
@@ -169,8 +172,8 @@ __global__ __launch_bounds__(THREADS) void log_probs_backward_kernel(Logits g, D
 
         __syncthreads();
         float total = 0.0f;
-        for (uint32_t j = threadIdx.x; j < in.given; j += THREADS) {
-            const uint32_t c = (uint32_t)in.tokens[(uint64_t)row * in.given + j];
+        for (uint32_t j = threadIdx.x; j < (in.given + 3) / 4 * 4; j += THREADS) {
+            const uint32_t c = j < in.given ? (uint32_t)in.tokens[(uint64_t)row * in.given + j] : ~0u;
             const float a = c < g.classes ? in.a[(uint64_t)row * in.given + j] : 0.0f;
             tokens[j] = c;
             deltas[j] = a;
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(THREADS) void log_probs_backward_kernel(Logits g, D
         const auto dense = [&](float z) __attribute__((always_inline)) {
             const float y = ex.scaled(z - m), log_p = Exp<T>::kUnit * fmaxf(y, -300.0f) - l;
             const float q = ENTROPY ? total + e * (log_p + h) : total;
-            return none ? 0.0f : -(probability<T>(y, l) * q) * g.inv;
+            return none ? 0.0f : -(probability<T>(z - m, l, ex) * q) * g.inv;
         };
         constexpr int kSlots = kMostGiven / THREADS > 1 ? kMostGiven / THREADS : 1;
         float fixed[kSlots];
@@ -194,25 +197,20 @@ __global__ __launch_bounds__(THREADS) void log_probs_backward_kernel(Logits g, D
             if (j >= in.given) continue;
             const uint32_t c = tokens[j];
             if (c >= g.classes || !p.has(c)) continue;
-            mine[i] = true;
-            float a = 0.0f;
-            for (uint32_t k = 0; k < in.given; ++k) {
-                if (tokens[k] != c) continue;
-                if (k < j) mine[i] = false;
-                a += deltas[k];
-            }
-            fixed[i] = dense(load1(logits, c)) + (none ? 0.0f : a * g.inv);
+            const Claim own = claim(tokens, deltas, in.given, j, c);
+            mine[i] = own.first;
+            fixed[i] = dense(load1(logits, c)) + (none ? 0.0f : own.sum * g.inv);
             if (OLD) fixed[i] += in.beta * load1(out, c);
         }
         __syncthreads();  // what logits_delta's old values, or the logits in its place, have been read for
         for (uint32_t v0 = p.v0; v0 < p.v1; v0 += kEach * THREADS) {
             u32x4v raw[kEach];
             float old[OLD ? kEach : 1][kVec<T>];
+            p.load(v0 + threadIdx.x, THREADS, raw);
+            if constexpr (OLD) {
 #pragma unroll
-            for (int u = 0; u < kEach; ++u) {
-                const uint32_t v = v0 + u * THREADS + threadIdx.x;
-                raw[u] = p.load(v);
-                if constexpr (OLD) p.load_other(out, v, old[u]);
+                for (int u = 0; u < kEach; ++u)
+                    if (v0 + u * THREADS + threadIdx.x < p.v1) p.load_other(out, v0 + u * THREADS + threadIdx.x, old[u]);
             }
 #pragma unroll
             for (int u = 0; u < kEach; ++u) {
@@ -223,9 +221,10 @@ __global__ __launch_bounds__(THREADS) void log_probs_backward_kernel(Logits g, D
                     z[i] = dense(z[i]);
                     if constexpr (OLD) z[i] += in.beta * old[u][i];
                 }
-                p.store_other(out, v0 + u * THREADS + threadIdx.x, z);
+                if (v0 + u * THREADS + threadIdx.x < p.v1) p.store_other(out, v0 + u * THREADS + threadIdx.x, z);
             }
         }
+        if (const uint32_t c = p.edge(); c != ~0u) store1(out, c, dense(load1(logits, c)) + (OLD ? in.beta * load1(out, c) : 0.0f));
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kSlots; ++i)
