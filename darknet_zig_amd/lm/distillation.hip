@@ -164,7 +164,8 @@ __device__ __forceinline__ Sums part_sums(const T *logits, const Part<T> &p, con
     for (uint32_t v0 = p.v0; v0 < p.v1; v0 += kEach * THREADS) {
         u32x4v raw[kEach];
         p.load(v0 + threadIdx.x, THREADS, raw);
-        add<T, false>(a, raw, ex);
+        float largest[kEach];
+        add<T, false>(a, raw, largest, ex);
     }
     const uint32_t edge = p.edge();
     add_one(a, edge != ~0u ? load1(logits, edge) : neg_inf(), ex);
@@ -270,9 +271,14 @@ struct DistillPlan {
 DistillPlan plan_distillation(int type, uint64_t rows, uint64_t classes) {
     const uint64_t vectors = classes / (type == DKZ_F32 ? 4 : 8);  // whole ones at most
     constexpr uint32_t kHeld[][2] = {{64, 4}, {256, 4}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}};
-    for (const auto &h : kHeld)
+    for (const auto &h : kHeld) {
+        // Few long rows leave the chip empty: two launches of several groups a row (65536 classes in bf16: 1 row 11.0 us, 13.3
+        // held; 64 rows 16.3 and 17.1; 128 rows 19.4 and 18.0. 131072: 1 row 11.0 and 20.7, 64 rows 19.0 and 25.0. 32768: 1 row
+        // 10.6 and 9.5).
+        if (rows <= 64 && h[0] * h[1] > 4096) break;
         if (vectors <= h[0] * h[1]) return {h[0], h[1], {0, 1, h[0] * h[1]}};
-    return {0, 0, plan_rows(type, rows, classes)};
+    }
+    return {0, 0, plan_joined_rows(type, rows, classes)};
 }
 
 template <class T>

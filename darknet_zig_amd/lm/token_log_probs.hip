@@ -21,25 +21,55 @@ struct Answers {
 
 // What a row's group writes, all of its threads having the row's sums and the first wave its list.
 template <class T, int THREADS>
-__device__ __forceinline__ void answer(const Logits &g, const Answers &out, uint32_t row, const Sums &a, uint64_t list) {
-    const float l = log_sum(a);
-    if (threadIdx.x == 0) {
-        out.stats[2 * (uint64_t)row] = a.m;
-        out.stats[2 * (uint64_t)row + 1] = l;
-        // l and -t / s are both at least 0: nothing cancels.
-        if (out.entropy != nullptr) out.entropy[row] = a.s == 0.0f ? 0.0f : l - Exp<T>::kUnit * (a.t / a.s);
+struct Answer {
+    static constexpr int kSlots = kMostGiven / THREADS;
+    uint32_t token[kSlots];
+    float z[kSlots];
+
+    // The given tokens and their logits, ahead of the row's sums.
+    __device__ __forceinline__ void begin(const Logits &g, const Answers &out, uint32_t row) {
+        const T *logits = static_cast<const T *>(g.p) + (uint64_t)row * g.pitch;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+            const uint32_t j = threadIdx.x + i * THREADS;
+            token[i] = j < out.given ? (uint32_t)out.tokens[(uint64_t)row * out.given + j] : ~0u;
+        }
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) z[i] = token[i] < g.classes ? load1(logits, token[i]) : 0.0f;
     }
-    const T *logits = static_cast<const T *>(g.p) + (uint64_t)row * g.pitch;
-    for (uint32_t j = threadIdx.x; j < out.given; j += THREADS) {
-        const uint64_t at = (uint64_t)row * out.given + j;
-        const uint32_t token = (uint32_t)out.tokens[at];
-        out.log_probs[at] = token < g.classes ? log_prob_of(load1(logits, token), a.m, l, g.inv) : 0.0f;
+    __device__ __forceinline__ void finish(const Logits &g, const Answers &out, uint32_t row, const Sums &a, uint64_t list) const {
+        const float l = log_sum(a);
+        if (threadIdx.x == 0) {
+            out.stats[2 * (uint64_t)row] = a.m;
+            out.stats[2 * (uint64_t)row + 1] = l;
+            // l and -t / s are both at least 0: nothing cancels.
+            if (out.entropy != nullptr) out.entropy[row] = a.s == 0.0f ? 0.0f : l - Exp<T>::kUnit * (a.t / a.s);
+        }
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+            const uint32_t j = threadIdx.x + i * THREADS;
+            if (j < out.given) out.log_probs[(uint64_t)row * out.given + j] = token[i] < g.classes ? log_prob_of(z[i], a.m, l, g.inv) : 0.0f;
+        }
+        if (threadIdx.x < out.top) {
+            const uint64_t at = (uint64_t)row * out.top + threadIdx.x;
+            const bool has = list != 0 && l == l;
+            out.top_tokens[at] = has ? (int)~(uint32_t)list : -1;
+            out.top_log_probs[at] = has ? log_prob_of(logit_of((uint32_t)(list >> 32)), a.m, l, g.inv) : l == l ? neg_inf() : l;
+        }
     }
-    if (threadIdx.x < out.top) {
-        const uint64_t at = (uint64_t)row * out.top + threadIdx.x;
-        out.top_tokens[at] = list != 0 ? (int)~(uint32_t)list : -1;
-        out.top_log_probs[at] = list != 0 ? log_prob_of(logit_of((uint32_t)(list >> 32)), a.m, l, g.inv) : neg_inf();
+};
+
+// The waves' lists joined two and two, in the first wave. keys: one a thread.
+template <int WAVES>
+__device__ __forceinline__ uint64_t join_lists(uint64_t list, uint64_t *keys) {
+    const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x & 63;
+#pragma unroll
+    for (uint32_t step = 1; step < WAVES; step *= 2) {
+        if (wave % (2 * step) == step) keys[threadIdx.x] = list;
+        __syncthreads();
+        if (wave % (2 * step) == 0) list = merged(list, keys[(wave + step) * kWave + kWave - 1 - lane]);
     }
+    return list;
 }
 
 // A group takes a part of a row: its sums in one pass, and its list of the largest.
@@ -47,79 +77,82 @@ template <class T, int THREADS, bool ENTROPY, bool TOP>
 __global__ __launch_bounds__(THREADS) void log_probs_kernel(Logits g, Answers out) {
     constexpr int kEach = kTileVectors, kWaves = THREADS / kWave;
     __shared__ Sums lds[kWaves];
-    __shared__ uint64_t keys[TOP ? kWaves * TopList::kRoom : 1];
+    __shared__ TopRoom rooms[TOP ? kWaves : 1];
+    __shared__ uint64_t keys[TOP ? THREADS : 1];
     const Exp<T> ex(g.inv);
-    const uint32_t wave = threadIdx.x / kWave;
     for (uint32_t group = blockIdx.x; group < g.rows * g.parts; group += gridDim.x) {
         const uint32_t row = group / g.parts, part = group - row * g.parts;
         const Part<T> p(g, row, part);
-        Sums a{neg_inf(), 0.0f, 0.0f};
-        TopList top(keys + wave * TopList::kRoom, TOP ? out.top : 1);
-        for (uint32_t v0 = p.v0; v0 < p.v1; v0 += kEach * THREADS) {
-            u32x4v raw[kEach];
-            p.load(v0 + threadIdx.x, THREADS, raw);
-            add<T, ENTROPY>(a, raw, ex);
-            if constexpr (TOP) {
-#pragma unroll
-                for (int u = 0; u < kEach; ++u) {
-                    float z[kVec<T>];
-                    unpack<T>(raw[u], z);
-                    const uint32_t c = p.class_of(v0 + u * THREADS + threadIdx.x);
-#pragma unroll
-                    for (uint32_t i = 0; i < kVec<T>; ++i) top.offer(key_of(z[i], c + i));
-                }
-            }
-        }
+        Answer<T, THREADS> answer;
+        if (g.parts == 1) answer.begin(g, out, row);
         const uint32_t edge = p.edge();
         const float at_edge = edge != ~0u ? load1(static_cast<const T *>(g.p) + (uint64_t)row * g.pitch, edge) : neg_inf();
+        Sums a{neg_inf(), 0.0f, 0.0f};
+        TopList<T> top(rooms[TOP ? threadIdx.x / kWave : 0], TOP ? out.top : 1);
+        for (uint32_t v0 = p.v0 + threadIdx.x; v0 - threadIdx.x < p.v1; v0 += kEach * THREADS) {
+            u32x4v raw[kEach];
+            float largest[kEach];
+            p.load(v0, THREADS, raw);
+            add<T, ENTROPY>(a, raw, largest, ex);
+            if constexpr (TOP) {
+                if (v0 - threadIdx.x == p.v0) top.begin(a.m);
+                top.tile(raw, largest, [&](int u) { return p.class_of(v0 + u * THREADS); });
+            }
+        }
         add_one(a, at_edge, ex);
-        if constexpr (TOP) top.offer(key_of(at_edge, edge));
         a = group_reduce<Sums, THREADS>(a, lds, [&](const Sums &x, const Sums &y) { return merge(x, y, ex); });
         uint64_t list = 0;
         if constexpr (TOP) {
+            top.offer(edge != ~0u ? key_of(at_edge, edge) : 0);
             top.finish();
-            list = top.list;
-            if constexpr (kWaves > 1) {
-                __syncthreads();
-                keys[threadIdx.x] = list;
-                __syncthreads();
-                if (wave == 0) {
-                    for (int w = 1; w < kWaves; ++w) list = merged(list, keys[w * kWave + kWave - 1 - threadIdx.x]);
-                }
-                __syncthreads();
-            }
+            list = join_lists<kWaves>(top.list, keys);
         }
         if (g.parts == 1) {
-            answer<T, THREADS>(g, out, row, a, list);
+            answer.finish(g, out, row, a, list);
         } else {
             if (threadIdx.x == 0) out.part_sums[group] = a;
             if (TOP && threadIdx.x < out.top) out.part_keys[(uint64_t)group * out.top + threadIdx.x] = list;
         }
+        if (TOP && kWaves > 1) __syncthreads();  // the keys' use
     }
 }
 
 // Joins a row's parts, a group of 256 threads a row.
 template <class T, bool TOP>
 __global__ __launch_bounds__(kBlock) void join_log_probs_kernel(Logits g, Answers out) {
-    constexpr int kWaves = kBlock / kWave;
+    constexpr int kWaves = kBlock / kWave, kAhead = 4;
     __shared__ Sums lds[kWaves];
-    __shared__ uint64_t keys[kBlock];
+    __shared__ uint64_t keys[TOP ? kBlock : 1];
     const Exp<T> ex(g.inv);
-    const uint32_t row = blockIdx.x, wave = threadIdx.x / kWave, lane = threadIdx.x & 63;
+    const uint32_t row = blockIdx.x, wave = threadIdx.x / kWave, back = kWave - 1 - (threadIdx.x & 63);
+    Answer<T, kBlock> answer;
+    answer.begin(g, out, row);
+    // A wave's lists, loaded a few at a time and from their ends.
+    const auto load = [&](uint64_t(&next)[kAhead], uint32_t p0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const uint32_t p = p0 + i * kWaves;
+            const uint32_t at = i == 0 && p0 == wave ? kWave - 1 - back : back;  // the first one is the list to begin with
+            next[i] = p < g.parts && at < out.top ? out.part_keys[((uint64_t)row * g.parts + p) * out.top + at] : 0;
+        }
+    };
+    uint64_t list = 0, next[kAhead];
+    if constexpr (TOP) load(next, wave);
     Sums a{neg_inf(), 0.0f, 0.0f};
     for (uint32_t p = threadIdx.x; p < g.parts; p += kBlock) a = merge(a, out.part_sums[(uint64_t)row * g.parts + p], ex);
     a = group_reduce<Sums, kBlock>(a, lds, [&](const Sums &x, const Sums &y) { return merge(x, y, ex); });
-    uint64_t list = 0;
     if constexpr (TOP) {
-        const uint32_t back = kWave - 1 - lane;
-        for (uint32_t p = wave; p < g.parts; p += kWaves)
-            list = merged(list, back < out.top ? out.part_keys[((uint64_t)row * g.parts + p) * out.top + back] : 0);
-        keys[threadIdx.x] = list;
-        __syncthreads();
-        if (wave == 0)
-            for (int w = 1; w < kWaves; ++w) list = merged(list, keys[w * kWave + back]);
+        for (uint32_t p = wave; p < g.parts; p += kAhead * kWaves) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (i == 0 && p == wave) list = next[0];
+                else if (p + i * kWaves < g.parts) list = merged(list, next[i]);
+            }
+            load(next, p + kAhead * kWaves);
+        }
+        list = join_lists<kWaves>(list, keys);
     }
-    answer<T, kBlock>(g, out, row, a, list);
+    answer.finish(g, out, row, a, list);
 }
 
 uint64_t part_bytes(uint64_t rows, const RowPlan &p, uint64_t top) {
@@ -252,7 +285,7 @@ extern "C" {
 
 int dkz_token_log_probs_workspace(int type, int rows, int classes, int top, size_t *bytes) {
     DKZ_REQUIRE(bytes != nullptr && logits_ok(type, rows, classes, classes, 1.0f) && top >= 0 && top <= kMostTop);
-    *bytes = (size_t)part_bytes((uint64_t)rows, plan_rows(type, rows, classes), (uint64_t)top);
+    *bytes = (size_t)part_bytes((uint64_t)rows, plan_joined_rows(type, rows, classes), (uint64_t)top);
     return 0;
 }
 
@@ -266,7 +299,7 @@ int dkz_token_log_probs(int type, int rows, int classes, int pitch, const void *
     DKZ_REQUIRE(stats != nullptr && (classes == 0 || logits != nullptr));
     DKZ_REQUIRE(given == 0 || (tokens != nullptr && log_probs_out != nullptr));
     DKZ_REQUIRE(top == 0 || (top_tokens != nullptr && top_log_probs != nullptr));
-    const RowPlan plan = plan_rows(type, rows, classes);
+    const RowPlan plan = plan_joined_rows(type, rows, classes);
     const uint64_t need = part_bytes(m, plan, (uint64_t)top);
     DKZ_REQUIRE_WORKSPACE(need);
     DKZ_REQUIRE(element_aligned(type, logits));
@@ -300,7 +333,7 @@ int dkz_token_log_probs_backward(int type, int rows, int classes, int pitch, con
     const Span writes[] = {{logits_delta, all}};
     const Span reads[] = {{onto ? nullptr : logits, all}, {tokens, 4 * n}, {stats, 8 * m}, {entropy, 4 * m}, {log_prob_deltas, 4 * n}, {entropy_deltas, 4 * m}};
     DKZ_REQUIRE(disjoint(writes, reads));
-    const RowPlan plan = plan_rows(type, rows, classes);
+    const RowPlan plan = plan_rows(type, rows, classes, ~0ull);
     const Logits g = make_logits(plan, logits, rows, classes, pitch, temperature);
     const Deltas in{tokens, stats, entropy, log_prob_deltas, entropy_deltas, logits_delta, beta, (uint32_t)given};
     const hipStream_t stream = current_stream();

@@ -88,8 +88,8 @@ int dkz_gated_backward(int type, int rows, int inputs, int hidden, int activatio
  * tokens and log_probs may be NULL where given is 0, as top_tokens and top_log_probs
  * where top is. temperature is 2^-64 .. 2^64. A row that has no class left has
  * m and l -infinity, log probabilities -infinity and entropy 0. A row with a NaN or
- * +infinity logit has NaN for l, log probabilities and entropy; a NaN counts as the
- * largest logit for the alternatives, not for m. */
+ * +infinity logit has NaN for l, log probabilities and entropy, and no alternatives:
+ * tokens -1 with NaN. m passes over NaNs. */
 int dkz_token_log_probs_workspace(int type, int rows, int classes, int top, size_t *bytes);
 int dkz_token_log_probs(int type, int rows, int classes, int pitch, const void *logits, float temperature, int given,
                         const int *tokens, int top, float *log_probs, float *entropy, float *stats, int *top_tokens,

@@ -112,8 +112,8 @@ def probability_error(y, l):
 
 
 def best(z, top):
-    """The classes of the `top` largest of a row, NaNs first, equal ones by class, -1 past the last that is not masked."""
-    order = np.lexsort((np.arange(z.size), np.where(np.isnan(z), 0.0, -z), ~np.isnan(z)))
+    """The classes of the `top` largest of a row, equal ones by class, -1 past the last that is not masked."""
+    order = np.lexsort((np.arange(z.size), -z))
     order = order[~np.isneginf(z[order])][:top]
     return np.concatenate([order, np.full(top - order.size, -1)]).astype(np.int64)
 
