@@ -36,14 +36,11 @@ int launch_f32_tiles(hipStream_t stream, const char *name, const Tiling &t, dim3
     return launch_on(stream, name, gemm_split_kernel<64, 64, AK, BK, false, Epi...>, grid, block, g, epi...);
 }
 
-// C (m x n, leading dimension ldc) = beta * C + op(A) op(B), or every element of the product to `epi`.
-// kRowMajor: A is m x k, B n x k; kColMajor: A is k x m, B k x n. `partial` has f32_partial_bytes.
+// run_f32's tiles, without the join of what they leave in pieces.
 template <Operand AK, Operand BK, class... Epi>
-int run_f32(hipStream_t stream, const char *name, const float *a, uint64_t lda, const float *b, uint64_t ldb, float beta, float *c, uint64_t ldc,
-            uint64_t m, uint64_t n, uint64_t k, float *partial, const Epi &...epi) {
-    if (m == 0 || n == 0) return 0;
-    const Tiling t = plan_f32(m, n, k);
-    SplitArgs g{};
+int run_f32_tiles(hipStream_t stream, const char *name, const float *a, uint64_t lda, const float *b, uint64_t ldb, float beta, float *c, uint64_t ldc,
+                  uint64_t m, uint64_t n, uint64_t k, float *partial, const Tiling &t, SplitArgs &g, const Epi &...epi) {
+    g = SplitArgs{};
     g.a = a;
     g.b = b;
     g.c = c;
@@ -74,10 +71,22 @@ int run_f32(hipStream_t stream, const char *name, const float *a, uint64_t lda, 
         total = t.full_tiles + g.runs;
     }
     DKZ_REQUIRE(total <= 0x7fffffffull);
-    DKZ_TRY((launch_f32_tiles<AK, BK, Epi...>(stream, name, t, dim3((uint32_t)total), g, epi...)));
+    return launch_f32_tiles<AK, BK, Epi...>(stream, name, t, dim3((uint32_t)total), g, epi...);
+}
+
+// C (m x n, leading dimension ldc) = beta * C + op(A) op(B), or every element of the product to `epi`.
+// kRowMajor: A is m x k, B n x k; kColMajor: A is k x m, B k x n. `partial` has f32_partial_bytes.
+template <Operand AK, Operand BK, class... Epi>
+int run_f32(hipStream_t stream, const char *name, const float *a, uint64_t lda, const float *b, uint64_t ldb, float beta, float *c, uint64_t ldc,
+            uint64_t m, uint64_t n, uint64_t k, float *partial, const Epi &...epi) {
+    if (m == 0 || n == 0) return 0;
+    const Tiling t = plan_f32(m, n, k);
+    SplitArgs g;
+    DKZ_TRY((run_f32_tiles<AK, BK, Epi...>(stream, name, a, lda, b, ldb, beta, c, ldc, m, n, k, partial, t, g, epi...)));
     const bool v4 = n % 4 == 0 && ldc % 4 == 0 && aligned16(c);
     const dim3 block(kBlock);
     if (t.stream) {
+        const uint32_t streamed = (uint32_t)((uint64_t)g.tiles_m * g.tiles_n * g.splits - t.full_tiles);
         const dim3 blocks(streamed * (t.bm * t.bn / 4 / kBlock));
         return v4 ? launch_on(stream, name, stream_reduce_kernel<true, Epi...>, blocks, block, g, epi...)
                   : launch_on(stream, name, stream_reduce_kernel<false, Epi...>, blocks, block, g, epi...);

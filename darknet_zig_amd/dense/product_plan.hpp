@@ -95,27 +95,40 @@ inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool n
 inline uint64_t packed_ld(uint64_t k) { return round_up(k, 8); }
 inline uint64_t packed_bytes(uint64_t rows, uint64_t k) { return k % 8 == 0 ? 0 : padded(2 * rows * packed_ld(k)); }
 
-// A thread a chunk of the copies of a (rows_a) and b (rows_b).
-__global__ __launch_bounds__(kBlock) void pack_kernel(const __bf16 *a, uint32_t rows_a, __bf16 *to_a, const __bf16 *b, uint32_t rows_b,
-                                                     __bf16 *to_b, uint32_t k, FastDiv chunks) {
-    uint32_t at = blockIdx.x * kBlock + threadIdx.x;
-    const uint32_t end_a = rows_a * chunks.d;
-    if (at >= end_a + rows_b * chunks.d) return;
-    const __bf16 *from = at < end_a ? a : b;
-    __bf16 *to = at < end_a ? to_a : to_b;
+// What is to be copied: rows_a rows of a, then rows_b of b, in chunks.
+struct PackArgs {
+    const __bf16 *a;
+    uint32_t rows_a;
+    __bf16 *to_a;
+    const __bf16 *b;
+    uint32_t rows_b;
+    __bf16 *to_b;
+    uint32_t k;
+    FastDiv chunks;  // of a row
+    uint64_t count() const { return ((uint64_t)rows_a + rows_b) * chunks.d; }
+};
+
+// Chunk `at` of the copies.
+__device__ __forceinline__ void pack_chunk(const PackArgs &g, uint32_t at) {
+    const uint32_t end_a = g.rows_a * g.chunks.d;
+    if (at >= end_a + g.rows_b * g.chunks.d) return;
+    const __bf16 *from = at < end_a ? g.a : g.b;
+    __bf16 *to = at < end_a ? g.to_a : g.to_b;
     at -= at < end_a ? 0 : end_a;
-    const uint32_t row = fdiv(at, chunks), c = (at - row * chunks.d) * 8;
-    const short *p = reinterpret_cast<const short *>(from) + (uint64_t)row * k + c;
+    const uint32_t row = fdiv(at, g.chunks), c = (at - row * g.chunks.d) * 8;
+    const short *p = reinterpret_cast<const short *>(from) + (uint64_t)row * g.k + c;
     s16x8 v = {};
-    if (c + 8 <= k) {
+    if (c + 8 <= g.k) {
         v = load_shifted(p);
     } else {
 #pragma unroll
         for (int i = 0; i < 7; ++i)
-            if (c + i < k) v[i] = p[i];
+            if (c + i < g.k) v[i] = p[i];
     }
     reinterpret_cast<s16x8 *>(to)[at] = v;
 }
+// A thread a chunk.
+__global__ __launch_bounds__(kBlock) void pack_kernel(PackArgs g) { pack_chunk(g, blockIdx.x * kBlock + threadIdx.x); }
 
 // A matrix as the products take it.
 struct Matrix {
@@ -123,18 +136,19 @@ struct Matrix {
     uint64_t ld;
 };
 
-// Copies a and b (null: left out) to the workspace where their rows are no whole chunks.
-inline int pack(hipStream_t stream, Matrix &a, uint64_t rows_a, Matrix &b, uint64_t rows_b, uint64_t k, Workspace &ws) {
-    if (k % 8 == 0) return 0;
+// a and b (null: left out) become copies in the workspace where their rows are no whole chunks; what is then to be copied.
+inline PackArgs pack_args(Matrix &a, uint64_t rows_a, Matrix &b, uint64_t rows_b, uint64_t k, Workspace &ws) {
+    if (k % 8 == 0) return {};
     const uint64_t ld = packed_ld(k), na = a.p != nullptr ? rows_a : 0, nb = b.p != nullptr ? rows_b : 0;
     __bf16 *to_a = ws.take<__bf16>(packed_bytes(rows_a, k) / 2), *to_b = ws.take<__bf16>(packed_bytes(rows_b, k) / 2);
-    const uint64_t chunks = (na + nb) * (ld / 8);
-    if (chunks != 0)
-        DKZ_TRY(launch_on(stream, "pack", pack_kernel, dim3(div_up(chunks, kBlock)), dim3(kBlock), a.p, (uint32_t)na, to_a, b.p, (uint32_t)nb, to_b,
-                          (uint32_t)k, make_fastdiv((uint32_t)(ld / 8))));
+    const PackArgs g{a.p, (uint32_t)na, to_a, b.p, (uint32_t)nb, to_b, (uint32_t)k, make_fastdiv((uint32_t)(ld / 8))};
     if (na) a = {to_a, ld};
     if (nb) b = {to_b, ld};
-    return 0;
+    return g;
+}
+inline int pack(hipStream_t stream, Matrix &a, uint64_t rows_a, Matrix &b, uint64_t rows_b, uint64_t k, Workspace &ws) {
+    const PackArgs g = pack_args(a, rows_a, b, rows_b, k, ws);
+    return g.count() != 0 ? launch_on(stream, "pack", pack_kernel, dim3(div_up(g.count(), kBlock)), dim3(kBlock), g) : 0;
 }
 
 // A size that a workspace is planned by, whatever the alignment of the operands.

@@ -209,6 +209,43 @@ __global__ __launch_bounds__(kBlock) void gate_kernel(const float *sums, float *
     }
 }
 
+// fp32, where K is cut: the join of both projections' pieces (in f64) and the output at once, a thread W units of a row.
+template <int W, bool EXP>
+__global__ __launch_bounds__(kBlock) void gate_join_kernel(const float *partial, uint32_t splits, uint32_t rows, uint32_t half, uint32_t units,
+                                                          const float *biases, float *sums, float *output, Gate gate) {
+    constexpr uint32_t kAhead = 8 / W;
+    const uint32_t i = blockIdx.x * kBlock + threadIdx.x, r = i / units, j = (i - r * units) * W;
+    if (r >= rows) return;
+    const uint64_t at = (uint64_t)r * 2 * half + j, size = (uint64_t)rows * 2 * half;
+    double s[2][W] = {};
+    for (uint32_t p = 0; p < splits; p += kAhead) {
+        Raw<float, W> x[kAhead][2];  // past the last piece: that one again, not added
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) x[u][h] = *reinterpret_cast<const Raw<float, W> *>(partial + min(p + u, splits - 1) * size + at + h * half);
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                for (int w = 0; w < W; ++w) s[h][w] += p + u < splits ? (double)x[u][h][w] : 0.0;
+    }
+    Raw<float, W> x, y, out;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const float g = (float)s[0][w], u = (float)s[1][w];
+        x[w] = biases != nullptr ? g + biases[j + w] : g;
+        y[w] = biases != nullptr ? u + biases[half + j + w] : u;
+        out[w] = activate_gate<float, EXP>(gate, x[w]) * y[w];
+    }
+    if (sums != nullptr) {
+        *reinterpret_cast<Raw<float, W> *>(sums + at) = x;
+        *reinterpret_cast<Raw<float, W> *>(sums + at + half) = y;
+    }
+    *reinterpret_cast<Raw<float, W> *>(output + (uint64_t)r * half + j) = out;
+}
+
 inline uint64_t paired_columns(uint64_t half) { return 2 * round_up(half, 8); }
 // Rows of both halves within the loads' 32-bit offsets of a tile's first.
 inline bool pairs_direct(const Matrix &x, const Matrix &w, uint64_t half) {
@@ -221,10 +258,27 @@ uint64_t forward_bytes(int type, uint64_t rows, uint64_t inputs, uint64_t hidden
     return packed + most_partial_bytes(rows, paired_columns(hidden), inputs, true);
 }
 
+// Pieces that a thread of gate_join_kernel adds up; the products of more have a join with sixteen threads an element.
+constexpr uint32_t kJoinPieces = 32;
+
 template <bool EXP>
 int forward_f32(hipStream_t stream, uint64_t rows, uint64_t inputs, uint64_t hidden, const Gate &gate, const float *input, const float *weights,
                 const float *biases, float *sums, float *output, Workspace ws) {
+    constexpr const char *kName = "gated_forward";
     float *own = ws.take<float>(rows * 2 * hidden), *partial = ws.take<float>(f32_partial_bytes(rows, 2 * hidden, inputs) / 4);
+    const Tiling t = plan_f32(rows, 2 * hidden, inputs);
+    if (t.splits > 1 && t.splits <= kJoinPieces) {
+        SplitArgs g;
+        DKZ_TRY((run_f32_tiles<kRowMajor, kRowMajor>(stream, kName, input, inputs, weights, inputs, 0.0f, (float *)nullptr, 2 * hidden, rows, 2 * hidden,
+                                                     inputs, partial, t, g)));
+        const bool fours = hidden % 4 == 0 && aligned16(output) && (sums == nullptr || aligned16(sums));
+        const uint32_t units = (uint32_t)(fours ? hidden / 4 : hidden);
+        const dim3 grid(div_up(rows * units, kBlock));
+        return fours ? launch_on(stream, kName, gate_join_kernel<4, EXP>, grid, dim3(kBlock), partial, t.splits, (uint32_t)rows, (uint32_t)hidden, units,
+                                 biases, sums, output, gate)
+                     : launch_on(stream, kName, gate_join_kernel<1, EXP>, grid, dim3(kBlock), partial, t.splits, (uint32_t)rows, (uint32_t)hidden, units,
+                                 biases, sums, output, gate);
+    }
     if (sums == nullptr) sums = own;
     LinearEpilogue<float, false> e;
     e.biases = biases;
@@ -239,7 +293,7 @@ int forward_f32(hipStream_t stream, uint64_t rows, uint64_t inputs, uint64_t hid
                                            2 * hidden, inputs, partial, e)));
     const uint64_t fours = (hidden + 3) / 4;
     const dim3 grid((uint32_t)std::min<uint64_t>((rows * fours + kBlock - 1) / kBlock, 1u << 16));
-    return launch_on(stream, "gated_forward", gate_kernel<EXP>, grid, dim3(kBlock), sums, output, (uint32_t)rows, (uint32_t)hidden, (uint32_t)fours, gate);
+    return launch_on(stream, kName, gate_kernel<EXP>, grid, dim3(kBlock), sums, output, (uint32_t)rows, (uint32_t)hidden, (uint32_t)fours, gate);
 }
 
 template <bool EXP>
@@ -264,73 +318,105 @@ int forward_bf16(hipStream_t stream, uint64_t rows, uint64_t inputs, uint64_t hi
 
 // ---- backward ----
 
-constexpr uint32_t kDeltaRows = 64;  // rows whose columns a workgroup of gate_delta_kernel sums
+constexpr uint32_t kDeltaRows = 64;    // rows a workgroup of gate_delta_kernel takes at once
+constexpr uint32_t kDeltaWhole = 128;  // rows up to which it takes all of its units'
+constexpr uint32_t kDeltaFill = 128;   // workgroups that are enough for eight units a thread
 
-// d(r, j) and d(r, half + j) to d, in rows of ldd (ldd's padding is 0; null: not stored), and the sums of
-// kDeltaRows rows' columns to `to` (null: not). A thread takes W units of eight rows; the eight sums of a
-// unit's threads are added in row order.
-template <class T, int W, bool EXP>
-__global__ __launch_bounds__(kBlock) void gate_delta_kernel(const T *sums, const T *delta, uint32_t rows, uint32_t half, Gate gate, T *d, uint32_t ldd,
-                                                           uint32_t blocks_c, float *to) {
+template <class T>
+struct GateDelta {
+    const T *sums, *delta;
+    uint32_t rows, half;
+    Gate gate;
+    T *d;  // null: not wanted
+    uint32_t ldd, blocks_c, blocks;
+    float beta, *to;  // null: not wanted
+    PackArgs pack;    // of T bf16: copies that the products need too, by the workgroups after the first `blocks`
+};
+
+// d(r, j) and d(r, half + j) to d, in rows of ldd (ldd's padding is 0), and the sums of kDeltaRows rows' columns to `to`. A
+// thread takes W units of eight rows; the eight sums of a unit's threads are added in row order. WHOLE: a workgroup takes all rows,
+// adds their sums in f64, and `to` is bias_updates itself. Bound by memory where it is large: 4096 rows of 8192 units, bf16, 56 us
+// (6.0 TB/s).
+template <class T, int W, bool EXP, bool WHOLE>
+__global__ __launch_bounds__(kBlock) void gate_delta_kernel(GateDelta<T> g) {
     constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes, kEach = kDeltaRows / kGroups;
     __shared__ float lds[2][kGroups][kLanes * W + 4];
-    const uint32_t x = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const uint32_t block_r = blockIdx.x / blocks_c, block_c = blockIdx.x - block_r * blocks_c;
+    if constexpr (sizeof(T) == 2) {
+        if (blockIdx.x >= g.blocks) return pack_chunk(g.pack, (blockIdx.x - g.blocks) * kBlock + threadIdx.x);
+    }
+    const uint32_t half = g.half, x = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const uint32_t block_r = blockIdx.x / g.blocks_c, block_c = blockIdx.x - block_r * g.blocks_c;
     const uint32_t j = (block_c * kLanes + x) * W;
     const bool in = j < half;  // W == 8: half is a multiple of it
-    const uint32_t r0 = block_r * kDeltaRows + group * kEach;
-    float total[2][W] = {};
-    constexpr uint32_t kBatch = 2;  // rows whose loads are on their way at once
+    constexpr uint32_t kBatch = W == 1 ? kEach : 2;  // rows whose loads are on their way at once
+    constexpr uint32_t kStored = (2 * kLanes * W + kBlock - 1) / kBlock;  // sums that a thread stores
+    double whole[kStored] = {};
+    for (uint32_t top = WHOLE ? 0 : block_r * kDeltaRows; top < g.rows; top += kDeltaRows) {
+        const uint32_t r0 = top + group * kEach;
+        float total[2][W] = {};
 #pragma unroll 1
-    for (uint32_t i0 = 0; i0 < kEach; i0 += kBatch) {
-        Raw<T, W> g[kBatch], up[kBatch], dl[kBatch];
+        for (uint32_t i0 = 0; i0 < kEach; i0 += kBatch) {
+            Raw<T, W> s[kBatch], up[kBatch], dl[kBatch];
 #pragma unroll
-        for (uint32_t i = 0; i < kBatch; ++i) {
-            const uint64_t r = min(r0 + i0 + i, rows - 1), at = in ? j : 0;
-            load_raw<T, RowRun, W>(sums, RowRun{r * 2 * half + at, W}, g[i]);
-            load_raw<T, RowRun, W>(sums, RowRun{r * 2 * half + half + at, W}, up[i]);
-            load_raw<T, RowRun, W>(delta, RowRun{r * half + at, W}, dl[i]);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < kBatch; ++i) {
-            const uint32_t r = r0 + i0 + i;
-            if (r >= rows || !in) break;
-            float dg[W], du[W];
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                float a;
-                const float slope = gate_slope<T, EXP>(gate, (float)g[i][w], a), v = (float)dl[i][w];
-                dg[w] = v * (float)up[i][w] * slope;
-                du[w] = v * a;
-                total[0][w] += dg[w];
-                total[1][w] += du[w];
+            for (uint32_t i = 0; i < kBatch; ++i) {
+                const uint64_t r = min(r0 + i0 + i, g.rows - 1), at = in ? j : 0;
+                load_raw<T, RowRun, W>(g.sums, RowRun{r * 2 * half + at, W}, s[i]);
+                load_raw<T, RowRun, W>(g.sums, RowRun{r * 2 * half + half + at, W}, up[i]);
+                load_raw<T, RowRun, W>(g.delta, RowRun{r * half + at, W}, dl[i]);
             }
-            if (d != nullptr) {
-                store_n(d, RowRun{(uint64_t)r * ldd + j, W}, dg);
-                store_n(d, RowRun{(uint64_t)r * ldd + half + j, W}, du);
+#pragma unroll
+            for (uint32_t i = 0; i < kBatch; ++i) {
+                const uint32_t r = r0 + i0 + i;
+                if (r >= g.rows || !in) break;
+                float dg[W], du[W];
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    float a;
+                    const float slope = gate_slope<T, EXP>(g.gate, (float)s[i][w], a), v = (float)dl[i][w];
+                    dg[w] = v * (float)up[i][w] * slope;
+                    du[w] = v * a;
+                    total[0][w] += dg[w];
+                    total[1][w] += du[w];
+                }
+                if (g.d != nullptr) {
+                    store_n(g.d, RowRun{(uint64_t)r * g.ldd + j, W}, dg);
+                    store_n(g.d, RowRun{(uint64_t)r * g.ldd + half + j, W}, du);
+                }
             }
         }
-    }
-    // The padding, at most seven elements a row.
-    if (d != nullptr && block_c == 0 && ldd > 2 * half) {
-        const uint32_t c = 2 * half + x;
-        if (c < ldd)
+        // The padding, at most seven elements a row.
+        if (g.d != nullptr && block_c == 0 && 2 * half + x < g.ldd)
             for (uint32_t i = 0; i < kEach; ++i)
-                if (r0 + i < rows) store1(d, (uint64_t)(r0 + i) * ldd + c, 0.0f);
+                if (r0 + i < g.rows) store1(g.d, (uint64_t)(r0 + i) * g.ldd + 2 * half + x, 0.0f);
+        if (g.to != nullptr) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int w = 0; w < W; ++w) lds[s][group][x * W + w] = total[s][w];
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < kStored; ++i) {
+                const uint32_t e = threadIdx.x + i * kBlock, s = e / (kLanes * W), c = e % (kLanes * W), unit = block_c * kLanes * W + c;
+                if (s >= 2 || unit >= half) continue;
+                float t = lds[s][0][c];
+#pragma unroll
+                for (uint32_t k = 1; k < kGroups; ++k) t += lds[s][k][c];
+                if constexpr (WHOLE) whole[i] += (double)t;
+                else g.to[(uint64_t)block_r * 2 * half + s * half + unit] = t;
+            }
+            if constexpr (WHOLE) __syncthreads();
+        }
+        if constexpr (!WHOLE) break;
     }
-    if (to == nullptr) return;
+    if constexpr (WHOLE) {
+        if (g.to == nullptr) return;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int w = 0; w < W; ++w) lds[s][group][x * W + w] = total[s][w];
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < 2 * kLanes * W; e += kBlock) {
-        const uint32_t s = e / (kLanes * W), c = e % (kLanes * W), unit = block_c * kLanes * W + c;
-        if (unit >= half) continue;
-        float t = lds[s][0][c];
-#pragma unroll
-        for (uint32_t i = 1; i < kGroups; ++i) t += lds[s][i][c];
-        to[(uint64_t)block_r * 2 * half + s * half + unit] = t;
+        for (uint32_t i = 0; i < kStored; ++i) {
+            const uint32_t e = threadIdx.x + i * kBlock, s = e / (kLanes * W), unit = block_c * kLanes * W + e % (kLanes * W);
+            if (s >= 2 || unit >= half) continue;
+            float &to = g.to[s * half + unit];
+            to = g.beta == 0.0f ? (float)whole[i] : g.beta * to + (float)whole[i];
+        }
     }
 }
 
@@ -353,15 +439,20 @@ BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t hi
     return p;
 }
 
+// bias_updates null: not wanted; sums: room for the sums of every kDeltaRows rows.
 template <class T, bool EXP>
-int run_gate_delta(hipStream_t stream, const T *sums, const T *delta, uint64_t rows, uint64_t hidden, const Gate &gate, T *d, uint64_t ldd, float *to) {
+int run_gate_delta(hipStream_t stream, GateDelta<T> g, float *sums, float *bias_updates) {
     constexpr const char *kName = "gated_backward_delta";
-    const bool eights = hidden % 8 == 0;
-    const uint32_t blocks_c = div_up(hidden, eights ? 256 : 32);
-    const dim3 grid(blocks_c * div_up(rows, kDeltaRows)), block(kBlock);
-    if (eights)
-        return launch_on(stream, kName, gate_delta_kernel<T, 8, EXP>, grid, block, sums, delta, (uint32_t)rows, (uint32_t)hidden, gate, d, (uint32_t)ldd, blocks_c, to);
-    return launch_on(stream, kName, gate_delta_kernel<T, 1, EXP>, grid, block, sums, delta, (uint32_t)rows, (uint32_t)hidden, gate, d, (uint32_t)ldd, blocks_c, to);
+    const bool whole = g.rows <= kDeltaWhole;
+    const uint32_t blocks_r = whole ? 1 : div_up(g.rows, kDeltaRows);
+    const bool eights = g.half % 8 == 0 && div_up(g.half, 256) * blocks_r >= kDeltaFill;
+    g.blocks_c = div_up(g.half, eights ? 256 : 32);
+    g.blocks = g.blocks_c * blocks_r;
+    g.to = bias_updates == nullptr ? nullptr : whole ? bias_updates : sums;
+    const dim3 grid(g.blocks + div_up(g.pack.count(), kBlock)), block(kBlock);
+    if (whole) return eights ? launch_on(stream, kName, gate_delta_kernel<T, 8, EXP, true>, grid, block, g) : launch_on(stream, kName, gate_delta_kernel<T, 1, EXP, true>, grid, block, g);
+    DKZ_TRY(eights ? launch_on(stream, kName, gate_delta_kernel<T, 8, EXP, false>, grid, block, g) : launch_on(stream, kName, gate_delta_kernel<T, 1, EXP, false>, grid, block, g));
+    return bias_updates != nullptr ? add_column_sums(stream, sums, blocks_r, 2 * (uint64_t)g.half, g.beta, bias_updates) : 0;
 }
 
 template <class T>
@@ -373,28 +464,33 @@ int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint6
     float *sums = ws.take<float>(plan.sum_bytes / 4), *partial = ws.take<float>(plan.partial_bytes / 4);
     const uint64_t ldd = delta_ld(type, hidden), n = 2 * hidden;
     const bool products = inputs != 0 && (weight_updates != nullptr || input_delta != nullptr);
-    const Gate gate = make_gate(act);
-    const T *s = static_cast<const T *>(sums_in), *delta = static_cast<const T *>(delta_in);
+    Matrix x{weight_updates != nullptr ? reinterpret_cast<const __bf16 *>(input) : nullptr, inputs};
+    Matrix w{input_delta != nullptr ? reinterpret_cast<const __bf16 *>(weights) : nullptr, inputs};
     if (rows != 0 && hidden != 0 && (products || bias_updates != nullptr)) {
-        T *to = products ? d : nullptr;
-        float *bias = bias_updates != nullptr ? sums : nullptr;
-        DKZ_TRY(gate_has_exp(act) ? (run_gate_delta<T, true>(stream, s, delta, rows, hidden, gate, to, ldd, bias))
-                                  : (run_gate_delta<T, false>(stream, s, delta, rows, hidden, gate, to, ldd, bias)));
+        GateDelta<T> g{};
+        g.sums = static_cast<const T *>(sums_in);
+        g.delta = static_cast<const T *>(delta_in);
+        g.rows = (uint32_t)rows;
+        g.half = (uint32_t)hidden;
+        g.gate = make_gate(act);
+        g.d = products ? d : nullptr;
+        g.ldd = (uint32_t)ldd;
+        g.beta = beta;
+        if (sizeof(T) == 2 && products) g.pack = pack_args(x, rows, w, n, inputs, ws);
+        DKZ_TRY(gate_has_exp(act) ? (run_gate_delta<T, true>(stream, g, sums, bias_updates)) : (run_gate_delta<T, false>(stream, g, sums, bias_updates)));
+    } else if (bias_updates != nullptr) {
+        DKZ_TRY(add_column_sums(stream, sums, 0, n, beta, bias_updates));  // no rows: beta * bias_updates
     }
-    if (bias_updates != nullptr) DKZ_TRY(add_column_sums(stream, sums, div_up(rows, kDeltaRows), n, beta, bias_updates));
     constexpr const char *kWeights = "gated_backward_weights", *kInput = "gated_backward_input";
     if constexpr (sizeof(T) == 4) {
-        const T *x = static_cast<const T *>(input), *w = static_cast<const T *>(weights);
+        const T *in = static_cast<const T *>(input), *wt = static_cast<const T *>(weights);
         if (weight_updates != nullptr)
-            DKZ_TRY((run_f32<kColMajor, kColMajor>(stream, kWeights, d, ldd, x, inputs, beta, static_cast<float *>(weight_updates), inputs, n, inputs,
+            DKZ_TRY((run_f32<kColMajor, kColMajor>(stream, kWeights, d, ldd, in, inputs, beta, static_cast<float *>(weight_updates), inputs, n, inputs,
                                                    rows, partial)));
         if (input_delta != nullptr)
-            DKZ_TRY((run_f32<kRowMajor, kColMajor>(stream, kInput, d, ldd, w, inputs, 0.0f, (float *)nullptr, inputs, rows, inputs, n, partial,
+            DKZ_TRY((run_f32<kRowMajor, kColMajor>(stream, kInput, d, ldd, wt, inputs, 0.0f, (float *)nullptr, inputs, rows, inputs, n, partial,
                                                    store_epilogue<T>(input_delta, input_residual, inputs, 0.0f))));
     } else {
-        Matrix x{weight_updates != nullptr ? static_cast<const T *>(input) : nullptr, inputs};
-        Matrix w{input_delta != nullptr ? static_cast<const T *>(weights) : nullptr, inputs};
-        if (rows != 0) DKZ_TRY(pack(stream, x, rows, w, n, inputs, ws));
         const Product to_input{d, ldd, w.p, w.ld, rows, inputs, n}, to_weights{d, ldd, x.p, x.ld, n, inputs, rows};
         DKZ_TRY(run_gradients(stream, kInput, input_delta != nullptr ? &to_input : nullptr, store_epilogue<T>(input_delta, input_residual, inputs, 0.0f),
                               kWeights, weight_updates != nullptr ? &to_weights : nullptr, store_epilogue<T>(weight_updates, nullptr, inputs, beta), partial));
