@@ -74,6 +74,16 @@ int run_f32_tiles(hipStream_t stream, const char *name, const float *a, uint64_t
     return launch_f32_tiles<AK, BK, Epi...>(stream, name, t, dim3((uint32_t)total), g, epi...);
 }
 
+// The join of streamed tiles' pieces.
+template <class... Epi>
+int join_f32_stream(hipStream_t stream, const char *name, const Tiling &t, const SplitArgs &g, const Epi &...epi) {
+    const uint32_t streamed = (uint32_t)((uint64_t)g.tiles_m * g.tiles_n * g.splits - t.full_tiles);
+    const dim3 blocks(streamed * (t.bm * t.bn / 4 / kBlock)), block(kBlock);
+    const bool v4 = g.n % 4 == 0 && g.ldc % 4 == 0 && aligned16(g.c);
+    return v4 ? launch_on(stream, name, stream_reduce_kernel<true, Epi...>, blocks, block, g, epi...)
+              : launch_on(stream, name, stream_reduce_kernel<false, Epi...>, blocks, block, g, epi...);
+}
+
 // C (m x n, leading dimension ldc) = beta * C + op(A) op(B), or every element of the product to `epi`.
 // kRowMajor: A is m x k, B n x k; kColMajor: A is k x m, B k x n. `partial` has f32_partial_bytes.
 template <Operand AK, Operand BK, class... Epi>
@@ -83,15 +93,10 @@ int run_f32(hipStream_t stream, const char *name, const float *a, uint64_t lda, 
     const Tiling t = plan_f32(m, n, k);
     SplitArgs g;
     DKZ_TRY((run_f32_tiles<AK, BK, Epi...>(stream, name, a, lda, b, ldb, beta, c, ldc, m, n, k, partial, t, g, epi...)));
+    if (t.stream) return join_f32_stream(stream, name, t, g, epi...);
+    if (g.splits == 1) return 0;
     const bool v4 = n % 4 == 0 && ldc % 4 == 0 && aligned16(c);
     const dim3 block(kBlock);
-    if (t.stream) {
-        const uint32_t streamed = (uint32_t)((uint64_t)g.tiles_m * g.tiles_n * g.splits - t.full_tiles);
-        const dim3 blocks(streamed * (t.bm * t.bn / 4 / kBlock));
-        return v4 ? launch_on(stream, name, stream_reduce_kernel<true, Epi...>, blocks, block, g, epi...)
-                  : launch_on(stream, name, stream_reduce_kernel<false, Epi...>, blocks, block, g, epi...);
-    }
-    if (g.splits == 1) return 0;
     const bool many = g.splits > 32;
     const dim3 blocks(div_up(m * n / (v4 ? 4 : 1), many ? kBlock / 16 : kBlock));
     if (v4)

@@ -6,6 +6,7 @@ namespace dkz {
 namespace {
 
 constexpr int kMostEntries = 256;
+constexpr uint64_t kMostParts = 64;  // of a row: each one's group joins all their sums
 
 struct Teacher {
     const int *tokens;
@@ -14,7 +15,7 @@ struct Teacher {
     void *delta;  // null: not wanted
     float scale, temperature;
     uint32_t top;
-    // Of rows in several parts: their sums, and the logits of the entries' classes, which the delta may overwrite.
+    // Of rows in parts: their sums, and the logits of the entries' classes, which the delta may overwrite.
     Sums *part_sums;
     float *entry_logits;  // [rows][kMostEntries]
 };
@@ -211,25 +212,7 @@ __global__ __launch_bounds__(THREADS, U == 16 ? 4 : U == 8 ? 6 : 8) void distill
     }
 }
 
-// A group takes a row: its sums, the loss, and the delta in a second pass.
-template <class T>
-__global__ __launch_bounds__(kBlock) void distillation_kernel(Logits g, Teacher t) {
-    __shared__ Sums sums[kBlock / kWave];
-    __shared__ Entries in;
-    const Exp<T> ex(g.inv);
-    for (uint32_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
-        RowOf<T> r(g, t, in, row);
-        if (row != blockIdx.x) __syncthreads();  // the last row's use of `in`
-        if (threadIdx.x < kWave) r.read();
-        const Part<T> p(g, row, 0);
-        const Sums a = part_sums<T, kBlock>(r.logits, p, ex, sums);
-        const float l = log_sum(a);
-        if (threadIdx.x < kWave) r.loss(a, l);
-        if (t.delta != nullptr) r.template write_again<kBlock>(p, a, l, ex);
-    }
-}
-
-// Rows in several parts: the sums of each, then the loss and the delta.
+// Rows in parts: the sums of each, then the loss and the delta.
 template <class T>
 __global__ __launch_bounds__(kBlock) void distillation_sums_kernel(Logits g, Teacher t) {
     __shared__ Sums sums[kBlock / kWave];
@@ -260,16 +243,16 @@ __global__ __launch_bounds__(kBlock) void distillation_delta_kernel(Logits g, Te
     if (t.delta != nullptr) r.template write_again<kBlock>(Part<T>(g, row, part), a, l, ex);
 }
 
-// How rows are taken: held by groups of `threads` with `vectors` a thread, or (threads 0) as `rows` says.
+// How rows are taken: held by groups of `threads` with `vectors` a thread, or (threads 0) in parts.
 struct DistillPlan {
     uint32_t threads, vectors;
     RowPlan rows;
-    uint64_t bytes(uint64_t n) const {
-        return threads != 0 || rows.parts == 1 ? 0 : padded(n * rows.parts * sizeof(Sums)) + padded(n * kMostEntries * 4);
-    }
+    uint64_t bytes(uint64_t n) const { return threads != 0 ? 0 : padded(n * rows.parts * sizeof(Sums)) + padded(n * kMostEntries * 4); }
 };
 DistillPlan plan_distillation(int type, uint64_t rows, uint64_t classes) {
     const uint64_t vectors = classes / (type == DKZ_F32 ? 4 : 8);  // whole ones at most
+    // 4096 rows of 65536 bf16 classes 216 us with 512 threads and 16 vectors, 249 with 1024 and 8, 348 with 1024 and 16; of 32768
+    // classes 117 with 512 and 8, 124 with 256 and 16, 140 with 1024 and 4.
     constexpr uint32_t kHeld[][2] = {{64, 4}, {256, 4}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}};
     for (const auto &h : kHeld) {
         // Few long rows leave the chip empty: two launches of several groups a row (65536 classes in bf16: 1 row 11.0 us, 13.3
@@ -278,7 +261,7 @@ DistillPlan plan_distillation(int type, uint64_t rows, uint64_t classes) {
         if (rows <= 64 && h[0] * h[1] > 4096) break;
         if (vectors <= h[0] * h[1]) return {h[0], h[1], {0, 1, h[0] * h[1]}};
     }
-    return {0, 0, plan_joined_rows(type, rows, classes)};
+    return {0, 0, plan_rows(type, rows, classes, kMostParts * rows)};
 }
 
 template <class T>
@@ -291,7 +274,6 @@ int distill(hipStream_t stream, const Logits &g, const DistillPlan &plan, const 
     if (plan.threads == 512 && plan.vectors == 8) return launch_on(stream, kName, distillation_held_kernel<T, 512, 8>, grid, block, g, t);
     if (plan.threads == 512) return launch_on(stream, kName, distillation_held_kernel<T, 512, 16>, grid, block, g, t);
     if (plan.threads == 1024) return launch_on(stream, kName, distillation_held_kernel<T, 1024, 16>, grid, block, g, t);
-    if (plan.rows.parts == 1) return launch_on(stream, kName, distillation_kernel<T>, grid, dim3(kBlock), g, t);
     DKZ_TRY(launch_on(stream, "distillation_sums", distillation_sums_kernel<T>, dim3(g.rows * g.parts), dim3(kBlock), g, t));
     return launch_on(stream, kName, distillation_delta_kernel<T>, dim3(t.delta != nullptr ? g.rows * g.parts : g.rows), dim3(kBlock), g, t);
 }

@@ -209,28 +209,48 @@ __global__ __launch_bounds__(kBlock) void gate_kernel(const float *sums, float *
     }
 }
 
-// fp32, where K is cut: the join of both projections' pieces (in f64) and the output at once, a thread W units of a row.
-template <int W, bool EXP>
+// fp32, where K is cut: the join of both projections' pieces (in f64) and the output at once, a thread W units of a row or
+// GROUPS threads, each taking every GROUPSth piece, for many pieces.
+template <int W, int GROUPS, bool EXP>
 __global__ __launch_bounds__(kBlock) void gate_join_kernel(const float *partial, uint32_t splits, uint32_t rows, uint32_t half, uint32_t units,
                                                           const float *biases, float *sums, float *output, Gate gate) {
-    constexpr uint32_t kAhead = 8 / W;
-    const uint32_t i = blockIdx.x * kBlock + threadIdx.x, r = i / units, j = (i - r * units) * W;
-    if (r >= rows) return;
+    constexpr uint32_t kAhead = 8 / W, kItems = kBlock / GROUPS;
+    const uint32_t i = blockIdx.x * kItems + threadIdx.x % kItems, group = threadIdx.x / kItems, r = i / units, j = (i - r * units) * W;
+    const bool in = r < rows;
     const uint64_t at = (uint64_t)r * 2 * half + j, size = (uint64_t)rows * 2 * half;
     double s[2][W] = {};
-    for (uint32_t p = 0; p < splits; p += kAhead) {
+    for (uint32_t p = group; in && p < splits; p += kAhead * GROUPS) {
         Raw<float, W> x[kAhead][2];  // past the last piece: that one again, not added
 #pragma unroll
         for (uint32_t u = 0; u < kAhead; ++u)
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) x[u][h] = *reinterpret_cast<const Raw<float, W> *>(partial + min(p + u, splits - 1) * size + at + h * half);
+            for (uint32_t h = 0; h < 2; ++h)
+                x[u][h] = *reinterpret_cast<const Raw<float, W> *>(partial + min(p + u * GROUPS, splits - 1) * size + at + h * half);
 #pragma unroll
         for (uint32_t u = 0; u < kAhead; ++u)
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
-                for (int w = 0; w < W; ++w) s[h][w] += p + u < splits ? (double)x[u][h][w] : 0.0;
+                for (int w = 0; w < W; ++w) s[h][w] += p + u * GROUPS < splits ? (double)x[u][h][w] : 0.0;
     }
+    if constexpr (GROUPS > 1) {
+        __shared__ double pieces[2][W][kBlock];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            pieces[0][w][threadIdx.x] = s[0][w];
+            pieces[1][w][threadIdx.x] = s[1][w];
+        }
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (uint32_t u = 1; u < GROUPS; ++u)
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                s[0][w] += pieces[0][w][threadIdx.x + u * kItems];
+                s[1][w] += pieces[1][w][threadIdx.x + u * kItems];
+            }
+    }
+    if (!in) return;
     Raw<float, W> x, y, out;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -258,26 +278,25 @@ uint64_t forward_bytes(int type, uint64_t rows, uint64_t inputs, uint64_t hidden
     return packed + most_partial_bytes(rows, paired_columns(hidden), inputs, true);
 }
 
-// Pieces that a thread of gate_join_kernel adds up; the products of more have a join with sixteen threads an element.
-constexpr uint32_t kJoinPieces = 32;
-
 template <bool EXP>
 int forward_f32(hipStream_t stream, uint64_t rows, uint64_t inputs, uint64_t hidden, const Gate &gate, const float *input, const float *weights,
                 const float *biases, float *sums, float *output, Workspace ws) {
-    constexpr const char *kName = "gated_forward";
+    constexpr const char *kName = "gated_forward", *kProduct = "gated_forward_product";
     float *own = ws.take<float>(rows * 2 * hidden), *partial = ws.take<float>(f32_partial_bytes(rows, 2 * hidden, inputs) / 4);
+    const uint32_t m = (uint32_t)rows, half = (uint32_t)hidden;
     const Tiling t = plan_f32(rows, 2 * hidden, inputs);
-    if (t.splits > 1 && t.splits <= kJoinPieces) {
-        SplitArgs g;
-        DKZ_TRY((run_f32_tiles<kRowMajor, kRowMajor>(stream, kName, input, inputs, weights, inputs, 0.0f, (float *)nullptr, 2 * hidden, rows, 2 * hidden,
+    SplitArgs g;
+    if (t.splits > 1) {
+        DKZ_TRY((run_f32_tiles<kRowMajor, kRowMajor>(stream, kProduct, input, inputs, weights, inputs, 0.0f, (float *)nullptr, 2 * hidden, rows, 2 * hidden,
                                                      inputs, partial, t, g)));
-        const bool fours = hidden % 4 == 0 && aligned16(output) && (sums == nullptr || aligned16(sums));
-        const uint32_t units = (uint32_t)(fours ? hidden / 4 : hidden);
-        const dim3 grid(div_up(rows * units, kBlock));
-        return fours ? launch_on(stream, kName, gate_join_kernel<4, EXP>, grid, dim3(kBlock), partial, t.splits, (uint32_t)rows, (uint32_t)hidden, units,
-                                 biases, sums, output, gate)
-                     : launch_on(stream, kName, gate_join_kernel<1, EXP>, grid, dim3(kBlock), partial, t.splits, (uint32_t)rows, (uint32_t)hidden, units,
-                                 biases, sums, output, gate);
+        const auto join = [&](auto kernel, uint32_t width, uint32_t groups) {
+            const uint32_t units = half / width;
+            return launch_on(stream, kName, kernel, dim3(div_up((uint64_t)m * units, kBlock / groups)), dim3(kBlock), partial, t.splits, m, half, units,
+                             biases, sums, output, gate);
+        };
+        if (t.splits > 32) return join(gate_join_kernel<1, 16, EXP>, 1, 16);
+        const bool fours = hidden % 4 == 0 && aligned16(output) && aligned16(sums);
+        return fours ? join(gate_join_kernel<4, 1, EXP>, 4, 1) : join(gate_join_kernel<1, 1, EXP>, 1, 1);
     }
     if (sums == nullptr) sums = own;
     LinearEpilogue<float, false> e;
@@ -285,15 +304,16 @@ int forward_f32(hipStream_t stream, uint64_t rows, uint64_t inputs, uint64_t hid
     e.residual = nullptr;
     e.activated = nullptr;
     e.output = sums;
-    e.ld = (uint32_t)(2 * hidden);
+    e.ld = 2 * half;
     e.act = kLinear;
     e.words = true;
     e.draws = make_draws(0.0f, 1.0f, 0, 0);
-    DKZ_TRY((run_f32<kRowMajor, kRowMajor>(stream, "gated_forward_product", input, inputs, weights, inputs, 0.0f, (float *)nullptr, 2 * hidden, rows,
-                                           2 * hidden, inputs, partial, e)));
+    DKZ_TRY((run_f32_tiles<kRowMajor, kRowMajor>(stream, kProduct, input, inputs, weights, inputs, 0.0f, (float *)nullptr, 2 * hidden, rows, 2 * hidden,
+                                                 inputs, partial, t, g, e)));
+    if (t.stream) DKZ_TRY(join_f32_stream(stream, kProduct, t, g, e));
     const uint64_t fours = (hidden + 3) / 4;
     const dim3 grid((uint32_t)std::min<uint64_t>((rows * fours + kBlock - 1) / kBlock, 1u << 16));
-    return launch_on(stream, kName, gate_kernel<EXP>, grid, dim3(kBlock), sums, output, (uint32_t)rows, (uint32_t)hidden, (uint32_t)fours, gate);
+    return launch_on(stream, kName, gate_kernel<EXP>, grid, dim3(kBlock), sums, output, m, half, (uint32_t)fours, gate);
 }
 
 template <bool EXP>

@@ -17,6 +17,7 @@ FORWARD = [
     128, 2832, 1552, SILU, 1), (BF16, 224, 2840, 24, SILU, 0), (BF16, 460, 205, 8616, RELU, 1), (BF16, 872, 952, 3632, RELU, 0), (BF16,
     1064, 265, 5784, SILU, 0), (BF16, 1334, 112, 10000, RELU, 0), (BF16, 1741, 264, 936, SILU, 0), (BF16, 1830, 69, 16, RELU, 0), (BF16,
     1830, 128, 7308, SILU, 1), (BF16, 3720, 5690, 30, RELU, 0), (BF16, 4267, 242, 2679, SILU, 0), (BF16, 4608, 96, 695, RELU, 1),
+    (F32, 48, 2768, 9464, SILU, 0), (F32, 88, 238, 3, SILU, 0), (F32, 3848, 13, 670, SILU, 0),
 ]
 
 BACKWARD = [
@@ -27,7 +28,9 @@ BACKWARD = [
     20, RELU, 0), (BF16, 1, 80, 2472, RELU, 0), (BF16, 8, 2367, 3049, RELU, 0), (BF16, 17, 248, 53, SILU, 1), (BF16, 17, 4064, 892,
     RELU, 1), (BF16, 59, 361, 240, SILU, 0), (BF16, 460, 205, 8616, RELU, 1), (BF16, 872, 952, 3632, RELU, 0), (BF16, 1741, 264, 936,
     SILU, 0), (BF16, 1886, 3304, 5, SILU, 1), (BF16, 4267, 242, 2679, SILU, 0), (BF16, 5832, 2652, 77, SILU, 1),
+    (F32, 5, 9, 36272, SILU, 1), (F32, 7, 8, 38488, RELU, 0), (BF16, 7, 16, 39224, SILU, 1), (BF16, 100, 16, 33800, RELU, 0),
+    (BF16, 857, 46, 5, RELU, 0), (BF16, 2863, 2712, 584, SILU, 0),
 ]
 
-# Rows and classes of logits: a wave a row, a workgroup, several.
-ROWS = [(5, 40), (600, 9001), (2, 65536)]
+# Rows and classes of logits: a wave a row, a workgroup, several; held in registers by groups of several sizes, read twice.
+ROWS = [(5, 40), (70, 4000), (66, 8001), (600, 9001), (65, 16001), (70, 32000), (66, 65003), (65, 131000), (65, 140001), (2, 65536), (3, 140001)]

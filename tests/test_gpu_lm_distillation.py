@@ -8,6 +8,7 @@ import pytest
 from darknet_zig_amd import gpu
 
 from . import dense_ref as ref
+from . import lm_cases as cases
 from . import lm_ref as lm
 from .dense_ref import BF16, F32, Pool, assert_within, buf
 from .test_gpu_lm_log_probs import make
@@ -111,7 +112,14 @@ def test_shapes_and_alignments(pool, kind, rows, classes, gap, top, shift):
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
-@pytest.mark.parametrize("rows,classes", [(4, 900), (3, 20000), (600, 4000)])
+@pytest.mark.parametrize("rows,classes", cases.ROWS)
+def test_every_kernel(pool, kind, rows, classes):
+    t, l = teacher(rows, 130, classes)
+    check(pool, kind, make(kind, rows, classes, classes + 1), classes, 1.0, t, l, scale=0.5)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("rows,classes", [(4, 900), (3, 20000), (600, 4000), (3, 70000)])
 @pytest.mark.parametrize("temperature", [0.5, 3.0])
 def test_onto_the_logits_and_without_a_delta(pool, kind, rows, classes, temperature):
     z = make(kind, rows, classes, classes + 5)

@@ -8,6 +8,7 @@ import pytest
 from darknet_zig_amd import gpu
 
 from . import dense_ref as ref
+from . import lm_cases as cases
 from . import lm_ref as lm
 from .dense_ref import BF16, F32, Pool, assert_within, buf
 
@@ -91,6 +92,15 @@ SHAPES = [(1, 1, 0, 1), (3, 2, 0, 2), (5, 7, 1, 5), (4, 63, 0, 64), (7, 64, 0, 3
 def test_shapes_and_alignments(pool, kind, rows, classes, gap, top, shift):
     z = make(kind, rows, classes, classes + gap)
     check(pool, kind, z, classes, 1.0, tokens_of(rows, 3, classes), top, True, shift)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("rows,classes", cases.ROWS)
+@pytest.mark.parametrize("entropy", [False, True])
+def test_every_kernel(pool, kind, rows, classes, entropy):
+    z = make(kind, rows, classes, classes + 1)
+    check(pool, kind, z, classes, 1.0, tokens_of(rows, 2, classes), 5 if entropy else 0, entropy)
+    run_backward(pool, kind, z, classes, 1.0, tokens_of(rows, 2, classes), entropy, beta=0.5)
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
