@@ -343,9 +343,14 @@ inline RowPlan plan_rows(int type, uint64_t rows, uint64_t classes, uint64_t fil
     const uint64_t want = std::min<uint64_t>(tiles, rows == 0 || fill == 0 ? 1 : fill / rows + (fill % rows != 0)), each = (tiles + want - 1) / want;
     return {kBlock, (uint32_t)((tiles + each - 1) / each), (uint32_t)(each * tile)};
 }
-// Where the parts' results are joined by another launch: one part from 256 rows on (50001 classes in bf16, top 5: 200 rows 19.1 us
-// in parts and 20.1, 300 rows 23.5 and 21.7, 500 rows 27.2 and 22.6).
-inline RowPlan plan_joined_rows(int type, uint64_t rows, uint64_t classes) { return plan_rows(type, rows, classes, rows < 256 ? 512 : 0); }
+// Where the parts' results are joined by another launch, which takes as long as three tiles: parts where they save more. (fp32, top
+// 20, us in parts and in one: 1 row of 2 tiles 11.7 and 8.8, of 4 11.9 and 12.2, of 5 12.3 and 13.6; 200 rows of 5 20.0 and 17.2.
+// bf16, top 5, 7 tiles: 200 rows 19.1 and 20.1, 300 rows 23.5 and 21.7.)
+inline RowPlan plan_joined_rows(int type, uint64_t rows, uint64_t classes) {
+    constexpr uint64_t kFill = 512, kJoinTiles = 3;
+    const uint64_t tile = kTileVectors * kBlock * (type == DKZ_F32 ? 4 : 8), tiles = (classes + tile - 1) / tile;
+    return plan_rows(type, rows, classes, kJoinTiles + (tiles * rows + kFill - 1) / kFill < tiles ? kFill : 0);
+}
 
 inline Logits make_logits(const RowPlan &plan, const void *p, int rows, int classes, int pitch, float temperature) {
     return {p, (uint64_t)pitch, (uint32_t)rows, (uint32_t)classes, plan.parts, plan.per, 1.0f / temperature};
