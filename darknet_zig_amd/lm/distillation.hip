@@ -166,7 +166,7 @@ __device__ __forceinline__ Sums part_sums(const T *logits, const Part<T> &p, con
         u32x4v raw[kEach];
         p.load(v0 + threadIdx.x, THREADS, raw);
         float largest[kEach];
-        add<T, false>(a, raw, largest, ex);
+        add_until<T, false>(a, raw, largest, v0 + threadIdx.x, THREADS, p.v1, ex);
     }
     const uint32_t edge = p.edge();
     add_one(a, edge != ~0u ? load1(logits, edge) : neg_inf(), ex);

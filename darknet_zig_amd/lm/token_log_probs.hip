@@ -93,7 +93,7 @@ __global__ __launch_bounds__(THREADS) void log_probs_kernel(Logits g, Answers ou
             u32x4v raw[kEach];
             float largest[kEach];
             p.load(v0, THREADS, raw);
-            add<T, ENTROPY>(a, raw, largest, ex);
+            add_until<T, ENTROPY>(a, raw, largest, v0, THREADS, p.v1, ex);
             if constexpr (TOP) {
                 if (v0 - threadIdx.x == p.v0) top.begin(a.m);
                 top.tile(raw, largest, [&](int u) { return p.class_of(v0 + u * THREADS); });
