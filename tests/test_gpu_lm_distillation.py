@@ -167,6 +167,18 @@ def test_specials_stay_in_their_rows(pool, kind, classes):
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("classes", [500, 20000, 70000])
+def test_logits_far_from_zero(pool, kind, classes):
+    """Rows whose logits are all large: only their distances matter."""
+    r = np.random.default_rng(2)
+    far = [0.0, 300.0, -300.0, 1e5, -1e5, 1e8, -1e8, 1e11, -1e11, 1e20, 1e30, -1e30]
+    z = np.stack([ref.rounded(f + np.maximum(3, abs(f) * 2.0**-7) * r.integers(-2, 3, classes), kind) for f in far])
+    tokens, logits = teacher(len(far), 5, classes)
+    for temperature in (1.0, 0.7):
+        check(pool, kind, z, classes, temperature, tokens, logits)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
 def test_no_classes_and_no_rows(pool, kind):
     t, l = np.zeros((3, 2), np.int32), np.zeros((3, 2), np.float32)
     dt, dl, loss = pool(t), pool(l), pool(n=3)

@@ -174,6 +174,18 @@ def test_extreme_temperatures(pool, kind):
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("entropy", [False, True])
+@pytest.mark.parametrize("classes", [500, 20000])
+def test_logits_far_from_zero(pool, kind, entropy, classes):
+    """Rows whose logits are all large: only their distances matter."""
+    r = np.random.default_rng(2)
+    far = [0.0, 300.0, -300.0, 1e5, -1e5, 1e8, -1e8, 1e11, -1e11, 1e20, 1e30, -1e30, 1e37, -1e37]
+    z = np.stack([ref.rounded(f + np.maximum(3, abs(f) * 2.0**-7) * r.integers(-2, 3, classes), kind) for f in far])
+    for temperature in (1.0, 0.7):
+        check(pool, kind, z, classes, temperature, tokens_of(len(far), 2, classes), 3, entropy)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
 def test_no_rows_and_no_classes(pool, kind):
     check(pool, kind, np.zeros((4, 0), np.float32), 0, 1.0, np.zeros((4, 2), np.int32), 3)
     gpu.tokenLogProbs(kind, 0, 10, 10, gpu.Buf(), 1.0, 1, None, 1, None, None, gpu.Buf(), None, None, None)
