@@ -31,6 +31,10 @@ constexpr TileKind kTileKinds[] = {{256, 256, 4, 2, 1, {1.62f}, 4.0f},
                                    {64, 64, 2, 2, 3, {0.24f, 0.37f, 0.55f}, 1.0f}};
 constexpr float kLaunchUs = 3.0f, kPartialBytesUs = 4e6f;  // a launch, and bytes of partials a us
 constexpr uint32_t kComputeUnits = 256;
+// What cutting K adds: the partials' way out and back and the launch that joins them.
+inline float join_us(uint64_t splits, uint64_t rows, uint64_t cols) {
+    return kLaunchUs + 2 * 4.0f / kPartialBytesUs * (float)(splits * rows * cols);
+}
 
 // How a product is cut: tiles of br x bc, each by wr x wc waves; K in `splits`
 // ranges of k_chunk. br 0: the kernel for few rows, bc its columns a workgroup.
@@ -73,7 +77,7 @@ inline ProductPlan plan_product(uint64_t rows, uint64_t cols, uint64_t k, bool n
             const uint64_t rounds = groups / slots, rest = groups % slots;
             float us = (float)rounds * ((float)chunk * t.slab[t.occupancy - 1] + t.fixed);
             if (rest) us += (float)chunk * t.slab[(rest - 1) / kComputeUnits] + t.fixed;
-            if (splits > 1) us += kLaunchUs + 2 * 4.0f / kPartialBytesUs * (float)(splits * rows * cols);
+            if (splits > 1) us += join_us(splits, rows, cols);
             if (us < least) {
                 least = us;
                 best = {t.br, t.bc, t.wr, t.wc, (uint32_t)splits, (uint32_t)(chunk * 64), direct, us};
@@ -178,6 +182,15 @@ inline ProductArgs product_args(const Product &x, const ProductPlan &p, float *p
 // workgroups of 256. A product of more takes several launches. (A multiple of the XCDs, so that xcd_run goes on as it was.)
 constexpr uint64_t kMostGroups = 1ull << 22;
 
+// Where K was cut.
+template <class Epi>
+int join_product(hipStream_t stream, const char *name, const ProductArgs &g, const Epi &epi) {
+    const uint64_t eights = (uint64_t)g.rows * (g.ldp / 8);
+    if (g.splits > 4) return launch_on(stream, name, join_kernel<8, Epi>, dim3(div_up(eights, kBlock / 8)), dim3(kBlock), g, epi);
+    if (g.splits > 1) return launch_on(stream, name, join_kernel<1, Epi>, dim3(div_up(eights, kBlock)), dim3(kBlock), g, epi);
+    return 0;
+}
+
 // `partial` has the plan's partial_bytes.
 template <bool VMC, bool UMC, class Epi>
 int run_product(hipStream_t stream, const char *name, const Product &x, const ProductPlan &p, float *partial, const Epi &epi) {
@@ -204,11 +217,7 @@ int run_product(hipStream_t stream, const char *name, const Product &x, const Pr
             DKZ_TRY(launch_on(stream, name, product_kernel<Tile64, VMC, UMC, true, Epi>, grid, four, g, epi));
         }
     }
-    if constexpr (Epi::kElementwise) {
-        const uint64_t eights = (uint64_t)g.rows * (g.ldp / 8);
-        if (g.splits > 4) return launch_on(stream, name, join_kernel<8, Epi>, dim3(div_up(eights, kBlock / 8)), dim3(kBlock), g, epi);
-        if (g.splits > 1) return launch_on(stream, name, join_kernel<1, Epi>, dim3(div_up(eights, kBlock)), dim3(kBlock), g, epi);
-    }
+    if constexpr (Epi::kElementwise) return join_product(stream, name, g, epi);
     return 0;
 }
 
@@ -221,50 +230,58 @@ int run_product(hipStream_t stream, const char *name, const Product &x, const Pr
 // 1 us slower paired) nor kinds of which a compute unit holds one (nothing runs
 // beside them). A whole backward pass, apart and paired: 64x1024x1024 17.3 and 11.5
 // us, 128x4096x1000 18.8 and 13.9, 768x768x3000 31.4 and 25.6, 1536^3 37.2 and 32.4.
-inline bool plan_pair(const Product &a, const Product &b, ProductPlan &pa, ProductPlan &pb) {
+// may_cut: the input gradient's K may be cut here too, as it is alone where the rows are few.
+inline bool plan_pair(const Product &a, const Product &b, ProductPlan &pa, ProductPlan &pb, bool may_cut = false) {
     float least = pa.us + pb.us + kLaunchUs;
     bool found = false;
-    if (pa.splits != 1 || pb.splits != 1 || !a.direct() || !b.direct() || a.rows == 0 || a.cols == 0 || b.rows == 0 || b.cols == 0) return false;
+    if ((pa.splits != 1 && !may_cut) || pb.splits != 1 || !a.direct() || !b.direct() || a.rows == 0 || a.cols == 0 || b.rows == 0 || b.cols == 0) return false;
+    const uint32_t most = may_cut ? pa.splits : 1;
     for (const TileKind &t : kTileKinds) {
         if (t.occupancy == 1) continue;
-        const uint64_t slabs_a = (a.k + 63) / 64, slabs_b = (b.k + 63) / 64;
-        const uint64_t tiles_a = (uint64_t)div_up(a.rows, t.br) * div_up(a.cols, t.bc), tiles_b = (uint64_t)div_up(b.rows, t.br) * div_up(b.cols, t.bc);
-        const uint64_t each = std::min<uint64_t>((tiles_a + tiles_b + kComputeUnits - 1) / kComputeUnits, t.occupancy);
-        const float us_a = (float)slabs_a * t.slab[each - 1] + t.fixed, us_b = (float)slabs_b * t.slab[each - 1] + t.fixed;
-        const float all = ((float)tiles_a * us_a + (float)tiles_b * us_b) / (float)(kComputeUnits * each);
-        // A product's tile takes as long as beside the others of its kind.
-        const auto alone = [&](uint64_t slabs, uint64_t tiles) {
-            return (float)slabs * t.slab[std::min<uint64_t>((tiles + kComputeUnits - 1) / kComputeUnits, t.occupancy) - 1] + t.fixed;
-        };
-        const float us = std::max(std::max(alone(slabs_a, tiles_a), alone(slabs_b, tiles_b)), all + 0.5f * std::min(us_a, us_b));
-        if (us >= least || tiles_a + tiles_b > 0x7fffffffull) continue;
-        least = us;
-        pa = {t.br, t.bc, t.wr, t.wc, 1, (uint32_t)(slabs_a * 64), true, us};
-        pb = {t.br, t.bc, t.wr, t.wc, 1, (uint32_t)(slabs_b * 64), true, us};
-        found = true;
+        for (uint32_t want = 1; want <= most; ++want) {
+            const uint64_t slabs_k = (a.k + 63) / 64, slabs_a = (slabs_k + want - 1) / want, slabs_b = (b.k + 63) / 64;
+            const uint64_t splits = slabs_a != 0 ? (slabs_k + slabs_a - 1) / slabs_a : 1;
+            const uint64_t tiles_a = splits * div_up(a.rows, t.br) * div_up(a.cols, t.bc), tiles_b = (uint64_t)div_up(b.rows, t.br) * div_up(b.cols, t.bc);
+            const uint64_t each = std::min<uint64_t>((tiles_a + tiles_b + kComputeUnits - 1) / kComputeUnits, t.occupancy);
+            const float us_a = (float)slabs_a * t.slab[each - 1] + t.fixed, us_b = (float)slabs_b * t.slab[each - 1] + t.fixed;
+            const float all = ((float)tiles_a * us_a + (float)tiles_b * us_b) / (float)(kComputeUnits * each);
+            // A product's tile takes as long as beside the others of its kind.
+            const auto alone = [&](uint64_t slabs, uint64_t tiles) {
+                return (float)slabs * t.slab[std::min<uint64_t>((tiles + kComputeUnits - 1) / kComputeUnits, t.occupancy) - 1] + t.fixed;
+            };
+            float us = std::max(std::max(alone(slabs_a, tiles_a), alone(slabs_b, tiles_b)), all + 0.5f * std::min(us_a, us_b));
+            if (splits > 1) us += join_us(splits, a.rows, a.cols);
+            if (us >= least || tiles_a + tiles_b > 0x7fffffffull) continue;
+            least = us;
+            pa = {t.br, t.bc, t.wr, t.wc, (uint32_t)splits, (uint32_t)(slabs_a * 64), true, us};
+            pb = {t.br, t.bc, t.wr, t.wc, 1, (uint32_t)(slabs_b * 64), true, us};
+            found = true;
+        }
     }
     return found;
 }
 
 template <class T, class Epi>
 int launch_pair(hipStream_t stream, const char *name, const ProductArgs &a, const Epi &epi_a, const ProductArgs &b, const Epi &epi_b) {
-    const uint32_t tiles_a = a.tiles_r * a.tiles_c, tiles_b = b.tiles_r * b.tiles_c;
-    return launch_on(stream, name, product_pair_kernel<T, Epi>, dim3(tiles_a + tiles_b), dim3(T::kThreads), a, epi_a, b, epi_b, tiles_a, a.k >= b.k);
+    const uint32_t tiles_a = a.tiles_r * a.tiles_c * a.splits, tiles_b = b.tiles_r * b.tiles_c;
+    DKZ_TRY(launch_on(stream, name, product_pair_kernel<T, Epi>, dim3(tiles_a + tiles_b), dim3(T::kThreads), a, epi_a, b, epi_b, tiles_a,
+                      std::min(a.k, a.k_chunk) >= b.k));
+    return join_product(stream, name, a, epi_a);
 }
 
 // The products of a backward pass, each null if it is not wanted.
 template <class Epi>
 int run_gradients(hipStream_t stream, const char *name_a, const Product *to_input, const Epi &epi_a, const char *name_b,
-                  const Product *to_weights, const Epi &epi_b, float *partial) {
+                  const Product *to_weights, const Epi &epi_b, float *partial, bool may_cut = false) {
     ProductPlan pa{}, pb{};
     if (to_input != nullptr) pa = plan_product(to_input->rows, to_input->cols, to_input->k, false, true, to_input->direct());
     if (to_weights != nullptr) pb = plan_product(to_weights->rows, to_weights->cols, to_weights->k, false, true, to_weights->direct());
-    if (to_input == nullptr || to_weights == nullptr || !plan_pair(*to_input, *to_weights, pa, pb)) {
+    if (to_input == nullptr || to_weights == nullptr || !plan_pair(*to_input, *to_weights, pa, pb, may_cut)) {
         if (to_weights != nullptr) DKZ_TRY((run_product<true, true>(stream, name_b, *to_weights, pb, partial, epi_b)));
         return to_input == nullptr ? 0 : run_product<false, true>(stream, name_a, *to_input, pa, partial, epi_a);
     }
     const Product &a = *to_input, &b = *to_weights;
-    const ProductArgs ga = product_args(a, pa, nullptr), gb = product_args(b, pb, nullptr);
+    const ProductArgs ga = product_args(a, pa, partial), gb = product_args(b, pb, nullptr);
     if (pa.bc == 128) return launch_pair<Tile64x128>(stream, name_a, ga, epi_a, gb, epi_b);
     return launch_pair<Tile64>(stream, name_a, ga, epi_a, gb, epi_b);
 }

@@ -513,7 +513,7 @@ int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint6
     } else {
         const Product to_input{d, ldd, w.p, w.ld, rows, inputs, n}, to_weights{d, ldd, x.p, x.ld, n, inputs, rows};
         DKZ_TRY(run_gradients(stream, kInput, input_delta != nullptr ? &to_input : nullptr, store_epilogue<T>(input_delta, input_residual, inputs, 0.0f),
-                              kWeights, weight_updates != nullptr ? &to_weights : nullptr, store_epilogue<T>(weight_updates, nullptr, inputs, beta), partial));
+                              kWeights, weight_updates != nullptr ? &to_weights : nullptr, store_epilogue<T>(weight_updates, nullptr, inputs, beta), partial, true));
     }
     return 0;
 }

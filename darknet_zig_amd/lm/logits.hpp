@@ -171,7 +171,7 @@ __device__ __forceinline__ void repacked(u32x4v &raw) { asm volatile("" : "+v"(r
 // end: as if it were not. Its products with e are summed as they are, although 0 * -infinity is NaN where a class is masked: then,
 // and where m * c is so large that r is no small number, the thread goes through its logits again, each in steps that cannot go
 // wrong. (bf16: about 8.5 instead of 12.6 issue slots a logit; 2000 rows of 50001 56.7 -> 50.8 us. fp32, in place of an exponential of under one ulp
-// with its own reduction: 1 row of 50001 13.0 -> 11.1 us, 2048 of 65536 105.8 -> 97.1.)
+// with its own reduction: 1 row of 65536 13.0 -> 11.1 us, 2048 of 65536 105.8 -> 97.1.)
 template <class T, bool MOMENT, int U, bool REPACK>
 __device__ __forceinline__ Sums sums_from(u32x4v (&raw)[U], float m, const Exp<T> &ex) {
     const float base = m == neg_inf() ? 0.0f : m;
