@@ -159,28 +159,32 @@ StoreEpilogue<T> store_epilogue(void *out, const void *add, uint64_t ld, float b
 
 // updates[c] = beta * updates[c] + the sum of column c of partial[chunks][cols],
 // in f64: a thread takes every eighth chunk of a column, and a column's eight
-// sums are added in order.
-__global__ __launch_bounds__(kBlock) void column_sums_kernel(const float *partial, uint32_t chunks, uint32_t cols, float beta,
-                                                            float *updates) {
-    constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes;
-    __shared__ double sums[kGroups][kLanes];
-    const uint32_t x = threadIdx.x % kLanes, group = threadIdx.x / kLanes, c = blockIdx.x * kLanes + x;
+// sums are added in order. `sums` is the workgroup's.
+constexpr uint32_t kSumLanes = 32, kSumGroups = kBlock / kSumLanes;
+__device__ __forceinline__ void column_sums(const float *partial, uint32_t chunks, uint32_t cols, float beta, float *updates, uint32_t block,
+                                            double (&sums)[kSumGroups][kSumLanes]) {
+    const uint32_t x = threadIdx.x % kSumLanes, group = threadIdx.x / kSumLanes, c = block * kSumLanes + x;
     double s = 0.0;
     if (c < cols) {
 #pragma unroll 4
-        for (uint32_t i = group; i < chunks; i += kGroups) s += (double)partial[(uint64_t)i * cols + c];
+        for (uint32_t i = group; i < chunks; i += kSumGroups) s += (double)partial[(uint64_t)i * cols + c];
     }
     sums[group][x] = s;
     __syncthreads();
     if (group != 0 || c >= cols) return;
 #pragma unroll
-    for (uint32_t i = 1; i < kGroups; ++i) s += sums[i][x];
+    for (uint32_t i = 1; i < kSumGroups; ++i) s += sums[i][x];
     updates[c] = beta == 0.0f ? (float)s : beta * updates[c] + (float)s;
+}
+__global__ __launch_bounds__(kBlock) void column_sums_kernel(const float *partial, uint32_t chunks, uint32_t cols, float beta,
+                                                            float *updates) {
+    __shared__ double sums[kSumGroups][kSumLanes];
+    column_sums(partial, chunks, cols, beta, updates, blockIdx.x, sums);
 }
 
 inline int add_column_sums(hipStream_t stream, const float *partial, uint64_t chunks, uint64_t cols, float beta, float *updates) {
     if (cols == 0) return 0;
-    return launch_on(stream, "bias_updates", column_sums_kernel, dim3(div_up(cols, 32)), dim3(kBlock), partial, (uint32_t)chunks,
+    return launch_on(stream, "bias_updates", column_sums_kernel, dim3(div_up(cols, kSumLanes)), dim3(kBlock), partial, (uint32_t)chunks,
                      (uint32_t)cols, beta, updates);
 }
 

@@ -261,18 +261,25 @@ inline bool plan_pair(const Product &a, const Product &b, ProductPlan &pa, Produ
     return found;
 }
 
-template <class T, class Epi>
-int launch_pair(hipStream_t stream, const char *name, const ProductArgs &a, const Epi &epi_a, const ProductArgs &b, const Epi &epi_b) {
-    const uint32_t tiles_a = a.tiles_r * a.tiles_c * a.splits, tiles_b = b.tiles_r * b.tiles_c;
-    DKZ_TRY(launch_on(stream, name, product_pair_kernel<T, Epi>, dim3(tiles_a + tiles_b), dim3(T::kThreads), a, epi_a, b, epi_b, tiles_a,
-                      std::min(a.k, a.k_chunk) >= b.k));
+// A launch of the two in groups_a + groups_b workgroups.
+struct PairLaunch {
+    template <class T, class Epi>
+    int run(hipStream_t stream, const char *name, const ProductArgs &a, const Epi &epi_a, const ProductArgs &b, const Epi &epi_b, uint32_t groups_a,
+            uint32_t groups_b, bool a_first) const {
+        return launch_on(stream, name, product_pair_kernel<T, Epi>, dim3(groups_a + groups_b), dim3(T::kThreads), a, epi_a, b, epi_b, groups_a, a_first);
+    }
+};
+template <class T, class Epi, class Pair>
+int launch_pair(hipStream_t stream, const char *name, const ProductArgs &a, const Epi &epi_a, const ProductArgs &b, const Epi &epi_b, Pair &pair) {
+    DKZ_TRY(pair.template run<T>(stream, name, a, epi_a, b, epi_b, a.tiles_r * a.tiles_c * a.splits, b.tiles_r * b.tiles_c,
+                                 std::min(a.k, a.k_chunk) >= b.k));
     return join_product(stream, name, a, epi_a);
 }
 
-// The products of a backward pass, each null if it is not wanted.
-template <class Epi>
+// The products of a backward pass, each null if it is not wanted; `pair` launches them where they are paired.
+template <class Epi, class Pair = PairLaunch>
 int run_gradients(hipStream_t stream, const char *name_a, const Product *to_input, const Epi &epi_a, const char *name_b,
-                  const Product *to_weights, const Epi &epi_b, float *partial, bool may_cut = false) {
+                  const Product *to_weights, const Epi &epi_b, float *partial, bool may_cut = false, Pair &&pair = {}) {
     ProductPlan pa{}, pb{};
     if (to_input != nullptr) pa = plan_product(to_input->rows, to_input->cols, to_input->k, false, true, to_input->direct());
     if (to_weights != nullptr) pb = plan_product(to_weights->rows, to_weights->cols, to_weights->k, false, true, to_weights->direct());
@@ -282,8 +289,8 @@ int run_gradients(hipStream_t stream, const char *name_a, const Product *to_inpu
     }
     const Product &a = *to_input, &b = *to_weights;
     const ProductArgs ga = product_args(a, pa, partial), gb = product_args(b, pb, nullptr);
-    if (pa.bc == 128) return launch_pair<Tile64x128>(stream, name_a, ga, epi_a, gb, epi_b);
-    return launch_pair<Tile64>(stream, name_a, ga, epi_a, gb, epi_b);
+    if (pa.bc == 128) return launch_pair<Tile64x128>(stream, name_a, ga, epi_a, gb, epi_b, pair);
+    return launch_pair<Tile64>(stream, name_a, ga, epi_a, gb, epi_b, pair);
 }
 
 }  // namespace

@@ -338,7 +338,8 @@ int forward_bf16(hipStream_t stream, uint64_t rows, uint64_t inputs, uint64_t hi
 
 // ---- backward ----
 
-constexpr uint32_t kDeltaRows = 64;    // rows a workgroup of gate_delta_kernel takes at once
+constexpr uint32_t kDeltaRows = 64;    // rows a workgroup of gate_delta_kernel takes at once,
+constexpr uint32_t kDeltaFew = 16;     // or, where that makes few workgroups
 constexpr uint32_t kDeltaWhole = 128;  // rows up to which it takes all of its units'
 constexpr uint32_t kDeltaFill = 128;   // workgroups that are enough for eight units a thread
 
@@ -353,13 +354,13 @@ struct GateDelta {
     PackArgs pack;    // of T bf16: copies that the products need too, by the workgroups after the first `blocks`
 };
 
-// d(r, j) and d(r, half + j) to d, in rows of ldd (ldd's padding is 0), and the sums of kDeltaRows rows' columns to `to`. A
+// d(r, j) and d(r, half + j) to d, in rows of ldd (ldd's padding is 0), and the sums of ROWS rows' columns to `to`. A
 // thread takes W units of eight rows; the eight sums of a unit's threads are added in row order. WHOLE: a workgroup takes all rows,
 // adds their sums in f64, and `to` is bias_updates itself. Bound by memory where it is large: 4096 rows of 8192 units, bf16, 56 us
 // (6.0 TB/s).
-template <class T, int W, bool EXP, bool WHOLE>
+template <class T, int W, bool EXP, bool WHOLE, uint32_t ROWS>
 __global__ __launch_bounds__(kBlock) void gate_delta_kernel(GateDelta<T> g) {
-    constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes, kEach = kDeltaRows / kGroups;
+    constexpr uint32_t kLanes = 32, kGroups = kBlock / kLanes, kEach = ROWS / kGroups;
     __shared__ float lds[2][kGroups][kLanes * W + 4];
     if constexpr (sizeof(T) == 2) {
         if (blockIdx.x >= g.blocks) return pack_chunk(g.pack, (blockIdx.x - g.blocks) * kBlock + threadIdx.x);
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(kBlock) void gate_delta_kernel(GateDelta<T> g) {
     constexpr uint32_t kBatch = W == 1 ? kEach : 2;  // rows whose loads are on their way at once
     constexpr uint32_t kStored = (2 * kLanes * W + kBlock - 1) / kBlock;  // sums that a thread stores
     double whole[kStored] = {};
-    for (uint32_t top = WHOLE ? 0 : block_r * kDeltaRows; top < g.rows; top += kDeltaRows) {
+    for (uint32_t top = WHOLE ? 0 : block_r * ROWS; top < g.rows; top += ROWS) {
         const uint32_t r0 = top + group * kEach;
         float total[2][W] = {};
 #pragma unroll 1
@@ -440,6 +441,14 @@ __global__ __launch_bounds__(kBlock) void gate_delta_kernel(GateDelta<T> g) {
     }
 }
 
+// Rows a workgroup takes, eight units a thread: 64 where that fills the chip; 16 else, whose loads wait in parallel and not one
+// after another (512 rows of 4096 units 10.0 -> 7.3 us). Not for single units, whose 64 rows' loads are on their way at once
+// (333 rows of 1503 8.6 -> 8.4, and more sums to add: 28.1 -> 28.6 with the products).
+inline uint32_t delta_rows(uint64_t rows, uint64_t half) {
+    const uint64_t blocks_c = div_up(half, 256);
+    const bool few = rows > kDeltaWhole && half % 8 == 0 && div_up(rows, kDeltaRows) * blocks_c < 512 && div_up(rows, kDeltaFew) * blocks_c >= kDeltaFill;
+    return few ? kDeltaFew : kDeltaRows;
+}
 inline uint64_t delta_ld(int type, uint64_t hidden) { return round_up(2 * hidden, type == DKZ_F32 ? 4 : 8); }
 
 struct BackwardPlan {
@@ -450,7 +459,7 @@ BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t hi
     BackwardPlan p;
     const uint64_t n = 2 * hidden;
     p.d_bytes = padded(rows * delta_ld(type, hidden) * type_size(type));
-    p.sum_bytes = padded(4 * n * div_up(rows, kDeltaRows));
+    p.sum_bytes = padded(4 * n * div_up(rows, delta_rows(rows, hidden)));
     p.packed = type == DKZ_F32 || rows == 0 ? 0 : packed_bytes(rows, inputs) + packed_bytes(n, inputs);
     if (type == DKZ_F32)
         p.partial_bytes = std::max(f32_partial_bytes(rows, inputs, n), f32_partial_bytes(n, inputs, rows));
@@ -459,21 +468,58 @@ BackwardPlan backward_plan(int type, uint64_t rows, uint64_t inputs, uint64_t hi
     return p;
 }
 
-// bias_updates null: not wanted; sums: room for the sums of every kDeltaRows rows.
+// Sums of rows' columns that are still to be added up, to bias_updates (as column_sums); cols 0: none.
+struct BiasSums {
+    const float *partial;
+    uint32_t chunks, cols;
+    float beta, *to;
+};
+
+// bias_updates null: not wanted; sums: room for the sums of every delta_rows rows, `left` what is to be done with them.
 template <class T, bool EXP>
-int run_gate_delta(hipStream_t stream, GateDelta<T> g, float *sums, float *bias_updates) {
+int run_gate_delta(hipStream_t stream, GateDelta<T> g, float *sums, float *bias_updates, BiasSums &left) {
     constexpr const char *kName = "gated_backward_delta";
     const bool whole = g.rows <= kDeltaWhole;
-    const uint32_t blocks_r = whole ? 1 : div_up(g.rows, kDeltaRows);
-    const bool eights = g.half % 8 == 0 && div_up(g.half, 256) * blocks_r >= kDeltaFill;
+    const uint32_t each = delta_rows(g.rows, g.half), blocks_r = whole ? 1 : div_up(g.rows, each);
+    const bool eights = g.half % 8 == 0 && (each == kDeltaFew || div_up(g.half, 256) * blocks_r >= kDeltaFill);
     g.blocks_c = div_up(g.half, eights ? 256 : 32);
     g.blocks = g.blocks_c * blocks_r;
     g.to = bias_updates == nullptr ? nullptr : whole ? bias_updates : sums;
     const dim3 grid(g.blocks + div_up(g.pack.count(), kBlock)), block(kBlock);
-    if (whole) return eights ? launch_on(stream, kName, gate_delta_kernel<T, 8, EXP, true>, grid, block, g) : launch_on(stream, kName, gate_delta_kernel<T, 1, EXP, true>, grid, block, g);
-    DKZ_TRY(eights ? launch_on(stream, kName, gate_delta_kernel<T, 8, EXP, false>, grid, block, g) : launch_on(stream, kName, gate_delta_kernel<T, 1, EXP, false>, grid, block, g));
-    return bias_updates != nullptr ? add_column_sums(stream, sums, blocks_r, 2 * (uint64_t)g.half, g.beta, bias_updates) : 0;
+    const auto run = [&](auto kernel) { return launch_on(stream, kName, kernel, grid, block, g); };
+    if (whole) return eights ? run(gate_delta_kernel<T, 8, EXP, true, kDeltaRows>) : run(gate_delta_kernel<T, 1, EXP, true, kDeltaRows>);
+    DKZ_TRY(each == kDeltaFew ? run(gate_delta_kernel<T, 8, EXP, false, kDeltaFew>)
+            : eights          ? run(gate_delta_kernel<T, 8, EXP, false, kDeltaRows>)
+                              : run(gate_delta_kernel<T, 1, EXP, false, kDeltaRows>));
+    if (bias_updates != nullptr) left = {sums, blocks_r, 2 * g.half, g.beta, bias_updates};
+    return 0;
 }
+
+// Both gradients, as product_pair_kernel, and, by the workgroups after their `groups`, the bias sums that are left (333x1001, 1503 units 28.1 -> 26.0 us
+// without a launch of theirs).
+template <class T, class Epi>
+__global__ __launch_bounds__(T::kThreads, 2) void gradients_kernel(ProductArgs a, Epi epi_a, ProductArgs b, Epi epi_b, uint32_t tiles_a, bool a_first,
+                                                                  uint32_t groups, BiasSums s) {
+    static_assert(T::kThreads == kBlock && lds_bytes<T, true>() >= sizeof(double[kSumGroups][kSumLanes]));
+    __shared__ __align__(1024) char lds[lds_bytes<T, true>()];
+    if (blockIdx.x >= groups)
+        return column_sums(s.partial, s.chunks, s.cols, s.beta, s.to, blockIdx.x - groups, *reinterpret_cast<double(*)[kSumGroups][kSumLanes]>(lds));
+    const uint32_t first = a_first ? tiles_a : groups - tiles_a, block = blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
+    if ((blockIdx.x < first) == a_first) product_tile<T, false, true, true>(a, epi_a, block, lds);
+    else product_tile<T, true, true, true>(b, epi_b, block, lds);
+}
+struct GradientsLaunch {
+    BiasSums &left;
+    template <class T, class Epi>
+    int run(hipStream_t stream, const char *name, const ProductArgs &a, const Epi &epi_a, const ProductArgs &b, const Epi &epi_b, uint32_t groups_a,
+            uint32_t groups_b, bool a_first) {
+        const BiasSums s = left;
+        left = {};
+        const uint32_t groups = groups_a + groups_b;
+        return launch_on(stream, name, gradients_kernel<T, Epi>, dim3(groups + div_up(s.cols, kSumLanes)), dim3(kBlock), a, epi_a, b, epi_b, groups_a,
+                         a_first, groups, s);
+    }
+};
 
 template <class T>
 int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint64_t hidden, int act, const void *input, const void *weights,
@@ -486,6 +532,7 @@ int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint6
     const bool products = inputs != 0 && (weight_updates != nullptr || input_delta != nullptr);
     Matrix x{weight_updates != nullptr ? reinterpret_cast<const __bf16 *>(input) : nullptr, inputs};
     Matrix w{input_delta != nullptr ? reinterpret_cast<const __bf16 *>(weights) : nullptr, inputs};
+    BiasSums left{};
     if (rows != 0 && hidden != 0 && (products || bias_updates != nullptr)) {
         GateDelta<T> g{};
         g.sums = static_cast<const T *>(sums_in);
@@ -497,7 +544,7 @@ int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint6
         g.ldd = (uint32_t)ldd;
         g.beta = beta;
         if (sizeof(T) == 2 && products) g.pack = pack_args(x, rows, w, n, inputs, ws);
-        DKZ_TRY(gate_has_exp(act) ? (run_gate_delta<T, true>(stream, g, sums, bias_updates)) : (run_gate_delta<T, false>(stream, g, sums, bias_updates)));
+        DKZ_TRY(gate_has_exp(act) ? (run_gate_delta<T, true>(stream, g, sums, bias_updates, left)) : (run_gate_delta<T, false>(stream, g, sums, bias_updates, left)));
     } else if (bias_updates != nullptr) {
         DKZ_TRY(add_column_sums(stream, sums, 0, n, beta, bias_updates));  // no rows: beta * bias_updates
     }
@@ -513,9 +560,9 @@ int backward(hipStream_t stream, int type, uint64_t rows, uint64_t inputs, uint6
     } else {
         const Product to_input{d, ldd, w.p, w.ld, rows, inputs, n}, to_weights{d, ldd, x.p, x.ld, n, inputs, rows};
         DKZ_TRY(run_gradients(stream, kInput, input_delta != nullptr ? &to_input : nullptr, store_epilogue<T>(input_delta, input_residual, inputs, 0.0f),
-                              kWeights, weight_updates != nullptr ? &to_weights : nullptr, store_epilogue<T>(weight_updates, nullptr, inputs, beta), partial, true));
+                              kWeights, weight_updates != nullptr ? &to_weights : nullptr, store_epilogue<T>(weight_updates, nullptr, inputs, beta), partial, true, GradientsLaunch{left}));
     }
-    return 0;
+    return left.cols != 0 ? add_column_sums(stream, left.partial, left.chunks, left.cols, left.beta, left.to) : 0;
 }
 
 bool sizes_ok(int type, int rows, int inputs, int hidden) {

@@ -30,7 +30,14 @@ BACKWARD = [
     SILU, 0), (BF16, 1886, 3304, 5, SILU, 1), (BF16, 4267, 242, 2679, SILU, 0), (BF16, 5832, 2652, 77, SILU, 1),
     (F32, 5, 9, 36272, SILU, 1), (F32, 7, 8, 38488, RELU, 0), (BF16, 7, 16, 39224, SILU, 1), (BF16, 100, 16, 33800, RELU, 0),
     (BF16, 857, 46, 5, RELU, 0), (BF16, 2863, 2712, 584, SILU, 0),
+    (BF16, 8896, 73, 16, SILU, 0), (BF16, 6776, 8, 1104, RELU, 0), (BF16, 3808, 8, 2232, SILU, 0), (F32, 1636, 8, 6320, RELU, 0), (F32, 2104,
+    12, 16, SILU, 0),
 ]
+
+# The same with some results alone (bias, weights, input).
+BACKWARD_PARTS = [((BF16, 16, 8, 21, SILU, 0), (1, 1, 0)), ((BF16, 16, 8, 21, SILU, 0), (1, 0, 1)), ((BF16, 16, 1560, 3877, RELU, 0), (1, 1, 0)),
+                  ((BF16, 333, 1001, 1503, SILU, 0), (0, 1, 1)), ((BF16, 333, 1001, 1503, SILU, 0), (1, 1, 0)), ((BF16, 333, 1001, 1503, SILU, 0), (1, 0, 1)),
+                  ((BF16, 300, 768, 1024, SILU, 0), (0, 1, 1)), ((BF16, 300, 768, 1024, RELU, 0), (1, 0, 0))]
 
 # Rows and classes of logits: a wave a row, a workgroup, several; held in registers by groups of several sizes, read twice.
 ROWS = [(5, 40), (70, 4000), (66, 8001), (600, 9001), (65, 16001), (70, 32000), (66, 65003), (65, 131000), (65, 140001), (2, 65536), (3, 140001)]

@@ -186,6 +186,12 @@ def test_backward_of_every_kernel(pool, case):
     run_backward(pool, kind, rows, inputs, hidden, act, shift=shift, beta=0.5)
 
 
+@pytest.mark.parametrize("case,want", cases.BACKWARD_PARTS, ids=str)
+def test_backward_of_some_results(pool, case, want):
+    kind, rows, inputs, hidden, act, shift = case
+    run_backward(pool, kind, rows, inputs, hidden, act, shift=shift, beta=0.5, want=want)
+
+
 @pytest.mark.parametrize("kind", [F32, BF16])
 def test_backward_without_rows_or_inputs(pool, kind):
     b, w = np.arange(12, dtype=np.float32), ref.rounded(np.arange(48).reshape(12, 4), kind)

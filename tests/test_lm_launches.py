@@ -23,12 +23,12 @@ def forward(kind, rows, inputs, hidden, act=SILU, shift=0, keep=True):
     gpu.gatedForward(kind, rows, inputs, hidden, act, buf(1, shift), buf(2, shift), buf(3), buf(4, shift) if keep else None, buf(5, shift), buf(6))
 
 
-def backward(kind, rows, inputs, hidden, act=SILU, shift=0):
+def backward(kind, rows, inputs, hidden, act=SILU, shift=0, want=(1, 1, 1)):
     from darknet_zig_amd import gpu
 
     shift *= 4 if kind == F32 else 2
-    gpu.gatedBackward(kind, rows, inputs, hidden, act, buf(1, shift), buf(2, shift), buf(3, shift), buf(4, shift), buf(5, shift), 0.5, buf(6),
-                      buf(7, shift), buf(8, shift), buf(9))
+    gpu.gatedBackward(kind, rows, inputs, hidden, act, buf(1, shift), buf(2, shift), buf(3, shift), buf(4, shift), buf(5, shift), 0.5,
+                      buf(6) if want[0] else None, buf(7, shift) if want[1] else None, buf(8, shift) if want[2] else None, buf(9))
 
 
 def log_probs(kind, rows, classes, top=5, entropy=True):
@@ -72,6 +72,8 @@ def kernels_of_the_cases():
         seen += recorded(lambda: forward(*case))
     for case in cases.BACKWARD:
         seen += recorded(lambda: backward(*case))
+    for case, want in cases.BACKWARD_PARTS:
+        seen += recorded(lambda: backward(*case, want))
     for kind in (F32, BF16):
         for rows, classes in cases.ROWS:
             for entropy in (False, True):
