@@ -230,9 +230,12 @@ int run_product(hipStream_t stream, const char *name, const Product &x, const Pr
 // 1 us slower paired) nor kinds of which a compute unit holds one (nothing runs
 // beside them). A whole backward pass, apart and paired: 64x1024x1024 17.3 and 11.5
 // us, 128x4096x1000 18.8 and 13.9, 768x768x3000 31.4 and 25.6, 1536^3 37.2 and 32.4.
-// may_cut: the input gradient's K may be cut here too, as it is alone where the rows are few.
+// may_cut: the input gradient's K may be cut here too, as it is alone where the rows are few, and how is chosen by what
+// is left of the longer tiles when the others have ended (gated blocks, apart, paired as before and so: 200x2048, 2048
+// units 38.7, 36.3 and 30.5 us, 512x1024, 4096 units 61.7, 51.2 and 44.4, 333x1001, 1503 units 31.8, 25.9 and 26.2).
 inline bool plan_pair(const Product &a, const Product &b, ProductPlan &pa, ProductPlan &pb, bool may_cut = false) {
-    float least = pa.us + pb.us + kLaunchUs;
+    const float apart = pa.us + pb.us + kLaunchUs;
+    float least = 1e30f;
     bool found = false;
     if ((pa.splits != 1 && !may_cut) || pb.splits != 1 || !a.direct() || !b.direct() || a.rows == 0 || a.cols == 0 || b.rows == 0 || b.cols == 0) return false;
     const uint32_t most = may_cut ? pa.splits : 1;
@@ -249,9 +252,16 @@ inline bool plan_pair(const Product &a, const Product &b, ProductPlan &pa, Produ
             const auto alone = [&](uint64_t slabs, uint64_t tiles) {
                 return (float)slabs * t.slab[std::min<uint64_t>((tiles + kComputeUnits - 1) / kComputeUnits, t.occupancy) - 1] + t.fixed;
             };
+            const float join = splits > 1 ? join_us(splits, a.rows, a.cols) : 0.0f;
             float us = std::max(std::max(alone(slabs_a, tiles_a), alone(slabs_b, tiles_b)), all + 0.5f * std::min(us_a, us_b));
-            if (splits > 1) us += join_us(splits, a.rows, a.cols);
-            if (us >= least || tiles_a + tiles_b > 0x7fffffffull) continue;
+            if (us + join >= apart || tiles_a + tiles_b > 0x7fffffffull) continue;
+            if (may_cut) {  // the longer tiles' slabs that are left, a compute unit's other tiles having ended
+                const uint64_t slabs = std::max(slabs_a, slabs_b), tiles = slabs_a > slabs_b ? tiles_a : tiles_b;
+                const float left = (float)slabs - all / t.slab[each - 1];
+                if (left > 0.0f) us = std::max(us, all + left * t.slab[std::min<uint64_t>((tiles + kComputeUnits - 1) / kComputeUnits, t.occupancy) - 1]);
+            }
+            us += join;
+            if (us >= least) continue;
             least = us;
             pa = {t.br, t.bc, t.wr, t.wc, (uint32_t)splits, (uint32_t)(slabs_a * 64), true, us};
             pb = {t.br, t.bc, t.wr, t.wc, 1, (uint32_t)(slabs_b * 64), true, us};
