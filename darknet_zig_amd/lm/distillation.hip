@@ -105,15 +105,17 @@ struct RowOf {
         finish();
     }
 
-    // The loss, by the first wave.
+    // The loss, by the first wave. temperature * (log p - log q) is temperature * (log p + l) - (z - m), which stays finite where
+    // a class is masked by the type's lowest value and the temperature is below 1.
     __device__ __forceinline__ void loss(const Sums &a, float l, bool store = true) const {
+        const bool left = a.m != neg_inf() || l != neg_inf();  // a class
         float sum = 0.0f;
         in.z[threadIdx.x] = z;
 #pragma unroll 1
         for (uint32_t j = threadIdx.x; j < t.top; j += kWave)
-            if (in.p[j] != 0.0f) sum += in.p[j] * (in.log_p[j] - log_prob_of(in.z[j], a.m, l, g.inv));
+            if (in.p[j] != 0.0f) sum += in.p[j] * (left ? t.temperature * (in.log_p[j] + l) - (in.z[j] - a.m) : -neg_inf());
         sum = lanes_reduce<kWave>(sum, [](float x, float y) { return x + y; });
-        if (threadIdx.x == 0 && store) t.loss[row] = t.temperature * (t.temperature * sum);
+        if (threadIdx.x == 0 && store) t.loss[row] = t.temperature * sum;
     }
 
     // Writes a part of the delta. vectors(f) calls f(v, logits of vector v) for this thread's vectors of the part.

@@ -86,7 +86,8 @@ int dkz_gated_backward(int type, int rows, int inputs, int hidden, int activatio
  *                                past the last other one the token is -1 and its log
  *                                probability -infinity.
  * tokens and log_probs may be NULL where given is 0, as top_tokens and top_log_probs
- * where top is. temperature is 2^-64 .. 2^64. A row that has no class left has
+ * where top is. temperature is 2^-64 .. 2^64. (fp32: what passes its range, the
+ * difference of two logits too, is infinite.) A row that has no class left has
  * m and l -infinity, log probabilities -infinity and entropy 0. A row with a NaN or
  * +infinity logit has NaN for l, log probabilities and entropy, and no alternatives:
  * tokens -1 with NaN. m passes over NaNs. */

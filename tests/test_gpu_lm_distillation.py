@@ -168,6 +168,20 @@ def test_specials_stay_in_their_rows(pool, kind, classes):
 
 @pytest.mark.parametrize("kind", [F32, BF16])
 @pytest.mark.parametrize("classes", [500, 20000, 70000])
+@pytest.mark.parametrize("temperature", [2.0**-60, 0.3, 0.7, 1.0])
+def test_masks_of_the_type_s_lowest_value(pool, kind, classes, temperature):
+    """A loss is finite where its formula's value is."""
+    lowest = -np.finfo(np.float32).max if kind == F32 else -float.fromhex("0x1.fep127")
+    z = make(kind, 5, classes, classes)
+    z[1, ::3] = z[3, 1:] = z[4] = lowest
+    t, l = teacher(5, 9, classes)
+    t[:, 0], t[3, 1] = 0, classes - 1
+    loss = check(pool, kind, z, classes, temperature, t, l)  # at most the temperature times 2^128
+    assert np.isfinite(loss).all()
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("classes", [500, 20000, 70000])
 def test_logits_far_from_zero(pool, kind, classes):
     """Rows whose logits are all large: only their distances matter."""
     r = np.random.default_rng(2)
