@@ -219,13 +219,15 @@ template <class T>
 __global__ __launch_bounds__(kBlock) void distillation_sums_kernel(Logits g, Teacher t) {
     __shared__ Sums sums[kBlock / kWave];
     const Exp<T> ex(g.inv);
-    const uint32_t row = blockIdx.x / g.parts, part = blockIdx.x - row * g.parts;
-    const T *logits = static_cast<const T *>(g.p) + (uint64_t)row * g.pitch;
-    const Sums a = part_sums<T, kBlock>(logits, Part<T>(g, row, part), ex, sums);
-    if (threadIdx.x == 0) t.part_sums[blockIdx.x] = a;
-    if (part == 0 && threadIdx.x < t.top) {
-        const uint32_t c = (uint32_t)t.tokens[(uint64_t)row * t.top + threadIdx.x];
-        if (c < g.classes) t.entry_logits[(uint64_t)row * kMostEntries + threadIdx.x] = load1(logits, c);
+    for (uint32_t group = blockIdx.x; group < g.rows * g.parts; group += gridDim.x) {
+        const uint32_t row = group / g.parts, part = group - row * g.parts;
+        const T *logits = static_cast<const T *>(g.p) + (uint64_t)row * g.pitch;
+        const Sums a = part_sums<T, kBlock>(logits, Part<T>(g, row, part), ex, sums);
+        if (threadIdx.x == 0) t.part_sums[group] = a;
+        if (part == 0 && threadIdx.x < t.top) {
+            const uint32_t c = (uint32_t)t.tokens[(uint64_t)row * t.top + threadIdx.x];
+            if (c < g.classes) t.entry_logits[(uint64_t)row * kMostEntries + threadIdx.x] = load1(logits, c);
+        }
     }
 }
 template <class T>
@@ -233,16 +235,19 @@ __global__ __launch_bounds__(kBlock) void distillation_delta_kernel(Logits g, Te
     __shared__ Sums sums[kBlock / kWave];
     __shared__ Entries in;
     const Exp<T> ex(g.inv);
-    // Without a delta a group a row suffices.
-    const uint32_t parts = t.delta != nullptr ? g.parts : 1, row = blockIdx.x / parts, part = blockIdx.x - row * parts;
-    RowOf<T> r(g, t, in, row);
-    if (threadIdx.x < kWave) r.read();
-    Sums a{neg_inf(), 0.0f, 0.0f};
-    for (uint32_t p = threadIdx.x; p < g.parts; p += kBlock) a = merge(a, t.part_sums[(uint64_t)row * g.parts + p], ex);
-    a = group_reduce<Sums, kBlock>(a, sums, [&](const Sums &x, const Sums &y) { return merge(x, y, ex); });
-    const float l = log_sum(a);
-    if (threadIdx.x < kWave) r.loss(a, l, part == 0);
-    if (t.delta != nullptr) r.template write_again<kBlock>(Part<T>(g, row, part), a, l, ex);
+    const uint32_t parts = t.delta != nullptr ? g.parts : 1;  // without a delta a group a row suffices
+    for (uint32_t group = blockIdx.x; group < g.rows * parts; group += gridDim.x) {
+        const uint32_t row = group / parts, part = group - row * parts;
+        if (group != blockIdx.x) __syncthreads();  // the last group's use of `in`
+        RowOf<T> r(g, t, in, row);
+        if (threadIdx.x < kWave) r.read();
+        Sums a{neg_inf(), 0.0f, 0.0f};
+        for (uint32_t p = threadIdx.x; p < g.parts; p += kBlock) a = merge(a, t.part_sums[(uint64_t)row * g.parts + p], ex);
+        a = group_reduce<Sums, kBlock>(a, sums, [&](const Sums &x, const Sums &y) { return merge(x, y, ex); });
+        const float l = log_sum(a);
+        if (threadIdx.x < kWave) r.loss(a, l, part == 0);
+        if (t.delta != nullptr) r.template write_again<kBlock>(Part<T>(g, row, part), a, l, ex);
+    }
 }
 
 // How rows are taken: held by groups of `threads` with `vectors` a thread, or (threads 0) in parts.
@@ -276,8 +281,11 @@ int distill(hipStream_t stream, const Logits &g, const DistillPlan &plan, const 
     if (plan.threads == 512 && plan.vectors == 8) return launch_on(stream, kName, distillation_held_kernel<T, 512, 8>, grid, block, g, t);
     if (plan.threads == 512) return launch_on(stream, kName, distillation_held_kernel<T, 512, 16>, grid, block, g, t);
     if (plan.threads == 1024) return launch_on(stream, kName, distillation_held_kernel<T, 1024, 16>, grid, block, g, t);
-    DKZ_TRY(launch_on(stream, "distillation_sums", distillation_sums_kernel<T>, dim3(g.rows * g.parts), dim3(kBlock), g, t));
-    return launch_on(stream, kName, distillation_delta_kernel<T>, dim3(t.delta != nullptr ? g.rows * g.parts : g.rows), dim3(kBlock), g, t);
+    // (The groups go round the rows' parts: a workgroup each would be more threads than a launch counts where the logits are a large
+    // part of the memory.)
+    const dim3 parts(plan.rows.groups(g.rows));
+    DKZ_TRY(launch_on(stream, "distillation_sums", distillation_sums_kernel<T>, parts, dim3(kBlock), g, t));
+    return launch_on(stream, kName, distillation_delta_kernel<T>, t.delta != nullptr ? parts : grid, dim3(kBlock), g, t);
 }
 
 }  // namespace

@@ -139,6 +139,18 @@ def test_a_launch_has_fewer_than_2_to_the_32_threads(call):
     assert most and all(0 < threads < 2**32 for threads in most.values()), most
 
 
+# Many rows of many classes, up to 2^38 logits: what parts of rows add up to.
+LARGEST_OF_PARTS = [(name, kind, rows, classes) for name in ("log_probs", "log_probs_backward", "distillation")
+                    for kind, rows, classes in [(F32, 1 << 20, 1 << 18), (BF16, 1 << 20, 1 << 18), (F32, 1000000, 65540), (BF16, 1000000, 131080),
+                                                (BF16, 511, 1 << 26), (F32, 1 << 14, 1 << 24)]]
+
+
+@pytest.mark.parametrize("call", [*LARGEST_OF_PARTS, ("distillation", F32, 1 << 20, 1 << 18, False)], ids=str)
+def test_many_long_rows_have_fewer_than_2_to_the_32_threads(call):
+    most = in_child("tests.test_lm_launches:grids_of", *call)
+    assert most and all(0 < threads < 2**32 for threads in most.values()), most
+
+
 # ---- what the compiler is told ----
 
 
