@@ -94,7 +94,8 @@ struct RowOf {
         const float log_s = logf(s), over = 1.0f / s;
 #pragma unroll 1
         for (uint32_t j = threadIdx.x; j - threadIdx.x < t.top; j += kWave) {
-            in.p[j] = in.p[j] == 0.0f ? 0.0f : in.p[j] * over;
+            // NaN: a NaN or infinity among them leaves no entry a probability.
+            in.p[j] = in.p[j] == 0.0f && (s == s || in.token[j] == ~0u) ? 0.0f : in.p[j] * over;
             in.log_p[j] -= log_s;
         }
         if (threadIdx.x == 0) in.mass = s;

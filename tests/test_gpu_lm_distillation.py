@@ -167,6 +167,32 @@ def test_specials_stay_in_their_rows(pool, kind, classes):
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("classes", [300, 30000, 140000])
+@pytest.mark.parametrize("special", [np.nan, np.inf])
+def test_a_teacher_s_special_is_in_all_of_its_entries(pool, kind, classes, special):
+    """No entry of such a row has a probability: the deltas of all their classes are NaN, those of the others as without."""
+    rows, top = 4, 70
+    z = make(kind, rows, classes, classes)
+    t = np.tile(np.arange(top, dtype=np.int32) * 3, (rows, 1))
+    l = np.random.default_rng(3).normal(size=(rows, top)).astype(np.float32)
+    t[1:, 5], t[1:, 68] = -1, classes  # no entries
+    l[2, 66] = l[3, 0] = special
+    l[3, 1], l[3, 2], l[1, 5], l[1, 68] = -np.inf, special, special, special
+    l[3, 4] = -1000.0
+    dz, dt, dl, loss, out = pool(z, kind), pool(t), pool(l), pool(n=rows), pool(kind=kind, n=(rows, classes))
+    ws = pool.work(gpu.distillationWorkspace(kind, rows, classes))
+    gpu.distillation(kind, rows, classes, classes, dz.buf, 1.0, top, dt.buf, dl.buf, None, 1.0, loss.buf, out.buf, buf(ws))
+    got, d = loss.get(), out.get()
+    assert np.isfinite(got[:2]).all() and np.isfinite(d[:2]).all() and np.isnan(got[2:]).all()
+    want = np.zeros((2, classes), bool)
+    for i in (0, 1):
+        want[i, t[2 + i][(t[2 + i] >= 0) & (t[2 + i] < classes)]] = True
+    assert (np.isnan(d[2:]) == want).all()
+    q = lm.Softmax(z, 1.0).p[2:]
+    assert_within(d[2:][~want], -q[~want], 2.0**-7 * q[~want] + 2.0**-120, "the others")
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
 @pytest.mark.parametrize("classes", [500, 20000, 70000])
 @pytest.mark.parametrize("temperature", [2.0**-60, 0.3, 0.7, 1.0])
 def test_masks_of_the_type_s_lowest_value(pool, kind, classes, temperature):
