@@ -352,8 +352,9 @@ __device__ __forceinline__ Claim claim(const uint32_t *tokens, const float *valu
     return r;
 }
 
-// log of the sum: of a row without a class left -infinity; NaN stays.
-__device__ __forceinline__ float log_sum(const Sums &a) { return a.s == 0.0f ? neg_inf() : logf(a.s); }
+// log of the sum: of a row without a class left -infinity; NaN stays. The largest logit's own term is 1, but for the rounding that
+// sums_from takes out of it again: a sum just below 1 is 1, so that no probability is above it.
+__device__ __forceinline__ float log_sum(const Sums &a) { return a.s == 0.0f ? neg_inf() : logf(a.s < 1.0f ? 1.0f : a.s); }
 
 // (z - m) / T - l, the log probability of a class. A row without a class left: -infinity.
 __device__ __forceinline__ float log_prob_of(float z, float m, float l, float inv) {

@@ -42,8 +42,11 @@ struct Answer {
         if (threadIdx.x == 0) {
             out.stats[2 * (uint64_t)row] = a.m;
             out.stats[2 * (uint64_t)row + 1] = l;
-            // l and -t / s are both at least 0: nothing cancels.
-            if (out.entropy != nullptr) out.entropy[row] = a.s == 0.0f ? 0.0f : l - Exp<T>::kUnit * (a.t / a.s);
+            // l and -t / s are both at least 0, the latter but for its rounding: nothing cancels. NaN stays.
+            if (out.entropy != nullptr) {
+                const float h = l - Exp<T>::kUnit * (a.t / a.s);
+                out.entropy[row] = a.s == 0.0f || h < 0.0f ? 0.0f : h;
+            }
         }
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {

@@ -193,6 +193,17 @@ def test_a_teacher_s_special_is_in_all_of_its_entries(pool, kind, classes, speci
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
+def test_one_class_left_that_the_teacher_has_is_no_loss(pool, kind):
+    rows, classes = 2000, 40
+    r = np.random.default_rng(4)
+    z = np.full((rows, classes), -np.inf, np.float32)
+    at = r.integers(0, classes, rows)
+    z[np.arange(rows), at] = ref.rounded(r.normal(size=rows) * 8, kind)
+    loss = check(pool, kind, z, classes, 0.7, at[:, None].astype(np.int32), np.ones((rows, 1), np.float32))
+    assert (loss == 0).all()
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
 @pytest.mark.parametrize("classes", [500, 20000, 70000])
 @pytest.mark.parametrize("temperature", [2.0**-60, 0.3, 0.7, 1.0])
 def test_masks_of_the_type_s_lowest_value(pool, kind, classes, temperature):

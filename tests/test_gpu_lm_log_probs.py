@@ -203,6 +203,28 @@ def test_more_rows_than_workgroups(pool):
     assert_within(lp[:, 0], want, err, "log_probs")
 
 
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("rows,classes", [(2000, 12), (1000, 900), (600, 5000), (3, 70000)])
+@pytest.mark.parametrize("entropy", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+def test_no_probability_is_above_1(pool, kind, rows, classes, entropy, temperature):
+    """Rows with one class left, or one far above the others: log probabilities are at most 0, entropies and log sums at least 0."""
+    r = np.random.default_rng(rows + classes)
+    for others in (-np.inf, -200.0, -30.0):
+        z = np.full((rows, classes), np.nan, np.float32)
+        m = ref.rounded(r.normal(size=(rows, 1)) * 8, kind)
+        z[:] = ref.rounded(m + others, kind)
+        at = r.integers(0, classes, rows)
+        z[np.arange(rows), at] = m[:, 0]
+        lp, h, stats, tt, tl = run(pool, kind, z, classes, temperature, at[:, None].astype(np.int32), 2, entropy)
+        assert (lp <= 0).all() and (stats[:, 1] >= 0).all() and (tl <= 0).all() and (tt[:, 0] == at).all()
+        assert h is None or (h >= 0).all()
+        s = lm.Softmax(z, temperature)
+        assert_within(stats[:, 1], s.l, s.l_err, "log sums")
+        if entropy:
+            assert_within(h, s.h, s.h_err, "entropy")
+
+
 def test_offsets_past_32_bits(pool):
     """Rows whose elements lie past 2^32 bytes and 2^31 elements: 33000 x 65600 bf16. (65001 classes: the sums are within
     U (34 + 6 (65001 / 4096 + 110)) = 5e-5, see lm_ref.Softmax.)"""
