@@ -202,6 +202,25 @@ def test_backward_without_rows_or_inputs(pool, kind):
 
 
 @pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("rows", [3, 300])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_backward_without_units_or_inputs(pool, kind, rows, shift):
+    """No units: the input's delta is the residual, or 0. No inputs: there are bias sums alone."""
+    for inputs in (1, 13, 264):
+        res = ref.rounded(np.random.default_rng(rows + inputs).normal(size=(rows, inputs)), kind)
+        dres, dx, out = (pool(res, kind, shift=shift) for _ in range(3))
+        ws = pool.work(gpu.gatedBackwardWorkspace(kind, rows, inputs, 0))
+        none = gpu.Buf()
+        gpu.gatedBackward(kind, rows, inputs, 0, SILU, dx.buf, none, none, none, dres.buf, 0.0, none, none, out.buf, buf(ws))
+        assert (out.get() == res).all()
+        gpu.gatedBackward(kind, rows, inputs, 0, SILU, dx.buf, none, none, none, dres.buf, 0.5, none, none, dres.buf, buf(ws))
+        assert (dres.get() == res).all() and (dx.get() == res).all()
+        gpu.gatedBackward(kind, rows, inputs, 0, SILU, dx.buf, none, none, none, None, 0.0, none, none, out.buf, buf(ws))
+        assert (out.get() == 0).all()
+    run_backward(pool, kind, rows, 0, 24, GELU, True, beta=0.5, shift=shift)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
 @pytest.mark.parametrize("act", GATES)
 def test_backward_over_the_range(pool, kind, act):
     """The two parts of d by themselves (identity weights): gates far from 0 give no NaN and the slopes of their limits."""
