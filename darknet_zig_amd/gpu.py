@@ -527,7 +527,8 @@ def batchnormBackward(
 # ---- the dense operators of libdkz_dense.so (include/dkz_dense.h): connected
 # layers with their epilogue, dropout without a stored mask, and softmax
 # cross-entropy without stored logits. `type` is F32 or BF16. Workspaces are
-# the caller's: allocate what the *Workspace function says, in bytes. ----
+# the caller's: allocate what the *Workspace function says, in bytes, for the call's
+# own sizes (fewer rows can need more). ----
 
 F32, BF16 = 0, 1
 
@@ -645,7 +646,7 @@ def linearCrossEntropyBackward(
 
 # ---- a token model's operators of libdkz_lm.so (include/dkz_lm.h): gated
 # feed-forward blocks, log probabilities of tokens and distillation from logits.
-# Workspaces as above. ----
+# Workspaces as above; those of calls on logits do for fewer rows too. ----
 
 SILU, GELU = 14, 15  # a gate's activations beside logistic, relu and linear
 

@@ -257,6 +257,7 @@ struct DistillPlan {
     RowPlan rows;
     uint64_t bytes(uint64_t n) const { return threads != 0 ? 0 : padded(n * rows.parts * sizeof(Sums)) + padded(n * kMostEntries * 4); }
 };
+constexpr uint64_t kFewRows = 64;
 DistillPlan plan_distillation(int type, uint64_t rows, uint64_t classes) {
     const uint64_t vectors = classes / (type == DKZ_F32 ? 4 : 8);  // whole ones at most
     // 4096 rows of 65536 bf16 classes 216 us with 512 threads and 16 vectors, 249 with 1024 and 8, 348 with 1024 and 16; of 32768
@@ -265,11 +266,16 @@ DistillPlan plan_distillation(int type, uint64_t rows, uint64_t classes) {
     for (const auto &h : kHeld) {
         // Few long rows leave the chip empty: two launches of several groups a row (65536 classes in bf16: 1 row 11.0 us, 13.3
         // held; 64 rows 16.3 and 17.1; 128 rows 19.4 and 18.0. 131072: 1 row 11.0 and 20.7, 64 rows 19.0 and 25.0. 32768: 1 row
-        // 10.6 and 9.5).
-        if (rows <= 64 && h[0] * h[1] > 4096) break;
+        // 10.6 and 9.5). One limit for all lengths, 65536 classes': at 131072 parts might do for more rows, which was not measured.
+        if (rows <= kFewRows && h[0] * h[1] > 4096) break;
         if (vectors <= h[0] * h[1]) return {h[0], h[1], {0, 1, h[0] * h[1]}};
     }
     return {0, 0, plan_rows(type, rows, classes, kMostParts * rows)};
+}
+// The most that any number of rows up to `rows` takes: those in parts take more the more they are.
+uint64_t most_bytes(int type, uint64_t rows, uint64_t classes) {
+    const uint64_t few = std::min(rows, kFewRows);
+    return std::max(plan_distillation(type, rows, classes).bytes(rows), plan_distillation(type, few, classes).bytes(few));
 }
 
 template <class T>
@@ -298,7 +304,7 @@ extern "C" {
 
 int dkz_distillation_workspace(int type, int rows, int classes, size_t *bytes) {
     DKZ_REQUIRE(bytes != nullptr && logits_ok(type, rows, classes, classes, 1.0f));
-    *bytes = (size_t)plan_distillation(type, rows, classes).bytes((uint64_t)rows);
+    *bytes = (size_t)most_bytes(type, (uint64_t)rows, (uint64_t)classes);
     return 0;
 }
 

@@ -388,10 +388,11 @@ inline RowPlan plan_rows(int type, uint64_t rows, uint64_t classes, uint64_t fil
 // Where the parts' results are joined by another launch, which takes as long as three tiles: parts where they save more. (fp32, top
 // 20, us in parts and in one: 1 row of 2 tiles 11.7 and 8.8, of 4 11.9 and 12.2, of 5 12.3 and 13.6; 200 rows of 5 20.0 and 17.2.
 // bf16, top 5, 7 tiles: 200 rows 19.1 and 20.1, 300 rows 23.5 and 21.7.)
+constexpr uint64_t kJoinFill = 512;
 inline RowPlan plan_joined_rows(int type, uint64_t rows, uint64_t classes) {
-    constexpr uint64_t kFill = 512, kJoinTiles = 3;
+    constexpr uint64_t kJoinTiles = 3;
     const uint64_t tile = kTileVectors * kBlock * (type == DKZ_F32 ? 4 : 8), tiles = (classes + tile - 1) / tile;
-    return plan_rows(type, rows, classes, kJoinTiles + (tiles * rows + kFill - 1) / kFill < tiles ? kFill : 0);
+    return plan_rows(type, rows, classes, kJoinTiles + (tiles * rows + kJoinFill - 1) / kJoinFill < tiles ? kJoinFill : 0);
 }
 
 inline Logits make_logits(const RowPlan &plan, const void *p, int rows, int classes, int pitch, float temperature) {

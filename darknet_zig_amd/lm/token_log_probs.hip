@@ -161,6 +161,12 @@ __global__ __launch_bounds__(kBlock) void join_log_probs_kernel(Logits g, Answer
 uint64_t part_bytes(uint64_t rows, const RowPlan &p, uint64_t top) {
     return p.parts == 1 ? 0 : padded(rows * p.parts * sizeof(Sums)) + padded(rows * p.parts * top * 8);
 }
+// The most that any number of rows up to `rows` takes: from kJoinFill on they have no parts.
+uint64_t most_part_bytes(int type, uint64_t rows, uint64_t classes, uint64_t top) {
+    uint64_t most = 0;
+    for (uint64_t r = 1; r <= std::min(rows, kJoinFill); ++r) most = std::max(most, part_bytes(r, plan_joined_rows(type, r, classes), top));
+    return most;
+}
 
 template <class T, bool ENTROPY, bool TOP>
 int run_log_probs(hipStream_t stream, const Logits &g, const RowPlan &plan, const Answers &out) {
@@ -288,7 +294,7 @@ extern "C" {
 
 int dkz_token_log_probs_workspace(int type, int rows, int classes, int top, size_t *bytes) {
     DKZ_REQUIRE(bytes != nullptr && logits_ok(type, rows, classes, classes, 1.0f) && top >= 0 && top <= kMostTop);
-    *bytes = (size_t)part_bytes((uint64_t)rows, plan_joined_rows(type, rows, classes), (uint64_t)top);
+    *bytes = (size_t)most_part_bytes(type, (uint64_t)rows, (uint64_t)classes, (uint64_t)top);
     return 0;
 }
 

@@ -29,7 +29,10 @@
  *     an input, but for the places named below.
  *   - The ops keep no scratch of their own: what they need is the caller's
  *     workspace (16-byte aligned device memory, contents irrelevant before and
- *     after; null where 0 bytes are needed). Calls with workspaces of their own
+ *     after; null where 0 bytes are needed). How much goes by a call's own sizes:
+ *     fewer rows can need more, since a product that leaves the chip empty is cut
+ *     into pieces, so that a workspace for several batch sizes is the largest of
+ *     theirs. Calls with workspaces of their own
  *     may overlap on any streams, host threads and captured graphs. (The stream is
  *     the process's: host threads that set streams of their own take a lock from
  *     dkz_set_stream to the call's return.) Nothing is allocated, copied to the

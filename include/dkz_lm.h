@@ -12,6 +12,10 @@
  * library's calls on this host thread. Deltas are the negative gradients of a loss,
  * as everywhere in the framework.
  *
+ * A workspace of a gated block goes by the call's own sizes, as dkz_dense.h's do: fewer
+ * rows can need more. What the queries of the calls on logits give does for any number
+ * of rows up to theirs.
+ *
  * Logits are rows of `classes` elements, each row `pitch` elements after the one
  * before (pitch >= classes); what lies between a row's end and the next row is
  * neither read nor written. rows, classes and pitch are 2^26 at most and

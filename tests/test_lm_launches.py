@@ -151,6 +151,63 @@ def test_many_long_rows_have_fewer_than_2_to_the_32_threads(call):
     assert most and all(0 < threads < 2**32 for threads in most.values()), most
 
 
+# ---- workspaces ----
+
+CLASSES = [0, 3, 1024, 16400, 32768, 40000, 50001, 65536, 65540, 131080, 262144, 1 << 20, 1 << 26]
+
+
+def workspaces(kind):
+    """What the queries of logits give for 0 to 1100 rows and some more of 2^26 classes at most, by classes and top."""
+    from darknet_zig_amd import gpu
+
+    load()
+    more = [*range(1101), 2000, 1 << 14, 1 << 20, 1 << 26]
+    out = []
+    for classes in CLASSES:
+        rows = [r for r in more if r * classes <= 1 << 38]
+        for top in (0, 5, 64):
+            out.append([f"log_probs {classes} {top}", [gpu.tokenLogProbsWorkspace(kind, r, classes, top) for r in rows]])
+        out.append([f"distillation {classes}", [gpu.distillationWorkspace(kind, r, classes) for r in rows]])
+    return out
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_a_workspace_of_logits_does_for_fewer_rows(kind):
+    found = in_child("tests.test_lm_launches:workspaces", kind)
+    for name, sizes in found:
+        assert sizes == sorted(sizes), (name, [(i, a, b) for i, (a, b) in enumerate(zip(sizes, sizes[1:])) if a > b][:5])
+    assert sum(sizes[-1] > 0 for _, sizes in found) > 20
+
+
+def refused_with_the_workspace_of(kind, most, classes):
+    """Of 1 .. `most` rows, those whose calls refuse a workspace for `most`."""
+    from darknet_zig_amd import gpu
+
+    load()
+    refused = []
+    words = lambda n: gpu.Buf(buf(9).ptr, n // 4) if n else None
+    for top in (0, 5):
+        ws = words(gpu.tokenLogProbsWorkspace(kind, most, classes, top))
+        for rows in range(1, most + 1):
+            try:
+                recorded(lambda: gpu.tokenLogProbs(kind, rows, classes, classes, buf(1), 1.0, 0, None, top, None, None, buf(5), buf(6), buf(7), ws))
+            except gpu.GpuError:
+                refused.append(("log_probs", top, rows))
+    ws = words(gpu.distillationWorkspace(kind, most, classes))
+    for rows in range(1, most + 1):
+        try:
+            recorded(lambda: gpu.distillation(kind, rows, classes, classes, buf(1), 1.0, 5, buf(2), buf(3), None, 1.0, buf(5), buf(6), ws))
+        except gpu.GpuError:
+            refused.append(("distillation", rows))
+    return refused
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("most,classes", [(600, 50001), (600, 65536), (300, 131080), (130, 150000)])
+def test_a_call_of_fewer_rows_takes_the_workspace(kind, most, classes):
+    assert in_child("tests.test_lm_launches:refused_with_the_workspace_of", kind, most, classes) == []
+
+
 # ---- what the compiler is told ----
 
 
