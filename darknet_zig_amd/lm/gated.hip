@@ -354,7 +354,9 @@ struct GateDelta {
     PackArgs pack;    // of T bf16: copies that the products need too, by the workgroups after the first `blocks`
 };
 
-// d(r, j) and d(r, half + j) to d, in rows of ldd (ldd's padding is 0), and the sums of ROWS rows' columns to `to`. A
+// d(r, j) and d(r, half + j) to d, in rows of ldd (ldd's padding is 0), and the sums of ROWS rows' columns to `to`. bf16: d is
+// rounded as it is stored, since the matrix instruction takes no wider operands (two of them a d would double the products'
+// time): the gradients are off by 0.0023 of their norm, by their own rounding alone 0.0017. The sums take it unrounded. A
 // thread takes W units of eight rows; the eight sums of a unit's threads are added in row order. WHOLE: a workgroup takes all rows,
 // adds their sums in f64, and `to` is bias_updates itself. Bound by memory where it is large: 4096 rows of 8192 units, bf16, 56 us
 // (6.0 TB/s).
